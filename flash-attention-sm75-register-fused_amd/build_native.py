@@ -47,6 +47,11 @@ HIP_SOURCES = [
     "fa_fwd_d64_keys_bf16.hip",
     "fa_bwd_d128.hip", "fa_bwd_d64.hip", "fa_bwd_d128_mask.hip", "fa_bwd_d64_mask.hip",
     "fa_bwd.hip",
+    "fa_paged_d128.hip", "fa_paged_d128_bf16.hip", "fa_paged_d128_fp8.hip",
+    "fa_paged_d128_bf16_fp8.hip",
+    "fa_paged_d64.hip", "fa_paged_d64_bf16.hip", "fa_paged_d64_fp8.hip",
+    "fa_paged_d64_bf16_fp8.hip",
+    "fa_paged.hip", "fa_paged_cache.hip", "fa_paged_capi.hip",
     "fa_fwd.hip", "fa_decode.hip", "fa_mask.hip", "fa_naive.hip", "fa_capi.hip",
 ]
 
@@ -127,7 +132,7 @@ def build_binding(verbose: bool = False) -> str:
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         f"-I{INCLUDE}", f"-I{py_inc}",
         *[f"-I{p}" for p in incs],
-        os.path.join(CSRC, "binding.cpp"),
+        os.path.join(CSRC, "binding.cpp"), os.path.join(CSRC, "binding_paged.cpp"),
         "-o", tmp,
         *[f"-L{p}" for p in libdirs],
         f"-L{OUT_DIR}",

@@ -426,6 +426,8 @@ torch::Tensor naive_attention_forward(torch::Tensor Q, torch::Tensor K, torch::T
 
 }  // namespace
 
+void bind_paged(pybind11::module_& m);  // binding_paged.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X (gfx950) fused attention forward, reference-compatible op set";
   m.def("naive_attention_forward", &naive_attention_forward);
@@ -445,6 +447,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("dO"), pybind11::arg("Q"), pybind11::arg("K"), pybind11::arg("V"),
         pybind11::arg("O"), pybind11::arg("LSE"), pybind11::arg("causal"),
         pybind11::arg("scale"), pybind11::arg("attn_mask") = pybind11::none());
+  bind_paged(m);
   m.def("abi_version", []() { return fa_sm75_abi_version(); });
   m.def("set_kernel_policy", [](int policy) {
     TORCH_CHECK(fa_sm75_set_kernel_policy(policy) == FA_OK,

@@ -13,12 +13,13 @@
 #include <mutex>
 #include <string>
 
+#include "fa_capi_error.h"
 #include "fa_internal.h"
 #include "flash_attn_sm75.h"
 
 namespace {
 
-thread_local char g_last_error[512] = "";
+thread_local char g_last_error[fa::kCapiErrorBytes] = "";
 
 // Which fused kernel fa_sm75_forward launches (process-wide).
 std::atomic<int> g_kernel_policy{FA_POLICY_AUTO};
@@ -30,6 +31,21 @@ int fail(int status, const char* fmt, ...) {
   va_end(ap);
   return status;
 }
+
+}  // namespace
+
+namespace fa {
+int capi_fail(int status, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return status;
+}
+char* capi_error_buffer() { return g_last_error; }
+}  // namespace fa
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

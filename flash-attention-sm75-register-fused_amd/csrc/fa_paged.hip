@@ -1,0 +1,81 @@
+// Attention over a paged cache: the plan, the launches, and the kernel that merges
+// the partials of cut units (fa_paged_attn.h).
+#include <algorithm>
+#include <numeric>
+
+#include "fa_internal.h"
+#include "fa_paged_attn.h"
+
+namespace fa {
+
+// The instances of fa_paged_d*.hip.
+#define FA_PAGED_EXTERN(D, BF, F8) \
+  extern template void launch_paged_attn<D, BF, F8>(const PagedArgs&, int, int64_t, hipStream_t);
+FA_PAGED_EXTERN(64, false, false) FA_PAGED_EXTERN(64, true, false)
+FA_PAGED_EXTERN(64, false, true) FA_PAGED_EXTERN(64, true, true)
+FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
+FA_PAGED_EXTERN(128, false, true) FA_PAGED_EXTERN(128, true, true)
+#undef FA_PAGED_EXTERN
+
+namespace {
+int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records
+  return 2ll * rows * (head_dim + 2) * (int64_t)sizeof(float);
+}
+}  // namespace
+
+PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
+                     int64_t workspace_bytes) {
+  PagedPlan p;
+  p.rows = max_query_len * a.group <= 16 ? 16 : 32;
+  p.classes = std::gcd(a.hkv, kNumXcds);
+  const int64_t resident = resident_fused_workgroups();
+  const int64_t room = workspace_bytes / (partial_bytes(p.rows, head_dim) * p.classes);
+  p.wgs = (int)std::min(resident / p.classes, room);
+  p.split = p.wgs > 0;
+  if (!p.split)  // a workgroup for every unit there can be
+    p.wgs = (int)((a.hkv / p.classes) *
+                  (((int64_t)a.tokens * a.group + p.rows - 1) / p.rows + a.batch));
+  p.workspace_bytes =
+      p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) : 0;
+  return p;
+}
+
+template <int D, bool BF16>
+void launch_paged_combine(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream) {
+  const dim3 g((unsigned)grid, kCombineY);
+  if (rows == 16)
+    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1>), g, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 2>), g, dim3(kThreads), 0, stream, a);
+}
+
+int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int head_dim,
+                           void* workspace, hipStream_t stream) {
+  PagedArgs a = args;
+  a.classes = plan.classes;
+  a.wgs = plan.wgs;
+  a.split = plan.split ? 1 : 0;
+  const int64_t grid = (int64_t)plan.wgs * plan.classes;
+  if (plan.split) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
+  }
+  const bool fp8 = a.ks != nullptr;
+#define FA_PAGED(D)                                                                     \
+  if (fp8) {                                                                            \
+    if (a.bf16) launch_paged_attn<D, true, true>(a, plan.rows, grid, stream);           \
+    else launch_paged_attn<D, false, true>(a, plan.rows, grid, stream);                 \
+  } else {                                                                              \
+    if (a.bf16) launch_paged_attn<D, true, false>(a, plan.rows, grid, stream);          \
+    else launch_paged_attn<D, false, false>(a, plan.rows, grid, stream);                \
+  }                                                                                     \
+  if (plan.split) {                                                                     \
+    if (a.bf16) launch_paged_combine<D, true>(a, plan.rows, grid, stream);              \
+    else launch_paged_combine<D, false>(a, plan.rows, grid, stream);                    \
+  }
+  if (head_dim == 64) { FA_PAGED(64) } else { FA_PAGED(128) }
+#undef FA_PAGED
+  return 0;
+}
+
+}  // namespace fa

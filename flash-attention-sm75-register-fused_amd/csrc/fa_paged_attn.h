@@ -1,0 +1,481 @@
+// Attention of new tokens over a paged cache, for units of at most 32 query
+// columns: one generated token of every sequence, or a few drafted ones.
+//
+// A unit is one (sequence, KV head, block of 16 NT query columns); column c of
+// the block is row r = 16 NT rb + c of the sequence's n * group rows, row r being
+// token r / group of query head kv_head * group + r % group.  All of them read
+// the same K and V rows, which is the work: streaming those from HBM once.
+//
+//   S^T = K Q^T     keys on the M side of 16x16x32 MFMAs, columns on N
+//   O^T = V^T P^T   P stays in the registers S^T left it in (the key order
+//                   inside a 32-key step is a permutation shared by P and V)
+//
+// 16x16x32 and not 32x32x16, as the other decode kernel has it: a K operand
+// read is then 16 rows of 64 bytes, and 16 consecutive keys lie in one page
+// whatever the page size (16 or more), so each read goes through one buffer
+// window whose base is scalar; and up to 16 columns cost half the matrix time.
+//
+// The four waves of a workgroup take every fourth 32-key tile of its key range
+// and run independently; their (max, sum, O) meet in LDS at the end.
+//
+// Softmax: running maximum per column, raised when some score outgrew it by more
+// than 2^kRescaleLog2 (the sums and O share the stale maximum, so nothing else
+// changes); sums of the unrounded P in 32 bits; P rounded to the 16-bit type for
+// the second product, at most half a step of it each.
+//
+// The plan.  The units of one class of KV heads (every classes-th head, so that
+// the workgroups of one XCD share heads) are laid end to end as a line of 32-key
+// tiles, and each of the class's workgroups takes an equal stretch of the line,
+// whatever mixture of sequences it covers: a batch of very different lengths
+// keeps every CU busy to the end.  A unit cut by a stretch's border leaves
+// partials (O, max, sum) in the workspace, at most two for each workgroup, which a
+// second kernel merges.  Stretches follow from the lengths alone, and partials
+// are merged in order, so the same call gives the same bits.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_paged.h"
+
+namespace fa {
+namespace {
+
+constexpr int kPTile = 32;       // keys of a wave's tile
+constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below
+
+__device__ __forceinline__ int wave_bcast(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ int64_t wave_bcast(int64_t x, int lane) {
+  return (int64_t)(uint32_t)wave_bcast((int)x, lane) |
+         ((int64_t)wave_bcast((int)(x >> 32), lane) << 32);
+}
+
+// Units of a sequence for one KV head, and the 32-key tiles each of them is on
+// the line: at least one, so that a sequence without keys has its rows written.
+template <int R>
+__device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& s) {
+  return (int)(((int64_t)s.n * a.group + R - 1) / R);
+}
+__device__ __forceinline__ int paged_tiles(const PagedArgs& a, const PagedSeq& s) {
+  return a.split ? max(1, (s.keys + kPTile - 1) / kPTile) : 1;
+}
+
+// Walks a class's line: total length, and the sequence that holds a position.
+// Called by whole waves; every lane gets the same answers.
+template <int R>
+struct PagedLine {
+  const PagedArgs& a;
+  int lane;
+  int heads;  // KV heads of the class
+  __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln) : a(args), lane(ln) {
+    heads = args.hkv / args.classes;
+  }
+  __device__ __forceinline__ int64_t length_of(const PagedSeq& s) const {
+    return (int64_t)heads * paged_blocks<R>(a, s) * paged_tiles(a, s);
+  }
+  // Inclusive prefix sum over the wave's lanes of sequence b0 + lane's length.
+  __device__ __forceinline__ int64_t prefix(int b0) const {
+    int64_t x = 0;
+    if (b0 + lane < a.batch) x = length_of(paged_seq(a, b0 + lane, [](const int32_t* p) { return *p; }));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(x, d);
+      if (lane >= d) x += y;
+    }
+    return x;
+  }
+  __device__ __forceinline__ int64_t total() const {
+    int64_t sum = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
+    return sum;
+  }
+  // The sequence b that holds position pos (0 <= pos < total), and where it starts.
+  __device__ __forceinline__ int find(int64_t pos, int64_t& start) const {
+    int64_t before = 0;
+    for (int b0 = 0;; b0 += 64) {
+      const int64_t x = prefix(b0);
+      const int64_t end = wave_bcast(x, 63);
+      if (pos < before + end || b0 + 64 >= a.batch) {
+        const uint64_t past = __builtin_amdgcn_ballot_w64(before + x > pos);
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        start = l > 0 ? before + wave_bcast(x, l - 1) : before;
+        return min(b0 + l, a.batch - 1);
+      }
+      before += end;
+    }
+  }
+};
+
+// Workgroups that share a class's line: all of them, unless stretches would
+// fall below kPMinTiles.
+__device__ __forceinline__ int paged_active(const PagedArgs& a, int64_t total) {
+  if (!a.split) return (int)min((int64_t)a.wgs, total);
+  return (int)min((int64_t)a.wgs, (total + kPMinTiles - 1) / kPMinTiles);
+}
+
+// Row r of a sequence's rows: the addresses of its Q, O and LSE.
+struct PagedRow {
+  int token, head;
+};
+__device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, const PagedSeq& s, int hkv, int r) {
+  const int i = r / a.group;
+  return {s.t0 + i, hkv * a.group + (r - i * a.group)};
+}
+
+__device__ __forceinline__ float natural_lse(float m2, float l) {
+  return ((m2 == -__builtin_inff() ? 0.0f : m2) + __builtin_log2f(l)) * 0.69314718055994530942f;
+}
+
+template <int D, bool BF16, bool FP8, int NT>
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
+  using E = Elem<BF16>;
+  constexpr int R = 16 * NT;
+  constexpr int KS = D / 32;  // contraction steps of S^T
+  constexpr int MT = D / 16;  // 16-dimension tiles of O^T
+  constexpr int CH = D / 8;   // 16-byte chunks of a 16-bit row
+  // A wave's V tile: 32 rows of D halves, 32-byte piece p of row r at p ^ swz(r)
+  // (the transposing reads take 32 bytes of 8 consecutive rows at once: eight
+  // different pieces of the 256-byte sweep of the banks).
+  constexpr int VT = kPTile * D;
+  constexpr int OP = D + 4;  // floats of an O row in the merge (rows 4 banks apart)
+  constexpr int V_BYTES = 4 * VT * 2, O_BYTES = 4 * R * OP * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
+  __shared__ float ml_lds[4][2][R];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int l16 = lane & 15;
+  const int g4 = lane >> 4;
+  const int cls = (int)blockIdx.x % a.classes;
+  const int wg = (int)blockIdx.x / a.classes;
+
+  const PagedLine<R> line(a, lane);
+  const int64_t total = line.total();
+  const int active = paged_active(a, total);
+  if (wg >= active) return;
+  int64_t pos = a.split ? wg * total / active : wg;
+  const int64_t end = a.split ? (wg + 1) * total / active : wg + 1;
+  int64_t seq_start;
+  int b = line.find(pos, seq_start);
+
+  auto swz = [](int r) { return D == 128 ? (r & 7) : ((r >> 1) & 3); };
+  _Float16* const vt = (_Float16*)lds + wave * VT;
+  const float c2 = a.c;
+
+  while (pos < end) {
+    const PagedSeq s = paged_seq(a, b, load_scalar);
+    const int blocks = paged_blocks<R>(a, s);
+    const int line_tiles = paged_tiles(a, s);
+    const int64_t len = (int64_t)line.heads * blocks * line_tiles;
+    if (pos >= seq_start + len) {  // on to the next sequence
+      seq_start += len;
+      if (++b >= a.batch) return;
+      continue;
+    }
+    const int unit = (int)((pos - seq_start) / line_tiles);
+    const int first = (int)(pos - seq_start - (int64_t)unit * line_tiles);  // on the line
+    const int here = (int)min((int64_t)(line_tiles - first), end - pos);
+    const int hc = unit / blocks;
+    const int rb = unit - hc * blocks;
+    const int hkv = hc * a.classes + cls;
+    const bool whole = !a.split || (first == 0 && here == line_tiles);
+    const int t_begin = a.split ? first : 0;
+    const int t_end = a.split ? first + here : (s.keys + kPTile - 1) / kPTile;
+    pos += here;
+
+    // Columns of this lane, one for each nt, and the last key each sees.
+    const int nrows = s.n * a.group;
+    int last[NT];
+    half8 qf[NT][KS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = rb * R + 16 * nt + l16;
+      const bool ok = r < nrows;
+      const PagedRow pr = paged_row(a, s, hkv, ok ? r : 0);
+      last[nt] = a.causal ? min(s.keys - 1, s.len - s.n + (pr.token - s.t0)) : s.keys - 1;
+      const _Float16* qp = a.q + pr.token * a.qt + pr.head * a.qh;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        // Dimensions of step kk that lane group g4 contracts: 8 of a 16-bit
+        // row's 64 bytes; of an 8-bit row's 64 bytes 16, over two steps.
+        const int dim = FP8 ? 64 * (kk >> 1) + 16 * g4 + 8 * (kk & 1) : 32 * kk + 8 * g4;
+        qf[nt][kk] = ok ? *(const half8*)(qp + dim) : (half8)(_Float16)0;
+        if (a.negate_q) qf[nt][kk] = negate16(qf[nt][kk]);
+      }
+    }
+    // Keys no row of the block sees are not read.
+    const int last_row = min(nrows, (rb + 1) * R) - 1;
+    const int sees = a.causal ? clamp_int(s.len - s.n + last_row / a.group + 1, 0, s.keys) : s.keys;
+    const int t_stop = min(t_end, (sees + kPTile - 1) / kPTile);
+
+    float4v o[NT][MT];
+    float m_run[NT], l_run[NT], thr[NT], mc[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[nt][mt] = (float4v)0.0f;
+      m_run[nt] = thr[nt] = -__builtin_inff();
+      l_run[nt] = mc[nt] = 0.0f;
+    }
+
+    for (int t = t_begin + wave; t < t_stop; t += 4) {
+      // The two 16-key pieces of the tile: their pages, and how many rows are keys.
+      int rows[2], page[2], off[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int key = t * kPTile + 16 * p;
+        rows[p] = clamp_int(sees - key, 0, 16);
+        off[p] = key & ((1 << a.page_shift) - 1);
+        page[p] = -1;
+        if (rows[p] > 0)
+          page[p] = load_scalar(a.table + b * a.table_stride + (key >> a.page_shift));
+        if (page[p] < 0 || page[p] >= a.num_pages) {
+          page[p] = 0;
+          rows[p] = 0;
+        }
+      }
+      float4v st[2][NT];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const __amdgpu_buffer_rsrc_t rk = make_rsrc(
+            a.k + page[p] * a.kp + hkv * a.kh + off[p] * a.kn, rows[p] * (int)a.kn);
+        half8 kf[KS];
+        if constexpr (FP8) {
+          const __amdgpu_buffer_rsrc_t rs = make_rsrc(
+              a.ks + page[p] * a.ksp + hkv * a.ksh + off[p] * a.ksn, rows[p] * (int)a.ksn);
+          const float sc = scale_of(__builtin_amdgcn_raw_buffer_load_b8(rs, l16 * (int)a.ksn, 0, 0));
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) {
+            const uint4v w = __builtin_bit_cast(
+                uint4v, __builtin_amdgcn_raw_buffer_load_b128(rk, l16 * (int)a.kn + 64 * i + 16 * g4, 0, 0));
+            kf[2 * i] = dequantise8<BF16>(w[0], w[1], sc);
+            kf[2 * i + 1] = dequantise8<BF16>(w[2], w[3], sc);
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk)
+            kf[kk] = __builtin_bit_cast(
+                half8, __builtin_amdgcn_raw_buffer_load_b128(rk, l16 * (int)a.kn + 64 * kk + 16 * g4, 0, 0));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          st[p][nt] = (float4v)0.0f;
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) st[p][nt] = E::mfma16(kf[kk], qf[nt][kk], st[p][nt]);
+        }
+        // V rows of the piece into the wave's tile.
+        const __amdgpu_buffer_rsrc_t rv = make_rsrc(
+            a.v + page[p] * a.vp + hkv * a.vh + off[p] * a.vn, rows[p] * (int)a.vn);
+        if constexpr (FP8) {
+          constexpr int QC = D / 16;  // 16-byte quarters of an 8-bit row
+          const __amdgpu_buffer_rsrc_t rs = make_rsrc(
+              a.vs + page[p] * a.vsp + hkv * a.vsh + off[p] * a.vsn, rows[p] * (int)a.vsn);
+#pragma unroll
+          for (int i = 0; i < 16 * QC / 64; ++i) {
+            const int row = (64 * i + lane) / QC, q = (64 * i + lane) % QC;
+            const float sc = scale_of(__builtin_amdgcn_raw_buffer_load_b8(rs, row * (int)a.vsn, 0, 0));
+            const uint4v w = __builtin_bit_cast(
+                uint4v, __builtin_amdgcn_raw_buffer_load_b128(rv, row * (int)a.vn + 16 * q, 0, 0));
+            const int rr = 16 * p + row;
+            _Float16* const dst = vt + rr * D + 16 * (q ^ swz(rr));
+            *(half8*)dst = dequantise8<BF16>(w[0], w[1], sc);
+            *(half8*)(dst + 8) = dequantise8<BF16>(w[2], w[3], sc);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 * CH / 64; ++i) {
+            const int row = (64 * i + lane) / CH, ch = (64 * i + lane) % CH;
+            const int rr = 16 * p + row;
+            *(half8*)(vt + rr * D + 8 * (ch ^ (2 * swz(rr)))) = __builtin_bit_cast(
+                half8, __builtin_amdgcn_raw_buffer_load_b128(rv, row * (int)a.vn + 16 * ch, 0, 0));
+          }
+        }
+      }
+      // Lane group g4 holds keys 16 p + 4 g4 + i of column l16.
+      half8 pf[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = t * kPTile + 16 * p + 4 * g4 + i;
+            if (key > last[nt] || rows[p] == 0) st[p][nt][i] = -__builtin_inff();
+            mx = fmaxf(mx, st[p][nt][i]);
+          }
+        if (__builtin_amdgcn_ballot_w64(mx > thr[nt]) != 0) {
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float m_new = fmaxf(m_run[nt], mx);
+          const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
+          const float alpha = m_run[nt] == -__builtin_inff()
+                                  ? 0.0f
+                                  : __builtin_amdgcn_exp2f((m_run[nt] - m_use) * c2);
+          l_run[nt] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) o[nt][mt] *= alpha;
+          m_run[nt] = m_new;
+          mc[nt] = m_use * c2;
+          thr[nt] = m_new + kRescaleLog2 / c2;
+        }
+        uint4v pw;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[p][nt][i], c2, -mc[nt]));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[p][nt][i + 1], c2, -mc[nt]));
+            l_run[nt] += p0;
+            l_run[nt] += p1;
+            pw[2 * p + (i >> 1)] = __builtin_bit_cast(unsigned, E::pack(p0, p1));
+          }
+        pf[nt] = __builtin_bit_cast(half8, pw);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        // Lane i of a 16-lane group names 4 dimensions of row i / 4 of the
+        // group's four; it receives dimension i of all four.
+        const int r0 = 4 * g4 + (l16 >> 2), r1 = r0 + 16;
+        const half4 lo = ds_read_tr16(vt + r0 * D + 16 * (mt ^ swz(r0)) + 4 * (l16 & 3));
+        const half4 hi = ds_read_tr16(vt + r1 * D + 16 * (mt ^ swz(r1)) + 4 * (l16 & 3));
+        const half8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[nt][mt] = E::mfma16(vf, pf[nt], o[nt][mt]);
+      }
+    }
+
+    // ---- the four waves' shares meet in LDS ---------------------------------
+    __syncthreads();  // the V tiles are free
+    float* const ow = (float*)lds;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float l = l_run[nt];
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      float m = m_run[nt];
+      const int c = 16 * nt + l16;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        *(float4v*)(ow + (wave * R + c) * OP + 16 * mt + 4 * g4) = o[nt][mt];
+      if (g4 == 0) {
+        ml_lds[wave][0][c] = m;
+        ml_lds[wave][1][c] = l;
+      }
+    }
+    __syncthreads();
+    // Thread: 4 dimensions of one column, columns in turns.
+    for (int it = threadIdx.x; it < R * (D / 4); it += kThreads) {
+      const int c = it / (D / 4), dim = 4 * (it - c * (D / 4));
+      const int r = rb * R + c;
+      if (r >= nrows) continue;
+      float mw[4], m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        mw[w] = ml_lds[w][0][c];
+        m = fmaxf(m, mw[w]);
+      }
+      const float m_use = m == -__builtin_inff() ? 0.0f : m;
+      float4v x = (float4v)0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f((mw[w] - m_use) * c2);
+        l += f * ml_lds[w][1][c];
+        x += f * *(const float4v*)(ow + (w * R + c) * OP + dim);
+      }
+      if (whole) {
+        const PagedRow pr = paged_row(a, s, hkv, r);
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        half4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = E::round(x[e] * inv);
+        *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
+        if (a.lse != nullptr && dim == 0)
+          a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m == -__builtin_inff() ? m : m * c2, l);
+      } else {
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0);
+        *(float4v*)(a.part_o + (slot * R + c) * D + dim) = x;
+        if (dim == 0) {
+          a.part_ml[(slot * R + c) * 2] = m == -__builtin_inff() ? m : m * c2;
+          a.part_ml[(slot * R + c) * 2 + 1] = l;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Merges the partials of the units that stretches cut.  Workgroup wg of a class
+// looks at the border between its stretch and the one before: where it is the
+// first border inside a unit, the unit's partials are slot 1 of the
+// workgroup before it and slot 0 of those from wg on that start inside it.
+// A wave takes a row: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+constexpr int kCombineY = 4;
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedArgs a) {
+  constexpr int R = 16 * NT;
+  constexpr int DL = D / 64;  // dimensions of a lane
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int cls = (int)blockIdx.x % a.classes;
+  const int wg = (int)blockIdx.x / a.classes;
+  const PagedLine<R> line(a, lane);
+  const int64_t total = line.total();
+  const int active = paged_active(a, total);
+  if (wg == 0 || wg >= active) return;
+  const int64_t border = wg * total / active;
+  int64_t seq_start;
+  const int b = line.find(border, seq_start);
+  const PagedSeq s = paged_seq(a, b, load_scalar);
+  const int blocks = paged_blocks<R>(a, s);
+  const int tiles = paged_tiles(a, s);
+  const int unit = (int)((border - seq_start) / tiles);
+  const int64_t u0 = seq_start + (int64_t)unit * tiles, u1 = u0 + tiles;
+  if (border == u0 || (wg - 1) * total / active > u0) return;
+  int pieces = 2;  // those of workgroups wg - 1 and wg
+  while ((wg - 1 + pieces) * total / active < u1 && wg - 1 + pieces < active) ++pieces;
+  const int hc = unit / blocks;
+  const int rb = unit - hc * blocks;
+  const int hkv = hc * a.classes + cls;
+  const int nrows = s.n * a.group;
+  auto slot = [&](int i) -> int64_t {
+    return 2 * ((int64_t)(wg - 1 + i) * a.classes + cls) + (i == 0 ? 1 : 0);
+  };
+  for (int c = wave + 4 * (int)blockIdx.y; c < R && rb * R + c < nrows; c += 4 * kCombineY) {
+    float m = -__builtin_inff(), l = 0.0f, x[DL];
+#pragma unroll
+    for (int e = 0; e < DL; ++e) x[e] = 0.0f;
+    for (int i = 0; i < pieces; ++i) {
+      const int64_t p = slot(i) * R + c;
+      const float mi = a.part_ml[2 * p], li = a.part_ml[2 * p + 1];
+      const float m_new = fmaxf(m, mi);
+      const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
+      const float f0 = __builtin_amdgcn_exp2f(m - m_use), f1 = __builtin_amdgcn_exp2f(mi - m_use);
+      l = l * f0 + li * f1;
+#pragma unroll
+      for (int e = 0; e < DL; ++e) x[e] = x[e] * f0 + a.part_o[p * D + DL * lane + e] * f1;
+      m = m_new;
+    }
+    const PagedRow pr = paged_row(a, s, hkv, rb * R + c);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh + DL * lane;
+#pragma unroll
+    for (int e = 0; e < DL; ++e) op[e] = Elem<BF16>::round(x[e] * inv);
+    if (a.lse != nullptr && lane == 0)
+      a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
+  }
+}
+
+}  // namespace
+
+template <int D, bool BF16, bool FP8>
+void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream) {
+  if (rows == 16)
+    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 1>), dim3((unsigned)grid), dim3(kThreads), 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 2>), dim3((unsigned)grid), dim3(kThreads), 0,
+                       stream, a);
+}
+
+}  // namespace fa

@@ -1,0 +1,6 @@
+// Attention over a paged cache, head_dim 64, bfloat16, 16-bit rows (see fa_paged_attn.h).
+#include "fa_paged_attn.h"
+
+namespace fa {
+template void launch_paged_attn<64, true, false>(const PagedArgs&, int, int64_t, hipStream_t);
+}  // namespace fa

@@ -332,6 +332,103 @@ int64_t fa_sm75_backward_workspace_size(const fa_bwd_params* p);
 
 #define FA_SM75_ABI_VERSION 7
 
+/* ---- Paged key/value cache -------------------------------------------------
+ * A pool of pages that the sequences of a serving batch share: page p holds
+ * page_size consecutive positions of one sequence, for every KV head.  K and V
+ * rows are in the model's 16-bit type, or (k_scale and v_scale set) in 8 bits:
+ * OCP e4m3 codes and one e8m0 scale (2^(byte - 127)) for each row, a row standing for
+ * codes * scale.  No reference counterpart (the reference has no cache).
+ * Everything on the device, block_table, seq_lens and cu_seqlens included: a captured
+ * call reads what they hold at each replay.  What they hold is checked there: a
+ * block_table entry outside [0, num_pages) names no page (rows there are not
+ * written, read as zeros, and hidden from every query), a length past the
+ * table's end counts as far as the table goes, and cu_seqlens is held to [0, tokens] and
+ * to rising. */
+typedef struct fa_paged_cache {
+  void* k;             /* page p, KV head h, row r at k + p k_stride_p + h k_stride_h + r k_stride_n */
+  void* v;
+  uint8_t* k_scale;    /* 8-bit rows: each row's scale, else NULL (both) */
+  uint8_t* v_scale;
+  const int32_t* block_table; /* [batch, max_pages], rows block_table_stride apart: entry i is
+                                 the page of positions [i page_size, (i + 1) page_size) */
+  const int32_t* seq_lens;    /* [batch]: tokens of each sequence, new ones included */
+  int64_t batch;
+  int64_t heads_kv;
+  int64_t head_dim;    /* 64 or 128 */
+  int64_t num_pages;
+  int64_t page_size;   /* a power of two, 16 or more */
+  int64_t max_pages;
+  int64_t block_table_stride;
+  /* Strides in elements: of K and V multiples of 16 bytes, head_dim contiguous. */
+  int64_t k_stride_p, k_stride_h, k_stride_n;
+  int64_t v_stride_p, v_stride_h, v_stride_n;
+  int64_t ks_stride_p, ks_stride_h, ks_stride_n;
+  int64_t vs_stride_p, vs_stride_h, vs_stride_n;
+} fa_paged_cache;
+
+/* New tokens' K and V.  Rows [cu_seqlens[b], cu_seqlens[b + 1]) are sequence b's last
+ * tokens, at positions seq_lens[b] - n .. seq_lens[b] - 1 for n of them; rows behind
+ * cu_seqlens[batch] are not used. */
+typedef struct fa_paged_rows {
+  const fa_half* k;    /* [tokens, heads_kv, head_dim], strides in elements (multiples of 8) */
+  const fa_half* v;
+  int64_t tokens;
+  int64_t k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+  const int32_t* cu_seqlens; /* [batch + 1], or NULL: row b is sequence b's one new token */
+  int dtype;           /* an fa_dtype */
+  void* stream;        /* hipStream_t; NULL selects the default stream */
+} fa_paged_rows;
+
+/* Writes new rows into their pages; positions before 0 or in no page are
+ * dropped.  8-bit rows: the scale is the smallest power of two s, from 2^-126 to
+ * 2^7 (binary16) or 2^119 (bfloat16), with |x| <= 448 s for every finite value
+ * (larger ones are stored as 448 s), codes are x / s rounded to nearest even, and
+ * infinities and NaN are stored as NaN.  Sequences of one call that share a page
+ * must not write the same positions of it.  Asynchronous on rows->stream. */
+int fa_sm75_paged_write(const fa_paged_cache* cache, const fa_paged_rows* rows);
+
+/* Reads positions [0, max_len) of every sequence into k and v, contiguous
+ * [batch, heads_kv, max_len, head_dim] of type dtype (an fa_dtype; 16-bit rows are
+ * copied as they are): zeros past a sequence's end and where it has no page. */
+int fa_sm75_paged_read(const fa_paged_cache* cache, fa_half* k, fa_half* v, int64_t max_len,
+                       int dtype, void* stream);
+
+/* Attention of new tokens over the cache (which holds their own rows already):
+ * O = softmax(scale * Q K^T) V.  With FA_CAUSAL_BOTTOM_RIGHT new token i of
+ * sequence b's n sees keys 0 .. seq_lens[b] - n + i, with FA_CAUSAL_NONE all of
+ * seq_lens[b]; keys in no page are seen by none.  A row that sees no key gets O = 0 and
+ * LSE = -inf.  Rows of O and lse behind cu_seqlens[batch] are left as they are. */
+typedef struct fa_paged_params {
+  const fa_paged_cache* cache;
+  const fa_half* q;    /* [tokens, heads_q, head_dim] */
+  fa_half* o;          /* [tokens, heads_q, head_dim] output */
+  float* lse;          /* optional [heads_q, tokens] fp32 natural-log row LSE, or NULL */
+  int64_t tokens;
+  int64_t heads_q;     /* a multiple of cache->heads_kv */
+  int64_t q_stride_t, q_stride_h;  /* elements, multiples of 8 */
+  int64_t o_stride_t, o_stride_h;
+  const int32_t* cu_seqlens; /* as in fa_paged_rows */
+  int64_t max_query_len; /* the most new tokens of one sequence, or 0 (not known): picks the
+                            kernel, results do not depend on its being right */
+  float scale;
+  int causal;          /* FA_CAUSAL_NONE or FA_CAUSAL_BOTTOM_RIGHT */
+  int dtype;           /* an fa_dtype: of Q and O, and of the rows of a 16-bit cache */
+  void* stream;        /* hipStream_t; NULL selects the default stream */
+  void* workspace;     /* optional device scratch, 16-byte aligned, or NULL: partial results of
+                          units whose keys are split; contents on entry do not matter; calls
+                          that share one race */
+  int64_t workspace_bytes; /* fa_sm75_paged_workspace_size() for full parallelism; with less
+                          the call still runs, on fewer workgroups */
+} fa_paged_params;
+
+/* Asynchronous on p->stream; allocates nothing.  Returns FA_OK or an fa_status. */
+int fa_sm75_paged_forward(const fa_paged_params* p);
+
+/* Workspace bytes fa_sm75_paged_forward can use (0 for invalid parameters too).  They
+ * depend on the sizes and the current device only, not on what the tables hold. */
+int64_t fa_sm75_paged_workspace_size(const fa_paged_params* p);
+
 /* ---- Reference launcher signatures ------------------------------------ */
 
 /* reference src/bindings/pytorch_extension.cpp:8-11,

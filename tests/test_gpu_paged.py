@@ -1,0 +1,372 @@
+"""The paged cache on the GPU against plain 64-bit references: writing, reading back, and
+attention over it, at the sizes, tables and masks where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+import flash_attention_sm75 as fa
+import paged_ref as ref
+from paged_ref import Cache
+
+pytestmark = pytest.mark.gpu
+
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+def attend(c, device, hq, seed=1, causal=True, scale=None, strided=False, one=None, **kw):
+    """Runs the call on a cache and checks O and LSE; returns them."""
+    g = torch.Generator().manual_seed(seed)
+    t = sum(c.news)
+    q = torch.randn(t, hq, c.d, generator=g).to(c.dtype)
+    args, scales = c.args(device, strided)
+    one = all(n == 1 for n in c.news) if one is None else one
+    o, lse = fa.flash_attention_paged(q.to(device), *args, cu_seqlens=None if one else c.cu.to(device),
+                                      causal="bottom_right" if causal else False, scale=scale,
+                                      return_lse=True, **scales, **kw)
+    want, want_lse, tol, lse_tol = ref.attention(c, q, causal, scale)
+    ref.check(o, want, tol, "O")
+    ref.check(lse, want_lse, lse_tol, "LSE")
+    return o, lse
+
+
+# ---- attention ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_single_tokens(device, d, dtype, q8, page):
+    """One token of each sequence: lengths around tiles and pages, empty ones among them."""
+    c = Cache([1, 0, 15, 16, 17, 31, 32, 33, 64, 65, 127, 128, 129, 300, 1000], 2, d, page, dtype, q8)
+    attend(c, device, 8)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (7, 1), (14, 2), (12, 12), (32, 8), (15, 3), (40, 2), (16, 16)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_heads(device, hq, hkv, q8):
+    """Groups of 1 to 20 query heads, KV heads that divide the eight XCDs and do not."""
+    attend(Cache([77, 300, 5], hkv, 64, 16, BF16, q8), device, hq)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("news", [[4, 4, 4], [1, 9, 2], [0, 3, 0], [70, 5, 33], [130, 1, 257]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_chunks(device, d, q8, news, causal):
+    """Several new tokens a sequence, none in some; the chunk can be the whole sequence."""
+    lens = [max(n, x) for n, x in zip(news, [130, 200, 257])]
+    attend(Cache(lens, 2, d, 16, FP16, q8, news=news), device, 6, causal=causal)
+
+
+def test_more_new_tokens_than_keys(device):
+    """seq_lens below the new tokens' count: the first tokens see no key and get zeros, LSE -inf."""
+    c = Cache([3, 0, 40], 2, 64, 16, BF16, False, news=[5, 2, 41])
+    o, lse = attend(c, device, 4)
+    assert (o[:2] == 0).all() and (lse[:, :2] == -math.inf).all()
+    assert (o[5:7] == 0).all() and (o[7] == 0).all()
+
+
+@pytest.mark.parametrize("page", [16, 32, 128, 1024])
+@pytest.mark.parametrize("q8", [False, True])
+def test_long(device, page, q8):
+    """Keys split over many workgroups, one long sequence among short ones."""
+    attend(Cache([9000, 3, 2500, 64], 2, 128, page, BF16, q8), device, 8)
+
+
+def test_one_long_sequence_few_heads(device):
+    attend(Cache([20011], 1, 64, 16, FP16, True), device, 7)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_missing_pages(device, q8):
+    """Entries that name no page hide their keys: -1, past the pool, the type's limits."""
+    c = Cache([500, 100, 40, 33], 2, 64, 16, FP16, q8, news=[3, 1, 2, 1],
+              gone=[(0, i) for i in range(9)] + [(1, 6), (2, 0), (2, 1), (2, 2)])
+    bad = [c.k.shape[0], 2 ** 31 - 1, -2 ** 31, -7]
+    for i, x in zip((3, 4, 5, 6), bad):
+        c.table[0, i] = x
+    o, lse = attend(c, device, 4)
+    assert (o[4:6] == 0).all() and (lse[:, 4:6] == -math.inf).all()  # no page of sequence 2 is left
+
+
+def test_length_past_the_table(device):
+    """seq_lens larger than the table has room for: the keys past it are in no page."""
+    c = Cache([100, 90], 2, 64, 16, FP16, False, news=[2, 1], width=3)
+    attend(c, device, 4)
+    c.seq_lens[1] = 2 ** 31 - 1  # as far as the type goes: every key of the table is seen
+    c.lens[1] = 48
+    c.rows[1] = [x[:, :48] for x in c.rows[1]]
+    (args, kw), q = c.args(device), torch.randn(3, 4, 64).half()
+    o = fa.flash_attention_paged(q.to(device), *args, cu_seqlens=c.cu.to(device), **kw)
+    want, _, tol, _ = ref.attention(c, q)
+    ref.check(o[2:], want[2:], tol[2:], "O")
+
+
+def test_shared_pages(device):
+    """Sequences that share a prefix's pages."""
+    c = Cache([96, 96, 50], 2, 64, 16, BF16, True)
+    c.table[1, :4] = c.table[0, :4]
+    for x in range(2):
+        c.rows[1][x][:, :64] = c.rows[0][x][:, :64]
+    attend(c, device, 6)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_strided(device, q8):
+    """[pages, page, H, D] storage, Q a slice of a wider projection, O written in place."""
+    c = Cache([50, 129], 2, 64, 32, FP16, q8, news=[5, 20])
+    attend(c, device, 4, strided=True)
+    (args, kw), g = c.args(device, True), torch.Generator().manual_seed(3)
+    wide = torch.randn(25, 12, 64, generator=g).half().to(device)
+    out = torch.full((25, 6, 64), 5.0, dtype=FP16, device=device)
+    got = fa.flash_attention_paged(wide[:, 2:6], *args, cu_seqlens=c.cu.to(device), out=out[:, 1:5], **kw)
+    assert got.data_ptr() == out[:, 1:5].data_ptr()
+    want, _, tol, _ = ref.attention(c, wide[:, 2:6].cpu())
+    ref.check(out[:, 1:5], want, tol, "O")
+    assert (out[:, 0] == 5).all() and (out[:, 5] == 5).all()
+
+
+def test_rows_behind_the_last_sequence(device):
+    """Rows of Q past cu_seqlens[B] are padding: their O and LSE rows are left as they are."""
+    c = Cache([50, 30], 2, 64, 16, FP16, False, news=[3, 1])
+    (args, kw), q = c.args(device), torch.randn(9, 4, 64).half()
+    q[4:] = math.nan
+    out = torch.full((9, 4, 64), 7.0, dtype=FP16, device=device)
+    fa.flash_attention_paged(q.to(device), *args, cu_seqlens=c.cu.to(device), out=out, **kw)
+    want, _, tol, _ = ref.attention(c, q[:4])
+    ref.check(out[:4], want, tol, "O")
+    assert (out[4:] == 7).all()
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-9, 2.0])
+def test_scales(device, scale):
+    attend(Cache([200, 10], 2, 64, 16, BF16, False, news=[2, 1]), device, 4, scale=scale)
+
+
+@pytest.mark.parametrize("news", [[1, 1], [40, 3]])
+@pytest.mark.parametrize("q8", [False, True])
+def test_nonfinite_rows(device, news, q8):
+    """A query's NaN stays in its row; NaN in a key hidden from a query does not reach it."""
+    c = Cache([400, 90], 1, 64, 16, BF16, q8, news=news)
+    (args, kw), g = c.args(device), torch.Generator().manual_seed(3)
+    t = sum(news)
+    q = torch.randn(t, 4, 64, generator=g).bfloat16()
+    q[0, 1, 5] = math.nan
+    o, lse = fa.flash_attention_paged(q.to(device), *args, cu_seqlens=c.cu.to(device), return_lse=True, **kw)
+    want, want_lse, tol, lse_tol = ref.attention(c, q.nan_to_num(0.0))
+    assert o[0, 1].isnan().all() and lse[1, 0].isnan()
+    keep = torch.ones(t, 4, dtype=torch.bool)
+    keep[0, 1] = False
+    ref.check(o.cpu()[keep], want[keep], tol[keep], "O")
+    ref.check(lse.cpu().T[keep], want_lse.T[keep], lse_tol.T[keep], "LSE")
+
+
+def test_peaked(device):
+    """Scores that keep rising along the keys raise the running maximum again and again."""
+    c = Cache([600], 1, 64, 16, FP16, False, news=[3])
+    up = torch.linspace(-1, 1, 600)[None, :, None]
+    k = (c.rows[0][0] * 0.1 + 12 * up).half()
+    for i in range(38):
+        p = int(c.table[0, i])
+        part = k[:, 16 * i:16 * i + 16]
+        c.k[p, :, :part.shape[1]] = part
+    c.rows[0][0] = k.double()
+    attend(c, device, 4)
+
+
+def test_max_query_len_is_a_hint(device):
+    """Wrong values of it choose another kernel and nothing else."""
+    c = Cache([150, 200], 2, 64, 16, BF16, False, news=[60, 1])
+    for hint in (1, 5, 60, 61, 10 ** 9):
+        attend(c, device, 8, max_query_len=hint)
+
+
+def test_index_tensors_are_held_to_their_ranges(device):
+    """cu_seqlens that falls or passes the rows writes nothing outside them."""
+    c = Cache([50, 30], 2, 64, 16, FP16, False, news=[3, 1])
+    (args, kw), q = c.args(device), torch.randn(4, 4, 64).half().to(device)
+    for cu in ([0, 3, 100], [0, -5, 4], [2 ** 31 - 1, 0, 1], [-2 ** 31, 2, 2 ** 31 - 1], [4, 4, 4]):
+        room = torch.full((12, 4, 64), 7.0, dtype=FP16, device=device)
+        cu = torch.tensor(cu, dtype=torch.int32, device=device)
+        fa.flash_attention_paged(q, *args, cu_seqlens=cu, out=room[4:8], **kw)
+        assert (room[:4] == 7).all() and (room[8:] == 7).all()
+    lens = torch.tensor([-5, -2 ** 31], dtype=torch.int32, device=device)
+    o = fa.flash_attention_paged(q, *args[:3], lens, cu_seqlens=c.cu.to(device), **kw)
+    assert (o == 0).all()
+
+
+def test_nothing_to_do(device):
+    c = Cache([5], 2, 64, 16, FP16, False)
+    args, _ = c.args(device)
+    empty = torch.empty(0, 4, 64, dtype=FP16, device=device)
+    cu = torch.zeros(2, dtype=torch.int32, device=device)
+    assert fa.flash_attention_paged(empty, *args, cu_seqlens=cu).shape == (0, 4, 64)
+    none = (args[0], args[1], args[2][:0], args[3][:0])
+    assert fa.flash_attention_paged(empty, *none).shape == (0, 4, 64)
+    out = torch.full((2, 4, 64), 3.0, dtype=FP16, device=device)
+    fa.flash_attention_paged(torch.zeros_like(out), *none, cu_seqlens=cu[:1], out=out)
+    assert (out == 3).all()
+    pool = (args[0][:0], args[1][:0], args[2], args[3])  # a pool without pages
+    o, lse = fa.flash_attention_paged(torch.ones(1, 4, 64, dtype=FP16, device=device), *pool, return_lse=True)
+    assert (o == 0).all() and (lse == -math.inf).all()
+
+
+def test_same_bits_every_time(device):
+    c = Cache([3000, 17, 900], 2, 128, 16, BF16, True, news=[2, 1, 3])
+    first = attend(c, device, 8)
+    for _ in range(3):
+        again = attend(c, device, 8)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ---- writing and reading ---------------------------------------------------------
+
+
+def written(c, device, k, v, cu, strided=False):
+    """The pools after a write over a NaN pool, as CPU tensors."""
+    (kc, vc, table, lens), kw = c.args(device, strided)
+    fa.paged_cache_write(k.to(device), v.to(device), kc, vc, table, lens, cu_seqlens=cu, **kw)
+    return [x.cpu() for x in (kc, vc, *kw.values())]
+
+
+def same(a, b):
+    a, b = (x.view(torch.uint8) if x.dtype == torch.float8_e8m0fnu else x.float() for x in (a, b))
+    return torch.equal(a.nan_to_num(123.0), b.nan_to_num(123.0)) if a.is_floating_point() else torch.equal(a, b)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_write(device, d, q8, dtype, strided):
+    """New rows arrive where the table says, everything else stays."""
+    news = [3, 0, 40, 1, 5]
+    c = Cache([20, 9, 77, 1, 3], 3, d, 16, dtype, q8, news=news, gone=[(2, 3)])
+    g = torch.Generator().manual_seed(9)
+    k, v = ((torch.randn(sum(news) + 2, 3, d, generator=g) * 3).to(dtype) for _ in "kv")
+    want = [x.clone() for x in (c.k, c.v, *((c.ks, c.vs) if q8 else ()))]
+    for b, n in enumerate(news):
+        for i in range(n):
+            pos, row = c.lens[b] - n + i, int(c.cu[b]) + i
+            if pos < 0 or c.table[b, pos // 16] < 0:
+                continue
+            p, r = int(c.table[b, pos // 16]), pos % 16
+            for x, new in enumerate((k, v)):
+                if q8:
+                    codes, scale = ref.quantise(new[row])
+                    want[x][p, :, r] = codes
+                    want[2 + x].view(torch.uint8)[p, :, r] = scale.view(torch.uint8)
+                else:
+                    want[x][p, :, r] = new[row]
+    for got, w in zip(written(c, device, k, v, c.cu.to(device), strided), want):
+        assert same(got, w)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_write_extremes(device, dtype):
+    """Rows of zeros, infinities, NaN, the type's limits, and every border of the scale."""
+    top, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    rows = [[0.0], [math.inf, 1.0], [math.nan, 3.0], [math.inf], [-math.inf, math.nan, top], [top], [-top],
+            [tiny], [tiny, -3 * tiny], [448.0], [449.0], [448.0 * 2, 1], [450.0 * 2], [0.4375], [0.438],
+            [57344.0, 65280.0 if dtype == FP16 else 3e38], [1.0, 2.0 ** -9, 2.0 ** -10, 2.0 ** -11, 3 * 2.0 ** -11],
+            [17.0, 18.0, 19.0, 21.0, 27.0, 29.0, 256.0]]
+    x = torch.zeros(len(rows), 1, 64)
+    for i, r in enumerate(rows):
+        x[i, 0, :len(r)] = torch.tensor(r, dtype=torch.float64).float()
+    x = x.to(dtype)
+    c = Cache([len(rows)], 1, 64, 32, dtype, True, news=[len(rows)])
+    k, v, ks, vs = written(c, device, x, -x, c.cu.to(device))
+    codes, scale = ref.quantise(x[:, 0])
+    p = int(c.table[0, 0])
+    assert same(k[p, 0, :len(rows)], codes) and same(ks[p, 0, :len(rows)], scale)
+    assert same(vs[p, 0, :len(rows)], scale)
+    # and back: exact 16-bit numbers
+    dev = [t.to(device) for t in (k, v, c.table, c.seq_lens)]
+    kr, _ = fa.paged_cache_read(*dev, max_len=len(rows), k_scale=ks.to(device), v_scale=vs.to(device), dtype=dtype)
+    want = codes.double() * scale.double()[:, None]
+    assert torch.equal(kr[0, 0].double().cpu().nan_to_num(9.9), want.nan_to_num(9.9))
+
+
+def test_write_single_tokens(device):
+    """Without cu_seqlens row b is sequence b's token; K and V as views of one projection."""
+    c = Cache([1, 16, 17, 0, 33], 2, 64, 16, BF16, False)
+    qkv = torch.randn(5, 3, 2, 64).bfloat16()
+    before = c.k.clone()
+    k, v = written(c, device, qkv[:, 1], qkv[:, 2], None)
+    for b, n in enumerate(c.lens):
+        if n:
+            p, r = int(c.table[b, (n - 1) // 16]), (n - 1) % 16
+            before[p, :, r] = qkv[b, 1]
+            assert torch.equal(v[p, :, r], qkv[b, 2])
+    assert same(k, before)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("q8,dtype", [(False, FP16), (False, BF16), (True, FP16), (True, BF16)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_read(device, d, q8, dtype, strided):
+    c = Cache([20, 0, 77, 1, 129], 3, d, 32, dtype, q8, gone=[(2, 0), (4, 2)])
+    args, kw = c.args(device, strided)
+    for max_len in (None, 1, 80, 200):
+        k, v = fa.paged_cache_read(*args, max_len=max_len, dtype=dtype if q8 else None, **kw)
+        longest = c.width * 32 if max_len is None else max_len
+        assert k.shape == (5, 3, longest, d) and k.dtype == dtype
+        for b, n in enumerate(c.lens):
+            held = c.held(b)
+            for got, rows in ((k, c.rows[b][0]), (v, c.rows[b][1])):
+                want = torch.zeros(3, longest, d, dtype=torch.float64)
+                m = min(n, longest)
+                want[:, :m] = torch.where(held[:m, None], rows[:, :m], 0.0)
+                assert torch.equal(got[b].double().cpu(), want)
+
+
+def test_read_nothing(device):
+    c = Cache([5, 3], 2, 64, 16, FP16, False)
+    args, _ = c.args(device)
+    assert fa.paged_cache_read(*args, max_len=0)[0].shape == (2, 2, 0, 64)
+    k, v = fa.paged_cache_read(args[0][:0], args[1][:0], *args[2:], max_len=20)
+    assert k.shape == (2, 2, 20, 64) and (k == 0).all() and (v == 0).all()
+
+
+# ---- together ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_a_batch_grows(device, q8):
+    """A serving loop: prompts in chunks, then single tokens; what is read back gives the other
+    kernels the same attention."""
+    d, hq, hkv, page, dtype = 64, 6, 2, 16, BF16
+    g = torch.Generator().manual_seed(5)
+    total = [75, 40]
+    c = Cache(total, hkv, d, page, dtype, q8, seed=11)  # its tables; the rows come from the writes
+    (kc, vc, table, _), kw = c.args(device)
+    new = [torch.randn(2, n, hkv, d, generator=g).to(dtype) for n in total]
+    done = [0, 0]
+    for step in ([30, 17], [33, 20], [1, 1], [1, 1], [10, 0], [0, 1]):
+        k, v = (torch.cat([new[b][x, done[b]:done[b] + n] for b, n in enumerate(step)]) for x in range(2))
+        done = [a + n for a, n in zip(done, step)]
+        lens = torch.tensor(done, dtype=torch.int32, device=device)
+        cu = torch.tensor([0, step[0], sum(step)], dtype=torch.int32, device=device)
+        fa.paged_cache_write(k.to(device), v.to(device), kc, vc, table, lens, cu_seqlens=cu, **kw)
+        q = torch.randn(sum(step), hq, d, generator=g).to(dtype)
+        o = fa.flash_attention_paged(q.to(device), kc, vc, table, lens, cu_seqlens=cu, **kw)
+        kr, vr = fa.paged_cache_read(kc, vc, table, lens, dtype=dtype, **kw)
+        for b, n in enumerate(step):
+            if n == 0:
+                continue
+            rows = [ref._through8(x[:done[b]]) if q8 else x[:done[b]].double() for x in new[b]]
+            c.rows[b] = [x.transpose(0, 1) for x in rows]
+            for got, want in ((kr, rows[0]), (vr, rows[1])):
+                assert torch.equal(got[b, :, :done[b]].double().cpu(), want.transpose(0, 1))
+                assert (got[b, :, done[b]:] == 0).all()
+            part = slice(int(cu[b]), int(cu[b]) + n)
+            dense = fa.flash_attention_forward_ex(q[part].to(device).transpose(0, 1)[None],
+                                                  kr[b:b + 1, :, :done[b]], vr[b:b + 1, :, :done[b]],
+                                                  causal="bottom_right")
+            one = Cache([done[b]], hkv, d, page, dtype, False, news=[n])
+            one.rows = [c.rows[b]]
+            want, _, tol, _ = ref.attention(one, q[part])
+            ref.check(o[part], want, tol, f"O of sequence {b}")
+            ref.check(dense[0].transpose(0, 1), want, 2 * tol, f"dense O of sequence {b}")
