@@ -28,7 +28,8 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   PagedPlan p;
   p.rows = max_query_len * a.group <= 16 ? 16 : 32;
   p.classes = std::gcd(a.hkv, kNumXcds);
-  const int64_t resident = resident_fused_workgroups();
+  const int64_t resident =  // (resident_fused_workgroups: two a CU)
+      resident_fused_workgroups() / 2 * paged_per_cu(head_dim, a.ks != nullptr, p.rows / 16);
   const int64_t room = workspace_bytes / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
   p.split = p.wgs > 0;

@@ -61,14 +61,17 @@ __device__ __forceinline__ int paged_tiles(const PagedArgs& a, const PagedSeq& s
 }
 
 // Walks a class's line: total length, and the sequence that holds a position.
-// Called by whole waves; every lane gets the same answers.
+// Called by whole waves; every lane gets the same answers.  The first 64
+// sequences are looked at once.
 template <int R>
 struct PagedLine {
   const PagedArgs& a;
   int lane;
   int heads;  // KV heads of the class
+  int64_t first;  // prefix(0)
   __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln) : a(args), lane(ln) {
     heads = args.hkv / args.classes;
+    first = prefix(0);
   }
   __device__ __forceinline__ int64_t length_of(const PagedSeq& s) const {
     return (int64_t)heads * paged_blocks<R>(a, s) * paged_tiles(a, s);
@@ -77,23 +80,28 @@ struct PagedLine {
   __device__ __forceinline__ int64_t prefix(int b0) const {
     int64_t x = 0;
     if (b0 + lane < a.batch) x = length_of(paged_seq(a, b0 + lane, [](const int32_t* p) { return *p; }));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
+    const int n = min(64, a.batch - b0);
+    for (int d = 1; d < n; d <<= 1) {
       const int64_t y = __shfl_up(x, d);
       if (lane >= d) x += y;
     }
-    return x;
+    return wave_bcast_last(x, n);
+  }
+  // (lanes past the last sequence hold the sum too)
+  __device__ __forceinline__ int64_t wave_bcast_last(int64_t x, int n) const {
+    const int64_t all = wave_bcast(x, n - 1);
+    return lane < n ? x : all;
   }
   __device__ __forceinline__ int64_t total() const {
-    int64_t sum = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
+    int64_t sum = wave_bcast(first, 63);
+    for (int b0 = 64; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
     return sum;
   }
   // The sequence b that holds position pos (0 <= pos < total), and where it starts.
   __device__ __forceinline__ int find(int64_t pos, int64_t& start) const {
     int64_t before = 0;
     for (int b0 = 0;; b0 += 64) {
-      const int64_t x = prefix(b0);
+      const int64_t x = b0 == 0 ? first : prefix(b0);
       const int64_t end = wave_bcast(x, 63);
       if (pos < before + end || b0 + 64 >= a.batch) {
         const uint64_t past = __builtin_amdgcn_ballot_w64(before + x > pos);
@@ -113,6 +121,12 @@ __device__ __forceinline__ int paged_active(const PagedArgs& a, int64_t total) {
   return (int)min((int64_t)a.wgs, (total + kPMinTiles - 1) / kPMinTiles);
 }
 
+// Workgroups of a CU at once: what their V tiles leave room for in 160 KB of LDS,
+// and their registers among 512 of a lane.
+__host__ __device__ constexpr int paged_per_cu(int d, bool fp8, int nt) {
+  return fp8 && nt == 1 ? (d == 64 ? 4 : 3) : d == 64 ? 3 : 2;
+}
+
 // Row r of a sequence's rows: the addresses of its Q, O and LSE.
 struct PagedRow {
   int token, head;
@@ -126,20 +140,34 @@ __device__ __forceinline__ float natural_lse(float m2, float l) {
   return ((m2 == -__builtin_inff() ? 0.0f : m2) + __builtin_log2f(l)) * 0.69314718055994530942f;
 }
 
+// Waits until at most N of the wave's vector loads are in flight (they land in
+// order), and keeps the LDS reads that depend on it behind the wait.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
+}
+
 template <int D, bool BF16, bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_attn_kernel(const PagedArgs a) {
   using E = Elem<BF16>;
   constexpr int R = 16 * NT;
   constexpr int KS = D / 32;  // contraction steps of S^T
   constexpr int MT = D / 16;  // 16-dimension tiles of O^T
-  constexpr int CH = D / 8;   // 16-byte chunks of a 16-bit row
+  constexpr int KL = FP8 ? KS / 2 : KS;         // K loads of a 16-key piece
+  constexpr int RL = FP8 ? D / 16 : D / 8;      // lanes that hold a V row, 16 bytes each
+  constexpr int VL = 16 * RL / 64;              // V loads of a piece
   // A wave's V tile: 32 rows of D halves, 32-byte piece p of row r at p ^ swz(r)
   // (the transposing reads take 32 bytes of 8 consecutive rows at once: eight
-  // different pieces of the 256-byte sweep of the banks).
+  // different pieces of the 256-byte sweep of the banks).  Two arrays, so that
+  // the compiler sees that loads in flight into one do not touch the other;
+  // an 8-bit cache's rows pass through registers and need one.
   constexpr int VT = kPTile * D;
-  constexpr int OP = D + 4;  // floats of an O row in the merge (rows 4 banks apart)
-  constexpr int V_BYTES = 4 * VT * 2, O_BYTES = 4 * R * OP * 4;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
+  constexpr bool TWO = !FP8 || NT == 2;
+  __shared__ __attribute__((aligned(1024))) _Float16 v_lds0[4 * VT];
+  __shared__ __attribute__((aligned(1024))) _Float16 v_lds1[TWO ? 4 * VT : 1];
+  static_assert(16 * D * 4 <= VT * 2, "a wave's O of 16 columns fits its V tile");
   __shared__ float ml_lds[4][2][R];
 
   const int lane = threadIdx.x & 63;
@@ -159,8 +187,24 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
   int b = line.find(pos, seq_start);
 
   auto swz = [](int r) { return D == 128 ? (r & 7) : ((r >> 1) & 3); };
-  _Float16* const vt = (_Float16*)lds + wave * VT;
+  _Float16* const vt0 = v_lds0 + wave * VT;
+  _Float16* const vt1 = v_lds1 + (TWO ? wave * VT : 0);
   const float c2 = a.c;
+
+  // Offsets inside a 16-key piece of what this lane loads: row l16 of K, 16 bytes
+  // at 16 g4 of each 64; VL times 64 / RL rows of V, RL lanes a row, in the
+  // order of the tile (16-bit rows go to LDS directly, lane l's 16 bytes at
+  // 16 l of each KB).
+  const int k_off = l16 * (int)a.kn + 16 * g4;
+  int v_off[VL];
+#pragma unroll
+  for (int i = 0; i < VL; ++i) {
+    const int row = (64 * i + lane) / RL, ch = (64 * i + lane) % RL;
+    v_off[i] = row * (int)a.vn + 16 * (FP8 ? ch : ch ^ (2 * swz(row)));
+  }
+  // Bases of the transposing reads: lane i of a 16-lane group names 4 dimensions
+  // of row i / 4 of the group's four; it receives dimension i of all four.
+  const int r0 = 4 * g4 + (l16 >> 2);
 
   while (pos < end) {
     const PagedSeq s = paged_seq(a, b, load_scalar);
@@ -203,9 +247,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
         if (a.negate_q) qf[nt][kk] = negate16(qf[nt][kk]);
       }
     }
-    // Keys no row of the block sees are not read.
+    // Keys no row of the block sees are not read (past `sees`); tiles up to `full`
+    // hide nothing from any of them.
     const int last_row = min(nrows, (rb + 1) * R) - 1;
     const int sees = a.causal ? clamp_int(s.len - s.n + last_row / a.group + 1, 0, s.keys) : s.keys;
+    const int full = a.causal ? clamp_int(s.len - s.n + rb * R / a.group + 1, 0, s.keys) : s.keys;
     const int t_stop = min(t_end, (sees + kPTile - 1) / kPTile);
 
     float4v o[NT][MT];
@@ -218,80 +264,73 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       l_run[nt] = mc[nt] = 0.0f;
     }
 
-    for (int t = t_begin + wave; t < t_stop; t += 4) {
-      // The two 16-key pieces of the tile: their pages, and how many rows are keys.
-      int rows[2], page[2], off[2];
+    // A tile in flight: which of its two pieces hold keys, and the registers that
+    // its loads fill.
+    struct Tile {
+      int rows[2];
+      uint4v k[2][KL];
+      uint4v v[FP8 ? 2 : 1][FP8 ? VL : 1];
+      unsigned ks[2], vs[2][FP8 ? VL : 1];
+    };
+    const int32_t* const entries = a.table + b * a.table_stride;
+    const uint8_t* const kh = a.k + hkv * a.kh;
+    const uint8_t* const vh = a.v + hkv * a.vh;
+    // Table entries of a tile's pieces (of the last page, past the table).
+    auto look_up = [&](int t, int (&e)[2]) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        e[p] = load_scalar(entries + min((t * kPTile + 16 * p) >> a.page_shift, a.max_pages - 1));
+    };
+    // Issues a tile's loads.  A piece in no page or past the keys reads through an
+    // empty window: zeros, and no traffic.
+    auto load = [&](int t, const int (&e)[2], Tile& x, _Float16* vt) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const int key = t * kPTile + 16 * p;
-        rows[p] = clamp_int(sees - key, 0, 16);
-        off[p] = key & ((1 << a.page_shift) - 1);
-        page[p] = -1;
-        if (rows[p] > 0)
-          page[p] = load_scalar(a.table + b * a.table_stride + (key >> a.page_shift));
-        if (page[p] < 0 || page[p] >= a.num_pages) {
-          page[p] = 0;
-          rows[p] = 0;
-        }
-      }
-      float4v st[2][NT];
+        const bool paged = e[p] >= 0 && e[p] < a.num_pages;
+        x.rows[p] = paged && t < t_stop ? clamp_int(sees - key, 0, 16) : 0;
+        const int64_t page = paged ? e[p] : 0;
+        const int off = key & ((1 << a.page_shift) - 1);
+        const __amdgpu_buffer_rsrc_t rk = make_rsrc(kh + page * a.kp + off * a.kn, x.rows[p] * (int)a.kn);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const __amdgpu_buffer_rsrc_t rk = make_rsrc(
-            a.k + page[p] * a.kp + hkv * a.kh + off[p] * a.kn, rows[p] * (int)a.kn);
-        half8 kf[KS];
+        for (int i = 0; i < KL; ++i)
+          x.k[p][i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 64 * i, 0, 0));
         if constexpr (FP8) {
-          const __amdgpu_buffer_rsrc_t rs = make_rsrc(
-              a.ks + page[p] * a.ksp + hkv * a.ksh + off[p] * a.ksn, rows[p] * (int)a.ksn);
-          const float sc = scale_of(__builtin_amdgcn_raw_buffer_load_b8(rs, l16 * (int)a.ksn, 0, 0));
+          const __amdgpu_buffer_rsrc_t rs =
+              make_rsrc(a.ks + page * a.ksp + hkv * a.ksh + off * a.ksn, x.rows[p] * (int)a.ksn);
+          x.ks[p] = __builtin_amdgcn_raw_buffer_load_b8(rs, l16 * (int)a.ksn, 0, 0);
+        }
+        const __amdgpu_buffer_rsrc_t rv = make_rsrc(vh + page * a.vp + off * a.vn, x.rows[p] * (int)a.vn);
+        if constexpr (FP8) {
+          const __amdgpu_buffer_rsrc_t rs =
+              make_rsrc(a.vs + page * a.vsp + hkv * a.vsh + off * a.vsn, x.rows[p] * (int)a.vsn);
 #pragma unroll
-          for (int i = 0; i < KS / 2; ++i) {
-            const uint4v w = __builtin_bit_cast(
-                uint4v, __builtin_amdgcn_raw_buffer_load_b128(rk, l16 * (int)a.kn + 64 * i + 16 * g4, 0, 0));
-            kf[2 * i] = dequantise8<BF16>(w[0], w[1], sc);
-            kf[2 * i + 1] = dequantise8<BF16>(w[2], w[3], sc);
+          for (int i = 0; i < VL; ++i) {
+            x.v[p][i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off[i], 0, 0));
+            x.vs[p][i] =
+                __builtin_amdgcn_raw_buffer_load_b8(rs, (64 * i + lane) / RL * (int)a.vsn, 0, 0);
           }
         } else {
 #pragma unroll
-          for (int kk = 0; kk < KS; ++kk)
-            kf[kk] = __builtin_bit_cast(
-                half8, __builtin_amdgcn_raw_buffer_load_b128(rk, l16 * (int)a.kn + 64 * kk + 16 * g4, 0, 0));
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          st[p][nt] = (float4v)0.0f;
-#pragma unroll
-          for (int kk = 0; kk < KS; ++kk) st[p][nt] = E::mfma16(kf[kk], qf[nt][kk], st[p][nt]);
-        }
-        // V rows of the piece into the wave's tile.
-        const __amdgpu_buffer_rsrc_t rv = make_rsrc(
-            a.v + page[p] * a.vp + hkv * a.vh + off[p] * a.vn, rows[p] * (int)a.vn);
-        if constexpr (FP8) {
-          constexpr int QC = D / 16;  // 16-byte quarters of an 8-bit row
-          const __amdgpu_buffer_rsrc_t rs = make_rsrc(
-              a.vs + page[p] * a.vsp + hkv * a.vsh + off[p] * a.vsn, rows[p] * (int)a.vsn);
-#pragma unroll
-          for (int i = 0; i < 16 * QC / 64; ++i) {
-            const int row = (64 * i + lane) / QC, q = (64 * i + lane) % QC;
-            const float sc = scale_of(__builtin_amdgcn_raw_buffer_load_b8(rs, row * (int)a.vsn, 0, 0));
-            const uint4v w = __builtin_bit_cast(
-                uint4v, __builtin_amdgcn_raw_buffer_load_b128(rv, row * (int)a.vn + 16 * q, 0, 0));
-            const int rr = 16 * p + row;
-            _Float16* const dst = vt + rr * D + 16 * (q ^ swz(rr));
-            *(half8*)dst = dequantise8<BF16>(w[0], w[1], sc);
-            *(half8*)(dst + 8) = dequantise8<BF16>(w[2], w[3], sc);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16 * CH / 64; ++i) {
-            const int row = (64 * i + lane) / CH, ch = (64 * i + lane) % CH;
-            const int rr = 16 * p + row;
-            *(half8*)(vt + rr * D + 8 * (ch ^ (2 * swz(rr)))) = __builtin_bit_cast(
-                half8, __builtin_amdgcn_raw_buffer_load_b128(rv, row * (int)a.vn + 16 * ch, 0, 0));
-          }
+          for (int i = 0; i < VL; ++i)
+            direct_load16_nt(rv, (lds_void*)(vt + (16 * p * RL + 64 * i) * 8), v_off[i]);
         }
       }
+    };
+
+    // Scores to probabilities of one tile, then P V.
+    auto compute = [&](int t, const int (&rows)[2], float4v (&st)[2][NT], const _Float16* vt, auto wait) {
       // Lane group g4 holds keys 16 p + 4 g4 + i of column l16.
+      if ((t + 1) * kPTile > full || rows[0] == 0 || rows[1] == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (t * kPTile + 16 * p + 4 * g4 + i > last[nt] || rows[p] == 0)
+                st[p][nt][i] = -__builtin_inff();
+      }
       half8 pf[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -299,11 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = t * kPTile + 16 * p + 4 * g4 + i;
-            if (key > last[nt] || rows[p] == 0) st[p][nt][i] = -__builtin_inff();
-            mx = fmaxf(mx, st[p][nt][i]);
-          }
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[p][nt][i]);
         if (__builtin_amdgcn_ballot_w64(mx > thr[nt]) != 0) {
           mx = fmaxf(mx, __shfl_xor(mx, 16));
           mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -332,41 +367,109 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
           }
         pf[nt] = __builtin_bit_cast(half8, pw);
       }
+      wait();
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        // Lane i of a 16-lane group names 4 dimensions of row i / 4 of the
-        // group's four; it receives dimension i of all four.
-        const int r0 = 4 * g4 + (l16 >> 2), r1 = r0 + 16;
         const half4 lo = ds_read_tr16(vt + r0 * D + 16 * (mt ^ swz(r0)) + 4 * (l16 & 3));
-        const half4 hi = ds_read_tr16(vt + r1 * D + 16 * (mt ^ swz(r1)) + 4 * (l16 & 3));
+        const half4 hi = ds_read_tr16(vt + (r0 + 16) * D + 16 * (mt ^ swz(r0)) + 4 * (l16 & 3));
         const half8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) o[nt][mt] = E::mfma16(vf, pf[nt], o[nt][mt]);
       }
+    };
+
+    int t = t_begin + wave;
+    if (t < t_stop) {
+      int e[2];
+      look_up(t, e);
+      if constexpr (FP8) {
+        // The tile's codes are converted, K's in registers and V's into LDS, and the
+        // next tile's loads go into the registers they leave.
+        Tile x;
+        load(t, e, x, nullptr);
+        look_up(t + 4, e);
+        for (; t < t_stop; t += 4) {
+          float4v st[2][NT];
+          const int rows[2] = {x.rows[0], x.rows[1]};
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+              const int row = 16 * p + (64 * i + lane) / RL, q = (64 * i + lane) % RL;
+              const float vs = scale_of(x.vs[p][i]);
+              _Float16* const dst = vt0 + row * D + 16 * (q ^ swz(row));
+              *(half8*)dst = dequantise8<BF16>(x.v[p][i][0], x.v[p][i][1], vs);
+              *(half8*)(dst + 8) = dequantise8<BF16>(x.v[p][i][2], x.v[p][i][3], vs);
+            }
+            const float ks = scale_of(x.ks[p]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) st[p][nt] = (float4v)0.0f;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+              const uint4v w = x.k[p][kk / 2];
+              const half8 kf = kk & 1 ? dequantise8<BF16>(w[2], w[3], ks) : dequantise8<BF16>(w[0], w[1], ks);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) st[p][nt] = E::mfma16(kf, qf[nt][kk], st[p][nt]);
+            }
+          }
+          load(t + 4, e, x, nullptr);
+          look_up(t + 8, e);
+          compute(t, rows, st, vt0, [] {});
+        }
+      } else {
+        Tile xa, xb;
+        load(t, e, xa, vt0);
+        look_up(t + 4, e);
+        auto step = [&](int tt, Tile& cur, Tile& nxt, const _Float16* vc, _Float16* vn) {
+          load(tt + 4, e, nxt, vn);
+          look_up(tt + 8, e);
+          float4v st[2][NT];
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              st[p][nt] = (float4v)0.0f;
+#pragma unroll
+              for (int kk = 0; kk < KS; ++kk)
+                st[p][nt] = E::mfma16(__builtin_bit_cast(half8, cur.k[p][kk]), qf[nt][kk], st[p][nt]);
+            }
+          // V of this tile has landed once only the next tile's loads are in flight.
+          compute(tt, cur.rows, st, vc, [] { wait_loads<2 * (KL + VL)>(); });
+        };
+        for (; t + 4 < t_stop; t += 8) {
+          step(t, xa, xb, vt0, vt1);
+          step(t + 4, xb, xa, vt1, vt0);
+        }
+        if (t < t_stop) step(t, xa, xb, vt0, vt1);
+      }
     }
 
     // ---- the four waves' shares meet in LDS ---------------------------------
-    __syncthreads();  // the V tiles are free
-    float* const ow = (float*)lds;
+    // No direct load is in flight into a V tile any more, and no wave reads one.
+    if constexpr (!FP8) wait_loads<0>();
+    __syncthreads();
+    // O of column c (16 of them to an array), 16-byte chunk d at d ^ c.
+    auto o_at = [&](int w, int c, int chunk) -> float4v* {
+      float* const base = (float*)(c < 16 || !TWO ? v_lds0 : v_lds1) + w * 16 * D;
+      return (float4v*)(base + (c & 15) * D + 4 * (chunk ^ (c & 15)));
+    };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float l = l_run[nt];
       l += __shfl_xor(l, 16);
       l += __shfl_xor(l, 32);
-      float m = m_run[nt];
       const int c = 16 * nt + l16;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        *(float4v*)(ow + (wave * R + c) * OP + 16 * mt + 4 * g4) = o[nt][mt];
+      for (int mt = 0; mt < MT; ++mt) *o_at(wave, c, 4 * mt + g4) = o[nt][mt];
       if (g4 == 0) {
-        ml_lds[wave][0][c] = m;
+        ml_lds[wave][0][c] = m_run[nt];
         ml_lds[wave][1][c] = l;
       }
     }
     __syncthreads();
     // Thread: 4 dimensions of one column, columns in turns.
     for (int it = threadIdx.x; it < R * (D / 4); it += kThreads) {
-      const int c = it / (D / 4), dim = 4 * (it - c * (D / 4));
+      const int c = it / (D / 4), ch = it - c * (D / 4), dim = 4 * ch;
       const int r = rb * R + c;
       if (r >= nrows) continue;
       float mw[4], m = -__builtin_inff(), l = 0.0f;
@@ -381,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       for (int w = 0; w < 4; ++w) {
         const float f = __builtin_amdgcn_exp2f((mw[w] - m_use) * c2);
         l += f * ml_lds[w][1][c];
-        x += f * *(const float4v*)(ow + (w * R + c) * OP + dim);
+        x += f * *o_at(w, c, ch);
       }
       if (whole) {
         const PagedRow pr = paged_row(a, s, hkv, r);
