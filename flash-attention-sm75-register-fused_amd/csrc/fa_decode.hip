@@ -1026,6 +1026,15 @@ int plan_splits(const DecodePlan& pl, int head_dim, int64_t most) {
 
 }  // namespace
 
+uint64_t merge_mark(uint64_t* flags, int64_t n, hipStream_t stream) {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  const hipError_t e = hipStreamIsCapturing(stream, &capture);
+  if (e != hipSuccess) (void)hipGetLastError();  // not this call's error
+  if (e == hipSuccess && capture == hipStreamCaptureStatusNone) return fresh_mark();
+  hipLaunchKernelGGL(fa_clear_flags, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, flags, n);
+  return kCapturedMark;
+}
+
 DecodePlan plan_decode(const FwdArgs& a, int batch, int head_dim, bool causal,
                        int64_t workspace_bytes) {
   DecodePlan pl;
@@ -1075,19 +1084,10 @@ int launch_decode_forward(const FwdArgs& a, const DecodePlan& pl, int head_dim, 
                   ? d.part_o + (int64_t)pl.units * pl.splits * pl.rows * head_dim
                   : nullptr;
   d.flags = nullptr;
-  d.mark = kCapturedMark;
+  d.mark = 0;
   if (pl.merge_in_kernel) {
     d.flags = reinterpret_cast<uint64_t*>(d.part_ml + (int64_t)pl.units * pl.splits * pl.rows * 2);
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    const hipError_t e = hipStreamIsCapturing(stream, &capture);
-    if (e != hipSuccess) (void)hipGetLastError();  // not this call's error
-    if (e == hipSuccess && capture == hipStreamCaptureStatusNone) {
-      d.mark = fresh_mark();
-    } else {
-      const int64_t n = (int64_t)pl.units * pl.splits;
-      hipLaunchKernelGGL(fa_clear_flags, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream,
-                         d.flags, n);
-    }
+    d.mark = merge_mark(d.flags, (int64_t)pl.units * pl.splits, stream);
   }
   if (a.bf16)
     launch_decode_typed<true>(d, pl, head_dim, causal, stream);

@@ -187,6 +187,10 @@ bool decode_eligible(const FwdArgs& a, int batch);
 // Splits for a workspace of `workspace_bytes`: as many as it has room for, down to one.
 DecodePlan plan_decode(const FwdArgs& a, int batch, int head_dim, bool causal,
                        int64_t workspace_bytes);
+// The mark of a call whose kernel merges its partials itself: one that no earlier
+// call's flags hold, or (under stream capture) a fixed one, with a kernel that
+// clears the call's n flags first.
+uint64_t merge_mark(uint64_t* flags, int64_t n, hipStream_t stream);
 int launch_decode_forward(const FwdArgs& a, const DecodePlan& plan, int head_dim, bool causal,
                           void* workspace, hipStream_t stream);
 

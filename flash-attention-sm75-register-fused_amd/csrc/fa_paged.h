@@ -58,6 +58,9 @@ struct PagedArgs {
   int split;
   float* part_o;
   float* part_ml;
+  uint64_t* flags;  // one for each of the two records of a workgroup
+  uint64_t mark;    // what a written record's flag holds (merge_mark)
+  int units;        // the most units a class can have
 };
 
 // Largest key count a block table may cover, and row stride (bytes) of a cache
@@ -72,6 +75,8 @@ int launch_paged_read(const PagedArgs& a, int head_dim, hipStream_t stream);
 struct PagedPlan {
   int classes, wgs, rows;  // rows: query columns of a unit
   bool split;
+  bool combine;       // some unit may have more partials than the kernel merges itself
+  int units, y;       // of the combine kernel's grid
   int64_t workspace_bytes;
 };
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
@@ -81,7 +86,7 @@ int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_d
 template <int D, bool BF16, bool FP8>
 void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream);
 template <int D, bool BF16>
-void launch_paged_combine(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream);
+void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream);
 
 }  // namespace fa
 

@@ -18,8 +18,8 @@ FA_PAGED_EXTERN(128, false, true) FA_PAGED_EXTERN(128, true, true)
 #undef FA_PAGED_EXTERN
 
 namespace {
-int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records
-  return 2ll * rows * (head_dim + 2) * (int64_t)sizeof(float);
+int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
+  return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
 }
 }  // namespace
 
@@ -33,17 +33,26 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   const int64_t room = workspace_bytes / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
   p.split = p.wgs > 0;
-  if (!p.split)  // a workgroup for every unit there can be
-    p.wgs = (int)((a.hkv / p.classes) *
-                  (((int64_t)a.tokens * a.group + p.rows - 1) / p.rows + a.batch));
+  // Units of a class: blocks of rows, the last of each sequence not full.
+  const int64_t blocks =
+      a.cu == nullptr ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
+                      : (int64_t)a.tokens * a.group / p.rows + std::min(a.batch, a.tokens);
+  p.units = (int)(a.hkv / p.classes * blocks);
+  if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) : 0;
+  // Stretches are kPMinTiles long at least, and there are wgs of them.
+  const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + kPTile - 1) / kPTile;
+  const int64_t pieces = std::min<int64_t>(p.wgs, tiles / kPMinTiles + 2);
+  p.y = (int)std::min<int64_t>(p.rows, max_query_len * a.group);
+  // (max_query_len may be wrong: rows are then up to p.rows)
+  p.combine = p.split && !paged_merges_itself((int)pieces, a.cu == nullptr ? p.y : p.rows, head_dim);
   return p;
 }
 
 template <int D, bool BF16>
-void launch_paged_combine(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream) {
-  const dim3 g((unsigned)grid, kCombineY);
+void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream) {
+  const dim3 g((unsigned)(a.units * a.classes), (unsigned)y);
   if (rows == 16)
     hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1>), g, dim3(kThreads), 0, stream, a);
   else
@@ -55,11 +64,14 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   PagedArgs a = args;
   a.classes = plan.classes;
   a.wgs = plan.wgs;
+  a.units = plan.units;
   a.split = plan.split ? 1 : 0;
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
   if (plan.split) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
+    a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);
+    a.mark = merge_mark(a.flags, 2 * grid, stream);
   }
   const bool fp8 = a.ks != nullptr;
 #define FA_PAGED(D)                                                                     \
@@ -70,9 +82,9 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
     if (a.bf16) launch_paged_attn<D, true, false>(a, plan.rows, grid, stream);          \
     else launch_paged_attn<D, false, false>(a, plan.rows, grid, stream);                \
   }                                                                                     \
-  if (plan.split) {                                                                     \
-    if (a.bf16) launch_paged_combine<D, true>(a, plan.rows, grid, stream);              \
-    else launch_paged_combine<D, false>(a, plan.rows, grid, stream);                    \
+  if (plan.combine) {                                                                   \
+    if (a.bf16) launch_paged_combine<D, true>(a, plan.rows, plan.y, stream);            \
+    else launch_paged_combine<D, false>(a, plan.rows, plan.y, stream);                  \
   }
   if (head_dim == 64) { FA_PAGED(64) } else { FA_PAGED(128) }
 #undef FA_PAGED

@@ -28,8 +28,9 @@
 // tiles, and each of the class's workgroups takes an equal stretch of the line,
 // whatever mixture of sequences it covers: a batch of very different lengths
 // keeps every CU busy to the end.  A unit cut by a stretch's border leaves
-// partials (O, max, sum) in the workspace, at most two for each workgroup, which a
-// second kernel merges.  Stretches follow from the lengths alone, and partials
+// partials (O, max, sum) in the workspace, at most two for each workgroup.  Where
+// they are few bytes the unit's last workgroup to finish merges them, else
+// a second kernel does.  Stretches follow from the lengths alone, and partials
 // are merged in order, so the same call gives the same bits.
 #pragma once
 
@@ -68,13 +69,15 @@ struct PagedLine {
   const PagedArgs& a;
   int lane;
   int heads;  // KV heads of the class
+  bool by_tiles;  // or by units
   int64_t first;  // prefix(0)
-  __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln) : a(args), lane(ln) {
+  __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln, bool tiles = true)
+      : a(args), lane(ln), by_tiles(tiles) {
     heads = args.hkv / args.classes;
     first = prefix(0);
   }
   __device__ __forceinline__ int64_t length_of(const PagedSeq& s) const {
-    return (int64_t)heads * paged_blocks<R>(a, s) * paged_tiles(a, s);
+    return (int64_t)heads * paged_blocks<R>(a, s) * (by_tiles ? paged_tiles(a, s) : 1);
   }
   // Inclusive prefix sum over the wave's lanes of sequence b0 + lane's length.
   __device__ __forceinline__ int64_t prefix(int b0) const {
@@ -96,6 +99,15 @@ struct PagedLine {
     int64_t sum = wave_bcast(first, 63);
     for (int b0 = 64; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
     return sum;
+  }
+  // Where sequence b starts.
+  __device__ __forceinline__ int64_t start_of(int b) const {
+    int64_t before = 0;
+    for (int b0 = 0;; b0 += 64) {
+      const int64_t x = b0 == 0 ? first : prefix(b0);
+      if (b < b0 + 64) return b == b0 ? before : before + wave_bcast(x, b - b0 - 1);
+      before += wave_bcast(x, 63);
+    }
   }
   // The sequence b that holds position pos (0 <= pos < total), and where it starts.
   __device__ __forceinline__ int find(int64_t pos, int64_t& start) const {
@@ -127,6 +139,47 @@ __host__ __device__ constexpr int paged_per_cu(int d, bool fp8, int nt) {
   return fp8 && nt == 1 ? (d == 64 ? 4 : 3) : d == 64 ? 3 : 2;
 }
 
+// The stretches of a class's line: of total / active tiles, the first ones a
+// tile longer.
+struct PagedStretch {
+  int64_t size;
+  int active, longer;
+  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int64_t total) {
+    active = paged_active(a, total);
+    size = 0;
+    longer = 0;
+    if (active > 0) {
+      size = total / active;
+      longer = (int)(total - size * active);
+    }
+  }
+  __device__ __forceinline__ int64_t start(int wg) const { return wg * size + min(wg, longer); }
+  __device__ __forceinline__ int holder(int64_t pos) const {  // the workgroup of a position
+    const int64_t p = pos - longer * (size + 1);
+    return (int)(p < 0 ? pos / (size + 1) : longer + p / size);
+  }
+};
+
+// The workgroups a unit on [u0, u1) of the line was cut into: from first on, each
+// with its record number slot(i) of the workspace.
+struct PagedPieces {
+  int first, count;
+  __device__ __forceinline__ PagedPieces(const PagedStretch& st, int64_t u0, int64_t u1) {
+    first = st.holder(u0);
+    count = st.holder(u1 - 1) - first + 1;
+  }
+  __device__ __forceinline__ int slot(const PagedArgs& a, int cls, int i) const {
+    return 2 * ((first + i) * a.classes + cls) + (i == 0 ? 1 : 0);
+  }
+};
+
+// Whether a unit's last workgroup merges its partials: one workgroup reads them
+// at about 50 bytes/ns.
+constexpr int kPMergeBytes = 128 << 10;
+__host__ __device__ constexpr bool paged_merges_itself(int pieces, int rows, int d) {
+  return pieces <= kThreads && (int64_t)pieces * rows * d * 4 <= kPMergeBytes;
+}
+
 // Row r of a sequence's rows: the addresses of its Q, O and LSE.
 struct PagedRow {
   int token, head;
@@ -147,6 +200,63 @@ __device__ __forceinline__ void wait_loads() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
   asm volatile("" ::: "memory");
+}
+
+// A merge of partials: the running maximum (log2 units), sum and O.  Where the
+// maximum is -inf every partial so far saw no key, with sum and O zero, or only
+// NaN scores, with both NaN; relative to 0 the weight of either is 2^-inf = 0, which
+// leaves the zeros and keeps the NaN.
+__device__ __forceinline__ float over_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
+constexpr int kPCoherent = 16;  // cache policy: the sc1 bit, coherent over the device's L2s
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+// O and LSE of row r of a sequence from its merged state, 4 dimensions.
+template <bool BF16>
+__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedSeq& s, int hkv, int r, int dim,
+                                          float m2, float l, float4v x) {
+  const PagedRow pr = paged_row(a, s, hkv, r);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  half4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = Elem<BF16>::round(x[e] * inv);
+  *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
+  if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+}
+
+// Folds up to BATCH partials, step apart from i0, into (m, l, x): all their loads
+// are in flight together.  `load` gives the record's (max, sum) and 4 dimensions.
+template <int BATCH, class LoadML, class LoadO>
+__device__ __forceinline__ void fold_partials(int i0, int step, int count, float& m, float& l, float4v& x,
+                                              LoadML load_ml, LoadO load_o) {
+  v2f ml[BATCH];
+  float4v o[BATCH];
+#pragma unroll
+  for (int u = 0; u < BATCH; ++u) {
+    const int i = min(i0 + u * step, count - 1);
+    ml[u] = load_ml(i);
+    o[u] = load_o(i);
+  }
+  float m_new = m;
+#pragma unroll
+  for (int u = 0; u < BATCH; ++u) {
+    if (i0 + u * step >= count) {  // the last one again: no weight
+      ml[u] = v2f{-__builtin_inff(), 0.0f};
+      o[u] = (float4v)0.0f;
+    }
+    m_new = fmaxf(m_new, ml[u][0]);
+  }
+  const float f = __builtin_amdgcn_exp2f(m - over_zero(m_new));
+  l *= f;
+  x *= f;
+#pragma unroll
+  for (int u = 0; u < BATCH; ++u) {
+    const float w = __builtin_amdgcn_exp2f(ml[u][0] - over_zero(m_new));
+    l += w * ml[u][1];
+    x += w * o[u];
+  }
+  m = m_new;
 }
 
 template <int D, bool BF16, bool FP8, int NT>
@@ -178,11 +288,10 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
   const int wg = (int)blockIdx.x / a.classes;
 
   const PagedLine<R> line(a, lane);
-  const int64_t total = line.total();
-  const int active = paged_active(a, total);
-  if (wg >= active) return;
-  int64_t pos = a.split ? wg * total / active : wg;
-  const int64_t end = a.split ? (wg + 1) * total / active : wg + 1;
+  const PagedStretch stretch(a, line.total());
+  if (wg >= stretch.active) return;
+  int64_t pos = stretch.start(wg);
+  const int64_t end = stretch.start(wg + 1);
   int64_t seq_start;
   int b = line.find(pos, seq_start);
 
@@ -486,86 +595,159 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
         l += f * ml_lds[w][1][c];
         x += f * *o_at(w, c, ch);
       }
+      const float m2 = m == -__builtin_inff() ? m : m * c2;
       if (whole) {
-        const PagedRow pr = paged_row(a, s, hkv, r);
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        half4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = E::round(x[e] * inv);
-        *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
-        if (a.lse != nullptr && dim == 0)
-          a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m == -__builtin_inff() ? m : m * c2, l);
+        store_row<BF16>(a, s, hkv, r, dim, m2, l, x);
       } else {
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0);
-        *(float4v*)(a.part_o + (slot * R + c) * D + dim) = x;
-        if (dim == 0) {
-          a.part_ml[(slot * R + c) * 2] = m == -__builtin_inff() ? m : m * c2;
-          a.part_ml[(slot * R + c) * 2 + 1] = l;
-        }
+        // Coherent over the L2s: the merging workgroup may be on another XCD.
+        const int64_t rec = (int64_t)(2 * (int)blockIdx.x + (first == 0 ? 1 : 0)) * R;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, x), make_rsrc(a.part_o + rec * D, R * D * 4),
+                                               (c * D + dim) * 4, 0, kPCoherent);
+        if (dim == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v2f{m2, l}),
+                                                make_rsrc(a.part_ml + rec * 2, R * 8), c * 8, 0, kPCoherent);
       }
+    }
+    if (whole) {
+      __syncthreads();  // the next unit's loads go into these tiles
+      continue;
+    }
+
+    // ---- the unit's last workgroup merges its partials -------------------------
+    // A workgroup's partials are acknowledged before it sets its flag, and its flag
+    // before it reads the others': the last flag to be set is set by a workgroup
+    // that sees them all.  Two that both do store the same values.
+    const int64_t u0 = seq_start + (int64_t)unit * line_tiles;
+    const PagedPieces pieces(stretch, u0, u0 + line_tiles);
+    const int nr = min(R, nrows - rb * R);
+    if (!paged_merges_itself(pieces.count, nr, D)) {
+      __syncthreads();
+      continue;
+    }
+    const __amdgpu_buffer_rsrc_t rf = make_rsrc(a.flags, 2 * (int)gridDim.x * 8);
+    wait_loads<0>();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, a.mark), rf,
+                                            (2 * (int)blockIdx.x + (first == 0 ? 1 : 0)) * 8, 0, kPCoherent);
+      wait_loads<0>();
+    }
+    __syncthreads();
+    bool set = true;
+    if ((int)threadIdx.x < pieces.count)
+      set = __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(
+                rf, pieces.slot(a, cls, threadIdx.x) * 8, 0, kPCoherent)) == a.mark;
+    if (!__syncthreads_and(set)) continue;
+    // Thread: 4 dimensions of a row, pieces grp, grp + groups, ...; the groups
+    // meet in LDS.  More items than threads: one group, items in turns.
+    const int items = nr * (D / 4);
+    const int groups = max(1, min(kThreads / items, pieces.count));
+    const int grp = groups > 1 ? (int)threadIdx.x / items : 0;
+    float4v* const xo = (float4v*)v_lds0;
+    float* const xm = (float*)(v_lds0 + 8 * kThreads);  // max, then sum
+    static_assert(kThreads * 24 <= 4 * VT * 2, "the merge's states fit the V tiles");
+    for (int it = (int)threadIdx.x - grp * items; grp < groups && it < items; it += kThreads) {
+      const int c = it / (D / 4), ch = it - c * (D / 4);
+      float m = -__builtin_inff(), l = 0.0f;
+      float4v x = (float4v)0.0f;
+      for (int i = grp; i < pieces.count; i += 8 * groups)
+        fold_partials<8>(
+            i, groups, pieces.count, m, l, x,
+            [&](int i) {
+              const int64_t rec = (int64_t)pieces.slot(a, cls, i) * R + c;
+              return __builtin_bit_cast(v2f, __builtin_amdgcn_raw_buffer_load_b64(make_rsrc(a.part_ml, INT32_MAX),
+                                                                                  (int)(rec * 8), 0, kPCoherent));
+            },
+            [&](int i) {
+              const int64_t rec = (int64_t)pieces.slot(a, cls, i) * R + c;
+              return __builtin_bit_cast(
+                  float4v, __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(a.part_o, INT32_MAX),
+                                                                 (int)((rec * D + 4 * ch) * 4), 0, kPCoherent));
+            });
+      if (groups > 1) {
+        xo[threadIdx.x] = x;
+        xm[threadIdx.x] = m;
+        xm[kThreads + threadIdx.x] = l;
+      } else {
+        store_row<BF16>(a, s, hkv, rb * R + c, 4 * ch, m, l, x);
+      }
+    }
+    __syncthreads();
+    if (groups > 1 && (int)threadIdx.x < items) {
+      float m = -__builtin_inff(), l = 0.0f;
+      float4v x = (float4v)0.0f;
+      for (int g = 0; g < groups; ++g) m = fmaxf(m, xm[g * items + threadIdx.x]);
+      for (int g = 0; g < groups; ++g) {
+        const float w = __builtin_amdgcn_exp2f(xm[g * items + threadIdx.x] - over_zero(m));
+        l += w * xm[kThreads + g * items + threadIdx.x];
+        x += w * xo[g * items + threadIdx.x];
+      }
+      const int c = (int)threadIdx.x / (D / 4);
+      store_row<BF16>(a, s, hkv, rb * R + c, 4 * ((int)threadIdx.x - c * (D / 4)), m, l, x);
     }
     __syncthreads();
   }
 }
 
-// Merges the partials of the units that stretches cut.  Workgroup wg of a class
-// looks at the border between its stretch and the one before: where it is the
-// first border inside a unit, the unit's partials are slot 1 of the
-// workgroup before it and slot 0 of those from wg on that start inside it.
-// A wave takes a row: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
-constexpr int kCombineY = 4;
+// Merges the partials of units whose last workgroup does not: a workgroup for each
+// unit of a class (blockIdx.x) and row (blockIdx.y, and every gridDim.y-th on).
+// The four waves take every fourth piece, D / 4 lanes each piece's row (with
+// several pieces at once where D / 4 < 64 lanes), and meet in LDS.
 template <int D, bool BF16, int NT>
 __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedArgs a) {
   constexpr int R = 16 * NT;
-  constexpr int DL = D / 64;  // dimensions of a lane
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  constexpr int LR = D / 4;               // lanes of a row
+  constexpr int GROUPS = kThreads / LR;   // pieces at once
+  __shared__ float4v xo[kThreads];
+  __shared__ float xm[2][kThreads];
   const int cls = (int)blockIdx.x % a.classes;
-  const int wg = (int)blockIdx.x / a.classes;
-  const PagedLine<R> line(a, lane);
+  const int index = (int)blockIdx.x / a.classes;  // of the class's units
+  const PagedLine<R> line(a, threadIdx.x & 63);
   const int64_t total = line.total();
-  const int active = paged_active(a, total);
-  if (wg == 0 || wg >= active) return;
-  const int64_t border = wg * total / active;
-  int64_t seq_start;
-  const int b = line.find(border, seq_start);
+  const PagedLine<R> units(a, threadIdx.x & 63, false);
+  if (index >= units.total()) return;
+  int64_t unit_start;
+  const int b = units.find(index, unit_start);
   const PagedSeq s = paged_seq(a, b, load_scalar);
-  const int blocks = paged_blocks<R>(a, s);
   const int tiles = paged_tiles(a, s);
-  const int unit = (int)((border - seq_start) / tiles);
-  const int64_t u0 = seq_start + (int64_t)unit * tiles, u1 = u0 + tiles;
-  if (border == u0 || (wg - 1) * total / active > u0) return;
-  int pieces = 2;  // those of workgroups wg - 1 and wg
-  while ((wg - 1 + pieces) * total / active < u1 && wg - 1 + pieces < active) ++pieces;
+  const int unit = (int)(index - unit_start);
+  const int64_t u0 = line.start_of(b) + (int64_t)unit * tiles;
+  const PagedStretch stretch(a, total);
+  const PagedPieces pieces(stretch, u0, u0 + tiles);
+  if (pieces.count == 1) return;
+  const int blocks = paged_blocks<R>(a, s);
   const int hc = unit / blocks;
   const int rb = unit - hc * blocks;
   const int hkv = hc * a.classes + cls;
-  const int nrows = s.n * a.group;
-  auto slot = [&](int i) -> int64_t {
-    return 2 * ((int64_t)(wg - 1 + i) * a.classes + cls) + (i == 0 ? 1 : 0);
-  };
-  for (int c = wave + 4 * (int)blockIdx.y; c < R && rb * R + c < nrows; c += 4 * kCombineY) {
-    float m = -__builtin_inff(), l = 0.0f, x[DL];
-#pragma unroll
-    for (int e = 0; e < DL; ++e) x[e] = 0.0f;
-    for (int i = 0; i < pieces; ++i) {
-      const int64_t p = slot(i) * R + c;
-      const float mi = a.part_ml[2 * p], li = a.part_ml[2 * p + 1];
-      const float m_new = fmaxf(m, mi);
-      const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
-      const float f0 = __builtin_amdgcn_exp2f(m - m_use), f1 = __builtin_amdgcn_exp2f(mi - m_use);
-      l = l * f0 + li * f1;
-#pragma unroll
-      for (int e = 0; e < DL; ++e) x[e] = x[e] * f0 + a.part_o[p * D + DL * lane + e] * f1;
-      m = m_new;
+  const int nr = min(R, s.n * a.group - rb * R);
+  if (paged_merges_itself(pieces.count, nr, D)) return;
+  const int grp = (int)threadIdx.x / LR, ch = (int)threadIdx.x % LR;
+  for (int c = blockIdx.y; c < nr; c += gridDim.y) {
+    float m = -__builtin_inff(), l = 0.0f;
+    float4v x = (float4v)0.0f;
+    for (int i = grp; i < pieces.count; i += 8 * GROUPS)
+      fold_partials<8>(
+          i, GROUPS, pieces.count, m, l, x,
+          [&](int i) { return *(const v2f*)(a.part_ml + ((int64_t)pieces.slot(a, cls, i) * R + c) * 2); },
+          [&](int i) {
+            return *(const float4v*)(a.part_o + ((int64_t)pieces.slot(a, cls, i) * R + c) * D + 4 * ch);
+          });
+    xo[threadIdx.x] = x;
+    xm[0][threadIdx.x] = m;
+    xm[1][threadIdx.x] = l;
+    __syncthreads();
+    if (grp == 0) {
+      for (int g = 1; g < GROUPS; ++g) m = fmaxf(m, xm[0][g * LR + ch]);
+      l = 0.0f;
+      x = (float4v)0.0f;
+      for (int g = 0; g < GROUPS; ++g) {
+        const float w = __builtin_amdgcn_exp2f(xm[0][g * LR + ch] - over_zero(m));
+        l += w * xm[1][g * LR + ch];
+        x += w * xo[g * LR + ch];
+      }
+      store_row<BF16>(a, s, hkv, rb * R + c, 4 * ch, m, l, x);
     }
-    const PagedRow pr = paged_row(a, s, hkv, rb * R + c);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh + DL * lane;
-#pragma unroll
-    for (int e = 0; e < DL; ++e) op[e] = Elem<BF16>::round(x[e] * inv);
-    if (a.lse != nullptr && lane == 0)
-      a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
+    __syncthreads();
   }
 }
 
