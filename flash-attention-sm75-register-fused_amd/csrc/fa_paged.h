@@ -77,6 +77,7 @@ struct PagedPlan {
   bool split;
   bool combine;       // some unit may have more partials than the kernel merges itself
   int units, y;       // of the combine kernel's grid
+  bool chunk;         // units of 128 rows (fa_paged_chunk.h)
   int64_t workspace_bytes;
 };
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
@@ -85,6 +86,8 @@ int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_d
                            void* workspace, hipStream_t stream);
 template <int D, bool BF16, bool FP8>
 void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream);
+template <int D, bool BF16, bool FP8>
+void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream);
 template <int D, bool BF16>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream);
 

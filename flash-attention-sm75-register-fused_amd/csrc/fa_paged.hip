@@ -5,12 +5,14 @@
 
 #include "fa_internal.h"
 #include "fa_paged_attn.h"
+#include "fa_paged_chunk.h"
 
 namespace fa {
 
 // The instances of fa_paged_d*.hip.
 #define FA_PAGED_EXTERN(D, BF, F8) \
-  extern template void launch_paged_attn<D, BF, F8>(const PagedArgs&, int, int64_t, hipStream_t);
+  extern template void launch_paged_attn<D, BF, F8>(const PagedArgs&, int, int64_t, hipStream_t); \
+  extern template void launch_paged_chunk<D, BF, F8>(const PagedArgs&, int64_t, hipStream_t);
 FA_PAGED_EXTERN(64, false, false) FA_PAGED_EXTERN(64, true, false)
 FA_PAGED_EXTERN(64, false, true) FA_PAGED_EXTERN(64, true, true)
 FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
@@ -23,9 +25,29 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
 }
 }  // namespace
 
+// Units of 128 rows, cut into pieces where they may be fewer than the GPU runs at once.
+static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace_bytes) {
+  PagedPlan p{};
+  p.chunk = true;
+  p.rows = kChunkRows;
+  p.classes = std::gcd(a.hkv, kNumXcds);
+  // A class's units, the last block of each sequence not full: at least and at most.
+  const int64_t heads = a.hkv / p.classes, rows = (int64_t)a.tokens * a.group;
+  const int64_t least = heads * ((rows + p.rows - 1) / p.rows);
+  p.units = (int)(heads * ((rows + (p.rows - 1ll) * std::min(a.batch, a.tokens)) / p.rows));
+  const int64_t record = (int64_t)p.rows * (head_dim + 2) * (int64_t)sizeof(float) * p.classes;
+  const int64_t wgs = resident_fused_workgroups() / p.classes;
+  p.split = least < wgs && std::max<int64_t>(wgs, p.units) <= workspace_bytes / record;
+  p.combine = p.split;
+  p.wgs = p.split ? (int)std::max<int64_t>(wgs, p.units) : p.units;
+  p.workspace_bytes = p.split ? p.wgs * record : 0;
+  return p;
+}
+
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
                      int64_t workspace_bytes) {
-  PagedPlan p;
+  if (max_query_len * a.group > 32) return plan_chunks(a, head_dim, workspace_bytes);
+  PagedPlan p{};
   p.rows = max_query_len * a.group <= 16 ? 16 : 32;
   p.classes = std::gcd(a.hkv, kNumXcds);
   const int64_t resident =  // (resident_fused_workgroups: two a CU)
@@ -52,6 +74,11 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
 
 template <int D, bool BF16>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream) {
+  if (rows == kChunkRows) {
+    hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16>),
+                       dim3((unsigned)(a.wgs * a.classes)), dim3(kThreads), 0, stream, a);
+    return;
+  }
   const dim3 g((unsigned)(a.units * a.classes), (unsigned)y);
   if (rows == 16)
     hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1>), g, dim3(kThreads), 0, stream, a);
@@ -67,7 +94,10 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   a.units = plan.units;
   a.split = plan.split ? 1 : 0;
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
-  if (plan.split) {
+  if (plan.split && plan.chunk) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + grid * plan.rows * head_dim;
+  } else if (plan.split) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);
@@ -75,7 +105,15 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   }
   const bool fp8 = a.ks != nullptr;
 #define FA_PAGED(D)                                                                     \
-  if (fp8) {                                                                            \
+  if (plan.chunk) {                                                                     \
+    if (fp8) {                                                                          \
+      if (a.bf16) launch_paged_chunk<D, true, true>(a, grid, stream);                   \
+      else launch_paged_chunk<D, false, true>(a, grid, stream);                         \
+    } else {                                                                            \
+      if (a.bf16) launch_paged_chunk<D, true, false>(a, grid, stream);                  \
+      else launch_paged_chunk<D, false, false>(a, grid, stream);                        \
+    }                                                                                   \
+  } else if (fp8) {                                                                            \
     if (a.bf16) launch_paged_attn<D, true, true>(a, plan.rows, grid, stream);           \
     else launch_paged_attn<D, false, true>(a, plan.rows, grid, stream);                 \
   } else {                                                                              \

@@ -1,0 +1,667 @@
+// Attention of a chunk of new tokens over a paged cache: units of 128 query rows.
+//
+// A unit is one (sequence, KV head, block of 128 rows), row r of a sequence being
+// token r / group of query head kv_head * group + r % group, so that a chunk of few
+// tokens fills a block with its heads, and all rows of a block read the same K and V.
+// One workgroup = 4 waves, wave w rows 32 w .. 32 w + 31; keys stream through LDS
+// in double-buffered tiles of 64.  The matrix formulation, the LDS layouts and the
+// step's schedule are the dense forward's (fa_fwd_kernel.h): S^T = K Q^T and O^T =
+// V^T P^T in 32x32x16 MFMAs, one query per lane, step j issuing the MFMAs of S_{j+1}
+// and P_j V_j slot by slot with the softmax of S_j, the operand reads and the
+// loads of K_{j+2} and V_{j+1} between them.
+//
+// Pages.  Each wave brings 16 consecutive keys of every tile, which lie in one page
+// whatever its size (16 or more): one table entry and one buffer window, whose base
+// is scalar, for all its loads.  Table entries are read through the scalar cache a
+// tile ahead.  Pieces that name no page read through an empty window (zeros) and
+// are masked.
+//
+// 8-bit rows go through registers: a wave converts its 16 rows of a tile once for the
+// workgroup (the codes times a power of two are 16-bit numbers) and writes them to LDS
+// in the layout the 16-bit rows arrive in.
+//
+// The plan.  Where there are fewer units than fill the GPU, each sequence's units are cut
+// into pieces of about equally many tiles, as short as lets all of them run at once;
+// the pieces' partials (O, max, sum) are merged by a second kernel.  Every workgroup
+// derives the cut from the lengths (ChunkCut).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_paged_units.h"
+
+namespace fa {
+namespace {
+
+constexpr int kChunkRows = 128;
+constexpr int kChunkMinTiles = 4;  // tiles a piece is not cut below
+
+// Rows a sequence's blocks and 64-key tiles.
+__device__ __forceinline__ int chunk_tiles(int keys) { return max(1, (keys + kBlockN - 1) / kBlockN); }
+
+__device__ __forceinline__ PagedSeq lane_seq(const PagedArgs& a, int b) {
+  if (b < a.batch) return paged_seq(a, b, [](const int32_t* p) { return *p; });
+  return PagedSeq{0, 0, 0, 0};
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
+// How a class's units are cut: each sequence's into ceil(tiles / len) pieces.  Called
+// by whole waves; the first 64 sequences (one a lane) are looked at once.
+struct ChunkCut {
+  const PagedArgs& a;
+  int lane, heads;
+  int units, tiles;  // of sequence `lane`: units, and the tiles of one
+  int len;
+
+  __device__ __forceinline__ void look(int b0, int& u, int& t) const {
+    if (b0 == 0) {
+      u = units;
+      t = tiles;
+      return;
+    }
+    const PagedSeq s = lane_seq(a, b0 + lane);
+    u = heads * paged_blocks<kChunkRows>(a, s);
+    t = chunk_tiles(s.keys);
+  }
+  __device__ __forceinline__ int pieces(int t) const { return len > 0 ? (t + len - 1) / len : 1; }
+  __device__ __forceinline__ int64_t items(int by) const {  // cut into pieces of `by` tiles
+    int64_t sum = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      int u, t;
+      look(b0, u, t);
+      sum += (int64_t)u * ((t + by - 1) / by);
+    }
+    return wave_sum(sum);
+  }
+
+  // The cut: the least of a few lengths from total / slots on with which all pieces
+  // run at once, total / (slots - units) being one of them; none where the units
+  // alone fill the GPU.
+  __device__ __forceinline__ ChunkCut(const PagedArgs& args, int ln) : a(args), lane(ln) {
+    heads = a.hkv / a.classes;
+    const PagedSeq s = lane_seq(a, lane);
+    units = heads * paged_blocks<kChunkRows>(a, s);
+    tiles = chunk_tiles(s.keys);
+    len = 0;
+    if (!a.split) return;
+    int64_t all_units = 0, total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      int u, t;
+      look(b0, u, t);
+      all_units += u;
+      total += (int64_t)u * t;
+    }
+    all_units = wave_sum(all_units);
+    total = wave_sum(total);
+    const int64_t room = a.wgs - all_units;
+    if (room <= 0) return;
+    const int64_t sure = (total + room - 1) / room, even = (total + a.wgs - 1) / a.wgs;
+    int64_t best = sure;
+    for (int k = 0; k < 5; ++k) {
+      const int64_t by = even + even * k / 8;
+      if (by >= sure) break;
+      if (items((int)by) <= a.wgs) {
+        best = by;
+        break;
+      }
+    }
+    len = __builtin_amdgcn_readfirstlane((int)max(best, (int64_t)kChunkMinTiles));
+  }
+
+  // Item `index` of the class: its sequence (-1: none), and its place there.
+  __device__ __forceinline__ int find(int64_t index, int& place) const {
+    int64_t before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      int u, t;
+      look(b0, u, t);
+      int64_t x = (int64_t)u * pieces(t);
+      const int n = min(64, a.batch - b0);
+      for (int d = 1; d < n; d <<= 1) {
+        const int64_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(lane < n && before + x > index);
+      if (past != 0) {
+        const int l = __builtin_ctzll(past);
+        place = (int)(index - (l > 0 ? before + wave_bcast(x, l - 1) : before));
+        return b0 + l;
+      }
+      before += wave_bcast(x, n - 1);
+    }
+    return -1;
+  }
+};
+
+// A unit of a sequence from its place: heads one after the other, blocks of a head
+// from the last (under the causal rule the longest) to the first.
+struct ChunkUnit {
+  int hkv, rb, piece, pieces;
+};
+__device__ __forceinline__ ChunkUnit chunk_unit(const PagedArgs& a, const ChunkCut& cut, const PagedSeq& s,
+                                                int cls, int place) {
+  ChunkUnit u;
+  const int blocks = paged_blocks<kChunkRows>(a, s);
+  u.pieces = cut.pieces(chunk_tiles(s.keys));
+  const int unit = place / u.pieces;
+  u.piece = place - unit * u.pieces;
+  const int hc = unit / blocks;
+  u.rb = blocks - 1 - (unit - hc * blocks);
+  u.hkv = hc * a.classes + cls;
+  return u;
+}
+
+template <int D, bool BF16, bool FP8>
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
+  constexpr bool DENSE = D == 64;
+  using L = std::conditional_t<DENSE, LdsDense<D>, Lds<D>>;
+  using E = Elem<BF16>;
+  constexpr int KK = D / 16;       // 16-wide contraction steps of S^T
+  constexpr int MT = D / 32;       // 32-row output tiles of O^T
+  constexpr int NS = 2 * KK;       // S^T MFMAs per tile
+  constexpr int NPV = 4 * MT;      // P V MFMAs per tile
+  constexpr int PFK = 3;           // K operand reads run this many MFMAs ahead
+  constexpr int PFV = 2;           // V operand reads run this many MFMAs ahead
+  constexpr int SEGQ = L::Segs / 4;            // 1 KB segments of a wave's 16 rows
+  constexpr int RL = D / 16;                   // FP8: lanes that hold a row's codes
+  constexpr int LQ = 16 * RL / 64;             // FP8: 16-byte loads of 16 rows
+  constexpr int LPW = FP8 ? 2 * LQ : 2 * SEGQ; // loads per wave and step
+  static_assert(SEGQ * 1024 == 16 * L::Pitch * 2, "a wave's segments are its 16 rows");
+
+  // Distinct objects, so that the compiler sees that loads in flight into one do
+  // not touch the tiles being read.
+  __shared__ __attribute__((aligned(1024))) _Float16 k_lds0[L::Tile];
+  __shared__ __attribute__((aligned(1024))) _Float16 k_lds1[L::Tile];
+  __shared__ __attribute__((aligned(1024))) _Float16 v_lds0[L::Tile];
+  __shared__ __attribute__((aligned(1024))) _Float16 v_lds1[L::Tile];
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int hi = lane >> 5;   // which half of the wave
+  const int ql = lane & 31;   // query column owned by this lane
+  const int grp = lane >> 4;  // 16-lane group (transposing reads)
+  const int gi = lane & 15;
+  const int cls = (int)blockIdx.x % a.classes;
+
+  const ChunkCut cut(a, lane);
+  int place;
+  const int b = __builtin_amdgcn_readfirstlane(cut.find((int)blockIdx.x / a.classes, place));
+  if (b < 0) return;
+  const PagedSeq s = paged_seq(a, b, load_scalar);
+  const ChunkUnit unit = chunk_unit(a, cut, s, cls, __builtin_amdgcn_readfirstlane(place));
+  const int hkv = unit.hkv;
+  const int nrows = s.n * a.group;
+  const int q0 = unit.rb * kChunkRows;
+  const int qw = q0 + 32 * wave;
+  const int row = qw + ql;
+  const int past = s.len - s.n;  // tokens before the new ones
+
+  // Keys the block's rows see, and this piece's tiles of them.
+  const int last_tok = (min(nrows, q0 + kChunkRows) - 1) / a.group;
+  const int kv_len = a.causal ? clamp_int(past + last_tok + 1, 0, s.keys) : s.keys;
+  const int block_tiles = (kv_len + kBlockN - 1) / kBlockN;
+  const int tile0 = (int)((int64_t)block_tiles * unit.piece / unit.pieces);
+  const int tile_end = (int)((int64_t)block_tiles * (unit.piece + 1) / unit.pieces);
+  // The last key this lane's row sees; keys below wave_full are seen by every row of
+  // the wave.
+  const int tok = min(row, nrows - 1) / a.group;
+  const int last_key = a.causal ? min(s.keys - 1, past + tok) : s.keys - 1;
+  const int wave_full = a.causal ? clamp_int(past + min(qw, nrows - 1) / a.group + 1, 0, s.keys) : s.keys;
+
+  // Q^T fragments (B operand of S^T), resident for the whole kernel.
+  half8 qf[KK];
+  {
+    const PagedRow pr = paged_row(a, s, hkv, min(row, nrows - 1));
+    const _Float16* qp = a.q + pr.token * a.qt + pr.head * a.qh + 8 * hi;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[kk] = *(const half8*)(qp + 16 * kk);
+      if (a.negate_q) qf[kk] = negate16(qf[kk]);
+    }
+  }
+
+  // What a lane loads of its wave's 16 rows: byte offsets from the first row.
+  // 16-bit rows go to LDS directly (lane l's 16 bytes at 16 l of each KB; padding
+  // lanes: past any window).
+  int koff[FP8 ? 1 : SEGQ], voff[FP8 ? 1 : SEGQ];
+  if constexpr (!FP8) {
+#pragma unroll
+    for (int i = 0; i < SEGQ; ++i) {
+      const int at = 1024 * i + 16 * lane;
+      const int r = at / (2 * L::Pitch);
+      const int within = at - r * (2 * L::Pitch);
+      if (DENSE || within < 2 * D) {
+        const int c = (within >> 4) ^ (DENSE ? dense_swizzle(r) : ((r >> 2) & 3));
+        koff[i] = r * (int)a.kn + 16 * c;
+        voff[i] = r * (int)a.vn + 16 * c;
+      } else {
+        koff[i] = voff[i] = -16;
+      }
+    }
+  }
+
+  // Table entries of a tile's four 16-key pieces, and what they say: the page of
+  // this wave's piece (-1: none) and which pieces are in no page.
+  const int32_t* const entries = a.table + b * a.table_stride;
+  auto look_up = [&](int j, int (&e)[4]) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      e[p] = load_scalar(entries + min((j * kBlockN + 16 * p) >> a.page_shift, a.max_pages - 1));
+  };
+  struct Pages {
+    int own;
+    unsigned gone;
+  };
+  auto pages_of = [&](const int (&e)[4]) -> Pages {
+    Pages x;
+    x.gone = 0;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) x.gone |= (unsigned)e[p] < (unsigned)a.num_pages ? 0u : 1u << p;
+    x.own = wave < 2 ? (wave == 0 ? e[0] : e[1]) : (wave == 2 ? e[2] : e[3]);
+    if ((x.gone >> wave) & 1) x.own = -1;
+    return x;
+  };
+  const uint8_t* const kh = a.k + hkv * a.kh;
+  const uint8_t* const vh = a.v + hkv * a.vh;
+  // Window of this wave's rows of tile j (empty past the piece's keys).
+  auto rows_of = [&](int j, int page) -> int {
+    return page >= 0 && j < tile_end ? clamp_int(kv_len - (j * kBlockN + 16 * wave), 0, 16) : 0;
+  };
+  auto window = [&](const uint8_t* base, int64_t sp, int64_t sn, int j, int page) {
+    const int off = (j * kBlockN + 16 * wave) & ((1 << a.page_shift) - 1);
+    return make_rsrc(base + (int64_t)max(page, 0) * sp + off * sn, rows_of(j, page) * (int)sn);
+  };
+
+  auto kbuf = [&](auto st) -> _Float16* { return decltype(st)::value % 2 == 0 ? k_lds0 : k_lds1; };
+  auto vbuf = [&](auto st) -> _Float16* { return decltype(st)::value % 2 == 0 ? v_lds0 : v_lds1; };
+  auto lds_seg = [&](_Float16* tile, int i) -> lds_void* {
+    int off = (SEGQ * wave + i) * 512;
+    asm volatile("" : "+s"(off));  // recomputed at each load, not kept in a register
+    return (lds_void*)(tile + off);
+  };
+
+  // 8-bit rows in flight: this wave's 16 rows of a K tile and of a V tile.
+  constexpr int LF = FP8 ? LQ : 1;
+  uint4v kr[LF], vr[LF];
+  unsigned ksr[LF], vsr[LF];
+  auto load_codes = [&](const uint8_t* base, int64_t sp, int64_t sn, const uint8_t* sbase, int64_t ssp,
+                        int64_t ssn, int j, int page, uint4v (&w)[LF], unsigned (&sc)[LF]) {
+    const __amdgpu_buffer_rsrc_t r = window(base, sp, sn, j, page);
+    const __amdgpu_buffer_rsrc_t rs = window(sbase, ssp, ssn, j, page);
+#pragma unroll
+    for (int i = 0; i < LF; ++i) {
+      const int rr = (64 * i + lane) / RL;
+      w[i] = __builtin_bit_cast(
+          uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, rr * (int)sn + 16 * (lane % RL), 0, 0));
+      sc[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, rr * (int)ssn, 0, 0);
+    }
+  };
+  // Half `h` of load i (8 codes) into its place of the tile.
+  auto store_codes = [&](_Float16* tile, const uint4v& w, unsigned sc, int i, int h) {
+    const int rr = 16 * wave + (64 * i + lane) / RL;
+    const int c = (2 * (lane % RL) + h) ^ (DENSE ? dense_swizzle(rr) : ((rr >> 2) & 3));
+    *(half8*)(tile + rr * L::Pitch + 8 * c) = dequantise8<BF16>(w[2 * h], w[2 * h + 1], scale_of(sc));
+  };
+  const uint8_t* const ksh = FP8 ? a.ks + hkv * a.ksh : nullptr;
+  const uint8_t* const vsh = FP8 ? a.vs + hkv * a.vsh : nullptr;
+  auto load_k8 = [&](int j, int page) { load_codes(kh, a.kp, a.kn, ksh, a.ksp, a.ksn, j, page, kr, ksr); };
+  auto load_v8 = [&](int j, int page) { load_codes(vh, a.vp, a.vn, vsh, a.vsp, a.vsn, j, page, vr, vsr); };
+
+  // Per-lane LDS bases of the operand reads (as in the dense forward).
+  const int sK = (ql >> 2) & 3;
+  const int k_base_even = ql * L::Pitch + 8 * (hi ^ sK);
+  const int k_base_odd = ql * L::Pitch + 8 * ((2 + hi) ^ sK);
+  const int v_row = 4 * hi + (gi >> 2);
+  const int v_c = 2 * (grp & 1) + ((gi & 3) >> 1);
+  const int v_base0 = v_row * L::Pitch + 8 * (v_c ^ hi) + 4 * (gi & 1);
+  const int v_base1 = (v_row + 8) * L::Pitch + 8 * (v_c ^ (hi + 2)) + 4 * (gi & 1);
+  int kd_base[DENSE ? KK : 1], vd_base0[DENSE ? MT : 1], vd_base1[DENSE ? MT : 1];
+  if constexpr (DENSE) {
+    const int sw = dense_swizzle(ql);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) kd_base[kk] = ql * L::Pitch + 8 * ((2 * kk + hi) ^ sw);
+    const int sw0 = dense_swizzle(v_row), sw1 = dense_swizzle(v_row + 8);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      vd_base0[mt] = v_row * L::Pitch + 8 * ((v_c + 4 * mt) ^ sw0) + 4 * (gi & 1);
+      vd_base1[mt] = (v_row + 8) * L::Pitch + 8 * ((v_c + 4 * mt) ^ sw1) + 4 * (gi & 1);
+    }
+  }
+  auto read_k = [&](const _Float16* Ks, int i) -> half8 {
+    const int t = i / KK, kk = i % KK;
+    if constexpr (DENSE) return *(const half8*)(Ks + kd_base[kk] + 32 * t * L::Pitch);
+    const int off = ((kk & 1) ? k_base_odd : k_base_even) + 32 * t * L::Pitch + 32 * (kk >> 1);
+    return *(const half8*)(Ks + off);
+  };
+  auto read_v = [&](const _Float16* Vs, int v) -> half8 {
+    const int ks = v / MT, mt = v % MT;
+    const int imm = 16 * ks * L::Pitch + (DENSE ? 0 : 32 * mt);
+    const half4 lo = ds_read_tr16(Vs + (DENSE ? vd_base0[DENSE ? mt : 0] : v_base0) + imm);
+    const half4 hi4 = ds_read_tr16(Vs + (DENSE ? vd_base1[DENSE ? mt : 0] : v_base1) + imm);
+    return __builtin_shufflevector(lo, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  float16v oacc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) oacc[mt] = (float16v)0.0f;
+  float m_run = -__builtin_inff();
+  float l_run = 0.0f;  // the lane's part of its row sum
+  const float c2 = a.c;
+  float16v s_buf[2][2];  // S^T of two tiles in flight
+  float mc = 0.0f;       // running max times c2 (exp2 offset)
+  float thr = -__builtin_inff();
+
+  // Masks tile j's scores where it hides a key from some row of the wave, and
+  // raises the running max when some row outgrew it by more than 2^kRescaleLog2.
+  // mx: the lane's max over its half of the row.
+  auto prepare = [&](int j, float16v (&sc)[2], float mx, unsigned gone) {
+    const int kstart = j * kBlockN;
+    if (kstart + kBlockN > wave_full || gone != 0) {
+      const int lim = last_key - kstart - 4 * hi;
+      static_for<32>([&](auto e_c) {
+        constexpr int e = decltype(e_c)::value;
+        constexpr int t = e >> 4, i = e & 15;
+        constexpr int off = 32 * t + 8 * (i >> 2) + (i & 3);
+        if (off > lim || ((gone >> (off >> 4)) & 1)) sc[t][i] = -__builtin_inff();
+      });
+      mx = -__builtin_inff();
+      static_for<32>([&](auto e_c) {
+        constexpr int e = decltype(e_c)::value;
+        mx = fmaxf(mx, sc[e >> 4][e & 15]);
+      });
+    }
+    if (__builtin_amdgcn_ballot_w64(mx > thr) != 0) {
+      const float m_new = fmaxf(m_run, halves_max(mx));
+      const float m_use = (m_new == -__builtin_inff()) ? 0.0f : m_new;
+      const float alpha =
+          (m_run == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f((m_run - m_use) * c2);
+      l_run *= alpha;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) oacc[mt] *= alpha;
+      m_run = m_new;
+      mc = m_use * c2;
+      thr = m_new + kRescaleLog2 / c2;
+    }
+  };
+
+  // Pages of tiles j + 1 and j + 2 at the start of step j, and the entries of
+  // tile j + 3 (in flight).
+  Pages pg1, pg2;
+  int ahead[4];
+
+  auto step = [&](int j, auto has_next_t, auto u_t) {
+    constexpr bool HAS_NEXT = decltype(has_next_t)::value;
+    constexpr int U = decltype(u_t)::value;
+    constexpr int ns = HAS_NEXT ? NS : 0;  // S MFMAs this step
+    const _Float16* Kn = kbuf(std::integral_constant<int, U + 1>{});
+    const _Float16* Vc = vbuf(std::integral_constant<int, U>{});
+    float16v (&s_cur)[2] = s_buf[U];
+    float16v (&s_nxt)[2] = s_buf[1 - U];
+
+    // Loads of K_{j+2} (into the buffer K_j used) and V_{j+1} (into V_{j-1}'s), one
+    // after each of the first MFMAs.  8-bit rows: those tiles' codes, loaded a step
+    // ago, are converted and stored, and the next tiles' loads follow.
+    __amdgpu_buffer_rsrc_t rk_next, rv_next;
+    const Pages now1 = pg1, now2 = pg2;
+    if constexpr (HAS_NEXT) {
+      pg1 = pg2;
+      pg2 = pages_of(ahead);
+      look_up(j + 4, ahead);
+      if constexpr (!FP8) {
+        rk_next = window(kh, a.kp, a.kn, j + 2, now2.own);
+        rv_next = window(vh, a.vp, a.vn, j + 1, now1.own);
+      }
+    }
+    _Float16* const k_dst = kbuf(std::integral_constant<int, U>{});
+    _Float16* const v_dst = vbuf(std::integral_constant<int, U + 1>{});
+    auto issue_load = [&](auto q_c) {
+      constexpr int q = decltype(q_c)::value;
+      if constexpr (FP8) {  // half a load's codes to LDS
+        constexpr int i = q / 4, h = q & 1;
+        if constexpr ((q & 2) == 0) store_codes(k_dst, kr[i], ksr[i], i, h);
+        else store_codes(v_dst, vr[i], vsr[i], i, h);
+        if constexpr (q == 4 * LQ - 1) {
+          load_k8(j + 3, pg2.own);
+          load_v8(j + 2, pg1.own);
+        }
+      } else if constexpr (q < SEGQ) {
+        direct_load16(rk_next, lds_seg(k_dst, q), koff[q]);
+      } else {
+        direct_load16(rv_next, lds_seg(v_dst, q - SEGQ), voff[q - SEGQ]);
+      }
+    };
+    constexpr int NL = FP8 ? 4 * LQ : LPW;
+
+    constexpr int NB = ns + NPV;            // MFMA slots
+    constexpr int PV_FIRST = ns;            // slot of the first P V MFMA
+    constexpr int PAIR_SLOTS = NB - MT;     // slots available to pairs
+    half8 kf[NS];
+    uint4v pf[4];
+    half8 vf[NPV];
+    constexpr auto pair_slot = [](int p) constexpr {
+      const int spread = (p * PAIR_SLOTS) / 16;
+      const int last_ok = PV_FIRST + (p / 4) * MT - 1;
+      return spread < last_ok ? spread : last_ok;
+    };
+    constexpr auto max_slot = [](int e) constexpr {
+      const int t = e >> 4, i = e & 15;
+      const int first = (t + 1) * KK + 2;
+      const int span = (t == 0 ? KK : NB - 1 - first);
+      const int sl = first + (i * span) / 16;
+      return sl < NB - 1 ? sl : NB - 1;
+    };
+    constexpr auto last_max_slot = [max_slot]() constexpr {
+      int m = 0;
+      for (int e = 0; e < 32; ++e) m = max_slot(e) > m ? max_slot(e) : m;
+      return m;
+    };
+    auto softmax_pair = [&](auto p_c) {
+      constexpr int p = decltype(p_c)::value;
+      constexpr int e = 2 * p;
+      constexpr int t = e >> 4, i = e & 15;
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[t][i], c2, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[t][i + 1], c2, -mc));
+      pf[2 * t + (i >> 3)][(i & 7) >> 1] = __builtin_bit_cast(unsigned, E::pack(p0, p1));
+      l_run += p0;
+      l_run += p1;
+      asm volatile("" : "+v"(l_run));  // keeps the sum in this slot
+    };
+    static_for<16>([&](auto p_c) {
+      if constexpr (pair_slot(decltype(p_c)::value) < 0) softmax_pair(p_c);
+    });
+    if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
+    static_for<(PFK < ns ? PFK : ns)>([&](auto i_c) {
+      kf[decltype(i_c)::value] = read_k(Kn, decltype(i_c)::value);
+    });
+    float mx_next = -__builtin_inff();
+    static_for<NB>([&](auto slot_c) {
+      constexpr int slot = decltype(slot_c)::value;
+      if constexpr (slot == (PV_FIRST >= PFV ? PV_FIRST - PFV : 0)) {
+        static_for<PFV>([&](auto v_c) {
+          vf[decltype(v_c)::value] = read_v(Vc, decltype(v_c)::value);
+        });
+      }
+      if constexpr (slot >= PV_FIRST && slot - PV_FIRST + PFV < NPV)
+        vf[slot - PV_FIRST + PFV] = read_v(Vc, slot - PV_FIRST + PFV);
+      if constexpr (slot < PV_FIRST) {
+        constexpr int i = slot;
+        if constexpr (i + PFK < ns) kf[i + PFK] = read_k(Kn, i + PFK);
+        constexpr int t = i / KK, kk = i % KK;
+        s_nxt[t] = E::mfma(kf[i], qf[kk], kk == 0 ? (float16v)0.0f : s_nxt[t]);
+      } else {
+        constexpr int v = slot - PV_FIRST;
+        constexpr int ks = v / MT, mt = v % MT;
+        oacc[mt] = E::mfma(vf[v], __builtin_bit_cast(half8, pf[ks]), oacc[mt]);
+      }
+      if constexpr (HAS_NEXT) {
+        static_for<NL>([&](auto q_c) {
+          constexpr int q = decltype(q_c)::value;
+          if constexpr ((q * (NB / 2)) / NL == slot) issue_load(q_c);
+        });
+        static_for<32>([&](auto e_c) {
+          constexpr int e = decltype(e_c)::value;
+          if constexpr (max_slot(e) == slot) mx_next = fmaxf(mx_next, s_nxt[e >> 4][e & 15]);
+        });
+        if constexpr (slot == last_max_slot()) asm volatile("" : "+v"(mx_next));
+      }
+      static_for<16>([&](auto p_c) {
+        if constexpr (pair_slot(decltype(p_c)::value) == slot) softmax_pair(p_c);
+      });
+      fence_schedule();
+    });
+    if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
+    if constexpr (HAS_NEXT) {
+      prepare(j + 1, s_nxt, mx_next, now1.gone);
+      // Direct loads have landed (codes in flight to registers need not have), and
+      // every wave is done with the buffers the next step's loads overwrite.
+      barrier_after_loads<FP8 ? 63 : 0>();
+    }
+  };
+
+  if (tile0 < tile_end) {
+    // ---- prologue: K_0, K_1 and V_0 into LDS; S_0 -----------------------------
+    int e0[4], e1[4], e2[4];
+    look_up(tile0, e0);
+    look_up(tile0 + 1, e1);
+    look_up(tile0 + 2, e2);
+    look_up(tile0 + 3, ahead);
+    const Pages pg0 = pages_of(e0);
+    pg1 = pages_of(e1);
+    pg2 = pages_of(e2);
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    if constexpr (FP8) {
+      load_k8(tile0, pg0.own);
+      load_v8(tile0, pg0.own);
+      static_for<LQ>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value;
+        static_for<2>([&](auto h_c) {
+          store_codes(k_lds0, kr[i], ksr[i], i, decltype(h_c)::value);
+          store_codes(v_lds0, vr[i], vsr[i], i, decltype(h_c)::value);
+        });
+      });
+      load_k8(tile0 + 1, pg1.own);
+      static_for<LQ>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value;
+        static_for<2>([&](auto h_c) { store_codes(k_lds1, kr[i], ksr[i], i, decltype(h_c)::value); });
+      });
+      load_k8(tile0 + 2, pg2.own);
+      load_v8(tile0 + 1, pg1.own);
+      barrier_after_loads<63>();
+    } else {
+      const __amdgpu_buffer_rsrc_t rk0 = window(kh, a.kp, a.kn, tile0, pg0.own);
+      const __amdgpu_buffer_rsrc_t rk1 = window(kh, a.kp, a.kn, tile0 + 1, pg1.own);
+      const __amdgpu_buffer_rsrc_t rv0 = window(vh, a.vp, a.vn, tile0, pg0.own);
+#pragma unroll
+      for (int i = 0; i < SEGQ; ++i) direct_load16(rk0, lds_seg(k_lds0, i), koff[i]);
+#pragma unroll
+      for (int i = 0; i < SEGQ; ++i) direct_load16(rk1, lds_seg(k_lds1, i), koff[i]);
+#pragma unroll
+      for (int i = 0; i < SEGQ; ++i) direct_load16(rv0, lds_seg(v_lds0, i), voff[i]);
+      barrier_after_loads<2 * SEGQ>();  // S_0 needs K_0 only
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s_buf[0][t] = (float16v)0.0f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        s_buf[0][t] = E::mfma(read_k(k_lds0, t * KK + kk), qf[kk], s_buf[0][t]);
+    }
+    float mx = -__builtin_inff();
+    static_for<32>([&](auto e_c) {
+      constexpr int e = decltype(e_c)::value;
+      mx = fmaxf(mx, s_buf[0][e >> 4][e & 15]);
+    });
+    prepare(tile0, s_buf[0], mx, pg0.gone);
+    // Step 0 writes K_2 into K_0's buffer: every wave must be done with it.
+    barrier_after_loads<FP8 ? 63 : 0>();
+    int j = tile0;
+    for (; j + 2 < tile_end; j += 2) {
+      step(j, Flag<true>{}, I0{});
+      step(j + 1, Flag<true>{}, I1{});
+    }
+    if (tile_end - j == 1) {
+      step(j, Flag<false>{}, I0{});
+    } else {
+      step(j, Flag<true>{}, I0{});
+      step(j + 1, Flag<false>{}, I1{});
+    }
+  }
+  // No direct load may land in LDS after the workgroup ends.
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+
+  const float l = halves_sum(l_run);
+  if (row >= nrows) return;
+  if (unit.pieces == 1) {
+    const PagedRow pr = paged_row(a, s, hkv, row);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        half4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = E::round(oacc[mt][4 * g + e] * inv);
+        *(half4*)(op + 32 * mt + 8 * g + 4 * hi) = v;
+      }
+    if (a.lse != nullptr && hi == 0)
+      a.lse[(int64_t)pr.head * a.tokens + pr.token] =
+          natural_lse(m_run == -__builtin_inff() ? m_run : m_run * c2, l);
+  } else {
+    const int64_t rec = (int64_t)blockIdx.x * kChunkRows + (row - q0);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(float4v*)(a.part_o + rec * D + 32 * mt + 8 * g + 4 * hi) =
+            float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
+    if (hi == 0)
+      *(v2f*)(a.part_ml + rec * 2) = v2f{m_run == -__builtin_inff() ? m_run : m_run * c2, l};
+  }
+}
+
+// Merges the pieces of cut units: the launch has the chunk kernel's workgroups, and of
+// a unit of p pieces each takes a p-th of the rows.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
+  constexpr int LR = D / 4;
+  const int lane = threadIdx.x & 63;
+  const int cls = (int)blockIdx.x % a.classes;
+  const ChunkCut cut(a, lane);
+  int place;
+  const int b = cut.find((int)blockIdx.x / a.classes, place);
+  if (b < 0) return;
+  const PagedSeq s = paged_seq(a, b, load_scalar);
+  const ChunkUnit unit = chunk_unit(a, cut, s, cls, place);
+  if (unit.pieces == 1) return;
+  const int ch = (int)threadIdx.x % LR;
+  const int rows = min(kChunkRows, s.n * a.group - unit.rb * kChunkRows);
+  const int r_end = rows * (unit.piece + 1) / unit.pieces;
+  for (int r = rows * unit.piece / unit.pieces + (int)threadIdx.x / LR; r < r_end; r += kThreads / LR) {
+    float m = -__builtin_inff(), l = 0.0f;
+    float4v x = (float4v)0.0f;
+    auto rec = [&](int i) -> int64_t {
+      return ((int64_t)blockIdx.x + (i - unit.piece) * a.classes) * kChunkRows + r;
+    };
+    for (int i = 0; i < unit.pieces; i += 8)
+      fold_partials<8>(
+          i, 1, unit.pieces, m, l, x, [&](int i) { return *(const v2f*)(a.part_ml + rec(i) * 2); },
+          [&](int i) { return *(const float4v*)(a.part_o + rec(i) * D + 4 * ch); });
+    store_row<BF16>(a, s, unit.hkv, unit.rb * kChunkRows + r, 4 * ch, m, l, x);
+  }
+}
+
+}  // namespace
+
+template <int D, bool BF16, bool FP8>
+void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream) {
+  hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+}
+
+}  // namespace fa

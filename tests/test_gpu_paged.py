@@ -15,18 +15,21 @@ FP16, BF16 = torch.float16, torch.bfloat16
 
 
 def attend(c, device, hq, seed=1, causal=True, scale=None, strided=False, one=None, **kw):
-    """Runs the call on a cache and checks O and LSE; returns them."""
+    """Runs the call on a cache, as the kernel for few and the one for many new tokens a
+    sequence take it, and checks O and LSE; returns the last."""
     g = torch.Generator().manual_seed(seed)
     t = sum(c.news)
     q = torch.randn(t, hq, c.d, generator=g).to(c.dtype)
     args, scales = c.args(device, strided)
     one = all(n == 1 for n in c.news) if one is None else one
-    o, lse = fa.flash_attention_paged(q.to(device), *args, cu_seqlens=None if one else c.cu.to(device),
-                                      causal="bottom_right" if causal else False, scale=scale,
-                                      return_lse=True, **scales, **kw)
     want, want_lse, tol, lse_tol = ref.attention(c, q, causal, scale)
-    ref.check(o, want, tol, "O")
-    ref.check(lse, want_lse, lse_tol, "LSE")
+    hints = [kw.pop("max_query_len")] if "max_query_len" in kw else [None] if one else [1, 10 ** 6]
+    for hint in hints:
+        o, lse = fa.flash_attention_paged(q.to(device), *args, cu_seqlens=None if one else c.cu.to(device),
+                                          causal="bottom_right" if causal else False, scale=scale,
+                                          return_lse=True, max_query_len=hint, **scales, **kw)
+        ref.check(o, want, tol, f"O (max_query_len={hint})")
+        ref.check(lse, want_lse, lse_tol, f"LSE (max_query_len={hint})")
     return o, lse
 
 
@@ -73,10 +76,20 @@ def test_more_new_tokens_than_keys(device):
 def test_long(device, page, q8):
     """Keys split over many workgroups, one long sequence among short ones."""
     attend(Cache([9000, 3, 2500, 64], 2, 128, page, BF16, q8), device, 8)
+    attend(Cache([5000, 3, 1500, 64], 2, 128, page, BF16, q8, news=[40, 2, 1, 64]), device, 8)
 
 
 def test_one_long_sequence_few_heads(device):
     attend(Cache([20011], 1, 64, 16, FP16, True), device, 7)
+    attend(Cache([20011], 1, 64, 16, FP16, True, news=[19]), device, 7)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q8", [False, True])
+def test_many_blocks(device, d, q8):
+    """More units than the GPU runs at once (none is cut), and one batch of few and of many."""
+    attend(Cache([700, 650, 300], 8, d, 64, BF16, q8, news=[700, 1, 300]), device, 32, max_query_len=700)
+    attend(Cache([1500, 65], 1, d, 32, FP16, q8, news=[190, 65]), device, 2, max_query_len=190)
 
 
 @pytest.mark.parametrize("q8", [False, True])
