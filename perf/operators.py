@@ -26,14 +26,14 @@ TOP = {"fp16": 7, "bf16": 119}
 
 
 def _fa():
-    """The package, imported where its calls are the ones that run."""
-    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                       "flash-attention-sm75-register-fused_amd", "src")
-    if src not in sys.path:
-        sys.path.insert(0, src)
-    import flash_attention_sm75
+    """The package, imported once, where its calls are the ones that run."""
+    if not hasattr(_fa, "package"):
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                                        "flash-attention-sm75-register-fused_amd", "src"))
+        import flash_attention_sm75
 
-    return flash_attention_sm75
+        _fa.package = flash_attention_sm75
+    return _fa.package
 
 
 def _case(name, op, dtype, q8, b, hq, hkv, d, page, lo, hi, n, new="all", gone=False, lse=False):
