@@ -107,6 +107,11 @@ __device__ __forceinline__ int load_scalar(const int32_t* p) { return *(cint32*)
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return max(lo, min(x, hi)); }
 
+// A value that is the same in every lane, in a scalar register: a clamp is done in
+// vector ones (v_med3), and a buffer window made of it would be taken for a
+// different one in each lane, its loads for a loop over them.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // One sequence: its rows [t0, t0 + n) of the new tokens, its length with them
 // and the keys its pages can hold of it.
 struct PagedSeq {
@@ -125,6 +130,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load lo
   s.len = max(0, load(a.lens + b));
   s.keys = min(s.len, a.max_pages << a.page_shift);
   return s;
+}
+// (b the same in every lane; all of it in scalar registers)
+__device__ __forceinline__ PagedSeq scalar_seq(const PagedArgs& a, int b) {
+  const PagedSeq s = paged_seq(a, uniform(b), load_scalar);
+  return {uniform(s.t0), uniform(s.n), uniform(s.len), uniform(s.keys)};
 }
 
 // The factor an e8m0 scale stands for (127: 1).  Only its exponent is used.

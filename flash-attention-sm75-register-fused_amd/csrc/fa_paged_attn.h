@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
   const int r0 = 4 * g4 + (l16 >> 2);
 
   while (pos < end) {
-    const PagedSeq s = paged_seq(a, b, load_scalar);
+    const PagedSeq s = scalar_seq(a, b);
     const int blocks = paged_blocks<R>(a, s);
     const int line_tiles = paged_tiles(a, s);
     const int64_t len = (int64_t)line.heads * blocks * line_tiles;
@@ -279,8 +279,10 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     // Keys no row of the block sees are not read (past `sees`); tiles up to `full`
     // hide nothing from any of them.
     const int last_row = min(nrows, (rb + 1) * R) - 1;
-    const int sees = a.causal ? clamp_int(s.len - s.n + last_row / a.group + 1, 0, s.keys) : s.keys;
-    const int full = a.causal ? clamp_int(s.len - s.n + rb * R / a.group + 1, 0, s.keys) : s.keys;
+    const int sees =
+        a.causal ? uniform(clamp_int(s.len - s.n + last_row / a.group + 1, 0, s.keys)) : s.keys;
+    const int full =
+        a.causal ? uniform(clamp_int(s.len - s.n + rb * R / a.group + 1, 0, s.keys)) : s.keys;
     const int t_stop = min(t_end, (sees + kPTile - 1) / kPTile);
 
     float4v o[NT][MT];
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
       for (int p = 0; p < 2; ++p) {
         const int key = t * kPTile + 16 * p;
         const bool paged = e[p] >= 0 && e[p] < a.num_pages;
-        x.rows[p] = paged && t < t_stop ? clamp_int(sees - key, 0, 16) : 0;
+        x.rows[p] = uniform(paged && t < t_stop ? clamp_int(sees - key, 0, 16) : 0);
         const int64_t page = paged ? e[p] : 0;
         const int off = key & ((1 << a.page_shift) - 1);
         const __amdgpu_buffer_rsrc_t rk = make_rsrc(kh + page * a.kp + off * a.kn, x.rows[p] * (int)a.kn);
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   if (index >= units.total()) return;
   int64_t unit_start;
   const int b = units.find(index, unit_start);
-  const PagedSeq s = paged_seq(a, b, load_scalar);
+  const PagedSeq s = scalar_seq(a, b);
   const int tiles = paged_tiles(a, s);
   const int unit = (int)(index - unit_start);
   const int64_t u0 = line.start_of(b) + (int64_t)unit * tiles;

@@ -48,7 +48,7 @@ __device__ __forceinline__ PagedSeq lane_seq(const PagedArgs& a, int b) {
 __device__ __forceinline__ int64_t wave_sum(int64_t x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
+  return wave_bcast(x, 0);  // the same in every lane, and known to be
 }
 
 // How a class's units are cut: each sequence's into ceil(tiles / len) pieces.  Called
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   int place;
   const int b = __builtin_amdgcn_readfirstlane(cut.find((int)blockIdx.x / a.classes, place));
   if (b < 0) return;
-  const PagedSeq s = paged_seq(a, b, load_scalar);
+  const PagedSeq s = scalar_seq(a, b);
   const ChunkUnit unit = chunk_unit(a, cut, s, cls, __builtin_amdgcn_readfirstlane(place));
   const int hkv = unit.hkv;
   const int nrows = s.n * a.group;
@@ -203,15 +203,16 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 
   // Keys the block's rows see, and this piece's tiles of them.
   const int last_tok = (min(nrows, q0 + kChunkRows) - 1) / a.group;
-  const int kv_len = a.causal ? clamp_int(past + last_tok + 1, 0, s.keys) : s.keys;
+  const int kv_len = a.causal ? uniform(clamp_int(past + last_tok + 1, 0, s.keys)) : s.keys;
   const int block_tiles = (kv_len + kBlockN - 1) / kBlockN;
-  const int tile0 = (int)((int64_t)block_tiles * unit.piece / unit.pieces);
-  const int tile_end = (int)((int64_t)block_tiles * (unit.piece + 1) / unit.pieces);
+  const int tile0 = unit.piece * (block_tiles / unit.pieces) + min(unit.piece, block_tiles % unit.pieces);
+  const int tile_end = tile0 + block_tiles / unit.pieces + (unit.piece < block_tiles % unit.pieces ? 1 : 0);
   // The last key this lane's row sees; keys below wave_full are seen by every row of
   // the wave.
   const int tok = min(row, nrows - 1) / a.group;
   const int last_key = a.causal ? min(s.keys - 1, past + tok) : s.keys - 1;
-  const int wave_full = a.causal ? clamp_int(past + min(qw, nrows - 1) / a.group + 1, 0, s.keys) : s.keys;
+  const int wave_full =
+      a.causal ? uniform(clamp_int(past + min(qw, nrows - 1) / a.group + 1, 0, s.keys)) : s.keys;
 
   // Q^T fragments (B operand of S^T), resident for the whole kernel.
   half8 qf[KK];
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const uint8_t* const vh = a.v + hkv * a.vh;
   // Window of this wave's rows of tile j (empty past the piece's keys).
   auto rows_of = [&](int j, int page) -> int {
-    return page >= 0 && j < tile_end ? clamp_int(kv_len - (j * kBlockN + 16 * wave), 0, 16) : 0;
+    return uniform(page >= 0 && j < tile_end ? clamp_int(kv_len - (j * kBlockN + 16 * wave), 0, 16) : 0);
   };
   auto window = [&](const uint8_t* base, int64_t sp, int64_t sn, int j, int page) {
     const int off = (j * kBlockN + 16 * wave) & ((1 << a.page_shift) - 1);
@@ -637,7 +638,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   int place;
   const int b = cut.find((int)blockIdx.x / a.classes, place);
   if (b < 0) return;
-  const PagedSeq s = paged_seq(a, b, load_scalar);
+  const PagedSeq s = scalar_seq(a, b);
   const ChunkUnit unit = chunk_unit(a, cut, s, cls, place);
   if (unit.pieces == 1) return;
   const int ch = (int)threadIdx.x % LR;
