@@ -25,6 +25,12 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
 }
 }  // namespace
 
+// Whether a line of `units` units stays below 2^31 tiles.
+static bool fits_line(const PagedArgs& a, int64_t units, int tile) {
+  const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + tile - 1) / tile;
+  return units * std::max<int64_t>(1, tiles) <= INT32_MAX;
+}
+
 // Units of 128 rows, cut into pieces where they may be fewer than the GPU runs at once.
 static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace_bytes) {
   PagedPlan p{};
@@ -35,11 +41,12 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace
   const int64_t heads = a.hkv / p.classes, rows = (int64_t)a.tokens * a.group;
   const int64_t least = heads * ((rows + p.rows - 1) / p.rows);
   p.units = (int)(heads * ((rows + (p.rows - 1ll) * std::min(a.batch, a.tokens)) / p.rows));
-  const int64_t record = (int64_t)p.rows * (head_dim + 2) * (int64_t)sizeof(float) * p.classes;
-  const int64_t wgs = resident_fused_workgroups() / p.classes;
-  p.split = least < wgs && std::max<int64_t>(wgs, p.units) <= workspace_bytes / record;
+  const int64_t record = 2ll * p.rows * (head_dim + 2) * (int64_t)sizeof(float) * p.classes;
+  const int64_t wgs = std::min<int64_t>(p.resident = resident_fused_workgroups() / p.classes,
+                                        workspace_bytes / record);
+  p.split = least < wgs && fits_line(a, p.units, kBlockN);
   p.combine = p.split;
-  p.wgs = p.split ? (int)std::max<int64_t>(wgs, p.units) : p.units;
+  p.wgs = p.split ? (int)wgs : p.units;
   p.workspace_bytes = p.split ? p.wgs * record : 0;
   return p;
 }
@@ -54,12 +61,12 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
       resident_fused_workgroups() / 2 * paged_per_cu(head_dim, a.ks != nullptr, p.rows / 16);
   const int64_t room = workspace_bytes / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
-  p.split = p.wgs > 0;
   // Units of a class: blocks of rows, the last of each sequence not full.
   const int64_t blocks =
       a.cu == nullptr ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
                       : (int64_t)a.tokens * a.group / p.rows + std::min(a.batch, a.tokens);
   p.units = (int)(a.hkv / p.classes * blocks);
+  p.split = p.wgs > 0 && fits_line(a, p.units, kPTile);
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) : 0;
@@ -92,11 +99,12 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   a.classes = plan.classes;
   a.wgs = plan.wgs;
   a.units = plan.units;
+  a.resident = plan.resident;
   a.split = plan.split ? 1 : 0;
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
   if (plan.split && plan.chunk) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + grid * plan.rows * head_dim;
+    a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
   } else if (plan.split) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;

@@ -45,123 +45,11 @@ namespace {
 constexpr int kPTile = 32;       // keys of a wave's tile
 constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below
 
-// 32-key tiles of each of a sequence's units on the line: at least one, so that a
-// sequence without keys has its rows written.
-__device__ __forceinline__ int paged_tiles(const PagedArgs& a, const PagedSeq& s) {
-  return a.split ? max(1, (s.keys + kPTile - 1) / kPTile) : 1;
-}
-
-// Walks a class's line: total length, and the sequence that holds a position.
-// Called by whole waves; every lane gets the same answers.  The first 64
-// sequences are looked at once.
-template <int R>
-struct PagedLine {
-  const PagedArgs& a;
-  int lane;
-  int heads;  // KV heads of the class
-  bool by_tiles;  // or by units
-  int64_t first;  // prefix(0)
-  __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln, bool tiles = true)
-      : a(args), lane(ln), by_tiles(tiles) {
-    heads = args.hkv / args.classes;
-    first = prefix(0);
-  }
-  __device__ __forceinline__ int64_t length_of(const PagedSeq& s) const {
-    return (int64_t)heads * paged_blocks<R>(a, s) * (by_tiles ? paged_tiles(a, s) : 1);
-  }
-  // Inclusive prefix sum over the wave's lanes of sequence b0 + lane's length.
-  __device__ __forceinline__ int64_t prefix(int b0) const {
-    int64_t x = 0;
-    if (b0 + lane < a.batch) x = length_of(paged_seq(a, b0 + lane, [](const int32_t* p) { return *p; }));
-    const int n = min(64, a.batch - b0);
-    for (int d = 1; d < n; d <<= 1) {
-      const int64_t y = __shfl_up(x, d);
-      if (lane >= d) x += y;
-    }
-    return wave_bcast_last(x, n);
-  }
-  // (lanes past the last sequence hold the sum too)
-  __device__ __forceinline__ int64_t wave_bcast_last(int64_t x, int n) const {
-    const int64_t all = wave_bcast(x, n - 1);
-    return lane < n ? x : all;
-  }
-  __device__ __forceinline__ int64_t total() const {
-    int64_t sum = wave_bcast(first, 63);
-    for (int b0 = 64; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
-    return sum;
-  }
-  // Where sequence b starts.
-  __device__ __forceinline__ int64_t start_of(int b) const {
-    int64_t before = 0;
-    for (int b0 = 0;; b0 += 64) {
-      const int64_t x = b0 == 0 ? first : prefix(b0);
-      if (b < b0 + 64) return b == b0 ? before : before + wave_bcast(x, b - b0 - 1);
-      before += wave_bcast(x, 63);
-    }
-  }
-  // The sequence b that holds position pos (0 <= pos < total), and where it starts.
-  __device__ __forceinline__ int find(int64_t pos, int64_t& start) const {
-    int64_t before = 0;
-    for (int b0 = 0;; b0 += 64) {
-      const int64_t x = b0 == 0 ? first : prefix(b0);
-      const int64_t end = wave_bcast(x, 63);
-      if (pos < before + end || b0 + 64 >= a.batch) {
-        const uint64_t past = __builtin_amdgcn_ballot_w64(before + x > pos);
-        const int l = past != 0 ? __builtin_ctzll(past) : 63;
-        start = l > 0 ? before + wave_bcast(x, l - 1) : before;
-        return min(b0 + l, a.batch - 1);
-      }
-      before += end;
-    }
-  }
-};
-
-// Workgroups that share a class's line: all of them, unless stretches would
-// fall below kPMinTiles.
-__device__ __forceinline__ int paged_active(const PagedArgs& a, int64_t total) {
-  if (!a.split) return (int)min((int64_t)a.wgs, total);
-  return (int)min((int64_t)a.wgs, (total + kPMinTiles - 1) / kPMinTiles);
-}
-
 // Workgroups of a CU at once: what their V tiles leave room for in 160 KB of LDS,
 // and their registers among 512 of a lane.
 __host__ __device__ constexpr int paged_per_cu(int d, bool fp8, int nt) {
   return fp8 && nt == 1 ? (d == 64 ? 4 : 3) : d == 64 ? 3 : 2;
 }
-
-// The stretches of a class's line: of total / active tiles, the first ones a
-// tile longer.
-struct PagedStretch {
-  int64_t size;
-  int active, longer;
-  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int64_t total) {
-    active = paged_active(a, total);
-    size = 0;
-    longer = 0;
-    if (active > 0) {
-      size = total / active;
-      longer = (int)(total - size * active);
-    }
-  }
-  __device__ __forceinline__ int64_t start(int wg) const { return wg * size + min(wg, longer); }
-  __device__ __forceinline__ int holder(int64_t pos) const {  // the workgroup of a position
-    const int64_t p = pos - longer * (size + 1);
-    return (int)(p < 0 ? pos / (size + 1) : longer + p / size);
-  }
-};
-
-// The workgroups a unit on [u0, u1) of the line was cut into: from first on, each
-// with its record number slot(i) of the workspace.
-struct PagedPieces {
-  int first, count;
-  __device__ __forceinline__ PagedPieces(const PagedStretch& st, int64_t u0, int64_t u1) {
-    first = st.holder(u0);
-    count = st.holder(u1 - 1) - first + 1;
-  }
-  __device__ __forceinline__ int slot(const PagedArgs& a, int cls, int i) const {
-    return 2 * ((first + i) * a.classes + cls) + (i == 0 ? 1 : 0);
-  }
-};
 
 // Whether a unit's last workgroup merges its partials: one workgroup reads them
 // at about 50 bytes/ns.
@@ -207,13 +95,13 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
   const int cls = (int)blockIdx.x % a.classes;
   const int wg = (int)blockIdx.x / a.classes;
 
-  const PagedLine<R> line(a, lane);
-  const PagedStretch stretch(a, line.total());
+  const PagedLine<R, kPTile> line(a, lane, a.split != 0);
+  const PagedStretch stretch(a, line.total(), a.split ? kPMinTiles : 1);
   if (wg >= stretch.active) return;
-  int64_t pos = stretch.start(wg);
-  const int64_t end = stretch.start(wg + 1);
-  int64_t seq_start;
-  int b = line.find(pos, seq_start);
+  int pos = stretch.start(wg);
+  const int end = stretch.start(wg + 1);
+  int seq_start;
+  int b = uniform(line.find(pos, seq_start));
 
   auto swz = [](int r) { return D == 128 ? (r & 7) : ((r >> 1) & 3); };
   _Float16* const vt0 = v_lds0 + wave * VT;
@@ -236,18 +124,18 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
   const int r0 = 4 * g4 + (l16 >> 2);
 
   while (pos < end) {
-    const PagedSeq s = scalar_seq(a, b);
+    const PagedSeq s = line.seq(b);
     const int blocks = paged_blocks<R>(a, s);
-    const int line_tiles = paged_tiles(a, s);
-    const int64_t len = (int64_t)line.heads * blocks * line_tiles;
+    const int line_tiles = line.tiles_of(s);
+    const int len = line.length_of(s);
     if (pos >= seq_start + len) {  // on to the next sequence
       seq_start += len;
       if (++b >= a.batch) return;
       continue;
     }
-    const int unit = (int)((pos - seq_start) / line_tiles);
-    const int first = (int)(pos - seq_start - (int64_t)unit * line_tiles);  // on the line
-    const int here = (int)min((int64_t)(line_tiles - first), end - pos);
+    const int unit = (pos - seq_start) / line_tiles;
+    const int first = pos - seq_start - unit * line_tiles;  // on the line
+    const int here = min(line_tiles - first, end - pos);
     const int hc = unit / blocks;
     const int rb = unit - hc * blocks;
     const int hkv = hc * a.classes + cls;
@@ -539,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     // A workgroup's partials are acknowledged before it sets its flag, and its flag
     // before it reads the others': the last flag to be set is set by a workgroup
     // that sees them all.  Two that both do store the same values.
-    const int64_t u0 = seq_start + (int64_t)unit * line_tiles;
+    const int u0 = seq_start + unit * line_tiles;
     const PagedPieces pieces(stretch, u0, u0 + line_tiles);
     const int nr = min(R, nrows - rb * R);
     if (!paged_merges_itself(pieces.count, nr, D)) {
@@ -624,17 +512,16 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   __shared__ float xm[2][kThreads];
   const int cls = (int)blockIdx.x % a.classes;
   const int index = (int)blockIdx.x / a.classes;  // of the class's units
-  const PagedLine<R> line(a, threadIdx.x & 63);
-  const int64_t total = line.total();
-  const PagedLine<R> units(a, threadIdx.x & 63, false);
+  const PagedLine<R, kPTile> line(a, threadIdx.x & 63, true);
+  const PagedLine<R, kPTile> units(a, threadIdx.x & 63, false);
   if (index >= units.total()) return;
-  int64_t unit_start;
-  const int b = units.find(index, unit_start);
-  const PagedSeq s = scalar_seq(a, b);
-  const int tiles = paged_tiles(a, s);
-  const int unit = (int)(index - unit_start);
-  const int64_t u0 = line.start_of(b) + (int64_t)unit * tiles;
-  const PagedStretch stretch(a, total);
+  int unit_start;
+  const int b = uniform(units.find(index, unit_start));
+  const PagedSeq s = line.seq(b);
+  const int tiles = line.tiles_of(s);
+  const int unit = index - unit_start;
+  const int u0 = line.start_of(b) + unit * tiles;
+  const PagedStretch stretch(a, line.total(), kPMinTiles);
   const PagedPieces pieces(stretch, u0, u0 + tiles);
   if (pieces.count == 1) return;
   const int blocks = paged_blocks<R>(a, s);

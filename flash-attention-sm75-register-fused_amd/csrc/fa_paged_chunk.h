@@ -20,10 +20,12 @@
 // workgroup (the codes times a power of two are 16-bit numbers) and writes them to LDS
 // in the layout the 16-bit rows arrive in.
 //
-// The plan.  Where there are fewer units than fill the GPU, each sequence's units are cut
-// into pieces of about equally many tiles, as short as lets all of them run at once;
-// the pieces' partials (O, max, sum) are merged by a second kernel.  Every workgroup
-// derives the cut from the lengths (ChunkCut).
+// The plan.  Where the units do not fill the GPU (SPLIT), each workgroup takes an equal
+// stretch of the class's line of 64-key tiles, as in the kernel for few columns; the
+// partials of units that stretches cut are merged by a second kernel.  Else a
+// workgroup takes a unit, each head's from its last block (under the causal rule the
+// longest) to its first; where all of them run at once, two a CU, the second half
+// of them in reverse, so that a CU gets a long and a short one.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -35,128 +37,9 @@ namespace fa {
 namespace {
 
 constexpr int kChunkRows = 128;
-constexpr int kChunkMinTiles = 4;  // tiles a piece is not cut below
+constexpr int kChunkMinTiles = 4;  // tiles a stretch is not cut below
 
-// Rows a sequence's blocks and 64-key tiles.
-__device__ __forceinline__ int chunk_tiles(int keys) { return max(1, (keys + kBlockN - 1) / kBlockN); }
-
-__device__ __forceinline__ PagedSeq lane_seq(const PagedArgs& a, int b) {
-  if (b < a.batch) return paged_seq(a, b, [](const int32_t* p) { return *p; });
-  return PagedSeq{0, 0, 0, 0};
-}
-
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return wave_bcast(x, 0);  // the same in every lane, and known to be
-}
-
-// How a class's units are cut: each sequence's into ceil(tiles / len) pieces.  Called
-// by whole waves; the first 64 sequences (one a lane) are looked at once.
-struct ChunkCut {
-  const PagedArgs& a;
-  int lane, heads;
-  int units, tiles;  // of sequence `lane`: units, and the tiles of one
-  int len;
-
-  __device__ __forceinline__ void look(int b0, int& u, int& t) const {
-    if (b0 == 0) {
-      u = units;
-      t = tiles;
-      return;
-    }
-    const PagedSeq s = lane_seq(a, b0 + lane);
-    u = heads * paged_blocks<kChunkRows>(a, s);
-    t = chunk_tiles(s.keys);
-  }
-  __device__ __forceinline__ int pieces(int t) const { return len > 0 ? (t + len - 1) / len : 1; }
-  __device__ __forceinline__ int64_t items(int by) const {  // cut into pieces of `by` tiles
-    int64_t sum = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      int u, t;
-      look(b0, u, t);
-      sum += (int64_t)u * ((t + by - 1) / by);
-    }
-    return wave_sum(sum);
-  }
-
-  // The cut: the least of a few lengths from total / slots on with which all pieces
-  // run at once, total / (slots - units) being one of them; none where the units
-  // alone fill the GPU.
-  __device__ __forceinline__ ChunkCut(const PagedArgs& args, int ln) : a(args), lane(ln) {
-    heads = a.hkv / a.classes;
-    const PagedSeq s = lane_seq(a, lane);
-    units = heads * paged_blocks<kChunkRows>(a, s);
-    tiles = chunk_tiles(s.keys);
-    len = 0;
-    if (!a.split) return;
-    int64_t all_units = 0, total = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      int u, t;
-      look(b0, u, t);
-      all_units += u;
-      total += (int64_t)u * t;
-    }
-    all_units = wave_sum(all_units);
-    total = wave_sum(total);
-    const int64_t room = a.wgs - all_units;
-    if (room <= 0) return;
-    const int64_t sure = (total + room - 1) / room, even = (total + a.wgs - 1) / a.wgs;
-    int64_t best = sure;
-    for (int k = 0; k < 5; ++k) {
-      const int64_t by = even + even * k / 8;
-      if (by >= sure) break;
-      if (items((int)by) <= a.wgs) {
-        best = by;
-        break;
-      }
-    }
-    len = __builtin_amdgcn_readfirstlane((int)max(best, (int64_t)kChunkMinTiles));
-  }
-
-  // Item `index` of the class: its sequence (-1: none), and its place there.
-  __device__ __forceinline__ int find(int64_t index, int& place) const {
-    int64_t before = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      int u, t;
-      look(b0, u, t);
-      int64_t x = (int64_t)u * pieces(t);
-      const int n = min(64, a.batch - b0);
-      for (int d = 1; d < n; d <<= 1) {
-        const int64_t y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-      }
-      const uint64_t past = __builtin_amdgcn_ballot_w64(lane < n && before + x > index);
-      if (past != 0) {
-        const int l = __builtin_ctzll(past);
-        place = (int)(index - (l > 0 ? before + wave_bcast(x, l - 1) : before));
-        return b0 + l;
-      }
-      before += wave_bcast(x, n - 1);
-    }
-    return -1;
-  }
-};
-
-// A unit of a sequence from its place: heads one after the other, blocks of a head
-// from the last (under the causal rule the longest) to the first.
-struct ChunkUnit {
-  int hkv, rb, piece, pieces;
-};
-__device__ __forceinline__ ChunkUnit chunk_unit(const PagedArgs& a, const ChunkCut& cut, const PagedSeq& s,
-                                                int cls, int place) {
-  ChunkUnit u;
-  const int blocks = paged_blocks<kChunkRows>(a, s);
-  u.pieces = cut.pieces(chunk_tiles(s.keys));
-  const int unit = place / u.pieces;
-  u.piece = place - unit * u.pieces;
-  const int hc = unit / blocks;
-  u.rb = blocks - 1 - (unit - hc * blocks);
-  u.hkv = hc * a.classes + cls;
-  return u;
-}
-
-template <int D, bool BF16, bool FP8>
+template <int D, bool BF16, bool FP8, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
   constexpr bool DENSE = D == 64;
   using L = std::conditional_t<DENSE, LdsDense<D>, Lds<D>>;
@@ -181,32 +64,59 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   __shared__ __attribute__((aligned(1024))) _Float16 v_lds1[L::Tile];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  const int cls = (int)blockIdx.x % a.classes;
+  const int wg = (int)blockIdx.x / a.classes;
+  const PagedLine<kChunkRows, kBlockN> line(a, threadIdx.x & 63, SPLIT);
+  const int total = line.total();
+  const PagedStretch stretch(a, total, SPLIT ? kChunkMinTiles : 1);
+  if (wg >= stretch.active) return;
+  int pos = stretch.start(wg);
+  const int end = stretch.start(wg + 1);
+  if constexpr (!SPLIT) {
+    if (a.causal && total <= a.resident && pos >= a.resident / 2) pos = total - 1 + a.resident / 2 - pos;
+  }
+  int seq_start;
+  int b = uniform(line.find(pos, seq_start));
+
+  do {
+  const PagedSeq s = line.seq(b);
+  const int blocks = paged_blocks<kChunkRows>(a, s);
+  const int line_tiles = line.tiles_of(s);
+  const int len = line.length_of(s);
+  if (pos >= seq_start + len) {  // on to the next sequence
+    seq_start += len;
+    if (++b >= a.batch) return;
+    continue;
+  }
+  const int unit = (pos - seq_start) / line_tiles;
+  const int first = pos - seq_start - unit * line_tiles;  // on the line
+  const int here = SPLIT ? min(line_tiles - first, end - pos) : 1;
+  const bool whole = !SPLIT || here == line_tiles;
+  pos += here;
+  const int hc = unit / blocks;
+  const int rb = blocks - 1 - (unit - hc * blocks);
+  const int hkv = hc * a.classes + cls;
+
+  // What depends on the lane is derived for each segment from an opaque lane index, so
+  // that none of it is kept in registers from one to the next.
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
   const int hi = lane >> 5;   // which half of the wave
   const int ql = lane & 31;   // query column owned by this lane
   const int grp = lane >> 4;  // 16-lane group (transposing reads)
   const int gi = lane & 15;
-  const int cls = (int)blockIdx.x % a.classes;
-
-  const ChunkCut cut(a, lane);
-  int place;
-  const int b = __builtin_amdgcn_readfirstlane(cut.find((int)blockIdx.x / a.classes, place));
-  if (b < 0) return;
-  const PagedSeq s = scalar_seq(a, b);
-  const ChunkUnit unit = chunk_unit(a, cut, s, cls, __builtin_amdgcn_readfirstlane(place));
-  const int hkv = unit.hkv;
   const int nrows = s.n * a.group;
-  const int q0 = unit.rb * kChunkRows;
+  const int q0 = rb * kChunkRows;
   const int qw = q0 + 32 * wave;
   const int row = qw + ql;
   const int past = s.len - s.n;  // tokens before the new ones
 
-  // Keys the block's rows see, and this piece's tiles of them.
+  // Keys the block's rows see, and this segment's tiles of them.
   const int last_tok = (min(nrows, q0 + kChunkRows) - 1) / a.group;
   const int kv_len = a.causal ? uniform(clamp_int(past + last_tok + 1, 0, s.keys)) : s.keys;
   const int block_tiles = (kv_len + kBlockN - 1) / kBlockN;
-  const int tile0 = unit.piece * (block_tiles / unit.pieces) + min(unit.piece, block_tiles % unit.pieces);
-  const int tile_end = tile0 + block_tiles / unit.pieces + (unit.piece < block_tiles % unit.pieces ? 1 : 0);
+  const int tile0 = SPLIT ? first : 0;
+  const int tile_end = SPLIT ? min(block_tiles, first + here) : block_tiles;
   // The last key this lane's row sees; keys below wave_full are seen by every row of
   // the wave.
   const int tok = min(row, nrows - 1) / a.group;
@@ -566,6 +476,39 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       for (int i = 0; i < SEGQ; ++i) direct_load16(rv0, lds_seg(v_lds0, i), voff[i]);
       barrier_after_loads<2 * SEGQ>();  // S_0 needs K_0 only
     }
+    if (qw >= nrows) {
+      // A wave without rows (a short block: a single token's heads) brings its share
+      // of the tiles and meets the barriers.
+      barrier_after_loads<FP8 ? 63 : 0>();
+      for (int j = tile0; j + 1 < tile_end; ++j) {
+        const Pages now1 = pg1, now2 = pg2;
+        pg1 = pg2;
+        pg2 = pages_of(ahead);
+        look_up(j + 4, ahead);
+        const bool odd = (j - tile0) & 1;
+        _Float16* const k_dst = odd ? k_lds1 : k_lds0;
+        _Float16* const v_dst = odd ? v_lds0 : v_lds1;
+        if constexpr (FP8) {
+          static_for<LQ>([&](auto i_c) {
+            constexpr int i = decltype(i_c)::value;
+            static_for<2>([&](auto h_c) {
+              store_codes(k_dst, kr[i], ksr[i], i, decltype(h_c)::value);
+              store_codes(v_dst, vr[i], vsr[i], i, decltype(h_c)::value);
+            });
+          });
+          load_k8(j + 3, pg2.own);
+          load_v8(j + 2, pg1.own);
+        } else {
+          const __amdgpu_buffer_rsrc_t rk = window(kh, a.kp, a.kn, j + 2, now2.own);
+          const __amdgpu_buffer_rsrc_t rv = window(vh, a.vp, a.vn, j + 1, now1.own);
+#pragma unroll
+          for (int i = 0; i < SEGQ; ++i) direct_load16(rk, lds_seg(k_dst, i), koff[i]);
+#pragma unroll
+          for (int i = 0; i < SEGQ; ++i) direct_load16(rv, lds_seg(v_dst, i), voff[i]);
+        }
+        barrier_after_loads<FP8 ? 63 : 0>();
+      }
+    } else {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s_buf[0][t] = (float16v)0.0f;
@@ -592,69 +535,80 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       step(j, Flag<true>{}, I0{});
       step(j + 1, Flag<false>{}, I1{});
     }
+    }
   }
-  // No direct load may land in LDS after the workgroup ends.
+  // No direct load may land in LDS after the workgroup, or the segment, ends.
   __builtin_amdgcn_s_waitcnt(0x0F70);
 
   const float l = halves_sum(l_run);
-  if (row >= nrows) return;
-  if (unit.pieces == 1) {
-    const PagedRow pr = paged_row(a, s, hkv, row);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+  const float m2 = m_run == -__builtin_inff() ? m_run : m_run * c2;
+  if (row < nrows) {
+    if (whole) {
+      const PagedRow pr = paged_row(a, s, hkv, row);
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        half4 v;
+        for (int g = 0; g < 4; ++g) {
+          half4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = E::round(oacc[mt][4 * g + e] * inv);
-        *(half4*)(op + 32 * mt + 8 * g + 4 * hi) = v;
-      }
-    if (a.lse != nullptr && hi == 0)
-      a.lse[(int64_t)pr.head * a.tokens + pr.token] =
-          natural_lse(m_run == -__builtin_inff() ? m_run : m_run * c2, l);
-  } else {
-    const int64_t rec = (int64_t)blockIdx.x * kChunkRows + (row - q0);
+          for (int e = 0; e < 4; ++e) v[e] = E::round(oacc[mt][4 * g + e] * inv);
+          *(half4*)(op + 32 * mt + 8 * g + 4 * hi) = v;
+        }
+      if (a.lse != nullptr && hi == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+    } else {
+      const int64_t rec = (2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0)) * kChunkRows + (row - q0);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *(float4v*)(a.part_o + rec * D + 32 * mt + 8 * g + 4 * hi) =
-            float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
-    if (hi == 0)
-      *(v2f*)(a.part_ml + rec * 2) = v2f{m_run == -__builtin_inff() ? m_run : m_run * c2, l};
+        for (int g = 0; g < 4; ++g)
+          *(float4v*)(a.part_o + rec * D + 32 * mt + 8 * g + 4 * hi) =
+              float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
+      if (hi == 0) *(v2f*)(a.part_ml + rec * 2) = v2f{m2, l};
+    }
   }
+  if constexpr (SPLIT) __syncthreads();  // the next segment's loads go into these tiles
+  } while (SPLIT && pos < end);
 }
 
-// Merges the pieces of cut units: the launch has the chunk kernel's workgroups, and of
-// a unit of p pieces each takes a p-th of the rows.
+// Merges the partials of units that stretches cut.  The workgroup of a border between
+// two stretches looks at the unit it lies in: of the unit's p - 1 borders each takes a
+// share of the rows, D / 4 lanes a row.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
   constexpr int LR = D / 4;
-  const int lane = threadIdx.x & 63;
   const int cls = (int)blockIdx.x % a.classes;
-  const ChunkCut cut(a, lane);
-  int place;
-  const int b = cut.find((int)blockIdx.x / a.classes, place);
-  if (b < 0) return;
-  const PagedSeq s = scalar_seq(a, b);
-  const ChunkUnit unit = chunk_unit(a, cut, s, cls, place);
-  if (unit.pieces == 1) return;
+  const int wg = (int)blockIdx.x / a.classes;
+  const PagedLine<kChunkRows, kBlockN> line(a, threadIdx.x & 63, true);
+  const PagedStretch stretch(a, line.total(), kChunkMinTiles);
+  if (wg == 0 || wg >= stretch.active) return;
+  const int border = stretch.start(wg);
+  int seq_start;
+  const int b = uniform(line.find(border, seq_start));
+  const PagedSeq s = line.seq(b);
+  const int tiles = line.tiles_of(s);
+  const int unit = (border - seq_start) / tiles;
+  const int u0 = seq_start + unit * tiles;
+  if (border == u0) return;
+  const PagedPieces pieces(stretch, u0, u0 + tiles);
+  const int blocks = paged_blocks<kChunkRows>(a, s);
+  const int hc = unit / blocks;
+  const int rb = blocks - 1 - (unit - hc * blocks);
+  const int hkv = hc * a.classes + cls;
   const int ch = (int)threadIdx.x % LR;
-  const int rows = min(kChunkRows, s.n * a.group - unit.rb * kChunkRows);
-  const int r_end = rows * (unit.piece + 1) / unit.pieces;
-  for (int r = rows * unit.piece / unit.pieces + (int)threadIdx.x / LR; r < r_end; r += kThreads / LR) {
+  const int rows = min(kChunkRows, s.n * a.group - rb * kChunkRows);
+  const int share = wg - pieces.first, shares = pieces.count - 1;  // from 1
+  const int r_end = rows * share / shares;
+  for (int r = rows * (share - 1) / shares + (int)threadIdx.x / LR; r < r_end; r += kThreads / LR) {
     float m = -__builtin_inff(), l = 0.0f;
     float4v x = (float4v)0.0f;
-    auto rec = [&](int i) -> int64_t {
-      return ((int64_t)blockIdx.x + (i - unit.piece) * a.classes) * kChunkRows + r;
-    };
-    for (int i = 0; i < unit.pieces; i += 8)
+    auto rec = [&](int i) -> int64_t { return (int64_t)pieces.slot(a, cls, i) * kChunkRows + r; };
+    for (int i = 0; i < pieces.count; i += 8)
       fold_partials<8>(
-          i, 1, unit.pieces, m, l, x, [&](int i) { return *(const v2f*)(a.part_ml + rec(i) * 2); },
+          i, 1, pieces.count, m, l, x, [&](int i) { return *(const v2f*)(a.part_ml + rec(i) * 2); },
           [&](int i) { return *(const float4v*)(a.part_o + rec(i) * D + 4 * ch); });
-    store_row<BF16>(a, s, unit.hkv, unit.rb * kChunkRows + r, 4 * ch, m, l, x);
+    store_row<BF16>(a, s, hkv, rb * kChunkRows + r, 4 * ch, m, l, x);
   }
 }
 
@@ -662,7 +616,9 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
 
 template <int D, bool BF16, bool FP8>
 void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream) {
-  hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  const dim3 g((unsigned)grid), t(kThreads);
+  if (a.split) hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true>), g, t, 0, stream, a);
+  else hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false>), g, t, 0, stream, a);
 }
 
 }  // namespace fa

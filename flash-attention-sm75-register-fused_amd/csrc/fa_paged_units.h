@@ -10,10 +10,19 @@
 namespace fa {
 namespace {
 
+// Lane `lane`'s value, the same in every lane.
 __device__ __forceinline__ int wave_bcast(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
-__device__ __forceinline__ int64_t wave_bcast(int64_t x, int lane) {
-  return (int64_t)(uint32_t)wave_bcast((int)x, lane) |
-         ((int64_t)wave_bcast((int)(x >> 32), lane) << 32);
+
+// Inclusive prefix sum over the wave's lanes: within rows of 16, then rows 0 and 2
+// into 1 and 3, then the lower half into the upper.
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
 }
 
 // Blocks of R rows of a sequence: its units for one KV head.
@@ -21,6 +30,100 @@ template <int R>
 __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& s) {
   return (int)(((int64_t)s.n * a.group + R - 1) / R);
 }
+
+// The line of a class of KV heads (every classes-th head): the units of its
+// sequences (blocks of R rows, for each head) end to end, each as long as its sequence
+// has tiles of T keys (one at least, so that the rows of a sequence without keys are
+// written too), or with tiles false of length one.  Below 2^31 in all (the launcher
+// sees to it).  Called by whole waves; the first 64 sequences, one a lane, are
+// looked at once.
+template <int R, int T>
+struct PagedLine {
+  const PagedArgs& a;
+  const int lane, heads;
+  const bool by_tiles;
+  PagedSeq own;  // sequence `lane`
+  int first;     // prefix(0)
+
+  __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln, bool tiles)
+      : a(args), lane(ln), heads(args.hkv / args.classes), by_tiles(tiles) {
+    own = look(lane);
+    first = wave_prefix(length_of(own));
+  }
+  __device__ __forceinline__ PagedSeq look(int b) const {
+    if (b < a.batch) return paged_seq(a, b, [](const int32_t* p) { return *p; });
+    return PagedSeq{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ int tiles_of(const PagedSeq& s) const {
+    return by_tiles ? max(1, (s.keys + T - 1) / T) : 1;
+  }
+  __device__ __forceinline__ int length_of(const PagedSeq& s) const {
+    return heads * paged_blocks<R>(a, s) * tiles_of(s);
+  }
+  // Inclusive prefix sum of the lengths of sequences b0 + lane.
+  __device__ __forceinline__ int prefix(int b0) const {
+    return b0 == 0 ? first : wave_prefix(length_of(look(b0 + lane)));
+  }
+  __device__ __forceinline__ int total() const {
+    int sum = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
+    return sum;
+  }
+  __device__ __forceinline__ PagedSeq seq(int b) const {
+    if (b >= 64) return scalar_seq(a, b);
+    return {wave_bcast(own.t0, b), wave_bcast(own.n, b), wave_bcast(own.len, b), wave_bcast(own.keys, b)};
+  }
+  // The sequence b that holds position pos (0 <= pos < total), and where it starts.
+  __device__ __forceinline__ int find(int pos, int& start) const {
+    int before = 0;
+    for (int b0 = 0;; b0 += 64) {
+      const int x = prefix(b0);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + x > pos);
+      if (past != 0 || b0 + 64 >= a.batch) {
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        start = l > 0 ? before + wave_bcast(x, l - 1) : before;
+        return min(b0 + l, a.batch - 1);
+      }
+      before += wave_bcast(x, 63);
+    }
+  }
+  // Where sequence b starts.
+  __device__ __forceinline__ int start_of(int b) const {
+    int before = 0;
+    for (int b0 = 0; b0 + 64 <= b; b0 += 64) before += wave_bcast(prefix(b0), 63);
+    return b % 64 == 0 ? before : before + wave_bcast(prefix(b / 64 * 64), b % 64 - 1);
+  }
+};
+
+// The stretches of a class's line, one for each workgroup of it: total / active tiles
+// long, the first ones a tile longer, and no shorter than `least` tiles.
+struct PagedStretch {
+  int size, active, longer;
+  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int total, int least) {
+    active = min(a.wgs, (total + least - 1) / least);
+    size = active > 0 ? total / active : 0;
+    longer = total - size * active;
+  }
+  __device__ __forceinline__ int start(int wg) const { return wg * size + min(wg, longer); }
+  __device__ __forceinline__ int holder(int pos) const {  // the workgroup of a position
+    const int p = pos - longer * (size + 1);
+    return p < 0 ? pos / (size + 1) : longer + p / size;
+  }
+};
+
+// The workgroups a unit on [u0, u1) of the line was cut into: from first on, each
+// with its record number slot(i) of the workspace.  A stretch starts inside at most one
+// unit that it does not start with, and ends inside at most one: two records.
+struct PagedPieces {
+  int first, count;
+  __device__ __forceinline__ PagedPieces(const PagedStretch& st, int u0, int u1) {
+    first = st.holder(u0);
+    count = st.holder(u1 - 1) - first + 1;
+  }
+  __device__ __forceinline__ int slot(const PagedArgs& a, int cls, int i) const {
+    return 2 * ((first + i) * a.classes + cls) + (i == 0 ? 1 : 0);
+  }
+};
 
 // Row r of a sequence's rows: the addresses of its Q, O and LSE.
 struct PagedRow {
