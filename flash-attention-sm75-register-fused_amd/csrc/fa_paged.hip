@@ -83,7 +83,7 @@ template <int D, bool BF16>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream) {
   if (rows == kChunkRows) {
     hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16>),
-                       dim3((unsigned)(a.wgs * a.classes)), dim3(kThreads), 0, stream, a);
+                       dim3((unsigned)(a.wgs * a.classes), kChunkCombineY), dim3(kThreads), 0, stream, a);
     return;
   }
   const dim3 g((unsigned)(a.units * a.classes), (unsigned)y);

@@ -144,26 +144,39 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     const int t_end = a.split ? first + here : (s.keys + kPTile - 1) / kPTile;
     pos += here;
 
-    // Columns of this lane, one for each nt, and the last key each sees.
+    // Columns of this lane, one for each nt: whether they hold a row, and the last
+    // key it sees.
     const int nrows = s.n * a.group;
+    const PagedRows row_of(a, s, hkv, rb * R);
     int last[NT];
     half8 qf[NT][KS];
+    auto load_q = [&] {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = rb * R + 16 * nt + l16;
-      const bool ok = r < nrows;
-      const PagedRow pr = paged_row(a, s, hkv, ok ? r : 0);
-      last[nt] = a.causal ? min(s.keys - 1, s.len - s.n + (pr.token - s.t0)) : s.keys - 1;
-      const _Float16* qp = a.q + pr.token * a.qt + pr.head * a.qh;
+      for (int nt = 0; nt < NT; ++nt) {
+        const int c = 16 * nt + l16;
+        const bool ok = rb * R + c < nrows;
+        const PagedRow pr = row_of(ok ? c : 0);
+        last[nt] = a.causal ? min(s.keys - 1, s.len - s.n + (pr.token - s.t0)) : s.keys - 1;
+        const _Float16* qp = a.q + pr.token * a.qt + pr.head * a.qh;
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        // Dimensions of step kk that lane group g4 contracts: 8 of a 16-bit
-        // row's 64 bytes; of an 8-bit row's 64 bytes 16, over two steps.
-        const int dim = FP8 ? 64 * (kk >> 1) + 16 * g4 + 8 * (kk & 1) : 32 * kk + 8 * g4;
-        qf[nt][kk] = ok ? *(const half8*)(qp + dim) : (half8)(_Float16)0;
-        if (a.negate_q) qf[nt][kk] = negate16(qf[nt][kk]);
+        for (int kk = 0; kk < KS; ++kk) {
+          // Dimensions of step kk that lane group g4 contracts: 8 of a 16-bit
+          // row's 64 bytes; of an 8-bit row's 64 bytes 16, over two steps.
+          const int dim = FP8 ? 64 * (kk >> 1) + 16 * g4 + 8 * (kk & 1) : 32 * kk + 8 * g4;
+          qf[nt][kk] = ok ? *(const half8*)(qp + dim) : (half8)(_Float16)0;
+        }
       }
-    }
+    };
+    // (behind the first tile's loads: it waits for Q)
+    auto sign_q = [&] {
+      fence_schedule();
+      if (a.negate_q) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) qf[nt][kk] = negate16(qf[nt][kk]);
+      }
+    };
     // Keys no row of the block sees are not read (past `sees`); tiles up to `full`
     // hide nothing from any of them.
     const int last_row = min(nrows, (rb + 1) * R) - 1;
@@ -301,12 +314,14 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     if (t < t_stop) {
       int e[2];
       look_up(t, e);
+      load_q();
       if constexpr (FP8) {
         // The tile's codes are converted, K's in registers and V's into LDS, and the
         // next tile's loads go into the registers they leave.
         Tile x;
         load(t, e, x, nullptr);
         look_up(t + 4, e);
+        sign_q();
         for (; t < t_stop; t += 4) {
           float4v st[2][NT];
           const int rows[2] = {x.rows[0], x.rows[1]};
@@ -339,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
         Tile xa, xb;
         load(t, e, xa, vt0);
         look_up(t + 4, e);
+        sign_q();
         auto step = [&](int tt, Tile& cur, Tile& nxt, const _Float16* vc, _Float16* vn) {
           load(tt + 4, e, nxt, vn);
           look_up(tt + 8, e);
@@ -407,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
       }
       const float m2 = m == -__builtin_inff() ? m : m * c2;
       if (whole) {
-        store_row<BF16>(a, s, hkv, r, dim, m2, l, x);
+        store_row<BF16>(a, row_of(c), dim, m2, l, x);
       } else {
         // Coherent over the L2s: the merging workgroup may be on another XCD.
         const int64_t rec = (int64_t)(2 * (int)blockIdx.x + (first == 0 ? 1 : 0)) * R;
@@ -479,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
         xm[threadIdx.x] = m;
         xm[kThreads + threadIdx.x] = l;
       } else {
-        store_row<BF16>(a, s, hkv, rb * R + c, 4 * ch, m, l, x);
+        store_row<BF16>(a, row_of(c), 4 * ch, m, l, x);
       }
     }
     __syncthreads();
@@ -493,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
         x += w * xo[g * items + threadIdx.x];
       }
       const int c = (int)threadIdx.x / (D / 4);
-      store_row<BF16>(a, s, hkv, rb * R + c, 4 * ((int)threadIdx.x - c * (D / 4)), m, l, x);
+      store_row<BF16>(a, row_of(c), 4 * ((int)threadIdx.x - c * (D / 4)), m, l, x);
     }
     __syncthreads();
   }
@@ -554,7 +570,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
         l += w * xm[1][g * LR + ch];
         x += w * xo[g * LR + ch];
       }
-      store_row<BF16>(a, s, hkv, rb * R + c, 4 * ch, m, l, x);
+      store_row<BF16>(a, PagedRows(a, s, hkv, rb * R)(c), 4 * ch, m, l, x);
     }
     __syncthreads();
   }

@@ -119,22 +119,26 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int tile_end = SPLIT ? min(block_tiles, first + here) : block_tiles;
   // The last key this lane's row sees; keys below wave_full are seen by every row of
   // the wave.
-  const int tok = min(row, nrows - 1) / a.group;
+  const PagedRows row_of(a, s, hkv, q0);
+  const int tok = row_of(min(row, nrows - 1) - q0).token - s.t0;
   const int last_key = a.causal ? min(s.keys - 1, past + tok) : s.keys - 1;
   const int wave_full =
       a.causal ? uniform(clamp_int(past + min(qw, nrows - 1) / a.group + 1, 0, s.keys)) : s.keys;
 
   // Q^T fragments (B operand of S^T), resident for the whole kernel.
   half8 qf[KK];
-  {
-    const PagedRow pr = paged_row(a, s, hkv, min(row, nrows - 1));
+  auto load_q = [&] {
+    const PagedRow pr = row_of(min(row, nrows - 1) - q0);
     const _Float16* qp = a.q + pr.token * a.qt + pr.head * a.qh + 8 * hi;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      qf[kk] = *(const half8*)(qp + 16 * kk);
-      if (a.negate_q) qf[kk] = negate16(qf[kk]);
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = *(const half8*)(qp + 16 * kk);
+  };
+  auto sign_q = [&] {  // (behind the first tiles' loads: it waits for Q)
+    if (a.negate_q) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) qf[kk] = negate16(qf[kk]);
     }
-  }
+  };
 
   // What a lane loads of its wave's 16 rows: byte offsets from the first row.
   // 16-bit rows go to LDS directly (lane l's 16 bytes at 16 l of each KB; padding
@@ -378,8 +382,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[t][i], c2, -mc));
       const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[t][i + 1], c2, -mc));
       pf[2 * t + (i >> 3)][(i & 7) >> 1] = __builtin_bit_cast(unsigned, E::pack(p0, p1));
-      l_run += p0;
-      l_run += p1;
+      l_run += p0 + p1;
       asm volatile("" : "+v"(l_run));  // keeps the sum in this slot
     };
     static_for<16>([&](auto p_c) {
@@ -441,6 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
     look_up(tile0 + 1, e1);
     look_up(tile0 + 2, e2);
     look_up(tile0 + 3, ahead);
+    load_q();
     const Pages pg0 = pages_of(e0);
     pg1 = pages_of(e1);
     pg2 = pages_of(e2);
@@ -463,6 +467,8 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       });
       load_k8(tile0 + 2, pg2.own);
       load_v8(tile0 + 1, pg1.own);
+      fence_schedule();
+      sign_q();
       barrier_after_loads<63>();
     } else {
       const __amdgpu_buffer_rsrc_t rk0 = window(kh, a.kp, a.kn, tile0, pg0.own);
@@ -474,6 +480,8 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       for (int i = 0; i < SEGQ; ++i) direct_load16(rk1, lds_seg(k_lds1, i), koff[i]);
 #pragma unroll
       for (int i = 0; i < SEGQ; ++i) direct_load16(rv0, lds_seg(v_lds0, i), voff[i]);
+      fence_schedule();
+      sign_q();
       barrier_after_loads<2 * SEGQ>();  // S_0 needs K_0 only
     }
     if (qw >= nrows) {
@@ -544,17 +552,27 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const float m2 = m_run == -__builtin_inff() ? m_run : m_run * c2;
   if (row < nrows) {
     if (whole) {
-      const PagedRow pr = paged_row(a, s, hkv, row);
+      const PagedRow pr = row_of(row - q0);
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+      _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh + 8 * hi;
+      // The half-waves hold 4 dimensions each of every 8; for two such groups the
+      // lower takes the first whole and the upper the second: 16-byte stores.
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          half4 v;
+        for (int g = 0; g < 4; g += 2) {
+          uint4v v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = E::round(oacc[mt][4 * g + e] * inv);
-          *(half4*)(op + 32 * mt + 8 * g + 4 * hi) = v;
+          for (int e = 0; e < 2; ++e) {
+            const unsigned x0 = __builtin_bit_cast(
+                unsigned, E::pack(oacc[mt][4 * g + 2 * e] * inv, oacc[mt][4 * g + 2 * e + 1] * inv));
+            const unsigned x1 = __builtin_bit_cast(
+                unsigned, E::pack(oacc[mt][4 * g + 4 + 2 * e] * inv, oacc[mt][4 * g + 5 + 2 * e] * inv));
+            const auto y = __builtin_amdgcn_permlane32_swap(x0, x1, false, false);
+            v[e] = y[0];
+            v[2 + e] = y[1];
+          }
+          *(uint4v*)(op + 32 * mt + 8 * g) = v;
         }
       if (a.lse != nullptr && hi == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
     } else {
@@ -574,7 +592,9 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 
 // Merges the partials of units that stretches cut.  The workgroup of a border between
 // two stretches looks at the unit it lies in: of the unit's p - 1 borders each takes a
-// share of the rows, D / 4 lanes a row.
+// share of the rows, D / 4 lanes a row.  kChunkCombineY workgroups for a border: a row's
+// partials are read at once and the next row's after them, so few rows each.
+constexpr int kChunkCombineY = 4;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
   constexpr int LR = D / 4;
@@ -596,11 +616,13 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int hc = unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int hkv = hc * a.classes + cls;
+  const PagedRows row_of(a, s, hkv, rb * kChunkRows);
   const int ch = (int)threadIdx.x % LR;
   const int rows = min(kChunkRows, s.n * a.group - rb * kChunkRows);
-  const int share = wg - pieces.first, shares = pieces.count - 1;  // from 1
-  const int r_end = rows * share / shares;
-  for (int r = rows * (share - 1) / shares + (int)threadIdx.x / LR; r < r_end; r += kThreads / LR) {
+  const int share = (wg - pieces.first - 1) * kChunkCombineY + (int)blockIdx.y;
+  const int shares = (pieces.count - 1) * kChunkCombineY;
+  const int r_end = rows * (share + 1) / shares;
+  for (int r = rows * share / shares + (int)threadIdx.x / LR; r < r_end; r += kThreads / LR) {
     float m = -__builtin_inff(), l = 0.0f;
     float4v x = (float4v)0.0f;
     auto rec = [&](int i) -> int64_t { return (int64_t)pieces.slot(a, cls, i) * kChunkRows + r; };
@@ -608,7 +630,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
       fold_partials<8>(
           i, 1, pieces.count, m, l, x, [&](int i) { return *(const v2f*)(a.part_ml + rec(i) * 2); },
           [&](int i) { return *(const float4v*)(a.part_o + rec(i) * D + 4 * ch); });
-    store_row<BF16>(a, s, hkv, rb * kChunkRows + r, 4 * ch, m, l, x);
+    store_row<BF16>(a, row_of(r), 4 * ch, m, l, x);
   }
 }
 

@@ -125,14 +125,30 @@ struct PagedPieces {
   }
 };
 
-// Row r of a sequence's rows: the addresses of its Q, O and LSE.
+// Rows of a block: row r0 + c of a sequence is token r / group of query head
+// kv_head * group + r % group.  The quotient of r0 is scalar; that of what is left and a
+// lane's c (below 2^22) comes from a product with 1 / group, whose error stays under the
+// 0.5 / group by which it is off a whole number.
 struct PagedRow {
   int token, head;
 };
-__device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, const PagedSeq& s, int hkv, int r) {
-  const int i = r / a.group;
-  return {s.t0 + i, hkv * a.group + (r - i * a.group)};
-}
+struct PagedRows {
+  int tok0, rem0, head0, group;
+  float inv;
+  __device__ __forceinline__ PagedRows(const PagedArgs& a, const PagedSeq& s, int hkv, int r0) {
+    group = a.group;
+    const int i = r0 / group;
+    tok0 = s.t0 + i;
+    rem0 = r0 - i * group;
+    head0 = hkv * group;
+    inv = 1.0f / (float)group;
+  }
+  __device__ __forceinline__ PagedRow operator()(int c) const {
+    const int x = rem0 + c;
+    const int i = (int)(((float)x + 0.5f) * inv);
+    return {tok0 + i, head0 + x - i * group};
+  }
+};
 
 __device__ __forceinline__ float natural_lse(float m2, float l) {
   return ((m2 == -__builtin_inff() ? 0.0f : m2) + __builtin_log2f(l)) * 0.69314718055994530942f;
@@ -148,11 +164,10 @@ constexpr int kPCoherent = 16;  // cache policy: the sc1 bit, coherent over the 
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-// O and LSE of row r of a sequence from its merged state, 4 dimensions.
+// O and LSE of a row from its merged state, 4 dimensions.
 template <bool BF16>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedSeq& s, int hkv, int r, int dim,
-                                          float m2, float l, float4v x) {
-  const PagedRow pr = paged_row(a, s, hkv, r);
+__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedRow pr, int dim, float m2, float l,
+                                          float4v x) {
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   half4 y;
 #pragma unroll
