@@ -57,8 +57,12 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   PagedPlan p{};
   p.rows = max_query_len * a.group <= 16 ? 16 : 32;
   p.classes = std::gcd(a.hkv, kNumXcds);
-  const int64_t resident =  // (resident_fused_workgroups: two a CU)
-      resident_fused_workgroups() / 2 * paged_per_cu(head_dim, a.ks != nullptr, p.rows / 16);
+  // Two workgroups a CU.  Head_dim 64 and 8-bit instances have room for three or four;
+  // with those a launch took longer (us, two against three: 32 sequences to 8192 keys d128
+  // 8 bits 68.3 / 70.7, 4 rows over 131072 keys 49.3 / 51.6, 16 to 32768 keys d64 39.6 /
+  // 41.0, 8 bits 32.1 / 32.4; 8 to 8192 keys without grouping d128 8 bits 29.3 / 33.5):
+  // stretches are shorter and more of them end inside a unit.
+  const int64_t resident = resident_fused_workgroups();
   const int64_t room = workspace_bytes / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
   // Units of a class: blocks of rows, the last of each sequence not full.

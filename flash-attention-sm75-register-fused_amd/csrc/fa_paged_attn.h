@@ -45,15 +45,11 @@ namespace {
 constexpr int kPTile = 32;       // keys of a wave's tile
 constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below
 
-// Workgroups of a CU at once: what their V tiles leave room for in 160 KB of LDS,
-// and their registers among 512 of a lane.
-__host__ __device__ constexpr int paged_per_cu(int d, bool fp8, int nt) {
-  return fp8 && nt == 1 ? (d == 64 ? 4 : 3) : d == 64 ? 3 : 2;
-}
-
 // Whether a unit's last workgroup merges its partials: one workgroup reads them
-// at about 50 bytes/ns.
-constexpr int kPMergeBytes = 128 << 10;
+// at about 50 bytes/ns, and the second kernel costs a launch 2.5 us where it has
+// nothing to do (16 sequences to 32768 keys d64 39.3 -> 36.9 us, 8 bits 32.9 -> 30.3,
+// without it).
+constexpr int kPMergeBytes = 256 << 10;
 __host__ __device__ constexpr bool paged_merges_itself(int pieces, int rows, int d) {
   return pieces <= kThreads && (int64_t)pieces * rows * d * 4 <= kPMergeBytes;
 }
@@ -68,7 +64,7 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 template <int D, bool BF16, bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_attn_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
   using E = Elem<BF16>;
   constexpr int R = 16 * NT;
   constexpr int KS = D / 32;  // contraction steps of S^T
@@ -136,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     const int unit = (pos - seq_start) / line_tiles;
     const int first = pos - seq_start - unit * line_tiles;  // on the line
     const int here = min(line_tiles - first, end - pos);
-    const int hc = unit / blocks;
+    const int hc = blocks == 1 ? unit : unit / blocks;
     const int rb = unit - hc * blocks;
     const int hkv = hc * a.classes + cls;
     const bool whole = !a.split || (first == 0 && here == line_tiles);
@@ -148,6 +144,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     // key it sees.
     const int nrows = s.n * a.group;
     const PagedRows row_of(a, s, hkv, rb * R);
+    const int past = s.len - s.n;  // tokens before the new ones
     int last[NT];
     half8 qf[NT][KS];
     auto load_q = [&] {
@@ -156,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
         const int c = 16 * nt + l16;
         const bool ok = rb * R + c < nrows;
         const PagedRow pr = row_of(ok ? c : 0);
-        last[nt] = a.causal ? min(s.keys - 1, s.len - s.n + (pr.token - s.t0)) : s.keys - 1;
+        last[nt] = a.causal ? min(s.keys - 1, past + (pr.token - s.t0)) : s.keys - 1;
         const _Float16* qp = a.q + pr.token * a.qt + pr.head * a.qh;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
@@ -179,11 +176,10 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
     };
     // Keys no row of the block sees are not read (past `sees`); tiles up to `full`
     // hide nothing from any of them.
-    const int last_row = min(nrows, (rb + 1) * R) - 1;
-    const int sees =
-        a.causal ? uniform(clamp_int(s.len - s.n + last_row / a.group + 1, 0, s.keys)) : s.keys;
-    const int full =
-        a.causal ? uniform(clamp_int(s.len - s.n + rb * R / a.group + 1, 0, s.keys)) : s.keys;
+    const int tok_first = uniform(row_of(0).token) - s.t0;
+    const int tok_last = uniform(row_of(min(nrows - rb * R, R) - 1).token) - s.t0;
+    const int sees = a.causal ? uniform(clamp_int(past + tok_last + 1, 0, s.keys)) : s.keys;
+    const int full = a.causal ? uniform(clamp_int(past + tok_first + 1, 0, s.keys)) : s.keys;
     const int t_stop = min(t_end, (sees + kPTile - 1) / kPTile);
 
     float4v o[NT][MT];
@@ -238,7 +234,10 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
               make_rsrc(a.vs + page * a.vsp + hkv * a.vsh + off * a.vsn, x.rows[p] * (int)a.vsn);
 #pragma unroll
           for (int i = 0; i < VL; ++i) {
-            x.v[p][i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off[i], 0, 0));
+            // Non-temporal, as the 16-bit rows' direct loads: whole lines that nobody
+            // reads again.  K's are read in halves and stay cached.
+            x.v[p][i] = __builtin_bit_cast(
+                uint4v, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off[i], 0, kPStreamed));
             x.vs[p][i] =
                 __builtin_amdgcn_raw_buffer_load_b8(rs, (64 * i + lane) / RL * (int)a.vsn, 0, 0);
           }
@@ -476,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, paged_per_cu(D, FP8, NT)) fa_paged_a
       const int c = it / (D / 4), ch = it - c * (D / 4);
       float m = -__builtin_inff(), l = 0.0f;
       float4v x = (float4v)0.0f;
-      for (int i = grp; i < pieces.count; i += 8 * groups)
-        fold_partials<8>(
+      for (int i = grp; i < pieces.count; i += 16 * groups)
+        fold_partials<16>(
             i, groups, pieces.count, m, l, x,
             [&](int i) {
               const int64_t rec = (int64_t)pieces.slot(a, cls, i) * R + c;

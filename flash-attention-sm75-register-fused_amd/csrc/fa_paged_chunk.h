@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int here = SPLIT ? min(line_tiles - first, end - pos) : 1;
   const bool whole = !SPLIT || here == line_tiles;
   pos += here;
-  const int hc = unit / blocks;
+  const int hc = blocks == 1 ? unit : unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int hkv = hc * a.classes + cls;
 
@@ -112,18 +112,18 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int past = s.len - s.n;  // tokens before the new ones
 
   // Keys the block's rows see, and this segment's tiles of them.
-  const int last_tok = (min(nrows, q0 + kChunkRows) - 1) / a.group;
+  const PagedRows row_of(a, s, hkv, q0);
+  const int last_tok = uniform(row_of(min(nrows - q0, kChunkRows) - 1).token) - s.t0;
   const int kv_len = a.causal ? uniform(clamp_int(past + last_tok + 1, 0, s.keys)) : s.keys;
   const int block_tiles = (kv_len + kBlockN - 1) / kBlockN;
   const int tile0 = SPLIT ? first : 0;
   const int tile_end = SPLIT ? min(block_tiles, first + here) : block_tiles;
   // The last key this lane's row sees; keys below wave_full are seen by every row of
   // the wave.
-  const PagedRows row_of(a, s, hkv, q0);
   const int tok = row_of(min(row, nrows - 1) - q0).token - s.t0;
   const int last_key = a.causal ? min(s.keys - 1, past + tok) : s.keys - 1;
   const int wave_full =
-      a.causal ? uniform(clamp_int(past + min(qw, nrows - 1) / a.group + 1, 0, s.keys)) : s.keys;
+      a.causal ? uniform(clamp_int(past + row_of(min(qw, nrows - 1) - q0).token - s.t0 + 1, 0, s.keys)) : s.keys;
 
   // Q^T fragments (B operand of S^T), resident for the whole kernel.
   half8 qf[KK];
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   if (border == u0) return;
   const PagedPieces pieces(stretch, u0, u0 + tiles);
   const int blocks = paged_blocks<kChunkRows>(a, s);
-  const int hc = unit / blocks;
+  const int hc = blocks == 1 ? unit : unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int hkv = hc * a.classes + cls;
   const PagedRows row_of(a, s, hkv, rb * kChunkRows);

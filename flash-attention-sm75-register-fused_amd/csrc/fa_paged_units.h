@@ -137,7 +137,7 @@ struct PagedRows {
   float inv;
   __device__ __forceinline__ PagedRows(const PagedArgs& a, const PagedSeq& s, int hkv, int r0) {
     group = a.group;
-    const int i = r0 / group;
+    const int i = r0 == 0 ? 0 : r0 / group;
     tok0 = s.t0 + i;
     rem0 = r0 - i * group;
     head0 = hkv * group;
@@ -160,7 +160,9 @@ __device__ __forceinline__ float natural_lse(float m2, float l) {
 // leaves the zeros and keeps the NaN.
 __device__ __forceinline__ float over_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
-constexpr int kPCoherent = 16;  // cache policy: the sc1 bit, coherent over the device's L2s
+// Cache policies of buffer accesses: the sc1 bit, coherent over the device's L2s; and the
+// nt bit, for what is read once.
+constexpr int kPCoherent = 16, kPStreamed = 2;
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
