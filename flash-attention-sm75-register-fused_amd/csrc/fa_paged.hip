@@ -19,6 +19,7 @@ FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
 FA_PAGED_EXTERN(128, false, true) FA_PAGED_EXTERN(128, true, true)
 #undef FA_PAGED_EXTERN
 
+
 namespace {
 int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
   return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
@@ -41,7 +42,7 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace
   const int64_t heads = a.hkv / p.classes, rows = (int64_t)a.tokens * a.group;
   const int64_t least = heads * ((rows + p.rows - 1) / p.rows);
   p.units = (int)(heads * ((rows + (p.rows - 1ll) * std::min(a.batch, a.tokens)) / p.rows));
-  const int64_t record = 2ll * p.rows * (head_dim + 2) * (int64_t)sizeof(float) * p.classes;
+  const int64_t record = partial_bytes(p.rows, head_dim) * p.classes;
   const int64_t wgs = std::min<int64_t>(p.resident = resident_fused_workgroups() / p.classes,
                                         workspace_bytes / record);
   p.split = least < wgs && fits_line(a, p.units, kBlockN);
@@ -106,10 +107,7 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   a.resident = plan.resident;
   a.split = plan.split ? 1 : 0;
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
-  if (plan.split && plan.chunk) {
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
-  } else if (plan.split) {
+  if (plan.split) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);

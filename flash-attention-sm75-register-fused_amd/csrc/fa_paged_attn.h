@@ -54,15 +54,6 @@ __host__ __device__ constexpr bool paged_merges_itself(int pieces, int rows, int
   return pieces <= kThreads && (int64_t)pieces * rows * d * 4 <= kPMergeBytes;
 }
 
-// Waits until at most N of the wave's vector loads are in flight (they land in
-// order), and keeps the LDS reads that depend on it behind the wait.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(N >= 0 && N < 64, "vmcnt range");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-  asm volatile("" ::: "memory");
-}
-
 template <int D, bool BF16, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
   using E = Elem<BF16>;
@@ -439,9 +430,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     }
 
     // ---- the unit's last workgroup merges its partials -------------------------
-    // A workgroup's partials are acknowledged before it sets its flag, and its flag
-    // before it reads the others': the last flag to be set is set by a workgroup
-    // that sees them all.  Two that both do store the same values.
     const int u0 = seq_start + unit * line_tiles;
     const PagedPieces pieces(stretch, u0, u0 + line_tiles);
     const int nr = min(R, nrows - rb * R);
@@ -449,20 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       __syncthreads();
       continue;
     }
-    const __amdgpu_buffer_rsrc_t rf = make_rsrc(a.flags, 2 * (int)gridDim.x * 8);
-    wait_loads<0>();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, a.mark), rf,
-                                            (2 * (int)blockIdx.x + (first == 0 ? 1 : 0)) * 8, 0, kPCoherent);
-      wait_loads<0>();
-    }
-    __syncthreads();
-    bool set = true;
-    if ((int)threadIdx.x < pieces.count)
-      set = __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(
-                rf, pieces.slot(a, cls, threadIdx.x) * 8, 0, kPCoherent)) == a.mark;
-    if (!__syncthreads_and(set)) continue;
+    if (!last_to_finish(a, pieces, cls, 2 * (int)blockIdx.x + (first == 0 ? 1 : 0), (int*)v_lds0)) continue;
     // Thread: 4 dimensions of a row, pieces grp, grp + groups, ...; the groups
     // meet in LDS.  More items than threads: one group, items in turns.
     const int items = nr * (D / 4);

@@ -22,7 +22,8 @@
 //
 // The plan.  Where the units do not fill the GPU (SPLIT), each workgroup takes an equal
 // stretch of the class's line of 64-key tiles, as in the kernel for few columns; the
-// partials of units that stretches cut are merged by a second kernel.  Else a
+// partials of units that stretches cut are merged by the unit's last workgroup where
+// they are few, else by a second kernel.  Else a
 // workgroup takes a unit, each head's from its last block (under the causal rule the
 // longest) to its first; where all of them run at once, two a CU, the second half
 // of them in reverse, so that a CU gets a long and a short one.
@@ -38,6 +39,117 @@ namespace {
 
 constexpr int kChunkRows = 128;
 constexpr int kChunkMinTiles = 4;  // tiles a stretch is not cut below
+
+// Rounds and stores two groups of 8 dimensions of a row.  The half-waves hold 4
+// dimensions each of both; the lower takes the first whole and the upper the
+// second: one 16-byte store.  `to`: the lane's 8.
+template <bool BF16>
+__device__ __forceinline__ void store_pair(_Float16* to, float4v x, float4v y, float inv) {
+  uint4v v;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const unsigned u0 =
+        __builtin_bit_cast(unsigned, Elem<BF16>::pack(x[2 * e] * inv, x[2 * e + 1] * inv));
+    const unsigned u1 =
+        __builtin_bit_cast(unsigned, Elem<BF16>::pack(y[2 * e] * inv, y[2 * e + 1] * inv));
+    const auto z = __builtin_amdgcn_permlane32_swap(u0, u1, false, false);
+    v[e] = z[0];
+    v[2 + e] = z[1];
+  }
+  *(uint4v*)to = v;
+}
+
+// Whether a unit's last workgroup merges its partials (it reads them at about 50
+// bytes/ns, 5 us for these many), or the second kernel.
+constexpr int kChunkMergeBytes = 256 << 10;
+__device__ __forceinline__ bool chunk_merges_itself(int pieces, int d) {
+  return (int64_t)pieces * kChunkRows * d * 4 <= kChunkMergeBytes;
+}
+
+// A record of the workspace: a block's partials in the order its waves' registers
+// hold them, so that 64 lanes store and load 1 KB at once (row by row, 16 bytes of
+// 32 rows at once, coherent stores took half of a short launch).  Group 4 mt + g of a wave:
+// dimensions 32 mt + 8 g + 4 (lane / 32) .. + 3 of its row lane % 32.
+template <int D>
+struct ChunkRecord {
+  static constexpr int Groups = D / 8;
+  __amdgpu_buffer_rsrc_t o, ml;
+  __device__ __forceinline__ ChunkRecord(const PagedArgs& a) {
+    o = make_rsrc(a.part_o, INT32_MAX);
+    ml = make_rsrc(a.part_ml, INT32_MAX);
+  }
+  __device__ __forceinline__ int o_at(int record, int wave, int group, int lane) const {
+    return (((record * 4 + wave) * Groups + group) * 64 + lane) * 16;
+  }
+  __device__ __forceinline__ int ml_at(int record, int wave, int ql) const {
+    return ((record * 4 + wave) * 32 + ql) * 8;
+  }
+};
+
+// Merges pairs of groups pair0 .. pair0 + 3 of a unit's partials, wave w its rows
+// 32 w .. + 31 (of `rows`), and stores them: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M)
+// l_i, M = max_i m_i.
+template <int D, bool BF16>
+__device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPieces& pieces, int cls,
+                                            const PagedRows& row_of, int rows, int pair0) {
+  constexpr int PAIRS = 4, AT = 4;  // at once; pieces at once
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hi = lane >> 5, ql = lane & 31;
+  const int r = 32 * wave + ql;
+  if (r >= rows) return;
+  const ChunkRecord<D> rec(a);
+  auto load_ml = [&](int i) {
+    return __builtin_bit_cast(v2f, __builtin_amdgcn_raw_buffer_load_b64(
+                                       rec.ml, rec.ml_at(pieces.slot(a, cls, i), wave, ql), 0, kPCoherent));
+  };
+  float m = -__builtin_inff();
+  for (int i0 = 0; i0 < pieces.count; i0 += 8) {
+    v2f ml[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) ml[u] = load_ml(min(i0 + u, pieces.count - 1));
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m = fmaxf(m, ml[u][0]);
+  }
+  float l = 0.0f;
+  float4v x[PAIRS][2];
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q) x[q][0] = x[q][1] = (float4v)0.0f;
+  for (int i0 = 0; i0 < pieces.count; i0 += AT) {
+    v2f ml[AT];
+    float4v o[AT][PAIRS][2];
+#pragma unroll
+    for (int u = 0; u < AT; ++u) {
+      const int i = min(i0 + u, pieces.count - 1);
+      const int record = pieces.slot(a, cls, i);
+      ml[u] = load_ml(i);
+#pragma unroll
+      for (int q = 0; q < PAIRS; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          o[u][q][e] = __builtin_bit_cast(
+              float4v, __builtin_amdgcn_raw_buffer_load_b128(
+                           rec.o, rec.o_at(record, wave, 2 * (pair0 + q) + e, lane), 0, kPCoherent));
+    }
+#pragma unroll
+    for (int u = 0; u < AT; ++u) {
+      if (i0 + u >= pieces.count) break;  // (the last one again)
+      const float w = __builtin_amdgcn_exp2f(ml[u][0] - over_zero(m));
+      l += w * ml[u][1];
+#pragma unroll
+      for (int q = 0; q < PAIRS; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[q][e] += w * o[u][q][e];
+    }
+  }
+  const PagedRow pr = row_of(r);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q) store_pair<BF16>(op + 16 * (pair0 + q) + 8 * hi, x[q][0], x[q][1], inv);
+  if (a.lse != nullptr && hi == 0 && pair0 == 0)
+    a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
+}
 
 template <int D, bool BF16, bool FP8, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
@@ -555,49 +667,57 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       const PagedRow pr = row_of(row - q0);
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh + 8 * hi;
-      // The half-waves hold 4 dimensions each of every 8; for two such groups the
-      // lower takes the first whole and the upper the second: 16-byte stores.
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int g = 0; g < 4; g += 2) {
-          uint4v v;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const unsigned x0 = __builtin_bit_cast(
-                unsigned, E::pack(oacc[mt][4 * g + 2 * e] * inv, oacc[mt][4 * g + 2 * e + 1] * inv));
-            const unsigned x1 = __builtin_bit_cast(
-                unsigned, E::pack(oacc[mt][4 * g + 4 + 2 * e] * inv, oacc[mt][4 * g + 5 + 2 * e] * inv));
-            const auto y = __builtin_amdgcn_permlane32_swap(x0, x1, false, false);
-            v[e] = y[0];
-            v[2 + e] = y[1];
-          }
-          *(uint4v*)(op + 32 * mt + 8 * g) = v;
-        }
+        for (int g = 0; g < 4; g += 2)
+          store_pair<BF16>(op + 32 * mt + 8 * g,
+                           float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]},
+                           float4v{oacc[mt][4 * g + 4], oacc[mt][4 * g + 5], oacc[mt][4 * g + 6],
+                                   oacc[mt][4 * g + 7]},
+                           inv);
       if (a.lse != nullptr && hi == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
     } else {
-      const int64_t rec = (2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0)) * kChunkRows + (row - q0);
+      // (see ChunkRecord; coherent over the L2s: the merging workgroup may be on
+      // another XCD)
+      const ChunkRecord<D> rec(a);
+      const int record = 2 * (int)blockIdx.x + (first == 0 ? 1 : 0);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          *(float4v*)(a.part_o + rec * D + 32 * mt + 8 * g + 4 * hi) =
-              float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
-      if (hi == 0) *(v2f*)(a.part_ml + rec * 2) = v2f{m2, l};
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(uint4v, float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2],
+                                                 oacc[mt][4 * g + 3]}),
+              rec.o, rec.o_at(record, wave, 4 * mt + g, lane), 0, kPCoherent);
+      if (hi == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v2f{m2, l}), rec.ml,
+                                              rec.ml_at(record, wave, ql), 0, kPCoherent);
     }
   }
-  if constexpr (SPLIT) __syncthreads();  // the next segment's loads go into these tiles
+  if constexpr (SPLIT) {
+    if (!whole) {
+      const int u0 = seq_start + unit * line_tiles;
+      const PagedPieces pieces(stretch, u0, u0 + line_tiles);
+      if (chunk_merges_itself(pieces.count, D) &&
+          last_to_finish(a, pieces, cls, 2 * (int)blockIdx.x + (first == 0 ? 1 : 0), (int*)k_lds0))
+        for (int pair = 0; pair < D / 16; pair += 4)
+          merge_chunk<D, BF16>(a, pieces, cls, row_of, nrows - q0, pair);
+    }
+    __syncthreads();  // the next segment's loads go into these tiles
+  }
   } while (SPLIT && pos < end);
 }
 
-// Merges the partials of units that stretches cut.  The workgroup of a border between
-// two stretches looks at the unit it lies in: of the unit's p - 1 borders each takes a
-// share of the rows, D / 4 lanes a row.  kChunkCombineY workgroups for a border: a row's
-// partials are read at once and the next row's after them, so few rows each.
-constexpr int kChunkCombineY = 4;
+// Merges the partials of units whose last workgroup does not.  The kChunkCombineY
+// workgroups of a border between two stretches look at the unit it lies in; all those
+// of the unit share its tasks, a pair of groups of one wave's 32 rows each.  Of a task
+// the workgroup's waves take every fourth piece, and meet in LDS.
+constexpr int kChunkCombineY = 2;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
-  constexpr int LR = D / 4;
+  __shared__ float4v xo[kWaves][2][64];
+  __shared__ float xml[kWaves][2][64];
   const int cls = (int)blockIdx.x % a.classes;
   const int wg = (int)blockIdx.x / a.classes;
   const PagedLine<kChunkRows, kBlockN> line(a, threadIdx.x & 63, true);
@@ -612,25 +732,77 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int u0 = seq_start + unit * tiles;
   if (border == u0) return;
   const PagedPieces pieces(stretch, u0, u0 + tiles);
+  if (chunk_merges_itself(pieces.count, D)) return;
   const int blocks = paged_blocks<kChunkRows>(a, s);
-  const int hc = blocks == 1 ? unit : unit / blocks;
+  const int hc = unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
-  const int hkv = hc * a.classes + cls;
-  const PagedRows row_of(a, s, hkv, rb * kChunkRows);
-  const int ch = (int)threadIdx.x % LR;
-  const int rows = min(kChunkRows, s.n * a.group - rb * kChunkRows);
+  const int rows = s.n * a.group - rb * kChunkRows;
+  const PagedRows row_of(a, s, hc * a.classes + cls, rb * kChunkRows);
+  const ChunkRecord<D> rec(a);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hi = lane >> 5, ql = lane & 31;
   const int share = (wg - pieces.first - 1) * kChunkCombineY + (int)blockIdx.y;
-  const int shares = (pieces.count - 1) * kChunkCombineY;
-  const int r_end = rows * (share + 1) / shares;
-  for (int r = rows * share / shares + (int)threadIdx.x / LR; r < r_end; r += kThreads / LR) {
+  for (int task = share; task < D / 16 * 4; task += (pieces.count - 1) * kChunkCombineY) {
+    const int pair = task / 4, rw = task % 4;  // (rows 32 rw ..)
+    constexpr int AT = 8;
     float m = -__builtin_inff(), l = 0.0f;
-    float4v x = (float4v)0.0f;
-    auto rec = [&](int i) -> int64_t { return (int64_t)pieces.slot(a, cls, i) * kChunkRows + r; };
-    for (int i = 0; i < pieces.count; i += 8)
-      fold_partials<8>(
-          i, 1, pieces.count, m, l, x, [&](int i) { return *(const v2f*)(a.part_ml + rec(i) * 2); },
-          [&](int i) { return *(const float4v*)(a.part_o + rec(i) * D + 4 * ch); });
-    store_row<BF16>(a, row_of(r), 4 * ch, m, l, x);
+    float4v x[2] = {(float4v)0.0f, (float4v)0.0f};
+    for (int i0 = wave; i0 < pieces.count; i0 += AT * kWaves) {
+      v2f ml[AT];
+      float4v o[AT][2];
+      float m_new = m;
+#pragma unroll
+      for (int u = 0; u < AT; ++u) {
+        const int record = pieces.slot(a, cls, min(i0 + u * kWaves, pieces.count - 1));
+        ml[u] = __builtin_bit_cast(
+            v2f, __builtin_amdgcn_raw_buffer_load_b64(rec.ml, rec.ml_at(record, rw, ql), 0, 0));
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          o[u][e] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    rec.o, rec.o_at(record, rw, 2 * pair + e, lane), 0, 0));
+      }
+#pragma unroll
+      for (int u = 0; u < AT; ++u) m_new = fmaxf(m_new, ml[u][0]);
+      const float f = __builtin_amdgcn_exp2f(m - over_zero(m_new));
+      l *= f;
+      x[0] *= f;
+      x[1] *= f;
+#pragma unroll
+      for (int u = 0; u < AT; ++u) {
+        if (i0 + u * kWaves >= pieces.count) break;  // (the last one again)
+        const float w = __builtin_amdgcn_exp2f(ml[u][0] - over_zero(m_new));
+        l += w * ml[u][1];
+        x[0] += w * o[u][0];
+        x[1] += w * o[u][1];
+      }
+      m = m_new;
+    }
+    xo[wave][0][lane] = x[0];
+    xo[wave][1][lane] = x[1];
+    xml[wave][0][lane] = m;
+    xml[wave][1][lane] = l;
+    __syncthreads();
+    const int r = 32 * rw + ql;
+    if (wave == 0 && r < rows) {
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, xml[w][0][lane]);
+      l = 0.0f;
+      x[0] = x[1] = (float4v)0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(xml[w][0][lane] - over_zero(m));
+        l += f * xml[w][1][lane];
+        x[0] += f * xo[w][0][lane];
+        x[1] += f * xo[w][1][lane];
+      }
+      const PagedRow pr = row_of(r);
+      store_pair<BF16>(a.o + pr.token * a.ot + pr.head * a.oh + 16 * pair + 8 * hi, x[0], x[1],
+                       l > 0.0f ? 1.0f / l : 0.0f);
+      if (a.lse != nullptr && hi == 0 && pair == 0)
+        a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
+    }
+    __syncthreads();
   }
 }
 

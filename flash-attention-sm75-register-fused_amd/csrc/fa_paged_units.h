@@ -178,23 +178,14 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const PagedRow pr,
   if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
 }
 
-// Folds up to BATCH partials, step apart from i0, into (m, l, x): all their loads
-// are in flight together.  `load` gives the record's (max, sum) and 4 dimensions.
-template <int BATCH, class LoadML, class LoadO>
-__device__ __forceinline__ void fold_partials(int i0, int step, int count, float& m, float& l, float4v& x,
-                                              LoadML load_ml, LoadO load_o) {
-  v2f ml[BATCH];
-  float4v o[BATCH];
-#pragma unroll
-  for (int u = 0; u < BATCH; ++u) {
-    const int i = min(i0 + u * step, count - 1);
-    ml[u] = load_ml(i);
-    o[u] = load_o(i);
-  }
+// Folds the first n (BATCH at most) of BATCH loaded partials into (m, l, x).
+template <int BATCH>
+__device__ __forceinline__ void fold_loaded(int n, v2f (&ml)[BATCH], float4v (&o)[BATCH], float& m, float& l,
+                                            float4v& x) {
   float m_new = m;
 #pragma unroll
   for (int u = 0; u < BATCH; ++u) {
-    if (i0 + u * step >= count) {  // the last one again: no weight
+    if (u >= n) {  // another one again: no weight
       ml[u] = v2f{-__builtin_inff(), 0.0f};
       o[u] = (float4v)0.0f;
     }
@@ -210,6 +201,62 @@ __device__ __forceinline__ void fold_partials(int i0, int step, int count, float
     x += w * o[u];
   }
   m = m_new;
+}
+
+// The same, step apart from i0 among count, all their loads in flight together: `load`
+// gives a record's (max, sum) and 4 dimensions.
+template <int BATCH, class LoadML, class LoadO>
+__device__ __forceinline__ void fold_partials(int i0, int step, int count, float& m, float& l, float4v& x,
+                                              LoadML load_ml, LoadO load_o) {
+  v2f ml[BATCH];
+  float4v o[BATCH];
+#pragma unroll
+  for (int u = 0; u < BATCH; ++u) {
+    const int i = min(i0 + u * step, count - 1);
+    ml[u] = load_ml(i);
+    o[u] = load_o(i);
+  }
+  fold_loaded<BATCH>((count - i0 + step - 1) / step, ml, o, m, l, x);
+}
+
+// Waits until at most N of the wave's vector loads and stores are in flight (they
+// land in order), and keeps the LDS reads that depend on it behind the wait.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
+}
+
+// Sets the flag of a workgroup's record, whose partials its waves have stored
+// coherently, and says whether every piece's flag of the unit is set (at most kThreads
+// pieces).  `scratch`: kWaves ints of LDS that the workgroup is done with.  A
+// workgroup's partials are acknowledged before it sets its flag, and its flag
+// before it reads the others': the last flag to be set is set by a workgroup that
+// sees them all.  Two that both do store the same values.
+__device__ __forceinline__ bool last_to_finish(const PagedArgs& a, const PagedPieces& pieces, int cls,
+                                               int record, int* scratch) {
+  const __amdgpu_buffer_rsrc_t rf = make_rsrc(a.flags, 2 * (int)gridDim.x * 8);
+  wait_loads<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, a.mark), rf, record * 8, 0, kPCoherent);
+    wait_loads<0>();
+  }
+  __syncthreads();
+  bool set = true;
+  if ((int)threadIdx.x < pieces.count)
+    set = __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(
+              rf, pieces.slot(a, cls, threadIdx.x) * 8, 0, kPCoherent)) == a.mark;
+  // (not __syncthreads_and, whose own LDS two workgroups a CU have no room for)
+  const bool all = __builtin_amdgcn_ballot_w64(!set) == 0;
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = all;
+  __syncthreads();
+  bool last = true;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) last = last && scratch[w] != 0;
+  __syncthreads();
+  return last;
 }
 
 }  // namespace
