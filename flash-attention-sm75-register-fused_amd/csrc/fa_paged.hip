@@ -71,7 +71,8 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
       a.cu == nullptr ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
                       : (int64_t)a.tokens * a.group / p.rows + std::min(a.batch, a.tokens);
   p.units = (int)(a.hkv / p.classes * blocks);
-  p.split = p.wgs > 0 && fits_line(a, p.units, kPTile);
+  // (Of very many units a workgroup each is balanced enough.)
+  p.split = p.wgs > 0 && p.units <= 16 * resident / p.classes && fits_line(a, p.units, kPTile);
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) : 0;

@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       const int c = it / (D / 4), ch = it - c * (D / 4);
       float m = -__builtin_inff(), l = 0.0f;
       float4v x = (float4v)0.0f;
-      for (int i = grp; i < pieces.count; i += 16 * groups)
-        fold_partials<16>(
+      for (int i = grp; i < pieces.count; i += 12 * groups)
+        fold_partials<12>(
             i, groups, pieces.count, m, l, x,
             [&](int i) {
               const int64_t rec = (int64_t)pieces.slot(a, cls, i) * R + c;

@@ -178,14 +178,23 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const PagedRow pr,
   if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
 }
 
-// Folds the first n (BATCH at most) of BATCH loaded partials into (m, l, x).
-template <int BATCH>
-__device__ __forceinline__ void fold_loaded(int n, v2f (&ml)[BATCH], float4v (&o)[BATCH], float& m, float& l,
-                                            float4v& x) {
+// Folds up to BATCH partials, step apart from i0 among count, into (m, l, x): all their
+// loads are in flight together.  `load` gives a record's (max, sum) and 4 dimensions.
+template <int BATCH, class LoadML, class LoadO>
+__device__ __forceinline__ void fold_partials(int i0, int step, int count, float& m, float& l, float4v& x,
+                                              LoadML load_ml, LoadO load_o) {
+  v2f ml[BATCH];
+  float4v o[BATCH];
+#pragma unroll
+  for (int u = 0; u < BATCH; ++u) {
+    const int i = min(i0 + u * step, count - 1);
+    ml[u] = load_ml(i);
+    o[u] = load_o(i);
+  }
   float m_new = m;
 #pragma unroll
   for (int u = 0; u < BATCH; ++u) {
-    if (u >= n) {  // another one again: no weight
+    if (i0 + u * step >= count) {  // the last one again: no weight
       ml[u] = v2f{-__builtin_inff(), 0.0f};
       o[u] = (float4v)0.0f;
     }
@@ -201,22 +210,6 @@ __device__ __forceinline__ void fold_loaded(int n, v2f (&ml)[BATCH], float4v (&o
     x += w * o[u];
   }
   m = m_new;
-}
-
-// The same, step apart from i0 among count, all their loads in flight together: `load`
-// gives a record's (max, sum) and 4 dimensions.
-template <int BATCH, class LoadML, class LoadO>
-__device__ __forceinline__ void fold_partials(int i0, int step, int count, float& m, float& l, float4v& x,
-                                              LoadML load_ml, LoadO load_o) {
-  v2f ml[BATCH];
-  float4v o[BATCH];
-#pragma unroll
-  for (int u = 0; u < BATCH; ++u) {
-    const int i = min(i0 + u * step, count - 1);
-    ml[u] = load_ml(i);
-    o[u] = load_o(i);
-  }
-  fold_loaded<BATCH>((count - i0 + step - 1) / step, ml, o, m, l, x);
 }
 
 // Waits until at most N of the wave's vector loads and stores are in flight (they

@@ -42,7 +42,7 @@ class Cache:
         self.seq_lens = torch.tensor(lens, dtype=torch.int32)
         self.cu = torch.tensor([0] + self.news, dtype=torch.int32).cumsum(0).int()
         nan = torch.full((pool, hkv, page, d), math.nan, dtype=dtype)
-        self.k, self.v = nan.clone(), nan.clone()
+        self.k, self.v, self.pages = nan.clone(), nan.clone(), pool
         self.rows = []  # per sequence [K, V] in the 16-bit type, [Hkv, len, D]
         for b, n in enumerate(lens):
             kv = [(torch.randn(hkv, n, d, generator=g) *
@@ -71,7 +71,7 @@ class Cache:
         pos = torch.arange(self.lens[b])
         ok = pos < self.width * self.page
         t = self.table[b][(pos // self.page).clamp(max=self.width - 1)]
-        return ok & (t >= 0) & (t < self.k.shape[0])
+        return ok & (t >= 0) & (t < self.pages)
 
     def args(self, device, strided=False):
         """(k, v, table, lens) and the keyword arguments of the calls, on `device`."""

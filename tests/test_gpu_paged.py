@@ -383,3 +383,190 @@ def test_a_batch_grows(device, q8):
             want, _, tol, _ = ref.attention(one, q[part])
             ref.check(o[part], want, tol, f"O of sequence {b}")
             ref.check(dense[0].transpose(0, 1), want, 2 * tol, f"dense O of sequence {b}")
+
+
+# ---- batches, shapes and tables at large ----------------------------------------------
+
+
+@pytest.mark.parametrize("hint", [1, 10 ** 6])
+@pytest.mark.parametrize("q8", [False, True])
+def test_many_sequences(device, q8, hint):
+    """More sequences than lanes, empty ones and ones without new tokens among them."""
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, 90, (150,), generator=g).tolist()
+    news = [min(n, int(x)) for n, x in zip(lens, torch.randint(0, 4, (150,), generator=g))]
+    lens[140], news[140] = 900, 60
+    c = Cache(lens, 2, 64, 16, BF16, q8, news=news)
+    attend(c, device, 6, max_query_len=hint)
+
+
+def test_write_many_sequences(device):
+    """The sequence of a row is found among more than 64 of them, many without new rows."""
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(1, 40, (200,), generator=g).tolist()
+    news = [min(n, int(x)) for n, x in zip(lens, torch.randint(0, 3, (200,), generator=g))]
+    c = Cache(lens, 1, 64, 16, FP16, False, news=news)
+    k = torch.randn(sum(news), 1, 64, generator=g).half()
+    want = c.k.clone()
+    for b, n in enumerate(news):
+        for i in range(n):
+            pos = lens[b] - n + i
+            want[int(c.table[b, pos // 16]), :, pos % 16] = k[int(c.cu[b]) + i]
+    got, _ = written(c, device, k, -k, c.cu.to(device))
+    assert same(got, want)
+
+
+@pytest.mark.parametrize("hq,hkv", [(160, 1), (33, 1), (48, 16), (24, 24)])
+def test_wide_groups(device, hq, hkv):
+    """More query heads to a KV head than a block of either kernel has rows."""
+    c = Cache([50, 7], hkv, 64, 16, FP16, True, news=[2, 1])
+    attend(c, device, hq)
+    attend(Cache([50, 7], hkv, 64, 16, FP16, False), device, hq, max_query_len=1)
+
+
+@pytest.mark.parametrize("page", [16, 4096])
+def test_table_wider_than_needed(device, page):
+    """A table with room for far longer sequences, its rows a slice of a wider one."""
+    c = Cache([130, 700], 2, 64, page, BF16, False, news=[3, 40])
+    (k, v, table, lens), kw = c.args(device)
+    wide = torch.full((2, 3000), 2 ** 30, dtype=torch.int32, device=device)
+    wide[:, 5:5 + table.shape[1]] = table
+    q = torch.randn(43, 4, 64).bfloat16()
+    want, _, tol, _ = ref.attention(c, q)
+    for hint in (1, 40):
+        o = fa.flash_attention_paged(q.to(device), k, v, wide[:, 5:2900], lens, cu_seqlens=c.cu.to(device),
+                                     max_query_len=hint, **kw)
+        ref.check(o, want, tol, "O")
+    kr, _ = fa.paged_cache_read(k, v, wide[:, 5:2900], lens, max_len=710, **kw)
+    assert torch.equal(kr[1, :, :700].double().cpu(), c.rows[1][0])
+
+
+def test_pool_past_32_bits(device):
+    """Pages, codes and scales whose byte offsets pass 2^32."""
+    pages, page, hkv, d = 300000, 64, 4, 64
+    for dtype in (torch.float8_e4m3fn, FP16):
+        k = torch.empty(pages, hkv, page, d, dtype=dtype, device=device)
+        v = torch.empty_like(k)
+        assert k.numel() * k.element_size() > 2 ** 32
+        kw = {}
+        if dtype == torch.float8_e4m3fn:
+            kw = {n: torch.empty(pages, hkv, page, dtype=torch.float8_e8m0fnu, device=device)
+                  for n in ("k_scale", "v_scale")}
+        table = torch.tensor([[pages - 1, 0, pages - 7], [5, pages // 2, -1]], dtype=torch.int32, device=device)
+        c = Cache([150, 100], hkv, d, page, FP16, bool(kw), news=[150, 100])
+        c.table, c.pages = table.cpu(), pages
+        g = torch.Generator().manual_seed(8)
+        new = [torch.randn(250, hkv, d, generator=g).half() for _ in "kv"]
+        c.rows = [[(ref._through8(x[p]) if kw else x[p].double()).transpose(0, 1) for x in new]
+                  for p in (slice(0, 150), slice(150, 250))]
+        lens, cu = c.seq_lens.to(device), c.cu.to(device)
+        fa.paged_cache_write(*(x.to(device) for x in new), k, v, table, lens, cu_seqlens=cu, **kw)
+        kr, vr = fa.paged_cache_read(k, v, table, lens, dtype=FP16, **kw)
+        for b, n in enumerate(c.lens):
+            assert torch.equal(kr[b, :, :n].double().cpu(), c.rows[b][0])
+            assert torch.equal(vr[b, :, :n].double().cpu(), c.rows[b][1])
+        q = torch.randn(250, 8, d, generator=g).half()
+        want, _, tol, _ = ref.attention(c, q)
+        for hint in (1, 150):
+            o = fa.flash_attention_paged(q.to(device), k, v, table, lens, cu_seqlens=cu, max_query_len=hint, **kw)
+            ref.check(o, want, tol, "O")
+        del k, v, kw, kr, vr
+        torch.cuda.empty_cache()
+
+
+def test_sweep(device):
+    """Seeded cases over the sizes, types, layouts and tables that the calls take."""
+    import os
+    import random
+
+    for seed in range(int(os.environ.get("FA_PAGED_SWEEP_CASES", "60"))):
+        r = random.Random(1000 + seed)
+        b = r.choice([1, 1, 2, 3, 7, 20])
+        lens = [r.choice([0, 1, r.randint(1, 64), r.randint(1, 400), r.randint(1, 1500 if b < 4 else 300)])
+                for _ in range(b)]
+        kind = r.choice(["one", "few", "chunk", "mixed"])
+        most = {"one": 1, "few": 5, "chunk": 300, "mixed": 90}[kind]
+        news = [1 if kind == "one" or (kind == "mixed" and r.random() < 0.7) else r.randint(0, most) for _ in lens]
+        if kind != "one" and r.random() < 0.7:
+            news = [min(n, x) for n, x in zip(news, lens)]
+        hkv, group = r.choice([(1, 1), (1, 7), (2, 4), (3, 2), (8, 4), (2, 1), (4, 9)])
+        d, dtype, q8, page = r.choice([64, 128]), r.choice([FP16, BF16]), r.random() < 0.5, r.choice([16, 32, 64, 256])
+        gone = [(i, r.randrange(-(-n // page))) for i, n in enumerate(lens) if n and r.random() < 0.2]
+        if sum(news) == 0:
+            continue
+        print(f"case {seed}: lens {lens} news {news} hkv {hkv} group {group} d {d} {dtype} q8 {q8} page {page}", flush=True)
+        c = Cache(lens, hkv, d, page, dtype, q8, seed=seed, news=news, gone=gone)
+        attend(c, device, hkv * group, seed=seed, causal=r.random() < 0.8, strided=r.random() < 0.3)
+
+
+# ---- streams and graphs ---------------------------------------------------------------
+
+
+def test_other_streams(device):
+    """Calls on streams of their own, at once, each with its own cache; and a cache whose calls
+    follow each other on one stream that is not the current one when it is read."""
+    caches = [Cache([400 + 50 * i, 33], 2, 64, 16, BF16, i % 2 == 1, seed=i, news=[1 + 20 * (i % 3), 1]) for i in range(4)]
+    streams = [torch.cuda.Stream() for _ in caches]
+    g = torch.Generator().manual_seed(1)
+    qs = [torch.randn(sum(c.news), 6, 64, generator=g).bfloat16() for c in caches]
+    on = [(c.args(device), q.to(device), c.cu.to(device)) for c, q in zip(caches, qs)]
+    torch.cuda.synchronize()
+    outs = [[] for _ in caches]
+    for _ in range(5):
+        for i, (s, ((args, kw), q, cu)) in enumerate(zip(streams, on)):
+            with torch.cuda.stream(s):
+                outs[i].append(fa.flash_attention_paged(q, *args, cu_seqlens=cu, max_query_len=21, **kw))
+    torch.cuda.synchronize()
+    for c, q, o in zip(caches, qs, outs):
+        want, _, tol, _ = ref.attention(c, q)
+        for x in o:
+            ref.check(x, want, tol, "O")
+            assert torch.equal(x, o[0])
+
+
+@pytest.mark.parametrize("most", [1, 70])
+@pytest.mark.parametrize("q8", [False, True])
+def test_captured(device, q8, most):
+    """A captured write, attention and read-back, replayed over tables, lengths and rows that
+    change in between, against eager calls, which run between the replays too."""
+    hkv, hq, d, page, dtype = 2, 8, 64, 16, FP16
+    c = Cache([900, 300, 64], hkv, d, page, dtype, q8, news=[most, 1, 1])
+    (k, v, table, lens), kw = c.args(device)
+    t = most + 2
+    cu = c.cu.to(device)
+    new = [torch.randn(t, hkv, d, device=device).to(dtype) for _ in "kv"]
+    q = torch.randn(t, hq, d, device=device).to(dtype)
+    out = torch.zeros_like(q)
+
+    def calls():
+        fa.paged_cache_write(*new, k, v, table, lens, cu_seqlens=cu, **kw)
+        fa.flash_attention_paged(q, k, v, table, lens, cu_seqlens=cu, max_query_len=most, out=out, **kw)
+        return fa.paged_cache_read(k, v, table, lens, max_len=901, dtype=dtype, **kw)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kr, vr = calls()
+    g = torch.Generator().manual_seed(6)
+    for step in range(4):
+        for x in new + [q]:
+            x.copy_(torch.randn(x.shape, generator=g))
+        lens.copy_(torch.tensor([900 - 37 * step, 300 - 100 * step, 64 - step], dtype=torch.int32))
+        rows = torch.randperm(3, generator=g).tolist()
+        table.copy_(c.table[rows][:, :])  # whose pages belong to whom
+        lens.copy_(torch.minimum(lens.cpu(), torch.tensor([c.lens[i] for i in rows], dtype=torch.int32)))
+        state = [x.clone() for x in (k, v, *kw.values())]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in (out, kr, vr, k, v, *kw.values())]
+        for x, y in zip((k, v, *kw.values()), state):
+            x.copy_(y)
+        out.zero_()
+        eager = calls()
+        torch.cuda.synchronize()
+        for a, b in zip(got, (out, *eager, k, v, *kw.values())):
+            assert same(a.cpu(), b.cpu()), step
