@@ -27,9 +27,9 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
 }  // namespace
 
 // Whether a line of `units` units stays below 2^31 tiles.
-static bool fits_line(const PagedArgs& a, int64_t units, int tile) {
+static bool fits_line(const PagedArgs& a, int64_t units, int tile, int ahead) {
   const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + tile - 1) / tile;
-  return units * std::max<int64_t>(1, tiles) <= INT32_MAX;
+  return units * (ahead + std::max<int64_t>(1, tiles)) <= INT32_MAX;
 }
 
 // Units of 128 rows, cut into pieces where they may be fewer than the GPU runs at once.
@@ -45,7 +45,7 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace
   const int64_t record = partial_bytes(p.rows, head_dim) * p.classes;
   const int64_t wgs = std::min<int64_t>(p.resident = resident_fused_workgroups() / p.classes,
                                         workspace_bytes / record);
-  p.split = least < wgs && fits_line(a, p.units, kBlockN);
+  p.split = least < wgs && fits_line(a, p.units, kBlockN, kChunkAhead);
   p.combine = p.split;
   p.wgs = p.split ? (int)wgs : p.units;
   p.workspace_bytes = p.split ? p.wgs * record : 0;
@@ -72,7 +72,7 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
                       : (int64_t)a.tokens * a.group / p.rows + std::min(a.batch, a.tokens);
   p.units = (int)(a.hkv / p.classes * blocks);
   // (Of very many units a workgroup each is balanced enough.)
-  p.split = p.wgs > 0 && p.units <= 16 * resident / p.classes && fits_line(a, p.units, kPTile);
+  p.split = p.wgs > 0 && p.units <= 16 * resident / p.classes && fits_line(a, p.units, kPTile, kPAhead);
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) : 0;

@@ -44,6 +44,7 @@ namespace {
 
 constexpr int kPTile = 32;       // keys of a wave's tile
 constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below
+constexpr int kPAhead = 3;       // another unit's cost, in tiles
 
 // Whether a unit's last workgroup merges its partials: one workgroup reads them
 // at about 50 bytes/ns, and the second kernel costs a launch 2.5 us where it has
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
   const int cls = (int)blockIdx.x % a.classes;
   const int wg = (int)blockIdx.x / a.classes;
 
-  const PagedLine<R, kPTile> line(a, lane, a.split != 0);
+  const PagedLine<R, kPTile, kPAhead> line(a, lane, a.split != 0);
   const PagedStretch stretch(a, line.total(), a.split ? kPMinTiles : 1);
   if (wg >= stretch.active) return;
   int pos = stretch.start(wg);
@@ -113,23 +114,26 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
   while (pos < end) {
     const PagedSeq s = line.seq(b);
     const int blocks = paged_blocks<R>(a, s);
-    const int line_tiles = line.tiles_of(s);
+    const int unit_len = line.unit_of(s);
     const int len = line.length_of(s);
     if (pos >= seq_start + len) {  // on to the next sequence
       seq_start += len;
       if (++b >= a.batch) return;
       continue;
     }
-    const int unit = (pos - seq_start) / line_tiles;
-    const int first = pos - seq_start - unit * line_tiles;  // on the line
-    const int here = min(line_tiles - first, end - pos);
+    const int unit = (pos - seq_start) / unit_len;
+    const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
+    const int u1 = seq_start + (unit + 1) * unit_len;
+    const int first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
+    pos = min(u1, end);
+    const int stop = pos - u0;
+    if (stop <= 0) break;
     const int hc = blocks == 1 ? unit : unit / blocks;
     const int rb = unit - hc * blocks;
     const int hkv = hc * a.classes + cls;
-    const bool whole = !a.split || (first == 0 && here == line_tiles);
-    const int t_begin = a.split ? first : 0;
-    const int t_end = a.split ? first + here : (s.keys + kPTile - 1) / kPTile;
-    pos += here;
+    const bool whole = first == 0 && pos == u1;
+    const int t_begin = first;
+    const int t_end = a.split ? stop : (s.keys + kPTile - 1) / kPTile;
 
     // Columns of this lane, one for each nt: whether they hold a row, and the last
     // key it sees.
@@ -430,8 +434,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     }
 
     // ---- the unit's last workgroup merges its partials -------------------------
-    const int u0 = seq_start + unit * line_tiles;
-    const PagedPieces pieces(stretch, u0, u0 + line_tiles);
+    const PagedPieces pieces(stretch, u0, u1);
     const int nr = min(R, nrows - rb * R);
     if (!paged_merges_itself(pieces.count, nr, D)) {
       __syncthreads();
@@ -502,17 +505,17 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   __shared__ float xm[2][kThreads];
   const int cls = (int)blockIdx.x % a.classes;
   const int index = (int)blockIdx.x / a.classes;  // of the class's units
-  const PagedLine<R, kPTile> line(a, threadIdx.x & 63, true);
-  const PagedLine<R, kPTile> units(a, threadIdx.x & 63, false);
+  const PagedLine<R, kPTile, kPAhead> line(a, threadIdx.x & 63, true);
+  const PagedLine<R, kPTile, kPAhead> units(a, threadIdx.x & 63, false);
   if (index >= units.total()) return;
   int unit_start;
   const int b = uniform(units.find(index, unit_start));
   const PagedSeq s = line.seq(b);
-  const int tiles = line.tiles_of(s);
+  const int unit_len = line.unit_of(s);
   const int unit = index - unit_start;
-  const int u0 = line.start_of(b) + unit * tiles;
+  const int u0 = line.start_of(b) + unit * unit_len;
   const PagedStretch stretch(a, line.total(), kPMinTiles);
-  const PagedPieces pieces(stretch, u0, u0 + tiles);
+  const PagedPieces pieces(stretch, u0 + line.ahead, u0 + unit_len);
   if (pieces.count == 1) return;
   const int blocks = paged_blocks<R>(a, s);
   const int hc = unit / blocks;

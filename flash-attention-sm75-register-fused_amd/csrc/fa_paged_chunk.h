@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kChunkRows = 128;
 constexpr int kChunkMinTiles = 4;  // tiles a stretch is not cut below
+constexpr int kChunkAhead = 3;     // another unit's cost, in tiles
 
 // Rounds and stores two groups of 8 dimensions of a row.  The half-waves hold 4
 // dimensions each of both; the lower takes the first whole and the upper the
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int cls = (int)blockIdx.x % a.classes;
   const int wg = (int)blockIdx.x / a.classes;
-  const PagedLine<kChunkRows, kBlockN> line(a, threadIdx.x & 63, SPLIT);
+  const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, SPLIT);
   const int total = line.total();
   const PagedStretch stretch(a, total, SPLIT ? kChunkMinTiles : 1);
   if (wg >= stretch.active) return;
@@ -193,18 +194,21 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   do {
   const PagedSeq s = line.seq(b);
   const int blocks = paged_blocks<kChunkRows>(a, s);
-  const int line_tiles = line.tiles_of(s);
+  const int unit_len = line.unit_of(s);
   const int len = line.length_of(s);
   if (pos >= seq_start + len) {  // on to the next sequence
     seq_start += len;
     if (++b >= a.batch) return;
     continue;
   }
-  const int unit = (pos - seq_start) / line_tiles;
-  const int first = pos - seq_start - unit * line_tiles;  // on the line
-  const int here = SPLIT ? min(line_tiles - first, end - pos) : 1;
-  const bool whole = !SPLIT || here == line_tiles;
-  pos += here;
+  const int unit = (pos - seq_start) / unit_len;
+  const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
+  const int u1 = seq_start + (unit + 1) * unit_len;
+  const int first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
+  pos = SPLIT ? min(u1, end) : u1;
+  const int stop = pos - u0;
+  if (SPLIT && stop <= 0) break;
+  const bool whole = !SPLIT || (first == 0 && pos == u1);
   const int hc = blocks == 1 ? unit : unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int hkv = hc * a.classes + cls;
@@ -229,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int kv_len = a.causal ? uniform(clamp_int(past + last_tok + 1, 0, s.keys)) : s.keys;
   const int block_tiles = (kv_len + kBlockN - 1) / kBlockN;
   const int tile0 = SPLIT ? first : 0;
-  const int tile_end = SPLIT ? min(block_tiles, first + here) : block_tiles;
+  const int tile_end = SPLIT ? min(block_tiles, stop) : block_tiles;
   // The last key this lane's row sees; keys below wave_full are seen by every row of
   // the wave.
   const int tok = row_of(min(row, nrows - 1) - q0).token - s.t0;
@@ -697,8 +701,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   }
   if constexpr (SPLIT) {
     if (!whole) {
-      const int u0 = seq_start + unit * line_tiles;
-      const PagedPieces pieces(stretch, u0, u0 + line_tiles);
+      const PagedPieces pieces(stretch, u0, u1);
       if (chunk_merges_itself(pieces.count, D) &&
           last_to_finish(a, pieces, cls, 2 * (int)blockIdx.x + (first == 0 ? 1 : 0), (int*)k_lds0))
         for (int pair = 0; pair < D / 16; pair += 4)
@@ -720,18 +723,18 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   __shared__ float xml[kWaves][2][64];
   const int cls = (int)blockIdx.x % a.classes;
   const int wg = (int)blockIdx.x / a.classes;
-  const PagedLine<kChunkRows, kBlockN> line(a, threadIdx.x & 63, true);
+  const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, true);
   const PagedStretch stretch(a, line.total(), kChunkMinTiles);
   if (wg == 0 || wg >= stretch.active) return;
   const int border = stretch.start(wg);
   int seq_start;
   const int b = uniform(line.find(border, seq_start));
   const PagedSeq s = line.seq(b);
-  const int tiles = line.tiles_of(s);
-  const int unit = (border - seq_start) / tiles;
-  const int u0 = seq_start + unit * tiles;
-  if (border == u0) return;
-  const PagedPieces pieces(stretch, u0, u0 + tiles);
+  const int unit_len = line.unit_of(s);
+  const int unit = (border - seq_start) / unit_len;
+  const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
+  if (border <= u0) return;
+  const PagedPieces pieces(stretch, u0, seq_start + (unit + 1) * unit_len);
   if (chunk_merges_itself(pieces.count, D)) return;
   const int blocks = paged_blocks<kChunkRows>(a, s);
   const int hc = unit / blocks;

@@ -34,31 +34,42 @@ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& 
 // The line of a class of KV heads (every classes-th head): the units of its
 // sequences (blocks of R rows, for each head) end to end, each as long as its sequence
 // has tiles of T keys (one at least, so that the rows of a sequence without keys are
-// written too), or with tiles false of length one.  Below 2^31 in all (the launcher
-// sees to it).  Called by whole waves; the first 64 sequences, one a lane, are
+// written too) and, where the sequences' lengths differ, H more in front of them, about
+// what it costs a workgroup to begin another unit (where they are equal the borders
+// of stretches often meet the units', which H would undo); or with tiles false of
+// length one.  Below 2^31 in all (the launcher sees to it).  Called by whole waves; the first 64 sequences, one a lane, are
 // looked at once.
-template <int R, int T>
+template <int R, int T, int H>
 struct PagedLine {
   const PagedArgs& a;
   const int lane, heads;
   const bool by_tiles;
+  int ahead;     // H or 0: a unit's first `ahead` are no tiles
   PagedSeq own;  // sequence `lane`
   int first;     // prefix(0)
 
   __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln, bool tiles)
       : a(args), lane(ln), heads(args.hkv / args.classes), by_tiles(tiles) {
     own = look(lane);
+    ahead = 0;
+    if (tiles) {
+      const int t = (own.keys + T - 1) / T;
+      const uint64_t there = __builtin_amdgcn_ballot_w64(own.n > 0);
+      const int t0 = there != 0 ? wave_bcast(t, __builtin_ctzll(there)) : 0;
+      if (__builtin_amdgcn_ballot_w64(own.n > 0 && t != t0) != 0) ahead = H;
+    }
     first = wave_prefix(length_of(own));
   }
   __device__ __forceinline__ PagedSeq look(int b) const {
     if (b < a.batch) return paged_seq(a, b, [](const int32_t* p) { return *p; });
     return PagedSeq{0, 0, 0, 0};
   }
-  __device__ __forceinline__ int tiles_of(const PagedSeq& s) const {
-    return by_tiles ? max(1, (s.keys + T - 1) / T) : 1;
+  // A unit's length on the line.
+  __device__ __forceinline__ int unit_of(const PagedSeq& s) const {
+    return by_tiles ? ahead + max(1, (s.keys + T - 1) / T) : 1;
   }
   __device__ __forceinline__ int length_of(const PagedSeq& s) const {
-    return heads * paged_blocks<R>(a, s) * tiles_of(s);
+    return heads * paged_blocks<R>(a, s) * unit_of(s);
   }
   // Inclusive prefix sum of the lengths of sequences b0 + lane.
   __device__ __forceinline__ int prefix(int b0) const {
@@ -111,7 +122,7 @@ struct PagedStretch {
   }
 };
 
-// The workgroups a unit on [u0, u1) of the line was cut into: from first on, each
+// The workgroups a unit whose tiles are [u0, u1) of the line was cut into: from first on, each
 // with its record number slot(i) of the workspace.  A stretch starts inside at most one
 // unit that it does not start with, and ends inside at most one: two records.
 struct PagedPieces {
