@@ -58,7 +58,7 @@ struct PagedArgs {
   int split;
   float* part_o;
   float* part_ml;
-  uint64_t* flags;  // one for each of the two records of a workgroup
+  uint64_t* flags;  // one for each of the two records of a workgroup, and one more
   uint64_t mark;    // what a written record's flag holds (merge_mark)
   int units;        // the most units a class can have
   int resident;     // the chunk kernel's workgroups of a class that run at once

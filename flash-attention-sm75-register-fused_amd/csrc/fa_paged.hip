@@ -24,6 +24,7 @@ namespace {
 int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
   return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
 }
+constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 16 bytes
 }  // namespace
 
 // Whether a line of `units` units stays below 2^31 tiles.
@@ -44,11 +45,11 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace
   p.units = (int)(heads * ((rows + (p.rows - 1ll) * std::min(a.batch, a.tokens)) / p.rows));
   const int64_t record = partial_bytes(p.rows, head_dim) * p.classes;
   const int64_t wgs = std::min<int64_t>(p.resident = resident_fused_workgroups() / p.classes,
-                                        workspace_bytes / record);
+                                        (workspace_bytes - kCombineWord) / record);
   p.split = least < wgs && fits_line(a, p.units, kBlockN, kChunkAhead);
   p.combine = p.split;
   p.wgs = p.split ? (int)wgs : p.units;
-  p.workspace_bytes = p.split ? p.wgs * record : 0;
+  p.workspace_bytes = p.split ? p.wgs * record + kCombineWord : 0;
   return p;
 }
 
@@ -64,7 +65,7 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   // 41.0, 8 bits 32.1 / 32.4; 8 to 8192 keys without grouping d128 8 bits 29.3 / 33.5):
   // stretches are shorter and more of them end inside a unit.
   const int64_t resident = resident_fused_workgroups();
-  const int64_t room = workspace_bytes / (partial_bytes(p.rows, head_dim) * p.classes);
+  const int64_t room = (workspace_bytes - kCombineWord) / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
   // Units of a class: blocks of rows, the last of each sequence not full.
   const int64_t blocks =
@@ -75,7 +76,7 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   p.split = p.wgs > 0 && p.units <= 16 * resident / p.classes && fits_line(a, p.units, kPTile, kPAhead);
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
-      p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) : 0;
+      p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) + kCombineWord : 0;
   // Stretches are kPMinTiles long at least, and there are wgs of them.
   const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + kPTile - 1) / kPTile;
   const int64_t pieces = std::min<int64_t>(p.wgs, tiles / kPMinTiles + 2);
@@ -112,7 +113,7 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + 2 * grid * plan.rows * head_dim;
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);
-    a.mark = merge_mark(a.flags, 2 * grid, stream);
+    a.mark = merge_mark(a.flags, 2 * grid + 1, stream);
   }
   const bool fp8 = a.ks != nullptr;
 #define FA_PAGED(D)                                                                     \

@@ -44,7 +44,10 @@ namespace {
 
 constexpr int kPTile = 32;       // keys of a wave's tile
 constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below
-constexpr int kPAhead = 3;       // another unit's cost, in tiles
+// Another unit's cost, in tiles (us without and with: 4 sequences of 2048 to 4096 keys d128
+// 8 bits 19.6 / 16.0, 32 of 4096 to 8192 132.0 / 130.5, 8 bits 68.8 / 68.0, 16 of 16384 to
+// 32768 d64 36.6 / 37.2; 8 of 8192 each d128, where it does not count, 45.2, with it 47.8).
+constexpr int kPAhead = 3;
 
 // Whether a unit's last workgroup merges its partials: one workgroup reads them
 // at about 50 bytes/ns, and the second kernel costs a launch 2.5 us where it has
@@ -437,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     const PagedPieces pieces(stretch, u0, u1);
     const int nr = min(R, nrows - rb * R);
     if (!paged_merges_itself(pieces.count, nr, D)) {
+      ask_combine(a);
       __syncthreads();
       continue;
     }
@@ -503,6 +507,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   constexpr int GROUPS = kThreads / LR;   // pieces at once
   __shared__ float4v xo[kThreads];
   __shared__ float xm[2][kThreads];
+  if (!combine_asked(a)) return;
   const int cls = (int)blockIdx.x % a.classes;
   const int index = (int)blockIdx.x / a.classes;  // of the class's units
   const PagedLine<R, kPTile, kPAhead> line(a, threadIdx.x & 63, true);

@@ -159,9 +159,10 @@ int make_forward(const fa_paged_params* p, fa::PagedArgs* a, bool* empty) {
   return FA_OK;
 }
 
+// (a checked call's: tokens > 0)
 int64_t longest_query(const fa_paged_params* p) {
   if (p->cu_seqlens == nullptr) return 1;
-  return p->max_query_len > 0 ? p->max_query_len : p->tokens;
+  return p->max_query_len > 0 && p->max_query_len < p->tokens ? p->max_query_len : p->tokens;
 }
 
 }  // namespace

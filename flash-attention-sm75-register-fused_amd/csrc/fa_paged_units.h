@@ -232,6 +232,16 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
+// The word behind the flags: whether some unit's partials are left to the second
+// kernel, whose workgroups else end at once.
+__device__ __forceinline__ uint64_t* combine_word(const PagedArgs& a) {
+  return a.flags + 2 * (int64_t)a.wgs * a.classes;
+}
+__device__ __forceinline__ void ask_combine(const PagedArgs& a) {
+  if (threadIdx.x == 0) *combine_word(a) = a.mark;
+}
+__device__ __forceinline__ bool combine_asked(const PagedArgs& a) { return *combine_word(a) == a.mark; }
+
 // Sets the flag of a workgroup's record, whose partials its waves have stored
 // coherently, and says whether every piece's flag of the unit is set (at most kThreads
 // pieces).  `scratch`: kWaves ints of LDS that the workgroup is done with.  A

@@ -192,7 +192,7 @@ def test_peaked(device):
 def test_max_query_len_is_a_hint(device):
     """Wrong values of it choose another kernel and nothing else."""
     c = Cache([150, 200], 2, 64, 16, BF16, False, news=[60, 1])
-    for hint in (1, 5, 60, 61, 10 ** 9):
+    for hint in (1, 5, 60, 61, 10 ** 9, 2 ** 63 - 1):
         attend(c, device, 8, max_query_len=hint)
 
 

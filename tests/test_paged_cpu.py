@@ -192,6 +192,19 @@ def test_forward_nulls_and_empty_calls(lib):
     assert lib.fa_sm75_paged_forward(ctypes.byref(params(cache(heads_kv=0)))) == 3
 
 
+def test_workspace_sizes(lib):
+    """Of the sizes alone, whole 16 bytes, none for a call that cannot split."""
+    c = cache(batch=4, heads_kv=8, head_dim=128, max_pages=512, block_table_stride=512,
+              **{f"{t}_stride_n": 128 for t in "kv"})
+    size = lambda **kw: lib.fa_sm75_paged_workspace_size(ctypes.byref(params(c, heads_q=32, **kw)))  # noqa: E731
+    one = size(tokens=4)
+    assert one > 0 and one % 16 == 0
+    few, chunk = size(tokens=16, cu_seqlens=0x1000, max_query_len=4), size(tokens=256, cu_seqlens=0x1000)
+    assert few > 0 and few % 16 == 0 and chunk > 0 and chunk % 16 == 0
+    assert size(tokens=256, cu_seqlens=0x1000, max_query_len=2 ** 63 - 1) == chunk
+    assert size(tokens=1 << 20, cu_seqlens=0x1000) == 0  # a workgroup for each block fills the GPU
+
+
 # ---- the Python calls ------------------------------------------------------------
 
 
