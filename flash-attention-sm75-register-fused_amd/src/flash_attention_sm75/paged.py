@@ -32,10 +32,9 @@ import torch
 import flash_attn_sm75_cuda as _C
 
 
-def _refuse_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() "
-                           "or on detached tensors")
+def _no_backward(name):
+    return RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() "
+                        "or on detached tensors")
 
 
 def paged_cache_write(K, V, k_cache, v_cache, block_table, seq_lens, cu_seqlens=None,
@@ -59,7 +58,9 @@ def paged_cache_write(K, V, k_cache, v_cache, block_table, seq_lens, cu_seqlens=
     Sequences of one call that share a page must not write the same positions
     of it (which of their values stays is not defined).
     """
-    _refuse_grad("paged_cache_write", K, V, k_cache, v_cache)
+    if torch.is_grad_enabled() and (K.requires_grad or V.requires_grad or k_cache.requires_grad
+                                    or v_cache.requires_grad):
+        raise _no_backward("paged_cache_write")
     _C.paged_cache_write(K, V, k_cache, v_cache, block_table, seq_lens, cu_seqlens, k_scale, v_scale)
 
 
@@ -75,7 +76,8 @@ def paged_cache_read(k_cache, v_cache, block_table, seq_lens, max_len=None, k_sc
         (K, V), each [B, H_kv, max_len, D]: what :func:`flash_attention_forward_ex`
         takes, zeros past a sequence's end and where it has no page.
     """
-    _refuse_grad("paged_cache_read", k_cache, v_cache)
+    if torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad):
+        raise _no_backward("paged_cache_read")
     if max_len is None:
         max_len = block_table.size(1) * k_cache.size(2) if block_table.dim() == 2 and k_cache.dim() == 4 else 0
     return _C.paged_cache_read(k_cache, v_cache, block_table, seq_lens, int(max_len), k_scale, v_scale,
@@ -106,7 +108,9 @@ def flash_attention_paged(Q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
         O [tokens, H_q, D] in Q's dtype, or (O, LSE).  A query that sees no key gets
         a zero row and LSE -inf.  Deterministic: the same call gives the same bits.
     """
-    _refuse_grad("flash_attention_paged", Q, k_cache, v_cache)
+    if torch.is_grad_enabled() and (Q.requires_grad or k_cache.requires_grad
+                                    or v_cache.requires_grad):
+        raise _no_backward("flash_attention_paged")
     if causal is False:
         code = 0
     elif causal == "bottom_right":
