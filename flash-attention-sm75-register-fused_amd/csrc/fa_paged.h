@@ -52,9 +52,12 @@ struct PagedArgs {
   int causal;    // token i of n of a sequence of len tokens sees key j iff j <= len - n + i
   float c;       // |scale| * log2(e), clamped away from 0
   int negate_q;  // scale < 0
-  // Plan: `classes` sequences of workgroups, class x holding KV heads x, x +
-  // classes, ...; wgs of them in each class (split), or one for each unit.
-  int classes, wgs;
+  // Quotients that every workgroup would begin with.
+  float inv_group;  // 1 / group
+  float rescale;    // kRescaleLog2 / c
+  // Plan: `classes` (2^class_shift) sequences of workgroups, class x holding the `heads` KV
+  // heads x, x + classes, ...; wgs of them in each class (split), or one for each unit.
+  int classes, class_shift, heads, wgs;
   int split;
   float* part_o;
   float* part_ml;
@@ -122,14 +125,16 @@ struct PagedSeq {
 template <class Load>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load load) {
   PagedSeq s;
+  const int len = load(a.lens + b);  // (all loads together)
   if (a.cu != nullptr) {
-    s.t0 = clamp_int(load(a.cu + b), 0, a.tokens);
-    s.n = clamp_int(load(a.cu + b + 1), s.t0, a.tokens) - s.t0;
+    const int t0 = load(a.cu + b), t1 = load(a.cu + b + 1);
+    s.t0 = clamp_int(t0, 0, a.tokens);
+    s.n = clamp_int(t1, s.t0, a.tokens) - s.t0;
   } else {
     s.t0 = min(b, a.tokens);
     s.n = b < a.tokens ? 1 : 0;
   }
-  s.len = max(0, load(a.lens + b));
+  s.len = max(0, len);
   s.keys = min(s.len, a.max_pages << a.page_shift);
   return s;
 }

@@ -103,7 +103,11 @@ void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t strea
 int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int head_dim,
                            void* workspace, hipStream_t stream) {
   PagedArgs a = args;
-  a.classes = plan.classes;
+  a.classes = plan.classes;  // (divides kNumXcds, a power of two)
+  a.class_shift = __builtin_ctz(plan.classes);
+  a.heads = a.hkv / a.classes;
+  a.inv_group = 1.0f / (float)a.group;
+  a.rescale = kRescaleLog2 / a.c;
   a.wgs = plan.wgs;
   a.units = plan.units;
   a.resident = plan.resident;

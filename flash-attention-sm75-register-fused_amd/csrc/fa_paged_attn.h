@@ -27,7 +27,8 @@
 // the workgroups of one XCD share heads) are laid end to end as a line of 32-key
 // tiles, and each of the class's workgroups takes an equal stretch of the line,
 // whatever mixture of sequences it covers: a batch of very different lengths
-// keeps every CU busy to the end.  A unit cut by a stretch's border leaves
+// keeps every CU busy to the end.  (Units that are all equally long are cut each for
+// itself instead, see PagedStretch.)  A unit cut by a stretch's border leaves
 // partials (O, max, sum) in the workspace, at most two for each workgroup.  Where
 // they are few bytes the unit's last workgroup to finish merges them, else
 // a second kernel does.  Stretches follow from the lengths alone, and partials
@@ -83,14 +84,17 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l16 = lane & 15;
   const int g4 = lane >> 4;
-  const int cls = (int)blockIdx.x % a.classes;
-  const int wg = (int)blockIdx.x / a.classes;
+  const int cls = (int)blockIdx.x & (a.classes - 1);
+  const int wg = (int)(blockIdx.x >> a.class_shift);
 
   const PagedLine<R, kPTile, kPAhead> line(a, lane, a.split != 0);
-  const PagedStretch stretch(a, line.total(), a.split ? kPMinTiles : 1);
+  const int total = line.total();
+  PagedStretch stretch = a.split ? PagedStretch(a, total, line.same, kPAhead, PagedStretch::Least<kPMinTiles>{})
+                                 : PagedStretch(a, total, 0, 0, PagedStretch::Least<1>{});
   if (wg >= stretch.active) return;
-  int pos = stretch.start(wg);
-  const int end = stretch.start(wg + 1);
+  int pos, end;
+  stretch.of(wg, pos, end);
+  asm volatile("" : "+v"(stretch.len), "+v"(stretch.cuts));  // (few scalar registers are left)
   int seq_start;
   int b = uniform(line.find(pos, seq_start));
 
@@ -119,19 +123,20 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     const int blocks = paged_blocks<R>(a, s);
     const int unit_len = line.unit_of(s);
     const int len = line.length_of(s);
-    if (pos >= seq_start + len) {  // on to the next sequence
+    if (pos >= seq_start + len || len == 0) {  // on to the next sequence
       seq_start += len;
       if (++b >= a.batch) return;
       continue;
     }
-    const int unit = (pos - seq_start) / unit_len;
+    const int unit = line.unit_at(pos - seq_start, unit_len, blocks);
     const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
     const int u1 = seq_start + (unit + 1) * unit_len;
     const int first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
+    if (u1 <= pos) return;  // (wrapped round)
     pos = min(u1, end);
     const int stop = pos - u0;
     if (stop <= 0) break;
-    const int hc = blocks == 1 ? unit : unit / blocks;
+    const int hc = blocks == 1 ? unit : (int)((unsigned)unit / (unsigned)blocks);
     const int rb = unit - hc * blocks;
     const int hkv = hc * a.classes + cls;
     const bool whole = first == 0 && pos == u1;
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
           for (int mt = 0; mt < MT; ++mt) o[nt][mt] *= alpha;
           m_run[nt] = m_new;
           mc[nt] = m_use * c2;
-          thr[nt] = m_new + kRescaleLog2 / c2;
+          thr[nt] = m_new + a.rescale;
         }
         uint4v pw;
 #pragma unroll
@@ -380,6 +385,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     // No direct load is in flight into a V tile any more, and no wave reads one.
     if constexpr (!FP8) wait_loads<0>();
     __syncthreads();
+    // What depends on the thread from here on is derived from an opaque index, so that none
+    // of it is made ready ahead of the tiles or kept through them.
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int t16 = tid & 15, t4 = (tid & 63) >> 4;
     // O of column c (16 of them to an array), 16-byte chunk d at d ^ c.
     auto o_at = [&](int w, int c, int chunk) -> float4v* {
       float* const base = (float*)(c < 16 || !TWO ? v_lds0 : v_lds1) + w * 16 * D;
@@ -390,17 +400,17 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       float l = l_run[nt];
       l += __shfl_xor(l, 16);
       l += __shfl_xor(l, 32);
-      const int c = 16 * nt + l16;
+      const int c = 16 * nt + t16;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) *o_at(wave, c, 4 * mt + g4) = o[nt][mt];
-      if (g4 == 0) {
+      for (int mt = 0; mt < MT; ++mt) *o_at(wave, c, 4 * mt + t4) = o[nt][mt];
+      if (t4 == 0) {
         ml_lds[wave][0][c] = m_run[nt];
         ml_lds[wave][1][c] = l;
       }
     }
     __syncthreads();
     // Thread: 4 dimensions of one column, columns in turns.
-    for (int it = threadIdx.x; it < R * (D / 4); it += kThreads) {
+    for (int it = tid; it < R * (D / 4); it += kThreads) {
       const int c = it / (D / 4), ch = it - c * (D / 4), dim = 4 * ch;
       const int r = rb * R + c;
       if (r >= nrows) continue;
@@ -437,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     }
 
     // ---- the unit's last workgroup merges its partials -------------------------
-    const PagedPieces pieces(stretch, u0, u1);
+    const PagedPieces pieces(stretch, a.wgs, u0, u1);
     const int nr = min(R, nrows - rb * R);
     if (!paged_merges_itself(pieces.count, nr, D)) {
       ask_combine(a);
@@ -449,11 +459,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     // meet in LDS.  More items than threads: one group, items in turns.
     const int items = nr * (D / 4);
     const int groups = max(1, min(kThreads / items, pieces.count));
-    const int grp = groups > 1 ? (int)threadIdx.x / items : 0;
+    const int grp = groups > 1 ? tid / items : 0;
     float4v* const xo = (float4v*)v_lds0;
     float* const xm = (float*)(v_lds0 + 8 * kThreads);  // max, then sum
     static_assert(kThreads * 24 <= 4 * VT * 2, "the merge's states fit the V tiles");
-    for (int it = (int)threadIdx.x - grp * items; grp < groups && it < items; it += kThreads) {
+    for (int it = tid - grp * items; grp < groups && it < items; it += kThreads) {
       const int c = it / (D / 4), ch = it - c * (D / 4);
       float m = -__builtin_inff(), l = 0.0f;
       float4v x = (float4v)0.0f;
@@ -472,25 +482,25 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
                                                                  (int)((rec * D + 4 * ch) * 4), 0, kPCoherent));
             });
       if (groups > 1) {
-        xo[threadIdx.x] = x;
-        xm[threadIdx.x] = m;
-        xm[kThreads + threadIdx.x] = l;
+        xo[tid] = x;
+        xm[tid] = m;
+        xm[kThreads + tid] = l;
       } else {
         store_row<BF16>(a, row_of(c), 4 * ch, m, l, x);
       }
     }
     __syncthreads();
-    if (groups > 1 && (int)threadIdx.x < items) {
+    if (groups > 1 && tid < items) {
       float m = -__builtin_inff(), l = 0.0f;
       float4v x = (float4v)0.0f;
-      for (int g = 0; g < groups; ++g) m = fmaxf(m, xm[g * items + threadIdx.x]);
+      for (int g = 0; g < groups; ++g) m = fmaxf(m, xm[g * items + tid]);
       for (int g = 0; g < groups; ++g) {
-        const float w = __builtin_amdgcn_exp2f(xm[g * items + threadIdx.x] - over_zero(m));
-        l += w * xm[kThreads + g * items + threadIdx.x];
-        x += w * xo[g * items + threadIdx.x];
+        const float w = __builtin_amdgcn_exp2f(xm[g * items + tid] - over_zero(m));
+        l += w * xm[kThreads + g * items + tid];
+        x += w * xo[g * items + tid];
       }
-      const int c = (int)threadIdx.x / (D / 4);
-      store_row<BF16>(a, row_of(c), 4 * ((int)threadIdx.x - c * (D / 4)), m, l, x);
+      const int c = tid / (D / 4);
+      store_row<BF16>(a, row_of(c), 4 * (tid - c * (D / 4)), m, l, x);
     }
     __syncthreads();
   }
@@ -508,8 +518,8 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   __shared__ float4v xo[kThreads];
   __shared__ float xm[2][kThreads];
   if (!combine_asked(a)) return;
-  const int cls = (int)blockIdx.x % a.classes;
-  const int index = (int)blockIdx.x / a.classes;  // of the class's units
+  const int cls = (int)blockIdx.x & (a.classes - 1);
+  const int index = (int)(blockIdx.x >> a.class_shift);  // of the class's units
   const PagedLine<R, kPTile, kPAhead> line(a, threadIdx.x & 63, true);
   const PagedLine<R, kPTile, kPAhead> units(a, threadIdx.x & 63, false);
   if (index >= units.total()) return;
@@ -519,8 +529,8 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   const int unit_len = line.unit_of(s);
   const int unit = index - unit_start;
   const int u0 = line.start_of(b) + unit * unit_len;
-  const PagedStretch stretch(a, line.total(), kPMinTiles);
-  const PagedPieces pieces(stretch, u0 + line.ahead, u0 + unit_len);
+  const PagedStretch stretch(a, line.total(), line.same, kPAhead, PagedStretch::Least<kPMinTiles>{});
+  const PagedPieces pieces(stretch, a.wgs, u0 + line.ahead, u0 + unit_len);
   if (pieces.count == 1) return;
   const int blocks = paged_blocks<R>(a, s);
   const int hc = unit / blocks;

@@ -38,7 +38,10 @@ namespace fa {
 namespace {
 
 constexpr int kChunkRows = 128;
-constexpr int kChunkMinTiles = 4;  // tiles a stretch is not cut below
+// Tiles a stretch is not cut below (us with 4, 5 and 6: one prompt of 320 tokens d128 17.9 /
+// 14.8 / 14.8, of 384 18.3 / 18.4 / 15.7, of 640 24.9 / 23.0 / 23.0, 64 tokens behind 936
+// 20.4 / 20.5 / 21.0).
+constexpr int kChunkMinTiles = 6;
 // Another unit's cost, in tiles (us without and with: 512 tokens of one sequence among 15
 // single ones of 1000 to 4096 keys d128 63.5 / 61.5, 777 of three of 1777 to 4000 d64
 // 51.9 / 51.3).
@@ -180,14 +183,14 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   __shared__ __attribute__((aligned(1024))) _Float16 v_lds1[L::Tile];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int cls = (int)blockIdx.x % a.classes;
-  const int wg = (int)blockIdx.x / a.classes;
+  const int cls = (int)blockIdx.x & (a.classes - 1);
+  const int wg = (int)(blockIdx.x >> a.class_shift);
   const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, SPLIT);
   const int total = line.total();
-  const PagedStretch stretch(a, total, SPLIT ? kChunkMinTiles : 1);
+  const PagedStretch stretch(a, total, line.same, kChunkAhead, PagedStretch::Least<SPLIT ? kChunkMinTiles : 1>{});
   if (wg >= stretch.active) return;
-  int pos = stretch.start(wg);
-  const int end = stretch.start(wg + 1);
+  int pos, end;
+  stretch.of(wg, pos, end);
   if constexpr (!SPLIT) {
     if (a.causal && total <= a.resident && pos >= a.resident / 2) pos = total - 1 + a.resident / 2 - pos;
   }
@@ -199,20 +202,21 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int blocks = paged_blocks<kChunkRows>(a, s);
   const int unit_len = line.unit_of(s);
   const int len = line.length_of(s);
-  if (pos >= seq_start + len) {  // on to the next sequence
+  if (pos >= seq_start + len || len == 0) {  // on to the next sequence
     seq_start += len;
     if (++b >= a.batch) return;
     continue;
   }
-  const int unit = (pos - seq_start) / unit_len;
+  const int unit = line.unit_at(pos - seq_start, unit_len, blocks);
   const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
   const int u1 = seq_start + (unit + 1) * unit_len;
   const int first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
+  if (SPLIT && u1 <= pos) return;  // (wrapped round)
   pos = SPLIT ? min(u1, end) : u1;
   const int stop = pos - u0;
   if (SPLIT && stop <= 0) break;
   const bool whole = !SPLIT || (first == 0 && pos == u1);
-  const int hc = blocks == 1 ? unit : unit / blocks;
+  const int hc = blocks == 1 ? unit : (int)((unsigned)unit / (unsigned)blocks);
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int hkv = hc * a.classes + cls;
 
@@ -419,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       for (int mt = 0; mt < MT; ++mt) oacc[mt] *= alpha;
       m_run = m_new;
       mc = m_use * c2;
-      thr = m_new + kRescaleLog2 / c2;
+      thr = m_new + a.rescale;
     }
   };
 
@@ -704,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   }
   if constexpr (SPLIT) {
     if (!whole) {
-      const PagedPieces pieces(stretch, u0, u1);
+      const PagedPieces pieces(stretch, a.wgs, u0, u1);
       if (!chunk_merges_itself(pieces.count, D)) {
         ask_combine(a);
       } else if (last_to_finish(a, pieces, cls, 2 * (int)blockIdx.x + (first == 0 ? 1 : 0), (int*)k_lds0)) {
@@ -727,22 +731,24 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   __shared__ float4v xo[kWaves][2][64];
   __shared__ float xml[kWaves][2][64];
   if (!combine_asked(a)) return;
-  const int cls = (int)blockIdx.x % a.classes;
-  const int wg = (int)blockIdx.x / a.classes;
+  const int cls = (int)blockIdx.x & (a.classes - 1);
+  const int wg = (int)(blockIdx.x >> a.class_shift);
   const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, true);
-  const PagedStretch stretch(a, line.total(), kChunkMinTiles);
+  const PagedStretch stretch(a, line.total(), line.same, kChunkAhead, PagedStretch::Least<kChunkMinTiles>{});
   if (wg == 0 || wg >= stretch.active) return;
-  const int border = stretch.start(wg);
+  int border, end;
+  stretch.of(wg, border, end);
   int seq_start;
   const int b = uniform(line.find(border, seq_start));
   const PagedSeq s = line.seq(b);
   const int unit_len = line.unit_of(s);
-  const int unit = (border - seq_start) / unit_len;
+  const int blocks = paged_blocks<kChunkRows>(a, s);
+  if (blocks == 0) return;
+  const int unit = line.unit_at(border - seq_start, unit_len, blocks);
   const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
   if (border <= u0) return;
-  const PagedPieces pieces(stretch, u0, seq_start + (unit + 1) * unit_len);
+  const PagedPieces pieces(stretch, a.wgs, u0, seq_start + (unit + 1) * unit_len);
   if (chunk_merges_itself(pieces.count, D)) return;
-  const int blocks = paged_blocks<kChunkRows>(a, s);
   const int hc = unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int rows = s.n * a.group - rb * kChunkRows;

@@ -28,7 +28,7 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // Blocks of R rows of a sequence: its units for one KV head.
 template <int R>
 __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& s) {
-  return (int)(((int64_t)s.n * a.group + R - 1) / R);
+  return (int)((unsigned)(s.n * a.group + R - 1) / R);  // (below 2^28)
 }
 
 // The line of a class of KV heads (every classes-th head): the units of its
@@ -37,39 +37,46 @@ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& 
 // written too) and, where the sequences' lengths differ, H more in front of them, about
 // what it costs a workgroup to begin another unit (where they are equal the borders
 // of stretches often meet the units', which H would undo); or with tiles false of
-// length one.  Below 2^31 in all (the launcher sees to it).  Called by whole waves; the first 64 sequences, one a lane, are
-// looked at once.
+// length one.  Below 2^31 in all (the launcher sees to it; only where cu_seqlens falls
+// again and again, so that sequences share rows, may positions wrap round, and then
+// units are held to those there are, and pieces to the workgroups).  Called by whole
+// waves; the first 64 sequences, one a lane, are looked at once.
 template <int R, int T, int H>
 struct PagedLine {
   const PagedArgs& a;
-  const int lane, heads;
+  const int lane;
   const bool by_tiles;
   int ahead;     // H or 0: a unit's first `ahead` are no tiles
+  int same;      // every unit's length, 0 where they differ or are not looked at
   PagedSeq own;  // sequence `lane`
   int first;     // prefix(0)
 
   __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln, bool tiles)
-      : a(args), lane(ln), heads(args.hkv / args.classes), by_tiles(tiles) {
+      : a(args), lane(ln), by_tiles(tiles) {
     own = look(lane);
     ahead = 0;
+    same = 0;
     if (tiles) {
-      const int t = (own.keys + T - 1) / T;
+      const int t = tiles_of(own);
       const uint64_t there = __builtin_amdgcn_ballot_w64(own.n > 0);
       const int t0 = there != 0 ? wave_bcast(t, __builtin_ctzll(there)) : 0;
       if (__builtin_amdgcn_ballot_w64(own.n > 0 && t != t0) != 0) ahead = H;
+      else if (a.batch <= 64) same = max(1, t0);
     }
     first = wave_prefix(length_of(own));
   }
   __device__ __forceinline__ PagedSeq look(int b) const {
-    if (b < a.batch) return paged_seq(a, b, [](const int32_t* p) { return *p; });
-    return PagedSeq{0, 0, 0, 0};
+    PagedSeq s = paged_seq(a, min(b, a.batch - 1), [](const int32_t* p) { return *p; });
+    if (b >= a.batch) s.n = 0;
+    return s;
   }
+  static __device__ __forceinline__ int tiles_of(const PagedSeq& s) { return (int)((unsigned)(s.keys + T - 1) / T); }
   // A unit's length on the line.
   __device__ __forceinline__ int unit_of(const PagedSeq& s) const {
-    return by_tiles ? ahead + max(1, (s.keys + T - 1) / T) : 1;
+    return by_tiles ? ahead + max(1, tiles_of(s)) : 1;
   }
   __device__ __forceinline__ int length_of(const PagedSeq& s) const {
-    return heads * paged_blocks<R>(a, s) * unit_of(s);
+    return a.heads * paged_blocks<R>(a, s) * unit_of(s);
   }
   // Inclusive prefix sum of the lengths of sequences b0 + lane.
   __device__ __forceinline__ int prefix(int b0) const {
@@ -98,6 +105,10 @@ struct PagedLine {
       before += wave_bcast(x, 63);
     }
   }
+  // The unit (of sequence s, `blocks` of them for each head) at rel from its start.
+  __device__ __forceinline__ int unit_at(int rel, int unit_len, int blocks) const {
+    return uniform((int)min((unsigned)rel / (unsigned)unit_len, (unsigned)(a.heads * blocks - 1)));
+  }
   // Where sequence b starts.
   __device__ __forceinline__ int start_of(int b) const {
     int before = 0;
@@ -106,19 +117,54 @@ struct PagedLine {
   }
 };
 
-// The stretches of a class's line, one for each workgroup of it: total / active tiles
-// long, the first ones a tile longer, and no shorter than `least` tiles.
+// The stretches of a class's line, one for each workgroup of it, and no shorter than `least`
+// tiles: of the whole line, total / active tiles each, or of every unit for itself where
+// all are equally long and that leaves a workgroup at most `more` tiles more, which is
+// what its beginning another unit costs (us, of the line and of units: one prompt of 448 tokens
+// d128 28.6 / 19.2, of 700 31.9 / 24.5, of 900 d64 8 bits 26.4 / 19.3; one token of 16
+// sequences of 4128 keys d128 8 bits 34.6 / 31.9, of 32 16 bits 86.0 / 82.1).  The first
+// ones of the line, or unit, are a tile longer.
 struct PagedStretch {
-  int size, active, longer;
-  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int total, int least) {
-    active = min(a.wgs, (total + least - 1) / least);
-    size = active > 0 ? total / active : 0;
-    longer = total - size * active;
+  int active;
+  int len, cuts;  // what is cut, and into how many
+  // LEAST: a constant, 1 where a stretch is a unit.
+  template <int LEAST>
+  struct Least {};
+  template <int LEAST>
+  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int total, int same, int more, Least<LEAST>) {
+    active = min(a.wgs, (total + LEAST - 1) / LEAST);
+    len = total;
+    cuts = active;
+    if (same > 0 && active > 0) {
+      // (a quotient past 2^21, where this is not exact, is more than there are workgroups)
+      const int count = max(1, (int)rintf((float)total * __builtin_amdgcn_rcpf((float)same)));
+      const int q = min(small_quotient(a.wgs, count), (int)((unsigned)(same + LEAST - 1) / LEAST));
+      if (q > 0 && same <= (int64_t)q * ((int)((unsigned)total / (unsigned)active) + more)) {
+        len = same;
+        cuts = q;
+        active = count * q;
+      }
+    }
+    active = uniform(active);
+    len = uniform(len);
+    cuts = uniform(cuts);
   }
-  __device__ __forceinline__ int start(int wg) const { return wg * size + min(wg, longer); }
+  // x / y, x below 2^21 (x + 0.5 is 0.5 / y at least off a multiple of y).
+  static __device__ __forceinline__ int small_quotient(int x, int y) {
+    return (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)y));
+  }
+  // Workgroup wg's (below active) stretch [pos, end).
+  __device__ __forceinline__ void of(int wg, int& pos, int& end) const {
+    const int u = wg < cuts ? 0 : small_quotient(wg, cuts), i = wg - u * cuts;
+    const int size = (int)((unsigned)len / (unsigned)cuts), longer = len - size * cuts;
+    pos = uniform(u * len + i * size + min(i, longer));
+    end = uniform(pos + size + (i < longer ? 1 : 0));
+  }
   __device__ __forceinline__ int holder(int pos) const {  // the workgroup of a position
-    const int p = pos - longer * (size + 1);
-    return p < 0 ? pos / (size + 1) : longer + p / size;
+    const int u = pos < len ? 0 : (int)((unsigned)pos / (unsigned)len), x = pos - u * len;
+    const int size = (int)((unsigned)len / (unsigned)cuts), longer = len - size * cuts;
+    const int p = x - longer * (size + 1);
+    return u * cuts + (int)(p < 0 ? (unsigned)x / (unsigned)(size + 1) : longer + (unsigned)p / (unsigned)size);
   }
 };
 
@@ -127,9 +173,14 @@ struct PagedStretch {
 // unit that it does not start with, and ends inside at most one: two records.
 struct PagedPieces {
   int first, count;
-  __device__ __forceinline__ PagedPieces(const PagedStretch& st, int u0, int u1) {
+  __device__ __forceinline__ PagedPieces(PagedStretch st, int wgs, int u0, int u1) {
+    // (opaque: what its divisions begin with is not to be made ready ahead of each launch)
+    asm volatile("" : "+v"(st.len), "+v"(st.cuts));
     first = st.holder(u0);
     count = st.holder(u1 - 1) - first + 1;
+    // (no change but on a line past 2^31, see PagedLine)
+    first = uniform(clamp_int(first, 0, wgs - 1));
+    count = uniform(clamp_int(count, 1, wgs - first));
   }
   __device__ __forceinline__ int slot(const PagedArgs& a, int cls, int i) const {
     return 2 * ((first + i) * a.classes + cls) + (i == 0 ? 1 : 0);
@@ -148,11 +199,16 @@ struct PagedRows {
   float inv;
   __device__ __forceinline__ PagedRows(const PagedArgs& a, const PagedSeq& s, int hkv, int r0) {
     group = a.group;
-    const int i = r0 == 0 ? 0 : r0 / group;
+    int i = 0;
+    if (r0 != 0) {
+      int g = group;
+      asm volatile("" : "+s"(g));  // (so too)
+      i = uniform((int)((unsigned)r0 / (unsigned)g));
+    }
     tok0 = s.t0 + i;
     rem0 = r0 - i * group;
     head0 = hkv * group;
-    inv = 1.0f / (float)group;
+    inv = a.inv_group;
   }
   __device__ __forceinline__ PagedRow operator()(int c) const {
     const int x = rem0 + c;

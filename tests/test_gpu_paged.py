@@ -92,6 +92,25 @@ def test_many_blocks(device, d, q8):
     attend(Cache([1500, 65], 1, d, 32, FP16, q8, news=[190, 65]), device, 2, max_query_len=190)
 
 
+@pytest.mark.parametrize("d,q8", [(64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("batch", [1, 2, 5, 33])
+def test_equal_lengths(device, d, q8, batch):
+    """Sequences of one length: cut into equal pieces each where that suits, whatever the
+    number of tiles, and along the line else."""
+    for keys in (31, 257, 320, 385, 600, 1025, 2100):
+        n = min(keys, max(1, 140 // batch))
+        c = Cache([keys] * batch, 2, d, 16, BF16, q8, news=[n] * batch, seed=keys)
+        attend(c, device, 6, seed=keys)
+        attend(c, device, 6, seed=keys, causal=False)
+    c = Cache([4097] * min(batch, 5), 2, d, 16, BF16, q8)
+    attend(c, device, 8)
+
+
+def test_unequal_lengths_of_equal_tiles(device):
+    c = Cache([385, 400, 448, 447], 1, 128, 16, FP16, False, news=[40, 1, 448, 3])
+    attend(c, device, 4)
+
+
 @pytest.mark.parametrize("q8", [False, True])
 def test_missing_pages(device, q8):
     """Entries that name no page hide their keys: -1, past the pool, the type's limits."""
@@ -208,6 +227,23 @@ def test_index_tensors_are_held_to_their_ranges(device):
     lens = torch.tensor([-5, -2 ** 31], dtype=torch.int32, device=device)
     o = fa.flash_attention_paged(q, *args[:3], lens, cu_seqlens=c.cu.to(device), **kw)
     assert (o == 0).all()
+
+
+@pytest.mark.parametrize("batch,most", [(4096, 1), (9000, 1)])
+def test_overlapping_sequences_past_32_bits(device, batch, most):
+    """cu_seqlens that falls again and again makes more tiles than 32 bits count: what is
+    written is not said, but nothing outside the rows is, and the call ends."""
+    page, keys = 1 << 15, 1 << 23
+    k = torch.zeros(1, 1, page, 64, dtype=torch.float8_e4m3fn, device=device)
+    s = torch.full((1, 1, page), 127, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+    table = torch.zeros(1, keys // page, dtype=torch.int32, device=device).expand(batch, -1).contiguous()
+    lens = torch.full((batch,), keys, dtype=torch.int32, device=device)
+    cu = torch.tensor(([0, 64] * batch)[:batch + 1], dtype=torch.int32, device=device)
+    room = torch.full((192, 1, 64), 7.0, dtype=FP16, device=device)
+    q = torch.randn(64, 1, 64, dtype=FP16, device=device)
+    fa.flash_attention_paged(q, k, k.clone(), table, lens, cu_seqlens=cu, k_scale=s, v_scale=s,
+                             out=room[64:128], max_query_len=most)
+    assert (room[:64] == 7).all() and (room[128:] == 7).all()
 
 
 def test_nothing_to_do(device):
