@@ -158,6 +158,38 @@ __device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPiece
     a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
 }
 
+// A class's stretches.  Where all units are equally long, of units, each into the number q
+// of pieces that costs least, unless along the line it costs less yet.  The costs are in
+// tiles, fitted to timings (us at q = 1, 2, 3, ..: one prompt of 512 tokens d128 17.8, 19.2;
+// of 900 24.6, 28.0; 500 tokens behind 1500 -, 32.6, 35.6, 34.5; 64 behind 936 -, 23.4, 21.0,
+// 20.1; one prompt of 800 d64 18.4, 17.5, 16.1; along the line against units: one prompt of
+// 1700 tokens d128 50.2 / 42.7, three of 900 d64 32.4 / 24.6, 800 tokens behind 3200 d128
+// 66.2 / 68.2): two workgroups on a CU slow each other down by a quarter; the merge costs so
+// much a piece, the more the more workgroups do it, at most what the second kernel does;
+// along the line a workgroup begins two units and most are cut.
+template <int D, class Line>
+__device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const PagedArgs& a, const Line& line) {
+  const int total = line.total(), same = line.same;
+  PagedStretch<kChunkMinTiles> s(a, total);
+  if (same > 0 && s.active > 0) {
+    const int count = s.units(same);
+    const int q = line.lane + 1;  // a lane each
+    const float full = 1.0f / (float)a.wgs;
+    auto slowed = [&](int wgs) { return 1.0f + 0.25f * fmaxf(0.0f, 2.0f * (float)wgs * full - 1.0f); };
+    const int most = s.small_quotient(same + q - 1, q);
+    const float piece = D == 128 ? 1.0f + 2.5f * (float)(count * q) * full : 1.7f;
+    float cost = (float)most * slowed(count * q) + (q > 1 ? fminf(piece * (float)q, 14.0f) : 0.0f);
+    if (count > a.wgs / q) cost = __builtin_inff();
+    float least = cost;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) least = fminf(least, __shfl_xor(least, m));
+    const float along = (float)total / (float)s.active * slowed(s.active) + 10.0f;
+    const uint64_t at = __builtin_amdgcn_ballot_w64(cost == least);
+    if (least < along) s.cut_units(count, same, __builtin_ctzll(at) + 1);
+  }
+  return s;
+}
+
 template <int D, bool BF16, bool FP8, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
   constexpr bool DENSE = D == 64;
@@ -186,13 +218,16 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
   const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, SPLIT);
-  const int total = line.total();
-  const PagedStretch stretch(a, total, line.same, kChunkAhead, PagedStretch::Least<SPLIT ? kChunkMinTiles : 1>{});
+  const auto stretch = [&] {
+    if constexpr (SPLIT) return chunk_stretch<D>(a, line);
+    else return PagedStretch<1>(a, line.total());
+  }();
   if (wg >= stretch.active) return;
   int pos, end;
   stretch.of(wg, pos, end);
   if constexpr (!SPLIT) {
-    if (a.causal && total <= a.resident && pos >= a.resident / 2) pos = total - 1 + a.resident / 2 - pos;
+    if (a.causal && stretch.len <= a.resident && pos >= a.resident / 2)
+      pos = stretch.len - 1 + a.resident / 2 - pos;
   }
   int seq_start;
   int b = uniform(line.find(pos, seq_start));
@@ -734,7 +769,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
   const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, true);
-  const PagedStretch stretch(a, line.total(), line.same, kChunkAhead, PagedStretch::Least<kChunkMinTiles>{});
+  const auto stretch = chunk_stretch<D>(a, line);
   if (wg == 0 || wg >= stretch.active) return;
   int border, end;
   stretch.of(wg, border, end);

@@ -117,37 +117,29 @@ struct PagedLine {
   }
 };
 
-// The stretches of a class's line, one for each workgroup of it, and no shorter than `least`
-// tiles: of the whole line, total / active tiles each, or of every unit for itself where
-// all are equally long and that leaves a workgroup at most `more` tiles more, which is
-// what its beginning another unit costs (us, of the line and of units: one prompt of 448 tokens
-// d128 28.6 / 19.2, of 700 31.9 / 24.5, of 900 d64 8 bits 26.4 / 19.3; one token of 16
-// sequences of 4128 keys d128 8 bits 34.6 / 31.9, of 32 16 bits 86.0 / 82.1).  The first
-// ones of the line, or unit, are a tile longer.
+// The stretches of a class's line, one for each workgroup of it, and no shorter than LEAST
+// tiles: of the whole line, total / active tiles each, or (cut_units) of every unit for
+// itself where all are equally long.  The first ones of the line, or unit, are a tile
+// longer.
+template <int LEAST>
 struct PagedStretch {
   int active;
   int len, cuts;  // what is cut, and into how many
-  // LEAST: a constant, 1 where a stretch is a unit.
-  template <int LEAST>
-  struct Least {};
-  template <int LEAST>
-  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int total, int same, int more, Least<LEAST>) {
-    active = min(a.wgs, (total + LEAST - 1) / LEAST);
-    len = total;
+  __device__ __forceinline__ PagedStretch(const PagedArgs& a, int total) {
+    active = uniform(min(a.wgs, (total + LEAST - 1) / LEAST));
+    len = uniform(total);
     cuts = active;
-    if (same > 0 && active > 0) {
-      // (a quotient past 2^21, where this is not exact, is more than there are workgroups)
-      const int count = max(1, (int)rintf((float)total * __builtin_amdgcn_rcpf((float)same)));
-      const int q = min(small_quotient(a.wgs, count), (int)((unsigned)(same + LEAST - 1) / LEAST));
-      if (q > 0 && same <= (int64_t)q * ((int)((unsigned)total / (unsigned)active) + more)) {
-        len = same;
-        cuts = q;
-        active = count * q;
-      }
-    }
-    active = uniform(active);
-    len = uniform(len);
-    cuts = uniform(cuts);
+  }
+  // Units of a line of them that are `same` tiles long (a quotient past 2^21, where this is
+  // not exact, is more than there are workgroups).
+  __device__ __forceinline__ int units(int same) const {
+    return max(1, (int)rintf((float)len * __builtin_amdgcn_rcpf((float)same)));
+  }
+  // Every unit into q stretches.
+  __device__ __forceinline__ void cut_units(int count, int same, int q) {
+    active = uniform(count * q);
+    len = uniform(same);
+    cuts = uniform(q);
   }
   // x / y, x below 2^21 (x + 0.5 is 0.5 / y at least off a multiple of y).
   static __device__ __forceinline__ int small_quotient(int x, int y) {
@@ -173,7 +165,8 @@ struct PagedStretch {
 // unit that it does not start with, and ends inside at most one: two records.
 struct PagedPieces {
   int first, count;
-  __device__ __forceinline__ PagedPieces(PagedStretch st, int wgs, int u0, int u1) {
+  template <int LEAST>
+  __device__ __forceinline__ PagedPieces(PagedStretch<LEAST> st, int wgs, int u0, int u1) {
     // (opaque: what its divisions begin with is not to be made ready ahead of each launch)
     asm volatile("" : "+v"(st.len), "+v"(st.cuts));
     first = st.holder(u0);
