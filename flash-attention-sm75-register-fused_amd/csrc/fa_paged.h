@@ -65,6 +65,7 @@ struct PagedArgs {
   uint64_t mark;    // what a written record's flag holds (merge_mark)
   int units;        // the most units a class can have
   int resident;     // the chunk kernel's workgroups of a class that run at once
+  int pieces;       // most pieces the chunk kernel may cut a unit into, 0: any number
 };
 
 // Largest key count a block table may cover, and row stride (bytes) of a cache
@@ -82,7 +83,7 @@ struct PagedPlan {
   bool combine;       // some unit may have more partials than the kernel merges itself
   int units, y;       // of the combine kernel's grid
   bool chunk;         // units of 128 rows (fa_paged_chunk.h)
-  int resident;
+  int resident, pieces;
   int64_t workspace_bytes;
 };
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,

@@ -67,11 +67,11 @@ __device__ __forceinline__ void store_pair(_Float16* to, float4v x, float4v y, f
 }
 
 // Whether a unit's last workgroup merges its partials (it reads them at about 50
-// bytes/ns, 5 us for these many), or the second kernel.
-constexpr int kChunkMergeBytes = 256 << 10;
-__device__ __forceinline__ bool chunk_merges_itself(int pieces, int d) {
-  return (int64_t)pieces * kChunkRows * d * 4 <= kChunkMergeBytes;
-}
+// bytes/ns, 6 us for these many), or the second kernel.  Where a launch has units enough
+// (plan_chunks), stretches are made long enough that none has more, and the second
+// kernel is not launched.
+constexpr int kChunkMergeBytes = 320 << 10;
+constexpr int chunk_pieces(int d) { return kChunkMergeBytes / (kChunkRows * d * 4); }
 
 // A record of the workspace: a block's partials in the order its waves' registers
 // hold them, so that 64 lanes store and load 1 KB at once (row by row, 16 bytes of
@@ -171,6 +171,11 @@ template <int D, class Line>
 __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const PagedArgs& a, const Line& line) {
   const int total = line.total(), same = line.same;
   PagedStretch<kChunkMinTiles> s(a, total);
+  if (a.pieces > 0 && s.active > 0) {
+    // (a unit as long as pieces - 1 stretches lies in one more at most)
+    const int least = (int)((unsigned)(line.longest() + a.pieces - 2) / (unsigned)(a.pieces - 1));
+    s.active = s.cuts = uniform(min(s.active, max(1, (int)((unsigned)total / (unsigned)least))));
+  }
   if (same > 0 && s.active > 0) {
     const int count = s.units(same);
     const int q = line.lane + 1;  // a lane each
@@ -179,7 +184,7 @@ __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const Page
     const int most = s.small_quotient(same + q - 1, q);
     const float piece = D == 128 ? 1.0f + 2.5f * (float)(count * q) * full : 1.7f;
     float cost = (float)most * slowed(count * q) + (q > 1 ? fminf(piece * (float)q, 14.0f) : 0.0f);
-    if (count > a.wgs / q) cost = __builtin_inff();
+    if (count > a.wgs / q || (a.pieces > 0 && q > a.pieces)) cost = __builtin_inff();
     float least = cost;
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) least = fminf(least, __shfl_xor(least, m));
@@ -744,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   if constexpr (SPLIT) {
     if (!whole) {
       const PagedPieces pieces(stretch, a.wgs, u0, u1);
-      if (!chunk_merges_itself(pieces.count, D)) {
+      if (pieces.count > chunk_pieces(D)) {
         ask_combine(a);
       } else if (last_to_finish(a, pieces, cls, 2 * (int)blockIdx.x + (first == 0 ? 1 : 0), (int*)k_lds0)) {
         for (int pair = 0; pair < D / 16; pair += 4)
@@ -783,7 +788,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
   if (border <= u0) return;
   const PagedPieces pieces(stretch, a.wgs, u0, seq_start + (unit + 1) * unit_len);
-  if (chunk_merges_itself(pieces.count, D)) return;
+  if (pieces.count <= chunk_pieces(D)) return;
   const int hc = unit / blocks;
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int rows = s.n * a.group - rb * kChunkRows;

@@ -25,6 +25,17 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return x;
 }
 
+// The largest of the lanes' values (all 0 or more), in the same steps.
+__device__ __forceinline__ int wave_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return wave_bcast(x, 63);
+}
+
 // Blocks of R rows of a sequence: its units for one KV head.
 template <int R>
 __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& s) {
@@ -86,6 +97,15 @@ struct PagedLine {
     int sum = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) sum += wave_bcast(prefix(b0), 63);
     return sum;
+  }
+  // The longest unit's tiles, 1 at least.
+  __device__ __forceinline__ int longest() const {
+    int most = 1;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
+      most = max(most, wave_max(s.n > 0 ? tiles_of(s) : 0));
+    }
+    return most;
   }
   __device__ __forceinline__ PagedSeq seq(int b) const {
     if (b >= 64) return scalar_seq(a, b);

@@ -106,6 +106,15 @@ def test_equal_lengths(device, d, q8, batch):
     attend(c, device, 8)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_long_unit_among_short_ones(device, d):
+    """Units enough that each is merged by its last workgroup, the longest many times the others."""
+    c = Cache([9000] + [70] * 40, 1, d, 64, BF16, False, news=[300] + [70] * 40)
+    attend(c, device, 8)
+    c = Cache([33] * 3 + [6000], 2, d, 16, FP16, True, news=[33] * 3 + [1200])
+    attend(c, device, 8)
+
+
 def test_unequal_lengths_of_equal_tiles(device):
     c = Cache([385, 400, 448, 447], 1, 128, 16, FP16, False, news=[40, 1, 448, 3])
     attend(c, device, 4)
