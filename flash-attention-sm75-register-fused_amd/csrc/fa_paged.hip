@@ -30,7 +30,7 @@ constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 1
 // Whether a line of `units` units stays below 2^31 tiles.
 static bool fits_line(const PagedArgs& a, int64_t units, int tile, int ahead) {
   const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + tile - 1) / tile;
-  return units * (ahead + std::max<int64_t>(1, tiles)) <= INT32_MAX;
+  return units * (ahead + std::max<int64_t>(1, tiles)) <= INT32_MAX - 64;  // (room to round up)
 }
 
 // Units of 128 rows, cut into pieces where they may be fewer than the GPU runs at once.

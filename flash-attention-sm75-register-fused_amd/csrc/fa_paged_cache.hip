@@ -147,7 +147,11 @@ __global__ void __launch_bounds__(kCacheThreads) fa_paged_write_kernel(const Pag
 }
 
 // Rows of [batch, hkv, max_len, D] out of the pages; zeros where a sequence
-// has no token or its page is gone.
+// has no token or its page is gone.  D / 8 lanes a row, 16 bytes of the output each; a
+// thread has one row, whose reads depend on each other (length, page, row), and it is the
+// many waves that keep the memory busy: 4 sequences to 8192 tokens of 8 heads d128, 235 MB,
+// 46.6 us (5.0 TB/s, what a large copy reaches); 7 to 8191 of 2 heads d64 8 bits, 38 MB,
+// 8.6 us (4.4 TB/s).
 template <int D, bool BF16, bool FP8>
 __global__ void __launch_bounds__(kCacheThreads) fa_paged_read_kernel(const PagedArgs a) {
   constexpr int LANES = D / 8;
