@@ -56,7 +56,8 @@ def paged_cache_write(K, V, k_cache, v_cache, block_table, seq_lens, cu_seqlens=
 
     Rows behind cu_seqlens[B], and positions that have no page, are left out.
     Sequences of one call that share a page must not write the same positions
-    of it (which of their values stays is not defined).
+    of it (which of their values stays is not defined), and K and V must not be views of
+    the rows that are written.
     """
     if torch.is_grad_enabled() and (K.requires_grad or V.requires_grad or k_cache.requires_grad
                                     or v_cache.requires_grad):
@@ -107,9 +108,12 @@ def flash_attention_paged(Q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
     Returns:
         O [tokens, H_q, D] in Q's dtype, or (O, LSE).  A query that sees no key gets
         a zero row and LSE -inf.  Deterministic: the same call gives the same bits.
+        What lies in hidden pages and past a sequence's end reaches no query; a new token's
+        V row that is not finite can reach its sequence's earlier tokens of the same call
+        (0 times NaN, as in a plain product).
     """
-    if torch.is_grad_enabled() and (Q.requires_grad or k_cache.requires_grad
-                                    or v_cache.requires_grad):
+    if torch.is_grad_enabled() and (Q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                                    or (out is not None and out.requires_grad)):
         raise _no_backward("flash_attention_paged")
     if causal is False:
         code = 0

@@ -189,7 +189,7 @@ def test_scales(device, scale):
 @pytest.mark.parametrize("news", [[1, 1], [40, 3]])
 @pytest.mark.parametrize("q8", [False, True])
 def test_nonfinite_rows(device, news, q8):
-    """A query's NaN stays in its row; NaN in a key hidden from a query does not reach it."""
+    """A query's NaN stays in its row (and the pool's unused rows, which hold NaN, reach none)."""
     c = Cache([400, 90], 1, 64, 16, BF16, q8, news=news)
     (args, kw), g = c.args(device), torch.Generator().manual_seed(3)
     t = sum(news)
@@ -378,6 +378,23 @@ def test_read(device, d, q8, dtype, strided):
                 m = min(n, longest)
                 want[:, :m] = torch.where(held[:m, None], rows[:, :m], 0.0)
                 assert torch.equal(got[b].double().cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_read_every_code_and_scale(device, dtype):
+    """Any code times any scale, also ones that no write leaves: rounded to the type, NaN for byte 255."""
+    code = torch.arange(1024) % 4 * 64 + torch.arange(64)[:, None]
+    codes = code.T.to(torch.uint8).reshape(1, 1, 1024, 64).contiguous().view(torch.float8_e4m3fn)
+    byte = (torch.arange(1024) // 4).to(torch.uint8)
+    scale = byte.reshape(1, 1, 1024).view(torch.float8_e8m0fnu)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=device)
+    lens = torch.tensor([1024], dtype=torch.int32, device=device)
+    k, v = fa.paged_cache_read(codes.to(device), codes.to(device), table, lens, k_scale=scale.to(device),
+                               v_scale=scale.to(device), dtype=dtype)
+    factor = torch.exp2(byte.double() - 127).masked_fill(byte == 255, math.nan)
+    want = (codes[0, 0].float().double() * factor[:, None]).to(dtype)
+    for got in (k, v):
+        assert torch.equal(got[0, 0].cpu().nan_to_num(nan=-1.5), want.nan_to_num(nan=-1.5))
 
 
 def test_read_nothing(device):

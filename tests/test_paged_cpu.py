@@ -238,6 +238,8 @@ def test_python_refusals():
         fa.flash_attention_paged(leaf, *args)
     with pytest.raises(RuntimeError, match="no backward pass"):
         fa.paged_cache_write(leaf, x, *args)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        fa.flash_attention_paged(x, *args, out=leaf)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):  # past that check
         fa.flash_attention_paged(leaf, *args)
 
