@@ -66,6 +66,7 @@ struct PagedArgs {
   int units;        // the most units a class can have
   int resident;     // the chunk kernel's workgroups of a class that run at once
   int pieces;       // most pieces the chunk kernel may cut a unit into, 0: any number
+  int stream_v;     // the chunk kernel reads V non-temporally
 };
 
 // Largest key count a block table may cover, and row stride (bytes) of a cache
@@ -84,6 +85,7 @@ struct PagedPlan {
   int units, y;       // of the combine kernel's grid
   bool chunk;         // units of 128 rows (fa_paged_chunk.h)
   int resident, pieces;
+  bool stream_v;
   int64_t workspace_bytes;
 };
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,

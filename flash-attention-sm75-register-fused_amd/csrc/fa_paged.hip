@@ -24,6 +24,7 @@ namespace {
 int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
   return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
 }
+constexpr int64_t kLastCacheBytes = 256 << 20;
 constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 16 bytes
 }  // namespace
 
@@ -34,7 +35,8 @@ static bool fits_line(const PagedArgs& a, int64_t units, int tile, int ahead) {
 }
 
 // Units of 128 rows, cut into pieces where they may be fewer than the GPU runs at once.
-static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace_bytes) {
+static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t max_query_len,
+                             int64_t workspace_bytes) {
   PagedPlan p{};
   p.chunk = true;
   p.rows = kChunkRows;
@@ -51,6 +53,14 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace
   // ones d128 60.9 / 59.1, one prompt of 700 tokens 21.8 / 20.3, three of 777 tokens d64 8 bits 50.7 / 47.5)
   const bool few = least * (chunk_pieces(head_dim) - 1) < wgs;
   p.combine = p.split && few;
+  // V non-temporally, where one block of a sequence reads it and the tables have room for
+  // more than stays in the 256 MB cache behind the L2s from one step to the next (us without
+  // and with: 16 tokens each of 16 sequences of 4096 to 8192 keys, 32 over 8 heads d128, 400
+  // MB 99.9 / 81.2, of 32 in 8 bits 118.7 / 108.8, 10 of 48 of 8192 to 16384 d64, 302 MB 68.2 /
+  // 63.8; in the cache: 16 of those 33.0 / 35.4, 16 in 8 bits d128 72.5 / 73.7).
+  const int64_t room = ((int64_t)a.max_pages << a.page_shift) * a.batch * a.hkv;
+  p.stream_v = max_query_len * a.group <= kChunkRows &&
+               room > kLastCacheBytes / (2 * head_dim * (a.ks != nullptr ? 1 : 2));
   p.pieces = few ? 0 : chunk_pieces(head_dim);
   p.wgs = p.split ? (int)wgs : p.units;
   p.workspace_bytes = p.split ? p.wgs * record + kCombineWord : 0;
@@ -59,7 +69,7 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t workspace
 
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
                      int64_t workspace_bytes) {
-  if (max_query_len * a.group > 32) return plan_chunks(a, head_dim, workspace_bytes);
+  if (max_query_len * a.group > 32) return plan_chunks(a, head_dim, max_query_len, workspace_bytes);
   PagedPlan p{};
   p.rows = max_query_len * a.group <= 16 ? 16 : 32;
   p.classes = std::gcd(a.hkv, kNumXcds);
@@ -116,6 +126,7 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   a.units = plan.units;
   a.resident = plan.resident;
   a.pieces = plan.pieces;
+  a.stream_v = plan.stream_v ? 1 : 0;
   a.split = plan.split ? 1 : 0;
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
   if (plan.split) {

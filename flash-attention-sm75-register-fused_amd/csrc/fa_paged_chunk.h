@@ -202,7 +202,8 @@ __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const Page
   return s;
 }
 
-template <int D, bool BF16, bool FP8, bool SPLIT>
+// STREAM: V's rows are read non-temporally (a sequence's only block is the one that reads them).
+template <int D, bool BF16, bool FP8, bool SPLIT, bool STREAM>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
   constexpr bool DENSE = D == 64;
   using L = std::conditional_t<DENSE, LdsDense<D>, Lds<D>>;
@@ -370,19 +371,25 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
     return (lds_void*)(tile + off);
   };
 
+  auto load_v16 = [](const __amdgpu_buffer_rsrc_t r, lds_void* to, int off) {
+    if constexpr (STREAM) direct_load16_nt(r, to, off);
+    else direct_load16(r, to, off);
+  };
+
   // 8-bit rows in flight: this wave's 16 rows of a K tile and of a V tile.
   constexpr int LF = FP8 ? LQ : 1;
   uint4v kr[LF], vr[LF];
   unsigned ksr[LF], vsr[LF];
   auto load_codes = [&](const uint8_t* base, int64_t sp, int64_t sn, const uint8_t* sbase, int64_t ssp,
-                        int64_t ssn, int j, int page, uint4v (&w)[LF], unsigned (&sc)[LF]) {
+                        int64_t ssn, int j, int page, uint4v (&w)[LF], unsigned (&sc)[LF], auto policy) {
     const __amdgpu_buffer_rsrc_t r = window(base, sp, sn, j, page);
     const __amdgpu_buffer_rsrc_t rs = window(sbase, ssp, ssn, j, page);
 #pragma unroll
     for (int i = 0; i < LF; ++i) {
       const int rr = (64 * i + lane) / RL;
       w[i] = __builtin_bit_cast(
-          uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, rr * (int)sn + 16 * (lane % RL), 0, 0));
+          uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, rr * (int)sn + 16 * (lane % RL), 0,
+                                                        decltype(policy)::value));
       sc[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, rr * (int)ssn, 0, 0);
     }
   };
@@ -394,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   };
   const uint8_t* const ksh = FP8 ? a.ks + hkv * a.ksh : nullptr;
   const uint8_t* const vsh = FP8 ? a.vs + hkv * a.vsh : nullptr;
-  auto load_k8 = [&](int j, int page) { load_codes(kh, a.kp, a.kn, ksh, a.ksp, a.ksn, j, page, kr, ksr); };
-  auto load_v8 = [&](int j, int page) { load_codes(vh, a.vp, a.vn, vsh, a.vsp, a.vsn, j, page, vr, vsr); };
+  auto load_k8 = [&](int j, int page) { load_codes(kh, a.kp, a.kn, ksh, a.ksp, a.ksn, j, page, kr, ksr, std::integral_constant<int, 0>{}); };
+  auto load_v8 = [&](int j, int page) { load_codes(vh, a.vp, a.vn, vsh, a.vsp, a.vsn, j, page, vr, vsr, std::integral_constant<int, STREAM ? kPStreamed : 0>{}); };
 
   // Per-lane LDS bases of the operand reads (as in the dense forward).
   const int sK = (ql >> 2) & 3;
@@ -517,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
       } else if constexpr (q < SEGQ) {
         direct_load16(rk_next, lds_seg(k_dst, q), koff[q]);
       } else {
-        direct_load16(rv_next, lds_seg(v_dst, q - SEGQ), voff[q - SEGQ]);
+        load_v16(rv_next, lds_seg(v_dst, q - SEGQ), voff[q - SEGQ]);
       }
     };
     constexpr int NL = FP8 ? 4 * LQ : LPW;
@@ -649,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 #pragma unroll
       for (int i = 0; i < SEGQ; ++i) direct_load16(rk1, lds_seg(k_lds1, i), koff[i]);
 #pragma unroll
-      for (int i = 0; i < SEGQ; ++i) direct_load16(rv0, lds_seg(v_lds0, i), voff[i]);
+      for (int i = 0; i < SEGQ; ++i) load_v16(rv0, lds_seg(v_lds0, i), voff[i]);
       fence_schedule();
       sign_q();
       barrier_after_loads<2 * SEGQ>();  // S_0 needs K_0 only
@@ -682,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 #pragma unroll
           for (int i = 0; i < SEGQ; ++i) direct_load16(rk, lds_seg(k_dst, i), koff[i]);
 #pragma unroll
-          for (int i = 0; i < SEGQ; ++i) direct_load16(rv, lds_seg(v_dst, i), voff[i]);
+          for (int i = 0; i < SEGQ; ++i) load_v16(rv, lds_seg(v_dst, i), voff[i]);
         }
         barrier_after_loads<FP8 ? 63 : 0>();
       }
@@ -873,8 +880,12 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
 template <int D, bool BF16, bool FP8>
 void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream) {
   const dim3 g((unsigned)grid), t(kThreads);
-  if (a.split) hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true>), g, t, 0, stream, a);
-  else hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false>), g, t, 0, stream, a);
+  if (a.split && a.stream_v)
+    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, true>), g, t, 0, stream, a);
+  else if (a.split)
+    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, false>), g, t, 0, stream, a);
+  else
+    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false, false>), g, t, 0, stream, a);
 }
 
 }  // namespace fa

@@ -115,6 +115,15 @@ def test_one_long_unit_among_short_ones(device, d):
     attend(c, device, 8)
 
 
+@pytest.mark.parametrize("d,q8,dtype", [(64, False, FP16), (64, True, BF16), (128, False, BF16), (128, True, FP16)])
+def test_wide_tables(device, d, q8, dtype):
+    """Tables with room for many more keys than there are: the same kernels, V read past the caches."""
+    lens, news = [700, 90, 1, 300, 2000], [20, 9, 1, 0, 32]
+    pages = (512 << 20) // (len(lens) * 2 * 2 * d * (1 if q8 else 2)) // 16
+    c = Cache(lens, 2, d, 16, dtype, q8, news=news, width=pages)
+    attend(c, device, 8, max_query_len=32)
+
+
 def test_unequal_lengths_of_equal_tiles(device):
     c = Cache([385, 400, 448, 447], 1, 128, 16, FP16, False, news=[40, 1, 448, 3])
     attend(c, device, 4)
