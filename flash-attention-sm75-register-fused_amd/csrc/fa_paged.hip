@@ -19,7 +19,6 @@ FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
 FA_PAGED_EXTERN(128, false, true) FA_PAGED_EXTERN(128, true, true)
 #undef FA_PAGED_EXTERN
 
-
 namespace {
 int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
   return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
@@ -145,7 +144,7 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
       if (a.bf16) launch_paged_chunk<D, true, false>(a, grid, stream);                  \
       else launch_paged_chunk<D, false, false>(a, grid, stream);                        \
     }                                                                                   \
-  } else if (fp8) {                                                                            \
+  } else if (fp8) {                                                                     \
     if (a.bf16) launch_paged_attn<D, true, true>(a, plan.rows, grid, stream);           \
     else launch_paged_attn<D, false, true>(a, plan.rows, grid, stream);                 \
   } else {                                                                              \

@@ -21,11 +21,11 @@
 // in the layout the 16-bit rows arrive in.
 //
 // The plan.  Where the units do not fill the GPU (SPLIT), each workgroup takes an equal
-// stretch of the class's line of 64-key tiles, as in the kernel for few columns; the
-// partials of units that stretches cut are merged by the unit's last workgroup where
-// they are few, else by a second kernel.  Else a
-// workgroup takes a unit, each head's from its last block (under the causal rule the
-// longest) to its first; where all of them run at once, two a CU, the second half
+// stretch of the class's line of 64-key tiles, as in the kernel for few columns, or where
+// all units are equally long a piece of one (chunk_stretch); the partials of units that are
+// cut are merged by the unit's last workgroup where they are few, else by a second
+// kernel.  Else a workgroup takes a unit, each head's from its last block (under the causal
+// rule the longest) to its first; where all of them run at once, two a CU, the second half
 // of them in reverse, so that a CU gets a long and a short one.
 //
 // What bounds it: as in the dense forward, the step (a tile's 32 MFMAs a wave, its softmax
@@ -401,8 +401,13 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   };
   const uint8_t* const ksh = FP8 ? a.ks + hkv * a.ksh : nullptr;
   const uint8_t* const vsh = FP8 ? a.vs + hkv * a.vsh : nullptr;
-  auto load_k8 = [&](int j, int page) { load_codes(kh, a.kp, a.kn, ksh, a.ksp, a.ksn, j, page, kr, ksr, std::integral_constant<int, 0>{}); };
-  auto load_v8 = [&](int j, int page) { load_codes(vh, a.vp, a.vn, vsh, a.vsp, a.vsn, j, page, vr, vsr, std::integral_constant<int, STREAM ? kPStreamed : 0>{}); };
+  auto load_k8 = [&](int j, int page) {
+    load_codes(kh, a.kp, a.kn, ksh, a.ksp, a.ksn, j, page, kr, ksr, std::integral_constant<int, 0>{});
+  };
+  auto load_v8 = [&](int j, int page) {
+    load_codes(vh, a.vp, a.vn, vsh, a.vsp, a.vsn, j, page, vr, vsr,
+               std::integral_constant<int, STREAM ? kPStreamed : 0>{});
+  };
 
   // Per-lane LDS bases of the operand reads (as in the dense forward).
   const int sK = (ql >> 2) & 3;
