@@ -90,9 +90,9 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) + kCombineWord : 0;
-  // Stretches are kPMinTiles long at least, and there are wgs of them.
+  // What the longest unit the tables have room for may be cut into.
   const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + kPTile - 1) / kPTile;
-  const int64_t pieces = std::min<int64_t>(p.wgs, tiles / kPMinTiles + 2);
+  const int64_t pieces = PagedStretch<kPMinTiles>::most_pieces(tiles, p.wgs);
   p.y = (int)std::min<int64_t>(p.rows, max_query_len * a.group);
   // (max_query_len may be wrong: rows are then up to p.rows)
   p.combine = p.split && !paged_merges_itself((int)pieces, a.cu == nullptr ? p.y : p.rows, head_dim);

@@ -51,7 +51,7 @@ namespace fa {
 namespace {
 
 constexpr int kPTile = 32;       // keys of a wave's tile
-constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below
+constexpr int kPMinTiles = 8;    // tiles a stretch is not cut below (but see PagedStretch)
 // Another unit's cost, in tiles (us without and with: 4 sequences of 2048 to 4096 keys d128
 // 8 bits 19.6 / 16.0, 32 of 4096 to 8192 132.0 / 130.5, 8 bits 68.8 / 68.0, 16 of 16384 to
 // 32768 d64 36.6 / 37.2; 8 of 8192 each d128, where it does not count, 45.2, with it 47.8).

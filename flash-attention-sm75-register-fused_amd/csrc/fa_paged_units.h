@@ -137,10 +137,12 @@ struct PagedLine {
   }
 };
 
-// The stretches of a class's line, one for each workgroup of it, and no shorter than LEAST
-// tiles: of the whole line, total / active tiles each, or (cut_units) of every unit for
-// itself where all are equally long.  The first ones of the line, or unit, are a tile
-// longer.
+// The stretches of a class's line, one for each workgroup of it: of the whole line, total /
+// active tiles each, or (cut_units) of every unit for itself where all are equally long.
+// The first ones of the line, or unit, are a tile longer.  There are at most as many as
+// stretches of LEAST tiles would be, rounded up: some may be shorter (nine tiles are two
+// stretches), but none is then longer than LEAST, and all of them together are at most LEAST - 1
+// short of it.
 template <int LEAST>
 struct PagedStretch {
   int active;
@@ -149,6 +151,13 @@ struct PagedStretch {
     active = uniform(min(a.wgs, (total + LEAST - 1) / LEAST));
     len = uniform(total);
     cuts = active;
+  }
+  // The most pieces a unit of `tiles` tiles is cut into.  Of `count` pieces all but the two
+  // ends are whole stretches, of LEAST (count - 2) - (LEAST - 1) tiles in all or more, and
+  // the ends have a tile each; of a unit cut for itself there are ceil(tiles / LEAST) at most.
+  static __host__ __device__ constexpr int64_t most_pieces(int64_t tiles, int64_t wgs) {
+    const int64_t pieces = (tiles + LEAST - 3) / LEAST + 2;
+    return pieces < wgs ? pieces : wgs;
   }
   // Units of a line of them that are `same` tiles long (a quotient past 2^21, where this is
   // not exact, is more than there are workgroups).
