@@ -34,8 +34,10 @@ class Call:
         self.hint = (max(news) if hint is None else hint) if cu else 1
 
     def __repr__(self):
-        return (f"{self.hkv * self.group} over {self.hkv} heads d{self.d} page {self.page} lens {self.lens} "
-                f"news {self.news} width {self.width} cu {self.cu} q8 {self.q8} max_query_len {self.hint}")
+        def short(x):
+            return str(x) if len(x) <= 16 else f"{len(x)} from {x[0]} to {x[-1]}"
+        return (f"{self.hkv * self.group} over {self.hkv} heads d{self.d} page {self.page} lens {short(self.lens)} "
+                f"news {short(self.news)} width {self.width} cu {self.cu} q8 {self.q8} max_query_len {self.hint}")
 
     def sizes(self):
         return (self.hkv, self.group, len(self.lens), sum(self.news), self.d, self.page.bit_length() - 1, self.width)
