@@ -200,8 +200,6 @@ int fa_sm75_paged_read(const fa_paged_cache* cache, fa_half* k, fa_half* v, int6
   if (max_len > (1 << 27) || (int64_t)a.batch * a.hkv > (1 << 27) ||
       max_len * a.batch * a.hkv > (1 << 27))
     return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv * max_len exceeds 2^27 rows");
-  if ((int64_t)a.batch * a.hkv > 65535)
-    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 65535");
   if (k == nullptr || v == nullptr)
     return capi_fail(FA_ERR_INVALID_ARGUMENT, "K and V must not be NULL");
   if (!aligned(k, 16) || !aligned(v, 16))

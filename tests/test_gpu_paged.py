@@ -414,6 +414,33 @@ def test_read_nothing(device):
     assert k.shape == (2, 2, 20, 64) and (k == 0).all() and (v == 0).all()
 
 
+@pytest.mark.parametrize("batch,hkv", [(2100, 64), (2, 1 << 16)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_read_many_sequences_and_heads(device, q8, batch, hkv):
+    """More heads of sequences than a dimension of the grid holds (65535)."""
+    d, page, max_len = 64, 16, 5
+    g = torch.Generator().manual_seed(7)
+    k, v = (torch.randn(2, hkv, page, d, generator=g).half() for _ in "kv")
+    kw = {}
+    if q8:
+        k, v = (x.float().to(torch.float8_e4m3fn) for x in (k, v))
+        kw = {n: torch.randint(120, 130, (2, hkv, page), generator=g, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+              for n in ("k_scale", "v_scale")}
+    table = torch.randint(-1, 2, (batch, 1), generator=g, dtype=torch.int32)
+    lens = torch.randint(0, 8, (batch,), generator=g, dtype=torch.int32)
+    got = fa.paged_cache_read(k.to(device), v.to(device), table.to(device), lens.to(device), max_len=max_len,
+                              dtype=FP16, **{n: x.to(device) for n, x in kw.items()})
+    pos = torch.arange(max_len)
+    held = (pos < lens[:, None]) & (table >= 0)
+    for out, pool, scale in zip(got, (k, v), ("k_scale", "v_scale")):
+        want = pool[:, :, :max_len].float()
+        if q8:  # (exact in binary16)
+            want = want * kw[scale][:, :, :max_len].float()[..., None]
+        want = want.half()[table[:, 0].clamp(min=0).long()]
+        want.masked_fill_(~held[:, None, :, None], 0.0)
+        assert torch.equal(out.cpu(), want)
+
+
 # ---- together ----------------------------------------------------------------------
 
 

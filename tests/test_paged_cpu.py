@@ -151,6 +151,13 @@ def test_read_refusals(lib, args, status, msg):
     assert msg in lib.fa_sm75_last_error()
 
 
+def test_read_takes_any_number_of_heads_and_sequences(lib):
+    """Only the rows in all are limited (the call ends at the pointer it is not given)."""
+    for kw, max_len in ((dict(batch=1024, heads_kv=64), 16), (dict(batch=1 << 20, heads_kv=128), 1)):
+        assert lib.fa_sm75_paged_read(ctypes.byref(cache(**kw)), 0, 0x10000, max_len, 0, None) == 1
+        assert b"must not be NULL" in lib.fa_sm75_last_error()
+
+
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(tokens=-1), 1, b"tokens must be non-negative"),
     (dict(tokens=1), 1, b"a token for each of the 2 sequences"),
