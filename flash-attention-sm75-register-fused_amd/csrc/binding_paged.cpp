@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <tuple>
+#include <utility>
 
 #include "flash_attn_sm75.h"
 
@@ -104,6 +105,40 @@ Tensor rows_view(const Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
+// Whether no byte from a's first element to its last lies between b's (strides not
+// negative).
+bool spans_apart(const Tensor& a, const Tensor& b) {
+  auto span = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    const auto first = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::pair<uintptr_t, uintptr_t>(first, first + (last + 1) * t.element_size());
+  };
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const auto x = span(a), y = span(b);
+  return x.second <= y.first || y.second <= x.first;
+}
+
+// Whether [tokens, heads, D] rows of one shape and type, a's and b's, share no memory: they
+// lie apart, or interleave in a buffer that holds both, in every token's stretch of it or in
+// every head's.  (False where neither can be seen from the strides.)
+bool rows_apart(const Tensor& a, const Tensor& b) {
+  if (spans_apart(a, b)) return true;
+  const int64_t d = a.size(2), st = a.stride(0), sh = a.size(1) == 1 ? d : a.stride(1);
+  const bool one = a.size(0) == 1;
+  if (!one && (st <= 0 || st != b.stride(0))) return false;
+  if (sh < d || (a.size(1) > 1 && sh != b.stride(1))) return false;
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
+  if (bytes % a.element_size() != 0) return false;
+  const int64_t delta = bytes / a.element_size();
+  // `width` elements of every `period`, b's delta behind a's.
+  auto apart = [delta](int64_t period, int64_t width) {
+    const int64_t r = (delta % period + period) % period;
+    return r >= width && r + width <= period;
+  };
+  return (!one && apart(st, (a.size(1) - 1) * sh + d)) || ((one || st % sh == 0) && apart(sh, d));
+}
+
 const int32_t* cu_pointer(const OptTensor& cu, const Tensor& k_cache, int64_t batch, int64_t tokens) {
   if (!cu.has_value()) {
     TORCH_CHECK(tokens == batch, "without cu_seqlens there is one new token for each of the ", batch,
@@ -195,13 +230,13 @@ std::tuple<Tensor, OptTensor> flash_attention_paged(
     TORCH_CHECK(O.sizes() == Q.sizes() && O.scalar_type() == Q.scalar_type() && O.device() == Q.device(),
                 "out must have Q's shape, dtype and device");
     // (other workgroups still read Q when the first rows of O are written)
-    for (const Tensor* t : {static_cast<const Tensor*>(&Q), static_cast<const Tensor*>(&k_cache),
-                            static_cast<const Tensor*>(&v_cache)})
-      TORCH_CHECK(O.numel() == 0 || !O.is_alias_of(*t), "out must not share Q's or the cache's memory");
     for (int i = 0; i < 2; ++i)
       TORCH_CHECK(O.size(i) <= 1 || O.stride(i) != 0, "out must not be an expanded view");
     TORCH_CHECK(O.numel() == 0 || rows_view(O).is_same(O),
                 "out must be 16-byte aligned, head_dim contiguous, its other strides multiples of 8");
+    bool apart = rows_apart(O, Q) && spans_apart(O, k_cache) && spans_apart(O, v_cache);
+    if (k_scale.has_value()) apart = apart && spans_apart(O, *k_scale) && spans_apart(O, *v_scale);
+    TORCH_CHECK(apart, "out must not share Q's or the cache's memory");
   } else {
     O = torch::empty(Q.sizes(), Q.options());
   }

@@ -102,8 +102,11 @@ def flash_attention_paged(Q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
             (all of the sequence's keys).
         scale: softmax scale (default 1/sqrt(D)).
         return_lse: also return the fp32 natural-log row LSE, [H_q, tokens].
-        out: a tensor like Q to write to; its rows behind cu_seqlens[B] are left as they
-            are (of a new tensor they are not defined, nor are the LSE's).
+        out: a tensor like Q to write to, 16-byte aligned, head_dim contiguous and the other
+            strides multiples of 8; it may be a view of the buffer Q is a view of (its rows
+            beside Q's, or its heads between them) but must share no element with Q or the
+            cache.  Its rows behind cu_seqlens[B] are left as they are (of a new tensor
+            they are not defined, nor are the LSE's).
 
     Returns:
         O [tokens, H_q, D] in Q's dtype, or (O, LSE).  A query that sees no key gets

@@ -190,6 +190,76 @@ def test_rows_behind_the_last_sequence(device):
     assert (out[4:] == 7).all()
 
 
+def fused(kind, t, h, d, device):
+    """Q and out of one buffer, no element in both."""
+    if kind == "halves of every row":
+        buf = torch.empty(t, 2 * h, d, dtype=FP16, device=device)
+        return buf, buf[:, :h], buf[:, h:]
+    if kind == "out first":
+        buf = torch.empty(t, 2 * h + 3, d, dtype=FP16, device=device)
+        return buf, buf[:, h + 2:2 * h + 2], buf[:, 1:h + 1]
+    if kind == "one behind the other":
+        buf = torch.empty(2, t, h, d, dtype=FP16, device=device)
+        return buf, buf[0], buf[1]
+    buf = torch.empty(t, h, 2, d, dtype=FP16, device=device)  # head by head
+    return buf, buf[:, :, 1], buf[:, :, 0]
+
+
+@pytest.mark.parametrize("news", [[5, 20], [1, 0]])
+@pytest.mark.parametrize("kind", ["halves of every row", "out first", "one behind the other", "head by head"])
+def test_out_beside_q(device, kind, news):
+    """out and Q as views of one buffer that share no element of it."""
+    c, t = Cache([50, 129], 2, 64, 32, FP16, False, news=news), sum(news)
+    (args, kw), g = c.args(device), torch.Generator().manual_seed(3)
+    q = torch.randn(t, 4, 64, generator=g).half()
+    want, _, tol, _ = ref.attention(c, q)
+    buf, at, out = fused(kind, t, 4, 64, device)
+    buf.fill_(9.0)
+    at.copy_(q)
+    got = fa.flash_attention_paged(at, *args, cu_seqlens=c.cu.to(device), out=out, **kw)
+    assert got.data_ptr() == out.data_ptr()
+    ref.check(out, want, tol, "O")
+    assert torch.equal(at.cpu(), q)
+    out.fill_(9.0)
+    at.fill_(9.0)
+    assert (buf == 9).all()
+
+
+def test_out_beside_the_cache(device):
+    """One allocation for the pools and the output."""
+    c = Cache([50, 129], 2, 64, 32, FP16, False, news=[5, 20])
+    (k, v, table, lens), _ = c.args(device)
+    n, q = k.numel(), torch.randn(25, 4, 64).half()
+    arena = torch.zeros(2 * n + q.numel(), dtype=FP16, device=device)
+    pools = [arena[i * n:(i + 1) * n].view(k.shape) for i in range(2)]
+    pools[0].copy_(k)
+    pools[1].copy_(v)
+    out = arena[2 * n:].view(q.shape)
+    fa.flash_attention_paged(q.to(device), *pools, table, lens, cu_seqlens=c.cu.to(device), out=out)
+    want, _, tol, _ = ref.attention(c, q)
+    ref.check(out, want, tol, "O")
+
+
+def test_out_that_overlaps_is_refused(device):
+    c = Cache([50, 129], 4, 64, 32, FP16, False, news=[5, 20])
+    (k, v, table, lens), _ = c.args(device)
+    cu = c.cu.to(device)
+    buf = torch.zeros(60, 9, 64, dtype=FP16, device=device)
+    q = buf[10:35, :4]
+    for out in (q, buf[10:35, 1:5], buf[10:35, 3:7], buf[11:36, :4], buf[34:59, 2:6], buf[9:34, 3:7],
+                k.view(-1, 4, 64)[:25], v.view(-1, 4, 64)[7:32]):
+        with pytest.raises(RuntimeError, match="must not share"):
+            fa.flash_attention_paged(q, k, v, table, lens, cu_seqlens=cu, out=out)
+    wide = torch.zeros(25, 5, 96, dtype=FP16, device=device)  # rows that overlap in part
+    with pytest.raises(RuntimeError, match="must not share"):
+        fa.flash_attention_paged(wide[:, :4, :64], k, v, table, lens, cu_seqlens=cu, out=wide[:, :4, 32:])
+    flat = torch.zeros(4000 * 64, dtype=FP16, device=device)  # strides of their own
+    a = flat.as_strided((25, 4, 64), (512, 64, 1))
+    for b in (flat.as_strided((25, 4, 64), (256, 64, 1), 256), flat.as_strided((25, 4, 64), (512, 128, 1), 256)):
+        with pytest.raises(RuntimeError, match="must not share"):
+            fa.flash_attention_paged(a, k, v, table, lens, cu_seqlens=cu, out=b)
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-9, 2.0])
 def test_scales(device, scale):
     attend(Cache([200, 10], 2, 64, 16, BF16, False, news=[2, 1]), device, 4, scale=scale)
