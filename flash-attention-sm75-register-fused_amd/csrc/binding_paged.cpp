@@ -155,6 +155,12 @@ void* current_stream(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
+// Tells autograd that a tensor was written to: a graph that kept its old values raises.
+// (Tensors of inference mode count no versions and are in no graph.)
+void written_to(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void paged_cache_write(Tensor K, Tensor V, Tensor k_cache, Tensor v_cache, Tensor block_table,
                        Tensor seq_lens, OptTensor cu_seqlens, OptTensor k_scale, OptTensor v_scale) {
   const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, true);
@@ -185,6 +191,12 @@ void paged_cache_write(Tensor K, Tensor V, Tensor k_cache, Tensor v_cache, Tenso
   r.stream = current_stream(k_cache);
   const int st = fa_sm75_paged_write(&c, &r);
   TORCH_CHECK(st == FA_OK, "paged_cache_write: ", fa_sm75_last_error());
+  written_to(k_cache);
+  written_to(v_cache);
+  if (k_scale.has_value()) {
+    written_to(*k_scale);
+    written_to(*v_scale);
+  }
 }
 
 std::tuple<Tensor, Tensor> paged_cache_read(Tensor k_cache, Tensor v_cache, Tensor block_table,
@@ -264,6 +276,7 @@ std::tuple<Tensor, OptTensor> flash_attention_paged(
   }
   const int st = fa_sm75_paged_forward(&p);
   TORCH_CHECK(st == FA_OK, "flash_attention_paged: ", fa_sm75_last_error());
+  if (out.has_value()) written_to(O);
   return {O, L};
 }
 

@@ -511,6 +511,51 @@ def test_read_many_sequences_and_heads(device, q8, batch, hkv):
         assert torch.equal(out.cpu(), want)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_what_is_written_counts_as_changed(device, q8):
+    """Autograd sees the writes: versions rise, also a view's base's, and a backward that kept the
+    old values raises, as after torch's own in-place operations."""
+    c = Cache([20, 9], 2, 64, 16, FP16, q8, news=[3, 1])
+    (k, v, table, lens), kw = c.args(device)
+    new = torch.randn(4, 2, 64, device=device).half()
+    changed = [k, v, *kw.values()]
+    before = [x._version for x in changed]
+    w = torch.ones((), device=device, requires_grad=True)
+    loss = (w * k.float().nan_to_num(0.0)).sum() if q8 else (w.half() * k).sum()  # the 16-bit pool is kept
+    fa.paged_cache_write(new, new, k, v, table, lens, cu_seqlens=c.cu.to(device), **kw)
+    assert all(x._version > n for x, n in zip(changed, before))
+    if q8:
+        loss.backward()  # (a copy was kept)
+    else:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = [x._version for x in changed]
+    q = torch.randn(4, 6, 64, device=device).half()
+    wide = torch.zeros(4, 8, 64, dtype=FP16, device=device)
+    version = wide._version
+    fa.flash_attention_paged(q, k, v, table, lens, cu_seqlens=c.cu.to(device), out=wide[:, 1:7], **kw)
+    assert wide._version > version and q._version == 0
+    fa.paged_cache_read(k, v, table, lens, dtype=FP16, **kw)
+    assert [x._version for x in changed] == before
+
+
+def test_inference_tensors(device):
+    """A cache and an output made in inference mode, used in it and outside of it."""
+    c = Cache([20, 9], 2, 64, 16, FP16, False, news=[3, 1])
+    with torch.inference_mode():
+        (k, v, table, lens), _ = c.args(device)
+        out = torch.zeros(4, 4, 64, dtype=FP16, device=device)
+    cu, new = c.cu.to(device), torch.randn(4, 2, 64, device=device).half()
+    got = []
+    for mode in (torch.inference_mode, torch.no_grad, torch.enable_grad):
+        with mode():
+            fa.paged_cache_write(new, new, k, v, table, lens, cu_seqlens=cu)
+            fa.flash_attention_paged(new.repeat(1, 2, 1), k, v, table, lens, cu_seqlens=cu, out=out)
+        got.append((k.cpu(), out.cpu()))
+    for pool, o in got[1:]:
+        assert same(pool, got[0][0]) and torch.equal(o, got[0][1])
+
+
 # ---- together ----------------------------------------------------------------------
 
 
