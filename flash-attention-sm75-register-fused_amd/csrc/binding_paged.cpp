@@ -6,8 +6,10 @@
 #include <torch/extension.h>
 
 #include <ATen/DeviceGuard.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 
+#include <initializer_list>
 #include <tuple>
 #include <utility>
 
@@ -155,6 +157,14 @@ void* current_stream(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
+// Refuses tensors that carry a forward-mode tangent, which the call would drop.
+void check_no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->_fw_grad(0).defined(), name, " has no forward-mode derivative: call it on the primals "
+                "(torch.autograd.forward_ad.unpack_dual)");
+}
+
 // Tells autograd that a tensor was written to: a graph that kept its old values raises.
 // (Tensors of inference mode count no versions and are in no graph.)
 void written_to(const Tensor& t) {
@@ -163,6 +173,7 @@ void written_to(const Tensor& t) {
 
 void paged_cache_write(Tensor K, Tensor V, Tensor k_cache, Tensor v_cache, Tensor block_table,
                        Tensor seq_lens, OptTensor cu_seqlens, OptTensor k_scale, OptTensor v_scale) {
+  check_no_tangent("paged_cache_write", {&K, &V, &k_cache, &v_cache});
   const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, true);
   for (const Tensor* t : {&K, &V}) {
     TORCH_CHECK(is_half_type(*t), "K and V must be FP16 or BF16");
@@ -202,6 +213,7 @@ void paged_cache_write(Tensor K, Tensor V, Tensor k_cache, Tensor v_cache, Tenso
 std::tuple<Tensor, Tensor> paged_cache_read(Tensor k_cache, Tensor v_cache, Tensor block_table,
                                             Tensor seq_lens, int64_t max_len, OptTensor k_scale,
                                             OptTensor v_scale, c10::optional<torch::ScalarType> dtype) {
+  check_no_tangent("paged_cache_read", {&k_cache, &v_cache});
   const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, false);
   TORCH_CHECK(max_len >= 0, "max_len must be non-negative, got ", max_len);
   TORCH_CHECK(dtype.has_value() || c.k_scale == nullptr, "a float8_e4m3fn cache needs a dtype to read to");
@@ -223,6 +235,7 @@ std::tuple<Tensor, OptTensor> flash_attention_paged(
     Tensor Q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens,
     OptTensor cu_seqlens, int64_t max_query_len, int64_t causal, double scale, OptTensor k_scale,
     OptTensor v_scale, bool return_lse, OptTensor out) {
+  check_no_tangent("flash_attention_paged", {&Q, &k_cache, &v_cache, out.has_value() ? &*out : &Q});
   const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, false);
   TORCH_CHECK(is_half_type(Q), "Q must be FP16 or BF16");
   TORCH_CHECK(Q.device() == k_cache.device(), "Q must be on the cache's device");

@@ -23,7 +23,8 @@ The index tensors stay on the device and are not looked at by the host, so a cal
 captured in a graph takes what they hold at each replay.
 
 The calls record no gradient: inputs that require one are refused while autograd
-records.
+records, and so are inputs with a forward-mode tangent.  What a call writes to counts as
+changed in place (tensor versions).
 """
 import math
 

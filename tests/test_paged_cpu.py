@@ -251,6 +251,39 @@ def test_python_refusals():
         fa.flash_attention_paged(leaf, *args)
 
 
+def test_tangents_are_refused():
+    """Forward-mode derivatives are not computed, so an input that carries one is not taken for a
+    plain tensor; with forward mode off, and of the primals, the calls go on (to the next check)."""
+    import flash_attention_sm75 as fa
+    import torch.autograd.forward_ad as fwd
+
+    c = Cache([5], 2, 64, 16, torch.float16, False)
+    (k, v, table, lens), _ = c.args("cpu")
+    x = torch.zeros(1, 2, 64, dtype=torch.float16)
+    calls = [lambda y, kc, vc: fa.paged_cache_write(y, x, kc, vc, table, lens),
+             lambda y, kc, vc: fa.paged_cache_write(x, y, kc, vc, table, lens),
+             lambda y, kc, vc: fa.flash_attention_paged(y, kc, vc, table, lens),
+             lambda y, kc, vc: fa.flash_attention_paged(x, kc, vc, table, lens, out=y)]
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        pool = fwd.make_dual(k, torch.ones_like(k))
+        with torch.no_grad():
+            for call in calls:
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(dual, k, v)
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(x, pool, v)
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(x, v, pool)
+                with pytest.raises(RuntimeError, match="CUDA"):
+                    call(fwd.unpack_dual(dual).primal, k, v)
+            for args in ((pool, v), (v, pool)):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    fa.paged_cache_read(*args, table, lens)
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="CUDA"):
+            fa.flash_attention_paged(dual, k, v, table, lens)
+
+
 # ---- the reference ------------------------------------------------------------------
 
 
