@@ -31,9 +31,11 @@
 // What bounds it: as in the dense forward, the step (a tile's 32 MFMAs a wave, its softmax
 // and 168 KB of LDS traffic a workgroup, two workgroups a CU: 1555 cycles each where the
 // MFMAs alone take 1024 at d128; of one workgroup alone 2558), 2048 tokens behind 6144 of 32
-// heads d128 232 to 245 us, 980 to 1040 TFLOP/s; in short launches what a workgroup does
-// before its first tile and after its last (7 us) and the merges (3 to 5 us): three
-// sequences of 1777 to 4000 keys, 777 new tokens each, 14 heads d64 8 bits, 47 us.
+// heads d128 232 to 248 us from one card to the next, 970 to 1040 TFLOP/s; in short launches
+// what a workgroup does before its first tile and after its last (7 us) and the merges (3 to 5
+// us); with 8-bit rows VALU instructions: three sequences of 1777 to 4000 keys, 777 new tokens
+// each, 14 heads d64, 47 to 51 us, issue 254 a wave and tile, of which the softmax is 112
+// (16-bit rows d128 179), and every 128-row unit converts all its K and V again.
 #pragma once
 
 #include <hip/hip_runtime.h>

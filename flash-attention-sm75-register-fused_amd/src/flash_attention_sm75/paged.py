@@ -71,7 +71,8 @@ def paged_cache_read(k_cache, v_cache, block_table, seq_lens, max_len=None, k_sc
     """The sequences' K and V out of their pages.
 
     Args:
-        max_len: positions to read (default: all that block_table has room for).
+        max_len: positions to read (default: all that block_table has room for);
+            B * H_kv * max_len is up to 2^27.
         dtype: float16 or bfloat16, for an 8-bit cache; a 16-bit one is read in its own.
 
     Returns:

@@ -352,14 +352,15 @@ typedef struct fa_paged_cache {
   const int32_t* block_table; /* [batch, max_pages], rows block_table_stride apart: entry i is
                                  the page of positions [i page_size, (i + 1) page_size) */
   const int32_t* seq_lens;    /* [batch]: tokens of each sequence, new ones included */
-  int64_t batch;
-  int64_t heads_kv;
+  int64_t batch;       /* up to 2^20 */
+  int64_t heads_kv;    /* up to 2^16 */
   int64_t head_dim;    /* 64 or 128 */
-  int64_t num_pages;
-  int64_t page_size;   /* a power of two, 16 or more */
-  int64_t max_pages;
+  int64_t num_pages;   /* below 2^31 */
+  int64_t page_size;   /* a power of two, 16 to 2^20 */
+  int64_t max_pages;   /* max_pages * page_size up to 2^30 */
   int64_t block_table_stride;
-  /* Strides in elements: of K and V multiples of 16 bytes, head_dim contiguous. */
+  /* Strides in elements: of K and V multiples of 16 bytes, head_dim contiguous, a row's
+   * (_n) up to 2^24 bytes. */
   int64_t k_stride_p, k_stride_h, k_stride_n;
   int64_t v_stride_p, v_stride_h, v_stride_n;
   int64_t ks_stride_p, ks_stride_h, ks_stride_n;
@@ -372,7 +373,7 @@ typedef struct fa_paged_cache {
 typedef struct fa_paged_rows {
   const fa_half* k;    /* [tokens, heads_kv, head_dim], strides in elements (multiples of 8) */
   const fa_half* v;
-  int64_t tokens;
+  int64_t tokens;      /* up to 2^24, tokens * heads_kv up to 2^26 */
   int64_t k_stride_t, k_stride_h;
   int64_t v_stride_t, v_stride_h;
   const int32_t* cu_seqlens; /* [batch + 1], or NULL: row b is sequence b's one new token */
@@ -390,7 +391,8 @@ int fa_sm75_paged_write(const fa_paged_cache* cache, const fa_paged_rows* rows);
 
 /* Reads positions [0, max_len) of every sequence into k and v, contiguous
  * [batch, heads_kv, max_len, head_dim] of type dtype (an fa_dtype; 16-bit rows are
- * copied as they are): zeros past a sequence's end and where it has no page. */
+ * copied as they are): zeros past a sequence's end and where it has no page.
+ * batch * heads_kv * max_len is up to 2^27. */
 int fa_sm75_paged_read(const fa_paged_cache* cache, fa_half* k, fa_half* v, int64_t max_len,
                        int dtype, void* stream);
 
@@ -404,8 +406,8 @@ typedef struct fa_paged_params {
   const fa_half* q;    /* [tokens, heads_q, head_dim] */
   fa_half* o;          /* [tokens, heads_q, head_dim] output */
   float* lse;          /* optional [heads_q, tokens] fp32 natural-log row LSE, or NULL */
-  int64_t tokens;
-  int64_t heads_q;     /* a multiple of cache->heads_kv */
+  int64_t tokens;      /* up to 2^24, tokens * heads_q + 32 * batch * heads_kv up to 2^27 */
+  int64_t heads_q;     /* a multiple of cache->heads_kv, up to 2^20 */
   int64_t q_stride_t, q_stride_h;  /* elements, multiples of 8 */
   int64_t o_stride_t, o_stride_h;
   const int32_t* cu_seqlens; /* as in fa_paged_rows */
