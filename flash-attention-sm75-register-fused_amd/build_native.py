@@ -51,7 +51,13 @@ HIP_SOURCES = [
     "fa_paged_d128_bf16_fp8.hip",
     "fa_paged_d64.hip", "fa_paged_d64_bf16.hip", "fa_paged_d64_fp8.hip",
     "fa_paged_d64_bf16_fp8.hip",
-    "fa_paged.hip", "fa_paged_cache.hip", "fa_paged_capi.hip",
+    "fa_paged_prefix_d128.hip", "fa_paged_prefix_d128_bf16.hip", "fa_paged_prefix_d128_fp8.hip",
+    "fa_paged_prefix_d128_bf16_fp8.hip",
+    "fa_paged_prefix_d64.hip", "fa_paged_prefix_d64_bf16.hip", "fa_paged_prefix_d64_fp8.hip",
+    "fa_paged_prefix_d64_bf16_fp8.hip",
+    "fa_paged_weigh_d128.hip", "fa_paged_weigh_d128_fp8.hip", "fa_paged_weigh_d64.hip",
+    "fa_paged_weigh_d64_fp8.hip",
+    "fa_paged.hip", "fa_paged_weigh.hip", "fa_paged_evict.hip", "fa_paged_cache.hip", "fa_paged_capi.hip",
     "fa_fwd.hip", "fa_decode.hip", "fa_mask.hip", "fa_naive.hip", "fa_capi.hip",
 ]
 

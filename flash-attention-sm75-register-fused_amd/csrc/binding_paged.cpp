@@ -1,5 +1,6 @@
 // PyTorch binding of the paged key/value cache (no reference counterpart):
-// paged_cache_write, paged_cache_read and flash_attention_paged.
+// paged_cache_write, paged_cache_read, paged_cache_evict, flash_attention_paged,
+// flash_attention_paged_prefix and paged_attention_weights.
 //
 // All checks run before any device work; the kernels are enqueued on the
 // current HIP stream of the cache's device and the host is not blocked.
@@ -231,12 +232,8 @@ std::tuple<Tensor, Tensor> paged_cache_read(Tensor k_cache, Tensor v_cache, Tens
   return {K, V};
 }
 
-std::tuple<Tensor, OptTensor> flash_attention_paged(
-    Tensor Q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens,
-    OptTensor cu_seqlens, int64_t max_query_len, int64_t causal, double scale, OptTensor k_scale,
-    OptTensor v_scale, bool return_lse, OptTensor out) {
-  check_no_tangent("flash_attention_paged", {&Q, &k_cache, &v_cache, out.has_value() ? &*out : &Q});
-  const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, false);
+// Checks the queries of a call over a cache; Q becomes rows that the kernels can read.
+void check_queries(Tensor& Q, const fa_paged_cache& c, const Tensor& k_cache) {
   TORCH_CHECK(is_half_type(Q), "Q must be FP16 or BF16");
   TORCH_CHECK(Q.device() == k_cache.device(), "Q must be on the cache's device");
   TORCH_CHECK(Q.dim() == 3, "Q must be [tokens, H_q, D]");
@@ -245,9 +242,21 @@ std::tuple<Tensor, OptTensor> flash_attention_paged(
   TORCH_CHECK(Q.size(2) == c.head_dim, "head_dim mismatch");
   TORCH_CHECK(c.heads_kv > 0 && Q.size(1) % c.heads_kv == 0, "heads mismatch: Q heads (", Q.size(1),
               ") not divisible by K/V heads (", c.heads_kv, ")");
+}
+
+// An attention call's parameters, checked, with the tensors they point into.
+struct Forward {
   fa_paged_params p{};
+  Tensor Q, O;
+  OptTensor L;
+};
+Forward make_forward(const fa_paged_cache& c, Tensor Q, const Tensor& k_cache, const Tensor& v_cache,
+                     const OptTensor& cu_seqlens, int64_t max_query_len, int64_t causal, double scale,
+                     const OptTensor& k_scale, const OptTensor& v_scale, bool return_lse, const OptTensor& out) {
+  check_queries(Q, c, k_cache);
+  Forward f;
+  fa_paged_params& p = f.p;
   p.cu_seqlens = cu_pointer(cu_seqlens, k_cache, c.batch, Q.size(0));
-  const at::OptionalDeviceGuard guard(at::device_of(k_cache));
   if (Q.numel() != 0) Q = rows_view(Q);
   Tensor O;
   if (out.has_value()) {
@@ -265,12 +274,11 @@ std::tuple<Tensor, OptTensor> flash_attention_paged(
   } else {
     O = torch::empty(Q.sizes(), Q.options());
   }
-  OptTensor L;
-  if (return_lse) L = torch::empty({Q.size(1), Q.size(0)}, Q.options().dtype(torch::kFloat32));
+  if (return_lse) f.L = torch::empty({Q.size(1), Q.size(0)}, Q.options().dtype(torch::kFloat32));
   p.cache = &c;
   p.q = static_cast<const fa_half*>(Q.data_ptr());
   p.o = static_cast<fa_half*>(O.data_ptr());
-  p.lse = return_lse ? L->data_ptr<float>() : nullptr;
+  p.lse = return_lse ? f.L->data_ptr<float>() : nullptr;
   p.tokens = Q.size(0);
   p.heads_q = Q.size(1);
   p.q_stride_t = eff_stride(Q, 0, 0); p.q_stride_h = eff_stride(Q, 1, 0);
@@ -280,17 +288,177 @@ std::tuple<Tensor, OptTensor> flash_attention_paged(
   p.causal = (int)causal;
   p.dtype = dtype_code(Q.scalar_type());
   p.stream = current_stream(k_cache);
-  const int64_t ws = fa_sm75_paged_workspace_size(&p);
-  Tensor work;  // lives until the launch is enqueued (stream-ordered reuse)
-  if (ws > 0) {
-    work = torch::empty({ws}, Q.options().dtype(torch::kUInt8));
-    p.workspace = work.data_ptr();
-    p.workspace_bytes = ws;
-  }
-  const int st = fa_sm75_paged_forward(&p);
+  f.Q = Q;
+  f.O = O;
+  return f;
+}
+
+// A workspace of the current stream's (stream-ordered reuse behind the launch).
+Tensor workspace(int64_t bytes, const Tensor& like) {
+  return bytes > 0 ? torch::empty({bytes}, like.options().dtype(torch::kUInt8)) : Tensor();
+}
+
+std::tuple<Tensor, OptTensor> flash_attention_paged(
+    Tensor Q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens,
+    OptTensor cu_seqlens, int64_t max_query_len, int64_t causal, double scale, OptTensor k_scale,
+    OptTensor v_scale, bool return_lse, OptTensor out) {
+  check_no_tangent("flash_attention_paged", {&Q, &k_cache, &v_cache, out.has_value() ? &*out : &Q});
+  const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, false);
+  const at::OptionalDeviceGuard guard(at::device_of(k_cache));
+  Forward f = make_forward(c, Q, k_cache, v_cache, cu_seqlens, max_query_len, causal, scale, k_scale, v_scale,
+                           return_lse, out);
+  f.p.workspace_bytes = fa_sm75_paged_workspace_size(&f.p);
+  const Tensor work = workspace(f.p.workspace_bytes, k_cache);
+  f.p.workspace = work.defined() ? work.data_ptr() : nullptr;
+  const int st = fa_sm75_paged_forward(&f.p);
   TORCH_CHECK(st == FA_OK, "flash_attention_paged: ", fa_sm75_last_error());
-  if (out.has_value()) written_to(O);
-  return {O, L};
+  if (out.has_value()) written_to(f.O);
+  return {f.O, f.L};
+}
+
+std::tuple<Tensor, OptTensor> flash_attention_paged_prefix(
+    Tensor Q, Tensor k_cache, Tensor v_cache, Tensor prefix_table, Tensor prefix_lens, Tensor block_table,
+    Tensor seq_lens, OptTensor cu_seqlens, OptTensor cu_prefix, int64_t max_query_len,
+    int64_t max_prefix_queries, int64_t causal, double scale, OptTensor k_scale, OptTensor v_scale,
+    bool return_lse, OptTensor out) {
+  check_no_tangent("flash_attention_paged_prefix", {&Q, &k_cache, &v_cache, out.has_value() ? &*out : &Q});
+  const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, false);
+  check_index(prefix_table, "prefix_table", 2, k_cache);
+  check_index(prefix_lens, "prefix_lens", 1, k_cache);
+  TORCH_CHECK(prefix_table.size(0) == prefix_lens.size(0), "prefix_table and prefix_lens must have as many rows");
+  TORCH_CHECK(prefix_table.size(1) <= 1 || prefix_table.stride(1) == 1, "prefix_table's rows must be contiguous");
+  TORCH_CHECK(prefix_lens.size(0) <= 1 || prefix_lens.stride(0) == 1, "prefix_lens must be contiguous");
+  fa_paged_prefix x{};
+  x.block_table = prefix_table.data_ptr<int32_t>();
+  x.lens = prefix_lens.data_ptr<int32_t>();
+  x.count = prefix_table.size(0);
+  x.max_pages = prefix_table.size(1);
+  x.block_table_stride = eff_stride(prefix_table, 0, prefix_table.size(1));
+  x.max_queries = max_prefix_queries;
+  if (cu_prefix.has_value()) {
+    check_index(*cu_prefix, "cu_prefix", 1, k_cache);
+    TORCH_CHECK(cu_prefix->size(0) == x.count + 1, "cu_prefix must have prefixes + 1 = ", x.count + 1, " entries");
+    TORCH_CHECK(cu_prefix->stride(0) == 1, "cu_prefix must be contiguous");
+    x.cu_prefix = cu_prefix->data_ptr<int32_t>();
+  } else {
+    TORCH_CHECK(x.count == 1, "without cu_prefix there is one prefix, got ", x.count);
+  }
+  const at::OptionalDeviceGuard guard(at::device_of(k_cache));
+  Forward f = make_forward(c, Q, k_cache, v_cache, cu_seqlens, max_query_len, causal, scale, k_scale, v_scale,
+                           return_lse, out);
+  f.p.workspace_bytes = fa_sm75_paged_prefix_workspace_size(&f.p, &x);
+  const Tensor work = workspace(f.p.workspace_bytes, k_cache);
+  f.p.workspace = work.defined() ? work.data_ptr() : nullptr;
+  const int st = fa_sm75_paged_prefix_forward(&f.p, &x);
+  TORCH_CHECK(st == FA_OK, "flash_attention_paged_prefix: ", fa_sm75_last_error());
+  if (out.has_value()) written_to(f.O);
+  return {f.O, f.L};
+}
+
+// Whether [B, H, n] rows of contiguous positions lie apart from each other.
+bool rows_disjoint(const Tensor& t) {
+  const int64_t n = t.size(2), b = t.size(0), h = t.size(1);
+  const int64_t sb = t.stride(0), sh = t.stride(1);
+  if (b <= 1) return h <= 1 || sh >= n;
+  if (h <= 1) return sb >= n;
+  return sb >= sh ? sh >= n && sb >= (h - 1) * sh + n : sb >= n && sh >= (b - 1) * sb + n;
+}
+
+Tensor paged_attention_weights(Tensor Q, Tensor LSE, Tensor k_cache, Tensor block_table, Tensor seq_lens,
+                               OptTensor cu_seqlens, int64_t max_len, int64_t max_query_len, int64_t causal,
+                               double scale, OptTensor k_scale, OptTensor add_to) {
+  check_no_tangent("paged_attention_weights", {&Q, &LSE, &k_cache, add_to.has_value() ? &*add_to : &Q});
+  const fa_paged_cache c = make_cache(k_cache, k_cache, block_table, seq_lens, k_scale, k_scale, false);
+  check_queries(Q, c, k_cache);
+  TORCH_CHECK(LSE.scalar_type() == torch::kFloat32, "LSE must be float32");
+  TORCH_CHECK(LSE.device() == k_cache.device(), "LSE must be on the cache's device");
+  TORCH_CHECK(LSE.dim() == 2 && LSE.size(0) == Q.size(1) && LSE.size(1) == Q.size(0),
+              "LSE must be [H_q, tokens]");
+  fa_paged_weigh_params p{};
+  p.cu_seqlens = cu_pointer(cu_seqlens, k_cache, c.batch, Q.size(0));
+  const at::OptionalDeviceGuard guard(at::device_of(k_cache));
+  if (Q.numel() != 0) Q = rows_view(Q);
+  LSE = LSE.contiguous();
+  Tensor W;
+  if (add_to.has_value()) {
+    W = *add_to;
+    TORCH_CHECK(W.scalar_type() == torch::kFloat32, "add_to must be float32");
+    TORCH_CHECK(W.device() == k_cache.device(), "add_to must be on the cache's device");
+    TORCH_CHECK(W.dim() == 3 && W.size(0) == c.batch && W.size(1) == c.heads_kv, "add_to must be [B, H_kv, max_len]");
+    TORCH_CHECK(W.size(2) <= 1 || W.stride(2) == 1, "add_to's positions must be contiguous");
+    TORCH_CHECK(W.numel() == 0 || rows_disjoint(W), "add_to's rows must not overlap");
+    bool apart = spans_apart(W, Q) && spans_apart(W, LSE) && spans_apart(W, k_cache);
+    if (k_scale.has_value()) apart = apart && spans_apart(W, *k_scale);
+    TORCH_CHECK(apart, "add_to must not share Q's, LSE's or the cache's memory");
+  } else {
+    TORCH_CHECK(max_len >= 0, "max_len must be non-negative, got ", max_len);
+    W = torch::empty({c.batch, c.heads_kv, max_len}, LSE.options());
+  }
+  p.cache = &c;
+  p.q = static_cast<const fa_half*>(Q.data_ptr());
+  p.lse = LSE.data_ptr<float>();
+  p.weights = W.data_ptr<float>();
+  p.weights_stride_b = eff_stride(W, 0, 0);
+  p.weights_stride_h = eff_stride(W, 1, 0);
+  p.max_len = W.size(2);
+  p.add = add_to.has_value();
+  p.tokens = Q.size(0);
+  p.heads_q = Q.size(1);
+  p.q_stride_t = eff_stride(Q, 0, 0); p.q_stride_h = eff_stride(Q, 1, 0);
+  p.max_query_len = max_query_len;
+  p.scale = (float)scale;
+  p.causal = (int)causal;
+  p.dtype = dtype_code(Q.scalar_type());
+  p.stream = current_stream(k_cache);
+  const int st = fa_sm75_paged_weigh(&p);
+  TORCH_CHECK(st == FA_OK, "paged_attention_weights: ", fa_sm75_last_error());
+  if (add_to.has_value()) written_to(W);
+  return W;
+}
+
+std::tuple<Tensor, Tensor> paged_cache_evict(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens,
+                                             Tensor weights, Tensor to_table, int64_t keep, int64_t recent,
+                                             OptTensor k_scale, OptTensor v_scale) {
+  check_no_tangent("paged_cache_evict", {&k_cache, &v_cache, &weights});
+  const fa_paged_cache c = make_cache(k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, true);
+  check_index(to_table, "to_table", 2, k_cache);
+  TORCH_CHECK(to_table.size(0) == c.batch, "to_table and block_table must have the same batch");
+  TORCH_CHECK(to_table.size(1) <= 1 || to_table.stride(1) == 1, "to_table's rows must be contiguous");
+  TORCH_CHECK(weights.scalar_type() == torch::kFloat32, "weights must be float32");
+  TORCH_CHECK(weights.device() == k_cache.device(), "weights must be on the cache's device");
+  TORCH_CHECK(weights.dim() == 3 && weights.size(0) == c.batch && weights.size(1) == c.heads_kv,
+              "weights must be [B, H_kv, max_len]");
+  TORCH_CHECK(keep >= 0, "keep must be non-negative, got ", keep);
+  const at::OptionalDeviceGuard guard(at::device_of(k_cache));
+  if (weights.size(2) > 1 && weights.stride(2) != 1) weights = weights.contiguous();
+  const auto new_lens = torch::empty({c.batch}, seq_lens.options());
+  const auto new_weights = torch::empty({c.batch, c.heads_kv, to_table.size(1) * c.page_size}, weights.options());
+  fa_paged_evict_params p{};
+  p.cache = &c;
+  p.weights = weights.data_ptr<float>();
+  p.weights_stride_b = eff_stride(weights, 0, 0);
+  p.weights_stride_h = eff_stride(weights, 1, 0);
+  p.weights_len = weights.size(2);
+  p.to_table = to_table.data_ptr<int32_t>();
+  p.to_pages = to_table.size(1);
+  p.to_table_stride = eff_stride(to_table, 0, to_table.size(1));
+  p.keep = keep;
+  p.recent = recent;
+  p.new_lens = new_lens.data_ptr<int32_t>();
+  p.new_weights = new_weights.data_ptr<float>();
+  p.stream = current_stream(k_cache);
+  p.workspace_bytes = fa_sm75_paged_evict_workspace_size(&p);
+  const Tensor work = workspace(p.workspace_bytes, k_cache);
+  p.workspace = work.defined() ? work.data_ptr() : nullptr;
+  const int st = fa_sm75_paged_evict(&p);
+  TORCH_CHECK(st == FA_OK, "paged_cache_evict: ", fa_sm75_last_error());
+  written_to(k_cache);
+  written_to(v_cache);
+  if (k_scale.has_value()) {
+    written_to(*k_scale);
+    written_to(*v_scale);
+  }
+  return {new_lens, new_weights};
 }
 
 }  // namespace
@@ -310,4 +478,17 @@ void bind_paged(pybind11::module_& m) {
         py::arg("max_query_len"), py::arg("causal"), py::arg("scale"),
         py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
         py::arg("return_lse") = false, py::arg("out") = py::none());
+  m.def("flash_attention_paged_prefix", &flash_attention_paged_prefix, py::arg("Q"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("prefix_table"), py::arg("prefix_lens"), py::arg("block_table"),
+        py::arg("seq_lens"), py::arg("cu_seqlens"), py::arg("cu_prefix"), py::arg("max_query_len"),
+        py::arg("max_prefix_queries"), py::arg("causal"), py::arg("scale"),
+        py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+        py::arg("return_lse") = false, py::arg("out") = py::none());
+  m.def("paged_attention_weights", &paged_attention_weights, py::arg("Q"), py::arg("LSE"), py::arg("k_cache"),
+        py::arg("block_table"), py::arg("seq_lens"), py::arg("cu_seqlens"), py::arg("max_len"),
+        py::arg("max_query_len"), py::arg("causal"), py::arg("scale"), py::arg("k_scale") = py::none(),
+        py::arg("add_to") = py::none());
+  m.def("paged_cache_evict", &paged_cache_evict, py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"),
+        py::arg("seq_lens"), py::arg("weights"), py::arg("to_table"), py::arg("keep"), py::arg("recent"),
+        py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
 }

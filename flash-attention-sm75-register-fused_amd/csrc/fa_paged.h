@@ -1,6 +1,7 @@
 // Paged key/value cache: kernel arguments, and the pieces its kernels share
 // (fa_paged_cache.hip: writing and reading rows, fa_paged_attn.h: attention
-// over the cache, fa_paged.hip: launchers).
+// over the cache, fa_paged.hip: launchers, fa_paged_weigh.h: the weights attention gave
+// the rows, fa_paged_evict.hip: eviction by them).
 //
 // Positions of a sequence are cut into pages of 2^page_shift tokens; entry i of
 // its row of the block table names the page of positions [i << page_shift,
@@ -67,7 +68,20 @@ struct PagedArgs {
   int resident;     // the chunk kernel's workgroups of a class that run at once
   int pieces;       // most pieces the chunk kernel may cut a unit into, 0: any number
   int stream_v;     // the chunk kernel reads V non-temporally
+
+  // Attention behind shared prefixes, in two launches.  Of the prefixes (stage kPrefix):
+  // `batch` of them, table, lens and max_pages theirs, prefix g's rows those of sequences
+  // groups[g] .. groups[g + 1] - 1 of `seqs`, of all where groups is nullptr; the rows' states
+  // (O unnormalised; max, sum) go to joint_o [tokens, hq, D] and joint_ml [tokens, hq, 2].  Of
+  // the sequences' own keys (stage kOwn): the states of rows whose sequence has one of the
+  // `prefixes` join theirs.
+  int stage;
+  const int32_t* groups;
+  int prefixes, seqs;
+  float* joint_o;
+  float* joint_ml;
 };
+constexpr int kPrefix = 1, kOwn = 2;  // PagedArgs::stage
 
 // Largest key count a block table may cover, and row stride (bytes) of a cache
 // tensor: a window over 64 of its rows stays within 31 bits.
@@ -92,12 +106,54 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
                      int64_t workspace_bytes);
 int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_dim,
                            void* workspace, hipStream_t stream);
-template <int D, bool BF16, bool FP8>
+// What joint_o and joint_ml take of a workspace.
+int64_t joint_bytes(const PagedArgs& a, int head_dim);
+// SHARE: instances of the two stages behind shared prefixes.
+template <int D, bool BF16, bool FP8, bool SHARE>
 void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream);
-template <int D, bool BF16, bool FP8>
+template <int D, bool BF16, bool FP8, bool SHARE>
 void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream);
-template <int D, bool BF16>
+template <int D, bool BF16, bool SHARE>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream);
+
+// The weights that attention gave the cached rows: out[b, h, j] (+)= sum over the new tokens
+// i of sequence b that see key j, and the query heads of KV head h, of exp(scale q k - lse).
+struct WeighArgs {
+  PagedArgs p;       // q, table, lens, ..; lse_in below in place of lse
+  const float* lse;  // [hq, tokens]
+  float* out;        // out[b, h, j] at b * sb + h * sh + j, j < max_len
+  int64_t sb, sh;
+  int max_len;
+  int add;           // to what is there; else positions without a row get 0
+  // Plan.
+  int run;           // 32-key tiles of a wave
+};
+struct WeighPlan {
+  int rows;  // query columns at once
+  int run;
+  int64_t grid;
+};
+WeighPlan plan_weigh(const WeighArgs& a, int head_dim, int64_t max_query_len);
+int launch_weigh(const WeighArgs& a, const WeighPlan& plan, int head_dim, hipStream_t stream);
+template <int D, bool BF16, bool FP8>
+void launch_weigh_few(const WeighArgs& a, int rows, int64_t grid, hipStream_t stream);
+
+// Eviction: which rows stay (select), and their copies to other pages (move).
+struct EvictArgs {
+  PagedArgs p;              // the cache; table and lens of what is there
+  const float* weights;     // [batch, hkv, >= room of the table], strides wb, wh
+  int64_t wb, wh;
+  const int32_t* to_table;  // [batch, to_pages], rows to_stride apart
+  int64_t to_stride;
+  int to_pages;
+  int keep, recent;
+  int32_t* new_lens;        // [batch]
+  float* new_weights;       // [batch, hkv, to_pages << page_shift]
+  int32_t* kept;            // workspace: [batch, hkv, slots] positions of the rows that stay
+  int slots;                // the most rows that can stay: min(keep, room of the table)
+};
+int64_t evict_workspace_bytes(const EvictArgs& a);
+int launch_evict(const EvictArgs& a, int head_dim, hipStream_t stream);
 
 }  // namespace fa
 
@@ -125,11 +181,21 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 struct PagedSeq {
   int t0, n, len, keys;
 };
-template <class Load>
+template <bool SHARE = false, class Load>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load load) {
   PagedSeq s;
   const int len = load(a.lens + b);  // (all loads together)
-  if (a.cu != nullptr) {
+  if (SHARE && a.stage == kPrefix) {  // a prefix: the rows of its sequences
+    int b0 = 0, b1 = a.seqs;
+    if (a.groups != nullptr) {
+      const int g0 = load(a.groups + b), g1 = load(a.groups + b + 1);
+      b0 = clamp_int(g0, 0, a.seqs);
+      b1 = clamp_int(g1, b0, a.seqs);
+    }
+    const int t0 = a.cu != nullptr ? load(a.cu + b0) : b0, t1 = a.cu != nullptr ? load(a.cu + b1) : b1;
+    s.t0 = clamp_int(t0, 0, a.tokens);
+    s.n = clamp_int(t1, s.t0, a.tokens) - s.t0;
+  } else if (a.cu != nullptr) {
     const int t0 = load(a.cu + b), t1 = load(a.cu + b + 1);
     s.t0 = clamp_int(t0, 0, a.tokens);
     s.n = clamp_int(t1, s.t0, a.tokens) - s.t0;
@@ -142,8 +208,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load lo
   return s;
 }
 // (b the same in every lane; all of it in scalar registers)
+template <bool SHARE = false>
 __device__ __forceinline__ PagedSeq scalar_seq(const PagedArgs& a, int b) {
-  const PagedSeq s = paged_seq(a, uniform(b), load_scalar);
+  const PagedSeq s = paged_seq<SHARE>(a, uniform(b), load_scalar);
   return {uniform(s.t0), uniform(s.n), uniform(s.len), uniform(s.keys)};
 }
 

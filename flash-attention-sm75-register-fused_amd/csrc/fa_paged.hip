@@ -10,14 +10,16 @@
 namespace fa {
 
 // The instances of fa_paged_d*.hip.
-#define FA_PAGED_EXTERN(D, BF, F8) \
-  extern template void launch_paged_attn<D, BF, F8>(const PagedArgs&, int, int64_t, hipStream_t); \
-  extern template void launch_paged_chunk<D, BF, F8>(const PagedArgs&, int64_t, hipStream_t);
+#define FA_PAGED_EXTERN_S(D, BF, F8, SH) \
+  extern template void launch_paged_attn<D, BF, F8, SH>(const PagedArgs&, int, int64_t, hipStream_t); \
+  extern template void launch_paged_chunk<D, BF, F8, SH>(const PagedArgs&, int64_t, hipStream_t);
+#define FA_PAGED_EXTERN(D, BF, F8) FA_PAGED_EXTERN_S(D, BF, F8, false) FA_PAGED_EXTERN_S(D, BF, F8, true)
 FA_PAGED_EXTERN(64, false, false) FA_PAGED_EXTERN(64, true, false)
 FA_PAGED_EXTERN(64, false, true) FA_PAGED_EXTERN(64, true, true)
 FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
 FA_PAGED_EXTERN(128, false, true) FA_PAGED_EXTERN(128, true, true)
 #undef FA_PAGED_EXTERN
+#undef FA_PAGED_EXTERN_S
 
 namespace {
 int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
@@ -66,6 +68,10 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t max_query
   return p;
 }
 
+int64_t joint_bytes(const PagedArgs& a, int head_dim) {
+  return ((int64_t)a.tokens * a.hq * (head_dim + 2) * (int64_t)sizeof(float) + 15) & ~(int64_t)15;
+}
+
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
                      int64_t workspace_bytes) {
   if (max_query_len * a.group > 32) return plan_chunks(a, head_dim, max_query_len, workspace_bytes);
@@ -81,8 +87,9 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   const int64_t room = (workspace_bytes - kCombineWord) / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
   // Units of a class: blocks of rows, the last of each sequence not full.
+  const bool ones = a.cu == nullptr && a.stage != kPrefix;  // one token in every sequence
   const int64_t blocks =
-      a.cu == nullptr ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
+      ones ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
                       : (int64_t)a.tokens * a.group / p.rows + std::min(a.batch, a.tokens);
   p.units = (int)(a.hkv / p.classes * blocks);
   // (Of very many units a workgroup each is balanced enough.)
@@ -95,22 +102,40 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   const int64_t pieces = PagedStretch<kPMinTiles>::most_pieces(tiles, p.wgs);
   p.y = (int)std::min<int64_t>(p.rows, max_query_len * a.group);
   // (max_query_len may be wrong: rows are then up to p.rows)
-  p.combine = p.split && !paged_merges_itself((int)pieces, a.cu == nullptr ? p.y : p.rows, head_dim);
+  p.combine = p.split && !paged_merges_itself((int)pieces, ones ? p.y : p.rows, head_dim);
   return p;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool SHARE>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream) {
   if (rows == kChunkRows) {
-    hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16>),
+    hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16, SHARE>),
                        dim3((unsigned)(a.wgs * a.classes), kChunkCombineY), dim3(kThreads), 0, stream, a);
     return;
   }
   const dim3 g((unsigned)(a.units * a.classes), (unsigned)y);
   if (rows == 16)
-    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1>), g, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1, SHARE>), g, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 2>), g, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 2, SHARE>), g, dim3(kThreads), 0, stream, a);
+}
+
+template <int D, bool BF16, bool FP8, bool SHARE>
+static void launch_planned(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
+  const int64_t grid = (int64_t)plan.wgs * plan.classes;
+  if (plan.chunk) launch_paged_chunk<D, BF16, FP8, SHARE>(a, grid, stream);
+  else launch_paged_attn<D, BF16, FP8, SHARE>(a, plan.rows, grid, stream);
+  if (plan.combine) launch_paged_combine<D, BF16, SHARE>(a, plan.rows, plan.y, stream);
+}
+template <int D, bool SHARE>
+static void launch_typed(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
+  if (a.ks != nullptr) {
+    if (a.bf16) launch_planned<D, true, true, SHARE>(a, plan, stream);
+    else launch_planned<D, false, true, SHARE>(a, plan, stream);
+  } else {
+    if (a.bf16) launch_planned<D, true, false, SHARE>(a, plan, stream);
+    else launch_planned<D, false, false, SHARE>(a, plan, stream);
+  }
 }
 
 int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int head_dim,
@@ -134,29 +159,13 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);
     a.mark = merge_mark(a.flags, 2 * grid + 1, stream);
   }
-  const bool fp8 = a.ks != nullptr;
-#define FA_PAGED(D)                                                                     \
-  if (plan.chunk) {                                                                     \
-    if (fp8) {                                                                          \
-      if (a.bf16) launch_paged_chunk<D, true, true>(a, grid, stream);                   \
-      else launch_paged_chunk<D, false, true>(a, grid, stream);                         \
-    } else {                                                                            \
-      if (a.bf16) launch_paged_chunk<D, true, false>(a, grid, stream);                  \
-      else launch_paged_chunk<D, false, false>(a, grid, stream);                        \
-    }                                                                                   \
-  } else if (fp8) {                                                                     \
-    if (a.bf16) launch_paged_attn<D, true, true>(a, plan.rows, grid, stream);           \
-    else launch_paged_attn<D, false, true>(a, plan.rows, grid, stream);                 \
-  } else {                                                                              \
-    if (a.bf16) launch_paged_attn<D, true, false>(a, plan.rows, grid, stream);          \
-    else launch_paged_attn<D, false, false>(a, plan.rows, grid, stream);                \
-  }                                                                                     \
-  if (plan.combine) {                                                                   \
-    if (a.bf16) launch_paged_combine<D, true>(a, plan.rows, plan.y, stream);            \
-    else launch_paged_combine<D, false>(a, plan.rows, plan.y, stream);                  \
+  if (a.stage != 0) {
+    if (head_dim == 64) launch_typed<64, true>(a, plan, stream);
+    else launch_typed<128, true>(a, plan, stream);
+  } else {
+    if (head_dim == 64) launch_typed<64, false>(a, plan, stream);
+    else launch_typed<128, false>(a, plan, stream);
   }
-  if (head_dim == 64) { FA_PAGED(64) } else { FA_PAGED(128) }
-#undef FA_PAGED
   return 0;
 }
 

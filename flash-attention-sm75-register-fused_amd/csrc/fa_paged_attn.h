@@ -85,7 +85,8 @@ __device__ __forceinline__ PagedStretch<kPMinTiles> paged_stretch(const PagedArg
   return s;
 }
 
-template <int D, bool BF16, bool FP8, int NT>
+// SHARE: either stage of attention behind shared prefixes (PagedArgs::stage).
+template <int D, bool BF16, bool FP8, int NT, bool SHARE>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
   using E = Elem<BF16>;
   constexpr int R = 16 * NT;
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
 
-  const PagedLine<R, kPTile, kPAhead> line(a, lane, a.split != 0);
+  const PagedLine<R, kPTile, kPAhead, SHARE> line(a, lane, a.split != 0);
   auto stretch = paged_stretch(a, line);
   if (wg >= stretch.active) return;
   int pos, end;
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     // key it sees.
     const int nrows = s.n * a.group;
     const PagedRows row_of(a, s, hkv, rb * R);
+    const PagedJoint joint = joint_of<SHARE>(a, b);
     const int past = s.len - s.n;  // tokens before the new ones
     int last[NT];
     half8 qf[NT][KS];
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       }
       const float m2 = m == -__builtin_inff() ? m : m * c2;
       if (whole) {
-        store_row<BF16>(a, row_of(c), dim, m2, l, x);
+        store_row<D, BF16>(a, joint, row_of(c), dim, m2, l, x);
       } else {
         // Coherent over the L2s: the merging workgroup may be on another XCD.
         const int64_t rec = (int64_t)(2 * (int)blockIdx.x + (first == 0 ? 1 : 0)) * R;
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
         xm[tid] = m;
         xm[kThreads + tid] = l;
       } else {
-        store_row<BF16>(a, row_of(c), 4 * ch, m, l, x);
+        store_row<D, BF16>(a, joint, row_of(c), 4 * ch, m, l, x);
       }
     }
     __syncthreads();
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
         x += w * xo[g * items + tid];
       }
       const int c = tid / (D / 4);
-      store_row<BF16>(a, row_of(c), 4 * (tid - c * (D / 4)), m, l, x);
+      store_row<D, BF16>(a, joint, row_of(c), 4 * (tid - c * (D / 4)), m, l, x);
     }
     __syncthreads();
   }
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
 // unit of a class (blockIdx.x) and row (blockIdx.y, and every gridDim.y-th on).
 // The four waves take every fourth piece, D / 4 lanes each piece's row (with
 // several pieces at once where D / 4 < 64 lanes), and meet in LDS.
-template <int D, bool BF16, int NT>
+template <int D, bool BF16, int NT, bool SHARE>
 __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedArgs a) {
   constexpr int R = 16 * NT;
   constexpr int LR = D / 4;               // lanes of a row
@@ -544,12 +546,13 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   if (!combine_asked(a)) return;
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int index = (int)(blockIdx.x >> a.class_shift);  // of the class's units
-  const PagedLine<R, kPTile, kPAhead> line(a, threadIdx.x & 63, true);
-  const PagedLine<R, kPTile, kPAhead> units(a, threadIdx.x & 63, false);
+  const PagedLine<R, kPTile, kPAhead, SHARE> line(a, threadIdx.x & 63, true);
+  const PagedLine<R, kPTile, kPAhead, SHARE> units(a, threadIdx.x & 63, false);
   if (index >= units.total()) return;
   int unit_start;
   const int b = uniform(units.find(index, unit_start));
   const PagedSeq s = line.seq(b);
+  const PagedJoint joint = joint_of<SHARE>(a, b);
   const int unit_len = line.unit_of(s);
   const int unit = index - unit_start;
   const int u0 = line.start_of(b) + unit * unit_len;
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
         l += w * xm[1][g * LR + ch];
         x += w * xo[g * LR + ch];
       }
-      store_row<BF16>(a, PagedRows(a, s, hkv, rb * R)(c), 4 * ch, m, l, x);
+      store_row<D, BF16>(a, joint, PagedRows(a, s, hkv, rb * R)(c), 4 * ch, m, l, x);
     }
     __syncthreads();
   }
@@ -594,13 +597,13 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
 
 }  // namespace
 
-template <int D, bool BF16, bool FP8>
+template <int D, bool BF16, bool FP8, bool SHARE>
 void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream) {
   if (rows == 16)
-    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 1>), dim3((unsigned)grid), dim3(kThreads), 0,
+    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 1, SHARE>), dim3((unsigned)grid), dim3(kThreads), 0,
                        stream, a);
   else
-    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 2>), dim3((unsigned)grid), dim3(kThreads), 0,
+    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 2, SHARE>), dim3((unsigned)grid), dim3(kThreads), 0,
                        stream, a);
 }
 

@@ -159,6 +159,143 @@ int make_forward(const fa_paged_params* p, fa::PagedArgs* a, bool* empty) {
   return FA_OK;
 }
 
+// Checks the prefixes of a forward call and fills both stages' arguments from its own ones.
+int make_prefix(const fa_paged_prefix* x, const fa::PagedArgs& a, fa::PagedArgs* prefix, fa::PagedArgs* own) {
+  if (x == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "prefix must not be NULL");
+  if (x->count < 0 || x->max_pages < 0 || x->block_table_stride < 0 || x->max_queries < 0)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "the prefixes' sizes and strides must be non-negative");
+  if (x->count > (1 << 20)) return capi_fail(FA_ERR_TOO_LARGE, "the prefixes exceed 2^20");
+  if (x->max_pages > fa::kPagedMaxKeys >> a.page_shift)
+    return capi_fail(FA_ERR_TOO_LARGE, "the prefixes' max_pages * page_size exceeds 2^30 tokens");
+  if (x->count > 0 && (x->lens == nullptr || (x->max_pages > 0 && x->block_table == nullptr)))
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "the prefixes' block_table and lens must not be NULL");
+  if (x->count != 1 && x->cu_prefix == nullptr)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "without cu_prefix there is one prefix, got %lld", (long long)x->count);
+  if (!aligned(x->block_table, 4) || !aligned(x->lens, 4) || !aligned(x->cu_prefix, 4))
+    return capi_fail(FA_ERR_MISALIGNED, "the prefixes' block_table, lens and cu_prefix must be 4-byte aligned");
+  if ((int64_t)a.tokens * a.hq + x->count * a.hkv * 32 > (1 << 27))
+    return capi_fail(FA_ERR_TOO_LARGE, "tokens * heads_q + 32 * prefixes * heads_kv exceeds 2^27");
+  *own = a;
+  own->groups = x->cu_prefix;
+  own->prefixes = (int)x->count;
+  own->seqs = a.batch;
+  own->stage = x->count > 0 ? fa::kOwn : 0;
+  *prefix = *own;
+  prefix->stage = fa::kPrefix;
+  prefix->batch = (int)x->count;
+  prefix->table = x->block_table;
+  prefix->lens = x->lens;
+  prefix->table_stride = x->block_table_stride;
+  prefix->max_pages = (int)x->max_pages;
+  prefix->causal = 0;
+  prefix->lse = nullptr;
+  return FA_OK;
+}
+
+// (a checked call's: tokens > 0)
+int64_t longest_shared(const fa_paged_prefix* x, const fa::PagedArgs& a) {
+  return x->max_queries > 0 && x->max_queries < a.tokens ? x->max_queries : a.tokens;
+}
+
+// Checks a call that sums weights; *nothing: no weight to write.
+int make_weigh(const fa_paged_weigh_params* p, fa::WeighArgs* w, bool* nothing) {
+  *w = fa::WeighArgs{};
+  if (p == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "params must not be NULL");
+  if (p->cache == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "cache must not be NULL");
+  fa_paged_cache c = *p->cache;  // V is not looked at
+  c.v = c.k;
+  c.v_scale = c.k_scale;
+  c.v_stride_p = c.k_stride_p; c.v_stride_h = c.k_stride_h; c.v_stride_n = c.k_stride_n;
+  c.vs_stride_p = c.ks_stride_p; c.vs_stride_h = c.ks_stride_h; c.vs_stride_n = c.ks_stride_n;
+  fa_paged_params f{};
+  f.cache = &c;
+  f.q = p->q;
+  f.o = const_cast<fa_half*>(p->q);  // (none is written)
+  f.lse = const_cast<float*>(p->lse);
+  f.tokens = p->tokens;
+  f.heads_q = p->heads_q;
+  f.q_stride_t = f.o_stride_t = p->q_stride_t;
+  f.q_stride_h = f.o_stride_h = p->q_stride_h;
+  f.cu_seqlens = p->cu_seqlens;
+  f.max_query_len = p->max_query_len;
+  f.scale = p->scale;
+  f.causal = p->causal;
+  f.dtype = p->dtype;
+  bool empty = true;
+  if (int st = make_forward(&f, &w->p, &empty)) return st;
+  if (!empty && p->lse == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "lse must not be NULL");
+  if (p->max_len < 0 || p->weights_stride_b < 0 || p->weights_stride_h < 0)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "max_len and the weights' strides must be non-negative");
+  if (p->max_len > fa::kPagedMaxKeys) return capi_fail(FA_ERR_TOO_LARGE, "max_len exceeds 2^30");
+  const int64_t pairs = (int64_t)w->p.batch * w->p.hkv;
+  *nothing = pairs == 0 || p->max_len == 0 || (empty && p->add);
+  if (*nothing) return FA_OK;
+  if (pairs > (1 << 22) || pairs * ((p->max_len + 31) / 32) > (1 << 28))
+    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 2^22, or batch * heads_kv * max_len 2^33");
+  if (p->weights == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "weights must not be NULL");
+  if (!aligned(p->weights, 4)) return capi_fail(FA_ERR_MISALIGNED, "weights must be 4-byte aligned");
+  if (empty) {  // no row: every weight is 0
+    w->p.tokens = 0;
+    w->p.group = 1;
+    w->p.c = 1.0f;
+  }
+  w->lse = p->lse;
+  w->out = p->weights;
+  w->sb = p->weights_stride_b;
+  w->sh = p->weights_stride_h;
+  w->max_len = (int)p->max_len;
+  w->add = p->add ? 1 : 0;
+  return FA_OK;
+}
+
+// Checks an eviction; *nothing: no sequence.
+int make_evict(const fa_paged_evict_params* p, fa::EvictArgs* e, bool* nothing) {
+  *e = fa::EvictArgs{};
+  if (p == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "params must not be NULL");
+  if (int st = make_cache(p->cache, FA_DTYPE_FP16, &e->p)) return st;  // (rows are copied as they are)
+  const fa::PagedArgs& a = e->p;
+  if (a.hkv == 0) return capi_fail(FA_ERR_INVALID_ARGUMENT, "heads_kv must be positive");
+  if (p->keep < 0 || p->recent < 0 || p->to_pages < 0 || p->weights_len < 0 || p->workspace_bytes < 0)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "keep, recent and sizes must be non-negative");
+  if (p->recent > p->keep)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "recent (%lld) must not exceed keep (%lld)", (long long)p->recent,
+                     (long long)p->keep);
+  if (p->weights_stride_b < 0 || p->weights_stride_h < 0 || p->to_table_stride < 0)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "strides must be non-negative");
+  if (p->to_pages > fa::kPagedMaxKeys >> a.page_shift)
+    return capi_fail(FA_ERR_TOO_LARGE, "to_pages * page_size exceeds 2^30 tokens");
+  const int64_t room = (int64_t)a.max_pages << a.page_shift, to_room = p->to_pages << a.page_shift;
+  const int64_t slots = p->keep < room ? p->keep : room;
+  if (to_room < slots)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "to_table has room for %lld rows, up to %lld stay", (long long)to_room,
+                     (long long)slots);
+  if (p->weights_len < room)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "weights must have block_table's room, %lld positions, got %lld",
+                     (long long)room, (long long)p->weights_len);
+  const int64_t pairs = (int64_t)a.batch * a.hkv;
+  *nothing = pairs == 0;
+  if (*nothing) return FA_OK;
+  if (pairs > (1 << 20) || pairs * slots > (1 << 30))
+    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 2^20, or the rows that stay 2^30");
+  if (p->new_lens == nullptr || (to_room > 0 && p->new_weights == nullptr) ||
+      (room > 0 && p->weights == nullptr) || (p->to_pages > 0 && p->to_table == nullptr))
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "weights, to_table, new_lens and new_weights must not be NULL");
+  if (!aligned(p->weights, 4) || !aligned(p->to_table, 4) || !aligned(p->new_lens, 4) || !aligned(p->new_weights, 4))
+    return capi_fail(FA_ERR_MISALIGNED, "weights, to_table, new_lens and new_weights must be 4-byte aligned");
+  e->weights = p->weights;
+  e->wb = p->weights_stride_b;
+  e->wh = p->weights_stride_h;
+  e->to_table = p->to_table;
+  e->to_stride = p->to_table_stride;
+  e->to_pages = (int)p->to_pages;
+  e->keep = (int)slots;
+  e->recent = (int)(p->recent < INT32_MAX ? p->recent : INT32_MAX);
+  e->new_lens = p->new_lens;
+  e->new_weights = p->new_weights;
+  e->slots = (int)slots;
+  return FA_OK;
+}
+
 // (a checked call's: tokens > 0)
 int64_t longest_query(const fa_paged_params* p) {
   if (p->cu_seqlens == nullptr) return 1;
@@ -229,6 +366,82 @@ int fa_sm75_paged_forward(const fa_paged_params* p) {
   const fa::PagedPlan plan = fa::plan_paged(a, head_dim, longest_query(p),
                                             p->workspace != nullptr ? p->workspace_bytes : 0);
   fa::launch_paged_attention(a, plan, head_dim, p->workspace, static_cast<hipStream_t>(p->stream));
+  return check_launch();
+}
+
+int64_t fa_sm75_paged_prefix_workspace_size(const fa_paged_params* p, const fa_paged_prefix* x) {
+  const fa::SavedError keep;  // a size is no error report
+  fa::PagedArgs a, prefix, own;
+  bool empty = true;
+  if (make_forward(p, &a, &empty) != FA_OK || empty || make_prefix(x, a, &prefix, &own) != FA_OK) return 0;
+  const int d = (int)p->cache->head_dim;
+  const int64_t rest = fa::plan_paged(own, d, longest_query(p), INT64_MAX).workspace_bytes;
+  if (own.stage == 0) return rest;
+  const int64_t first = fa::plan_paged(prefix, d, longest_shared(x, a), INT64_MAX).workspace_bytes;
+  return fa::joint_bytes(a, d) + (first > rest ? first : rest);
+}
+
+int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix* x) {
+  fa::capi_clear_error();
+  fa::PagedArgs a, prefix, own;
+  bool empty = true;
+  if (int st = make_forward(p, &a, &empty)) return st;
+  if (empty) return FA_OK;
+  if (int st = make_prefix(x, a, &prefix, &own)) return st;
+  const int d = (int)p->cache->head_dim;
+  const hipStream_t stream = static_cast<hipStream_t>(p->stream);
+  char* work = static_cast<char*>(p->workspace);
+  int64_t bytes = p->workspace != nullptr ? p->workspace_bytes : 0;
+  if (own.stage != 0) {
+    const int64_t joint = fa::joint_bytes(a, d);
+    if (bytes < joint)
+      return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes at least, got %lld",
+                       (long long)joint, (long long)bytes);
+    prefix.joint_o = own.joint_o = reinterpret_cast<float*>(work);
+    prefix.joint_ml = own.joint_ml = own.joint_o + (int64_t)a.tokens * a.hq * d;
+    work += joint;
+    bytes -= joint;
+    const fa::PagedPlan plan = fa::plan_paged(prefix, d, longest_shared(x, a), bytes);
+    fa::launch_paged_attention(prefix, plan, d, work, stream);
+  }
+  const fa::PagedPlan plan = fa::plan_paged(own, d, longest_query(p), bytes);
+  fa::launch_paged_attention(own, plan, d, work, stream);
+  return check_launch();
+}
+
+int fa_sm75_paged_weigh(const fa_paged_weigh_params* p) {
+  fa::capi_clear_error();
+  fa::WeighArgs w;
+  bool nothing = true;
+  if (int st = make_weigh(p, &w, &nothing)) return st;
+  if (nothing) return FA_OK;
+  const int64_t longest = p->cu_seqlens == nullptr ? 1
+                          : p->max_query_len > 0 && p->max_query_len < p->tokens ? p->max_query_len : p->tokens;
+  const int d = (int)p->cache->head_dim;
+  fa::launch_weigh(w, fa::plan_weigh(w, d, longest), d, static_cast<hipStream_t>(p->stream));
+  return check_launch();
+}
+
+int64_t fa_sm75_paged_evict_workspace_size(const fa_paged_evict_params* p) {
+  const fa::SavedError keep;  // a size is no error report
+  fa::EvictArgs e;
+  bool nothing = true;
+  return make_evict(p, &e, &nothing) != FA_OK || nothing ? 0 : fa::evict_workspace_bytes(e);
+}
+
+int fa_sm75_paged_evict(const fa_paged_evict_params* p) {
+  fa::capi_clear_error();
+  fa::EvictArgs e;
+  bool nothing = true;
+  if (int st = make_evict(p, &e, &nothing)) return st;
+  if (nothing) return FA_OK;
+  const int64_t need = fa::evict_workspace_bytes(e);
+  if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need))
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes, got %lld", (long long)need,
+                     (long long)(p->workspace != nullptr ? p->workspace_bytes : 0));
+  if (!aligned(p->workspace, 16)) return capi_fail(FA_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  e.kept = static_cast<int32_t*>(p->workspace);
+  fa::launch_evict(e, (int)p->cache->head_dim, static_cast<hipStream_t>(p->stream));
   return check_launch();
 }
 

@@ -75,6 +75,36 @@ __device__ __forceinline__ void store_pair(_Float16* to, float4v x, float4v y, f
   *(uint4v*)to = v;
 }
 
+// O and LSE of a row from its merged state: pairs of groups pair0 .. pair0 + N - 1, 16
+// dimensions each, of which a half-wave holds 4 hi .. + 3 and 8 + 4 hi .. + 3.
+template <int D, bool BF16, int N>
+__device__ __forceinline__ void store_pairs(const PagedArgs& a, const PagedJoint joint, const PagedRow pr, int hi,
+                                            int pair0, float m2, float l, float4v (&x)[N][2]) {
+  if (joint.out) {
+    const int64_t row = joint_row(a, pr);
+    float* const to = a.joint_o + row * D + 16 * pair0 + 4 * hi;
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) *(float4v*)(to + 16 * q + 8 * e) = x[q][e];
+    if (hi == 0 && pair0 == 0) *(v2f*)(a.joint_ml + 2 * row) = v2f{m2, l};
+    return;
+  }
+  if (joint.in) {
+    const JointState<D> j(a, pr, m2, l);
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) x[q][e] = j.x(16 * (pair0 + q) + 4 * hi + 8 * e, x[q][e]);
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+#pragma unroll
+  for (int q = 0; q < N; ++q) store_pair<BF16>(op + 16 * (pair0 + q) + 8 * hi, x[q][0], x[q][1], inv);
+  if (a.lse != nullptr && hi == 0 && pair0 == 0)
+    a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+}
+
 // Whether a unit's last workgroup merges its partials (it reads them at about 50
 // bytes/ns, 6 us for these many), or the second kernel.  Where a launch has units enough
 // (plan_chunks), stretches are made long enough that none has more, and the second
@@ -107,7 +137,7 @@ struct ChunkRecord {
 // l_i, M = max_i m_i.
 template <int D, bool BF16>
 __device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPieces& pieces, int cls,
-                                            const PagedRows& row_of, int rows, int pair0) {
+                                            const PagedJoint joint, const PagedRows& row_of, int rows, int pair0) {
   constexpr int PAIRS = 4, AT = 4;  // at once; pieces at once
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -158,13 +188,7 @@ __device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPiece
         for (int e = 0; e < 2; ++e) x[q][e] += w * o[u][q][e];
     }
   }
-  const PagedRow pr = row_of(r);
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
-#pragma unroll
-  for (int q = 0; q < PAIRS; ++q) store_pair<BF16>(op + 16 * (pair0 + q) + 8 * hi, x[q][0], x[q][1], inv);
-  if (a.lse != nullptr && hi == 0 && pair0 == 0)
-    a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
+  store_pairs<D, BF16, PAIRS>(a, joint, row_of(r), hi, pair0, m, l, x);
 }
 
 // A class's stretches.  Where all units are equally long, of units, each into the number q
@@ -205,7 +229,8 @@ __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const Page
 }
 
 // STREAM: V's rows are read non-temporally (a sequence's only block is the one that reads them).
-template <int D, bool BF16, bool FP8, bool SPLIT, bool STREAM>
+// SHARE: either stage of attention behind shared prefixes (PagedArgs::stage).
+template <int D, bool BF16, bool FP8, bool SPLIT, bool STREAM, bool SHARE>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
   constexpr bool DENSE = D == 64;
   using L = std::conditional_t<DENSE, LdsDense<D>, Lds<D>>;
@@ -232,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
-  const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, SPLIT);
+  const PagedLine<kChunkRows, kBlockN, kChunkAhead, SHARE> line(a, threadIdx.x & 63, SPLIT);
   const auto stretch = [&] {
     if constexpr (SPLIT) return chunk_stretch<D>(a, line);
     else return PagedStretch<1>(a, line.total());
@@ -734,21 +759,18 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 
   const float l = halves_sum(l_run);
   const float m2 = m_run == -__builtin_inff() ? m_run : m_run * c2;
+  const PagedJoint joint = joint_of<SHARE>(a, b);
   if (row < nrows) {
     if (whole) {
-      const PagedRow pr = row_of(row - q0);
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh + 8 * hi;
+      float4v x[D / 16][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int q = 0; q < D / 16; ++q)
 #pragma unroll
-        for (int g = 0; g < 4; g += 2)
-          store_pair<BF16>(op + 32 * mt + 8 * g,
-                           float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]},
-                           float4v{oacc[mt][4 * g + 4], oacc[mt][4 * g + 5], oacc[mt][4 * g + 6],
-                                   oacc[mt][4 * g + 7]},
-                           inv);
-      if (a.lse != nullptr && hi == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+        for (int e = 0; e < 2; ++e) {
+          const int mt = q / 2, g = 2 * (q % 2) + e;
+          x[q][e] = float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
+        }
+      store_pairs<D, BF16, D / 16>(a, joint, row_of(row - q0), hi, 0, m2, l, x);
     } else {
       // (see ChunkRecord; coherent over the L2s: the merging workgroup may be on
       // another XCD)
@@ -774,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
         ask_combine(a);
       } else if (last_to_finish(a, pieces, cls, 2 * (int)blockIdx.x + (first == 0 ? 1 : 0), (int*)k_lds0)) {
         for (int pair = 0; pair < D / 16; pair += 4)
-          merge_chunk<D, BF16>(a, pieces, cls, row_of, nrows - q0, pair);
+          merge_chunk<D, BF16>(a, pieces, cls, joint, row_of, nrows - q0, pair);
       }
     }
     __syncthreads();  // the next segment's loads go into these tiles
@@ -787,14 +809,14 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 // of the unit share its tasks, a pair of groups of one wave's 32 rows each.  Of a task
 // the workgroup's waves take every fourth piece, and meet in LDS.
 constexpr int kChunkCombineY = 2;
-template <int D, bool BF16>
+template <int D, bool BF16, bool SHARE>
 __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
   __shared__ float4v xo[kWaves][2][64];
   __shared__ float xml[kWaves][2][64];
   if (!combine_asked(a)) return;
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
-  const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, true);
+  const PagedLine<kChunkRows, kBlockN, kChunkAhead, SHARE> line(a, threadIdx.x & 63, true);
   const auto stretch = chunk_stretch<D>(a, line);
   if (wg == 0 || wg >= stretch.active) return;
   int border, end;
@@ -814,6 +836,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int rows = s.n * a.group - rb * kChunkRows;
   const PagedRows row_of(a, s, hc * a.classes + cls, rb * kChunkRows);
+  const PagedJoint joint = joint_of<SHARE>(a, b);
   const ChunkRecord<D> rec(a);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -872,11 +895,8 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
         x[0] += f * xo[w][0][lane];
         x[1] += f * xo[w][1][lane];
       }
-      const PagedRow pr = row_of(r);
-      store_pair<BF16>(a.o + pr.token * a.ot + pr.head * a.oh + 16 * pair + 8 * hi, x[0], x[1],
-                       l > 0.0f ? 1.0f / l : 0.0f);
-      if (a.lse != nullptr && hi == 0 && pair == 0)
-        a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
+      float4v y[1][2] = {{x[0], x[1]}};
+      store_pairs<D, BF16, 1>(a, joint, row_of(r), hi, pair, m, l, y);
     }
     __syncthreads();
   }
@@ -884,15 +904,21 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
 
 }  // namespace
 
-template <int D, bool BF16, bool FP8>
+// (Behind shared prefixes V is not read non-temporally: a prefix's rows are read by all its blocks.)
+template <int D, bool BF16, bool FP8, bool SHARE>
 void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream) {
   const dim3 g((unsigned)grid), t(kThreads);
-  if (a.split && a.stream_v)
-    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, true>), g, t, 0, stream, a);
-  else if (a.split)
-    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, false>), g, t, 0, stream, a);
-  else
-    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false, false>), g, t, 0, stream, a);
+  if (!a.split) {
+    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false, false, SHARE>), g, t, 0, stream, a);
+    return;
+  }
+  if constexpr (!SHARE) {
+    if (a.stream_v) {
+      hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, true, SHARE>), g, t, 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, false, SHARE>), g, t, 0, stream, a);
 }
 
 }  // namespace fa

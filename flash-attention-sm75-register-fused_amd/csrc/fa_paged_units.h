@@ -52,7 +52,7 @@ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& 
 // again and again, so that sequences share rows, may positions wrap round, and then
 // units are held to those there are, and pieces to the workgroups).  Called by whole
 // waves; the first 64 sequences, one a lane, are looked at once.
-template <int R, int T, int H>
+template <int R, int T, int H, bool SHARE = false>
 struct PagedLine {
   const PagedArgs& a;
   const int lane;
@@ -77,7 +77,7 @@ struct PagedLine {
     first = wave_prefix(length_of(own));
   }
   __device__ __forceinline__ PagedSeq look(int b) const {
-    PagedSeq s = paged_seq(a, min(b, a.batch - 1), [](const int32_t* p) { return *p; });
+    PagedSeq s = paged_seq<SHARE>(a, min(b, a.batch - 1), [](const int32_t* p) { return *p; });
     if (b >= a.batch) s.n = 0;
     return s;
   }
@@ -108,7 +108,7 @@ struct PagedLine {
     return most;
   }
   __device__ __forceinline__ PagedSeq seq(int b) const {
-    if (b >= 64) return scalar_seq(a, b);
+    if (b >= 64) return scalar_seq<SHARE>(a, b);
     return {wave_bcast(own.t0, b), wave_bcast(own.n, b), wave_bcast(own.len, b), wave_bcast(own.keys, b)};
   }
   // The sequence b that holds position pos (0 <= pos < total), and where it starts.
@@ -255,10 +255,61 @@ constexpr int kPCoherent = 16, kPStreamed = 2;
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
+// What becomes of a unit's merged states behind shared prefixes: they are kept (of a prefix), or
+// join those of their rows over the prefix (of a sequence that has one).
+struct PagedJoint {
+  bool out, in;
+};
+template <bool SHARE>
+__device__ __forceinline__ PagedJoint joint_of(const PagedArgs& a, int b) {
+  PagedJoint j = {false, false};
+  if constexpr (SHARE) {
+    j.out = a.stage == kPrefix;
+    j.in = !j.out;
+    if (j.in && a.groups != nullptr) {
+      const int first = load_scalar(a.groups), behind = load_scalar(a.groups + a.prefixes);
+      j.in = b >= first && b < behind;
+    }
+  }
+  return j;
+}
+__device__ __forceinline__ int64_t joint_row(const PagedArgs& a, const PagedRow pr) {
+  return (int64_t)pr.token * a.hq + pr.head;
+}
+// A row's own state (m, l, and its x through `x`) joined with the one over its prefix:
+// M = max(m, m'), l = 2^(m - M) l + 2^(m' - M) l', x likewise; all in 32 bits, one rounding
+// to the 16-bit type after both.
+template <int D>
+struct JointState {
+  float f, fp;
+  const float* o;
+  __device__ __forceinline__ JointState(const PagedArgs& a, const PagedRow pr, float& m, float& l) {
+    const int64_t row = joint_row(a, pr);
+    const v2f p = *(const v2f*)(a.joint_ml + 2 * row);
+    o = a.joint_o + row * D;
+    const float top = fmaxf(m, p[0]);
+    f = __builtin_amdgcn_exp2f(m - over_zero(top));
+    fp = __builtin_amdgcn_exp2f(p[0] - over_zero(top));
+    l = f * l + fp * p[1];
+    m = top;
+  }
+  __device__ __forceinline__ float4v x(int dim, float4v own) const { return f * own + fp * *(const float4v*)(o + dim); }
+};
+
 // O and LSE of a row from its merged state, 4 dimensions.
-template <bool BF16>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedRow pr, int dim, float m2, float l,
-                                          float4v x) {
+template <int D, bool BF16>
+__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedJoint joint, const PagedRow pr, int dim,
+                                          float m2, float l, float4v x) {
+  if (joint.out) {
+    const int64_t row = joint_row(a, pr);
+    *(float4v*)(a.joint_o + row * D + dim) = x;
+    if (dim == 0) *(v2f*)(a.joint_ml + 2 * row) = v2f{m2, l};
+    return;
+  }
+  if (joint.in) {
+    const JointState<D> j(a, pr, m2, l);
+    x = j.x(dim, x);
+  }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   half4 y;
 #pragma unroll

@@ -1,0 +1,7 @@
+// The weights attention gave a paged cache's rows, head_dim 128, e4m3 rows (see fa_paged_weigh.h).
+#include "fa_paged_weigh.h"
+
+namespace fa {
+template void launch_weigh_few<128, false, true>(const WeighArgs&, int, int64_t, hipStream_t);
+template void launch_weigh_few<128, true, true>(const WeighArgs&, int, int64_t, hipStream_t);
+}  // namespace fa

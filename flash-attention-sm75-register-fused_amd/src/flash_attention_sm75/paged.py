@@ -1,4 +1,5 @@
-"""Paged key/value cache: writing new tokens, reading them back, attention over it.
+"""Paged key/value cache: writing new tokens, reading them back, attention over it, prefixes
+that sequences share, the weight that attention gave each row, and eviction by it.
 
 No reference counterpart (the reference has neither a cache nor a decode path).
 
@@ -36,6 +37,22 @@ import flash_attn_sm75_cuda as _C
 def _no_backward(name):
     return RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() "
                         "or on detached tensors")
+
+
+def _causal_code(causal):
+    if causal is False:
+        return 0
+    if causal == "bottom_right":
+        return 2
+    raise ValueError(f"causal must be 'bottom_right' or False, got {causal!r}")
+
+
+def _hint(value, name):
+    if value is None:
+        return 0
+    if value < 0:
+        raise ValueError(f"{name} must be non-negative, got {value}")
+    return int(value)
 
 
 def paged_cache_write(K, V, k_cache, v_cache, block_table, seq_lens, cu_seqlens=None,
@@ -120,19 +137,114 @@ def flash_attention_paged(Q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
     if torch.is_grad_enabled() and (Q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
                                     or (out is not None and out.requires_grad)):
         raise _no_backward("flash_attention_paged")
-    if causal is False:
-        code = 0
-    elif causal == "bottom_right":
-        code = 2
-    else:
-        raise ValueError(f"causal must be 'bottom_right' or False, got {causal!r}")
+    code = _causal_code(causal)
     if scale is None:
         scale = 1.0 / math.sqrt(Q.size(-1))
-    if max_query_len is None:
-        max_query_len = 0
-    elif max_query_len < 0:
-        raise ValueError(f"max_query_len must be non-negative, got {max_query_len}")
     o, lse = _C.flash_attention_paged(Q, k_cache, v_cache, block_table, seq_lens, cu_seqlens,
-                                      int(max_query_len), code, float(scale), k_scale, v_scale,
+                                      _hint(max_query_len, "max_query_len"), code, float(scale), k_scale, v_scale,
                                       bool(return_lse), out)
     return (o, lse) if return_lse else o
+
+
+def flash_attention_paged_prefix(Q, k_cache, v_cache, prefix_table, prefix_lens, block_table, seq_lens,
+                                 cu_seqlens=None, cu_prefix=None, max_query_len=None,
+                                 max_prefix_queries=None, causal="bottom_right", scale=None, k_scale=None,
+                                 v_scale=None, return_lse=False, out=None):
+    """Attention of new tokens whose sequences share prefixes (an instruction, a document): a
+    prefix's rows are read once for all of its sequences.
+
+    What :func:`flash_attention_paged` gives where each sequence's table lists its prefix's pages
+    first, with these differences: block_table and seq_lens are of a sequence's own tokens
+    (new ones included) and do not count its prefix, whose length need not fill its last page.
+
+    Args:
+        prefix_table: [G, max_prefix_pages] int32, the pages of each prefix, as block_table.
+        prefix_lens: [G] int32, tokens of each prefix.
+        cu_prefix: [G + 1] int32, rising: sequences cu_prefix[g] .. cu_prefix[g + 1] - 1 have
+            prefix g, those before cu_prefix[0] and from cu_prefix[G] on none.  None: there is
+            one prefix, and every sequence has it.
+        max_prefix_queries: the most new tokens behind one prefix, if the caller knows: a hint
+            as max_query_len.
+        causal: by which a new token sees its sequence's own keys; it sees all of its prefix.
+
+        The others, and what is returned, are those of :func:`flash_attention_paged`; LSE is
+        over the prefix and the own keys.
+    """
+    if torch.is_grad_enabled() and (Q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                                    or (out is not None and out.requires_grad)):
+        raise _no_backward("flash_attention_paged_prefix")
+    code = _causal_code(causal)
+    if scale is None:
+        scale = 1.0 / math.sqrt(Q.size(-1))
+    o, lse = _C.flash_attention_paged_prefix(
+        Q, k_cache, v_cache, prefix_table, prefix_lens, block_table, seq_lens, cu_seqlens, cu_prefix,
+        _hint(max_query_len, "max_query_len"), _hint(max_prefix_queries, "max_prefix_queries"), code,
+        float(scale), k_scale, v_scale, bool(return_lse), out)
+    return (o, lse) if return_lse else o
+
+
+def paged_attention_weights(Q, LSE, k_cache, block_table, seq_lens, cu_seqlens=None, max_len=None,
+                            max_query_len=None, causal="bottom_right", scale=None, k_scale=None, add_to=None):
+    """The weight that attention gave each cached row: its probabilities, summed over the new
+    tokens and the query heads that share its KV head.
+
+    Args:
+        Q, k_cache, block_table, seq_lens, cu_seqlens, max_query_len, causal, scale, k_scale: the
+            attention call's.
+        LSE: the log-sum-exp it returned, [H_q, tokens] float32; a row of -inf adds nothing.
+        max_len: positions to weigh (default: all that block_table has room for).
+        add_to: [B, H_kv, max_len] float32, positions contiguous: the weights are added to
+            those of the positions that hold a row, the others are left as they are.  Its rows
+            must not overlap, nor share memory with the other tensors.
+
+    Returns:
+        weights [B, H_kv, max_len] float32 (add_to where that is given): entry j is position j's;
+        0 past a sequence's end and where it has no page.  Deterministic: the same call gives the
+        same bits.
+
+    The rows of a shared prefix get theirs from a call over its table (prefix_table, prefix_lens, and for
+    cu_seqlens the bounds of its sequences' tokens) with causal=False and the LSE of
+    :func:`flash_attention_paged_prefix`.  A key that is not finite gives its own weight only;
+    a query or LSE that is NaN gives every row it sees NaN.
+    """
+    if torch.is_grad_enabled() and (Q.requires_grad or LSE.requires_grad or k_cache.requires_grad
+                                    or (add_to is not None and add_to.requires_grad)):
+        raise _no_backward("paged_attention_weights")
+    code = _causal_code(causal)
+    if scale is None:
+        scale = 1.0 / math.sqrt(Q.size(-1))
+    if max_len is None:
+        max_len = block_table.size(1) * k_cache.size(2) if block_table.dim() == 2 and k_cache.dim() == 4 else 0
+    elif add_to is not None:
+        raise ValueError("max_len goes without add_to, whose size says it")
+    return _C.paged_attention_weights(Q, LSE, k_cache, block_table, seq_lens, cu_seqlens, int(max_len),
+                                      _hint(max_query_len, "max_query_len"), code, float(scale), k_scale, add_to)
+
+
+def paged_cache_evict(k_cache, v_cache, block_table, seq_lens, weights, to_table, keep, recent=0,
+                      k_scale=None, v_scale=None):
+    """Cuts each sequence to ``keep`` rows, for each KV head those that attention gave most
+    weight: they are copied, in order, to other pages.
+
+    Args:
+        weights: [B, H_kv, max_len] float32, max_len at least what block_table has room for: of each
+            position (:func:`paged_attention_weights`).
+        to_table: [B, max_to_pages] int32, the pages that the rows go to, with room for keep rows (or for
+            as many as block_table has room for).  None of them may be one of block_table's that hold
+            rows, and none may be listed twice; rows whose place has no page are dropped.
+        keep: rows that stay (all, where a sequence holds no more).
+        recent: those of the sequence's last ``recent`` positions (at most keep) stay whatever their weights.
+
+    Of the other rows the heaviest stay; of equal ones those at the lowest positions; NaN
+    counts as less than any number.  Positions without a page hold no row, so what is kept
+    closes up over them.  block_table's rows and seq_lens are left as they are, and its pages may be shared
+    between sequences; the caller goes on with to_table and what is returned:
+
+    Returns:
+        (seq_lens, weights): [B] int32, rows that stayed; [B, H_kv, max_to_pages * page_size] float32, their
+        weights, 0 behind them.
+    """
+    if torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad or weights.requires_grad):
+        raise _no_backward("paged_cache_evict")
+    return _C.paged_cache_evict(k_cache, v_cache, block_table, seq_lens, weights, to_table, int(keep), int(recent),
+                                k_scale, v_scale)

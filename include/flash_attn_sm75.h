@@ -431,6 +431,88 @@ int fa_sm75_paged_forward(const fa_paged_params* p);
  * depend on the sizes and the current device only, not on what the tables hold. */
 int64_t fa_sm75_paged_workspace_size(const fa_paged_params* p);
 
+/* Attention of sequences that share a prefix, whose rows are read once for all of them.
+ * Sequences cu_prefix[g] .. cu_prefix[g + 1] - 1 of the call's batch have prefix g: their new
+ * tokens see all of its keys, whatever p->causal is, and their own (the cache's block_table
+ * and seq_lens, which do not count the prefix) by p->causal; sequences before cu_prefix[0] and
+ * from cu_prefix[count] on have none.  The pages are the cache's.  cu_prefix is held to
+ * [0, batch] and to rising. */
+typedef struct fa_paged_prefix {
+  const int32_t* block_table; /* [count, max_pages], rows block_table_stride apart, as the cache's */
+  const int32_t* lens;        /* [count]: tokens of each prefix */
+  int64_t count;              /* up to 2^20, tokens * heads_q + 32 * count * heads_kv up to 2^27 */
+  int64_t max_pages;          /* max_pages * page_size up to 2^30 */
+  int64_t block_table_stride;
+  const int32_t* cu_prefix;   /* [count + 1], or NULL: one prefix, of every sequence */
+  int64_t max_queries;        /* the most new tokens behind one prefix, or 0 (not known): a hint
+                                 as max_query_len */
+} fa_paged_prefix;
+
+/* As fa_sm75_paged_forward (p->lse: over the prefix and the own keys), but for the workspace:
+ * it is needed, for the 32-bit states of the rows over their prefixes, tokens * heads_q *
+ * (head_dim + 2) floats (and 12 bytes), whose size in whole 16 bytes is the least taken. */
+int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix* prefix);
+int64_t fa_sm75_paged_prefix_workspace_size(const fa_paged_params* p, const fa_paged_prefix* prefix);
+
+/* The weight that attention gave each cached row: for KV head h and position j of sequence b
+ * the sum of exp(scale q k - lse) over the new tokens that see j and the query heads of h's
+ * group, lse the log-sum-exp of fa_sm75_paged_forward or fa_sm75_paged_prefix_forward (a row of -inf adds
+ * nothing).  A prefix's rows get theirs from a call over its table, whose cu_seqlens bounds its
+ * sequences' tokens, with FA_CAUSAL_NONE. */
+typedef struct fa_paged_weigh_params {
+  const fa_paged_cache* cache; /* its V is not looked at */
+  const fa_half* q;    /* [tokens, heads_q, head_dim] */
+  const float* lse;    /* [heads_q, tokens] */
+  float* weights;      /* [batch, heads_kv, max_len], strides in elements, positions contiguous */
+  int64_t weights_stride_b, weights_stride_h;
+  int64_t max_len;     /* positions up to max_len are weighed; batch * heads_kv up to 2^22, times
+                          max_len up to 2^33 */
+  int add;             /* nonzero: add to what is there (positions without a row are left as they
+                          are); 0: write (they get 0) */
+  int64_t tokens;      /* as in fa_paged_params, as all that follows */
+  int64_t heads_q;
+  int64_t q_stride_t, q_stride_h;
+  const int32_t* cu_seqlens;
+  int64_t max_query_len;
+  float scale;
+  int causal;
+  int dtype;
+  void* stream;
+} fa_paged_weigh_params;
+
+/* Asynchronous on p->stream; needs no workspace.  The same call gives the same bits. */
+int fa_sm75_paged_weigh(const fa_paged_weigh_params* p);
+
+/* Eviction: of each sequence and KV head, min(keep, rows it holds) rows stay: those of its last
+ * `recent` positions, and of the others the ones of the largest weights (of equal ones those at
+ * the lowest positions; NaN is less than any number).  Row number r of them, in their order, is
+ * copied to position r of to_table's row (K, V and scales; dropped where that has no page), its
+ * weight to new_weights[b, h, r]; the rest of new_weights is 0, and new_lens[b] the number of rows that
+ * stayed.  to_table's pages must be none of block_table's that hold rows, and each be listed once; rows of
+ * theirs that none is copied to are left as they are. */
+typedef struct fa_paged_evict_params {
+  const fa_paged_cache* cache;
+  const float* weights;     /* [batch, heads_kv, weights_len], strides in elements, positions contiguous */
+  int64_t weights_stride_b, weights_stride_h;
+  int64_t weights_len;      /* at least max_pages * page_size */
+  const int32_t* to_table;  /* [batch, to_pages], rows to_table_stride apart */
+  int64_t to_pages;         /* to_pages * page_size at least keep, or as many as block_table has
+                               room for */
+  int64_t to_table_stride;
+  int64_t keep, recent;     /* 0 <= recent <= keep; batch * heads_kv up to 2^20, times keep up to 2^30 */
+  int32_t* new_lens;        /* [batch] */
+  float* new_weights;       /* contiguous [batch, heads_kv, to_pages * page_size] */
+  void* stream;
+  void* workspace;          /* 16-byte aligned, fa_sm75_paged_evict_workspace_size() bytes; calls that
+                               share one race */
+  int64_t workspace_bytes;
+} fa_paged_evict_params;
+
+/* Asynchronous on p->stream; allocates nothing. */
+int fa_sm75_paged_evict(const fa_paged_evict_params* p);
+/* Workspace bytes the call needs (0 for invalid parameters too): of the sizes alone. */
+int64_t fa_sm75_paged_evict_workspace_size(const fa_paged_evict_params* p);
+
 /* ---- Reference launcher signatures ------------------------------------ */
 
 /* reference src/bindings/pytorch_extension.cpp:8-11,
