@@ -378,6 +378,10 @@ Tensor paged_attention_weights(Tensor Q, Tensor LSE, Tensor k_cache, Tensor bloc
   p.cu_seqlens = cu_pointer(cu_seqlens, k_cache, c.batch, Q.size(0));
   const at::OptionalDeviceGuard guard(at::device_of(k_cache));
   if (Q.numel() != 0) Q = rows_view(Q);
+  // (views wider than fa_paged_weigh_params takes)
+  if (Q.numel() != 0 && (eff_stride(Q, 0, 0) >= 1 << 23 || eff_stride(Q, 1, 0) >= 1 << 23 ||
+                         33 * eff_stride(Q, 0, 0) + Q.size(1) / c.heads_kv * eff_stride(Q, 1, 0) >= 1 << 30))
+    Q = Q.contiguous();
   LSE = LSE.contiguous();
   Tensor W;
   if (add_to.has_value()) {
@@ -410,6 +414,9 @@ Tensor paged_attention_weights(Tensor Q, Tensor LSE, Tensor k_cache, Tensor bloc
   p.causal = (int)causal;
   p.dtype = dtype_code(Q.scalar_type());
   p.stream = current_stream(k_cache);
+  p.workspace_bytes = fa_sm75_paged_weigh_workspace_size(&p);
+  const Tensor work = workspace(p.workspace_bytes, k_cache);
+  p.workspace = work.defined() ? work.data_ptr() : nullptr;
   const int st = fa_sm75_paged_weigh(&p);
   TORCH_CHECK(st == FA_OK, "paged_attention_weights: ", fa_sm75_last_error());
   if (add_to.has_value()) written_to(W);

@@ -126,17 +126,25 @@ struct WeighArgs {
   int max_len;
   int add;           // to what is there; else positions without a row get 0
   // Plan.
-  int run;           // 32-key tiles of a wave
+  int run;           // few rows: 32-key tiles of a wave
+  int split;         // more: units may be cut (with a workspace)
+  float* partial;
+  uint64_t* flags;
+  uint64_t mark;     // what a written part's flag holds (merge_mark)
 };
 struct WeighPlan {
-  int rows;  // query columns at once
+  int rows;  // rows at once: 16 or 32, 0 for the kernel of more
   int run;
   int64_t grid;
+  bool split;
+  int64_t workspace_bytes;
 };
-WeighPlan plan_weigh(const WeighArgs& a, int head_dim, int64_t max_query_len);
-int launch_weigh(const WeighArgs& a, const WeighPlan& plan, int head_dim, hipStream_t stream);
+WeighPlan plan_weigh(const WeighArgs& a, int64_t max_query_len, int64_t workspace_bytes);
+int launch_weigh(const WeighArgs& a, const WeighPlan& plan, int head_dim, void* workspace, hipStream_t stream);
 template <int D, bool BF16, bool FP8>
 void launch_weigh_few(const WeighArgs& a, int rows, int64_t grid, hipStream_t stream);
+template <int D, bool BF16, bool FP8>
+void launch_weigh_chunk(const WeighArgs& a, int64_t grid, hipStream_t stream);
 
 // Eviction: which rows stay (select), and their copies to other pages (move).
 struct EvictArgs {
@@ -151,9 +159,11 @@ struct EvictArgs {
   float* new_weights;       // [batch, hkv, to_pages << page_shift]
   int32_t* kept;            // workspace: [batch, hkv, slots] positions of the rows that stay
   int slots;                // the most rows that can stay: min(keep, room of the table)
+  int* counts;              // workspace: a histogram for each row, digit and chunk
+  int chunks;               // workgroups of a row
 };
 int64_t evict_workspace_bytes(const EvictArgs& a);
-int launch_evict(const EvictArgs& a, int head_dim, hipStream_t stream);
+int launch_evict(const EvictArgs& a, int head_dim, void* workspace, hipStream_t stream);
 
 }  // namespace fa
 

@@ -221,17 +221,24 @@ int make_weigh(const fa_paged_weigh_params* p, fa::WeighArgs* w, bool* nothing) 
   f.scale = p->scale;
   f.causal = p->causal;
   f.dtype = p->dtype;
+  f.workspace = p->workspace;
+  f.workspace_bytes = p->workspace_bytes;
   bool empty = true;
   if (int st = make_forward(&f, &w->p, &empty)) return st;
   if (!empty && p->lse == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "lse must not be NULL");
+  // 32 rows of one KV head's queries are read through one window, by products of 24 bits.
+  constexpr int64_t kStride = 1 << 23;
+  if (!empty && (p->q_stride_t >= kStride || p->q_stride_h >= kStride || w->p.group >= kStride ||
+                 33 * p->q_stride_t + w->p.group * p->q_stride_h >= 1 << 30))
+    return capi_fail(FA_ERR_TOO_LARGE, "Q's strides must be below 2^23, and a group's heads and 33 tokens within 2^30 elements");
   if (p->max_len < 0 || p->weights_stride_b < 0 || p->weights_stride_h < 0)
     return capi_fail(FA_ERR_INVALID_ARGUMENT, "max_len and the weights' strides must be non-negative");
   if (p->max_len > fa::kPagedMaxKeys) return capi_fail(FA_ERR_TOO_LARGE, "max_len exceeds 2^30");
   const int64_t pairs = (int64_t)w->p.batch * w->p.hkv;
   *nothing = pairs == 0 || p->max_len == 0 || (empty && p->add);
   if (*nothing) return FA_OK;
-  if (pairs > (1 << 22) || pairs * ((p->max_len + 31) / 32) > (1 << 28))
-    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 2^22, or batch * heads_kv * max_len 2^33");
+  if (pairs > (1 << 22) || pairs * ((p->max_len + 31) / 32) > (1 << 26))
+    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 2^22, or batch * heads_kv * max_len 2^31");
   if (p->weights == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "weights must not be NULL");
   if (!aligned(p->weights, 4)) return capi_fail(FA_ERR_MISALIGNED, "weights must be 4-byte aligned");
   if (empty) {  // no row: every weight is 0
@@ -275,8 +282,8 @@ int make_evict(const fa_paged_evict_params* p, fa::EvictArgs* e, bool* nothing) 
   const int64_t pairs = (int64_t)a.batch * a.hkv;
   *nothing = pairs == 0;
   if (*nothing) return FA_OK;
-  if (pairs > (1 << 20) || pairs * slots > (1 << 30))
-    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 2^20, or the rows that stay 2^30");
+  if (pairs > (1 << 20) || pairs * slots > (1 << 29))
+    return capi_fail(FA_ERR_TOO_LARGE, "batch * heads_kv exceeds 2^20, or the rows that stay 2^29");
   if (p->new_lens == nullptr || (to_room > 0 && p->new_weights == nullptr) ||
       (room > 0 && p->weights == nullptr) || (p->to_pages > 0 && p->to_table == nullptr))
     return capi_fail(FA_ERR_INVALID_ARGUMENT, "weights, to_table, new_lens and new_weights must not be NULL");
@@ -297,9 +304,12 @@ int make_evict(const fa_paged_evict_params* p, fa::EvictArgs* e, bool* nothing) 
 }
 
 // (a checked call's: tokens > 0)
+int64_t longest_query(const int32_t* cu_seqlens, int64_t max_query_len, int64_t tokens) {
+  if (cu_seqlens == nullptr) return 1;
+  return max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens;
+}
 int64_t longest_query(const fa_paged_params* p) {
-  if (p->cu_seqlens == nullptr) return 1;
-  return p->max_query_len > 0 && p->max_query_len < p->tokens ? p->max_query_len : p->tokens;
+  return longest_query(p->cu_seqlens, p->max_query_len, p->tokens);
 }
 
 }  // namespace
@@ -409,16 +419,23 @@ int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix
   return check_launch();
 }
 
+int64_t fa_sm75_paged_weigh_workspace_size(const fa_paged_weigh_params* p) {
+  const fa::SavedError keep;  // a size is no error report
+  fa::WeighArgs w;
+  bool nothing = true;
+  if (make_weigh(p, &w, &nothing) != FA_OK || nothing) return 0;
+  return fa::plan_weigh(w, longest_query(p->cu_seqlens, p->max_query_len, p->tokens), INT64_MAX).workspace_bytes;
+}
+
 int fa_sm75_paged_weigh(const fa_paged_weigh_params* p) {
   fa::capi_clear_error();
   fa::WeighArgs w;
   bool nothing = true;
   if (int st = make_weigh(p, &w, &nothing)) return st;
   if (nothing) return FA_OK;
-  const int64_t longest = p->cu_seqlens == nullptr ? 1
-                          : p->max_query_len > 0 && p->max_query_len < p->tokens ? p->max_query_len : p->tokens;
-  const int d = (int)p->cache->head_dim;
-  fa::launch_weigh(w, fa::plan_weigh(w, d, longest), d, static_cast<hipStream_t>(p->stream));
+  const fa::WeighPlan plan = fa::plan_weigh(w, longest_query(p->cu_seqlens, p->max_query_len, p->tokens),
+                                            p->workspace != nullptr ? p->workspace_bytes : 0);
+  fa::launch_weigh(w, plan, (int)p->cache->head_dim, p->workspace, static_cast<hipStream_t>(p->stream));
   return check_launch();
 }
 
@@ -440,8 +457,7 @@ int fa_sm75_paged_evict(const fa_paged_evict_params* p) {
     return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes, got %lld", (long long)need,
                      (long long)(p->workspace != nullptr ? p->workspace_bytes : 0));
   if (!aligned(p->workspace, 16)) return capi_fail(FA_ERR_MISALIGNED, "workspace must be 16-byte aligned");
-  e.kept = static_cast<int32_t*>(p->workspace);
-  fa::launch_evict(e, (int)p->cache->head_dim, static_cast<hipStream_t>(p->stream));
+  fa::launch_evict(e, (int)p->cache->head_dim, p->workspace, static_cast<hipStream_t>(p->stream));
   return check_launch();
 }
 

@@ -23,8 +23,6 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kSelBins = 2048;
-// Keys held in LDS (128 KB); those of later positions are made again from the weights.
-constexpr int kSelHeld = 32768;
 constexpr unsigned kRecentKey = 0xffffffffu;
 
 // An integer that orders as the weights do: NaN below all (1; 0 is no row), -0 as 0.
@@ -34,141 +32,263 @@ __device__ __forceinline__ unsigned order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of the waves' values before this one's, and of all; `scratch` is free again behind it.
-struct Before {
-  int before, all;
+// One (sequence, KV head): what it holds and where that goes.
+struct SelRow {
+  const EvictArgs& e;
+  const float* w;
+  const int32_t* entries;
+  int b, h, keys, recent_from, from_room, room;
+  int32_t* kept;
+  float* to_w;
+  __device__ __forceinline__ SelRow(const EvictArgs& args, int pair) : e(args) {
+    const PagedArgs& a = e.p;
+    b = (int)((unsigned)pair / (unsigned)a.hkv);
+    h = pair - b * a.hkv;
+    const int len = max(0, a.lens[b]);
+    from_room = a.max_pages << a.page_shift;
+    keys = min(len, from_room);
+    recent_from = len - min(e.recent, len);
+    w = e.weights + b * e.wb + h * e.wh;
+    entries = a.table + b * a.table_stride;
+    kept = e.kept + (int64_t)pair * e.slots;
+    room = e.to_pages << a.page_shift;
+    to_w = e.new_weights + (int64_t)pair * room;
+  }
 };
-__device__ __forceinline__ Before across_waves(int x, int wave, int* scratch) {
-  if ((threadIdx.x & 63) == 0) scratch[wave] = x;
+
+// kSelBlock positions of a row, a wave's kSelKeys * 64 next to each other, in registers.  (Loads do
+// not wait for the sequence's length: the weights have the table's room.)
+constexpr int kSelKeys = 8;
+constexpr int kSelBlock = kSelKeys * kSelThreads;
+struct SelBlock {
+  unsigned k[kSelKeys];
+  float x[kSelKeys];
+  int j0;  // this lane's first; 64 apart
+  __device__ __forceinline__ SelBlock(const SelRow& row, int base, int end, int wave, int lane) {
+    j0 = base + wave * (64 * kSelKeys) + lane;
+    int page[kSelKeys];
+#pragma unroll
+    for (int u = 0; u < kSelKeys; ++u) {
+      const int j = j0 + 64 * u;
+      const bool there = j < row.from_room;
+      x[u] = there ? row.w[j] : 0.0f;
+      page[u] = there ? row.entries[j >> row.e.p.page_shift] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kSelKeys; ++u) {
+      const int j = j0 + 64 * u;
+      const bool held = j < min(end, row.keys) && page[u] >= 0 && page[u] < row.e.p.num_pages;
+      k[u] = !held ? 0 : j >= row.recent_from ? kRecentKey : order_key(x[u]);
+    }
+  }
+};
+
+// The search: keys that stay are above `bound` where they differ from it under `mask`; `need`
+// more of those that agree do.
+struct Search {
+  unsigned bound, mask;
+  int need, shift;  // shift: 21, 10, 0
+  __device__ __forceinline__ int width() const { return shift == 0 ? 1 << 10 : kSelBins; }
+  __device__ __forceinline__ int digit(unsigned k) const { return (k >> shift) & (width() - 1); }
+  __device__ __forceinline__ void count(const SelBlock& x, int* bins) const {
+#pragma unroll
+    for (int u = 0; u < kSelKeys; ++u)
+      if (x.k[u] != 0 && (x.k[u] & mask) == bound) atomicAdd(&bins[digit(x.k[u])], 1);
+  }
+};
+
+// What a workgroup shares in the search of one digit.
+struct SelShared {
+  int waves[kSelWaves];
+  int found[2];
+};
+// The waves' values summed over those before this one, and over all (one barrier; `waves` is not
+// written again).
+__device__ __forceinline__ int2 across_waves(int x, int wave, int lane, int* waves) {
+  if (lane == 0) waves[wave] = x;
   __syncthreads();
-  Before r = {0, 0};
+  int2 r = {0, 0};
 #pragma unroll
   for (int i = 0; i < kSelWaves; ++i) {
-    const int y = scratch[i];
-    r.before += i < wave ? y : 0;
-    r.all += y;
+    const int y = waves[i];
+    r.x += i < wave ? y : 0;
+    r.y += y;
   }
-  __syncthreads();
   return r;
 }
-
 __device__ __forceinline__ int wave_sum(int x) {
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m);
   return x;
 }
 
-// A workgroup for each (sequence, KV head); a wave has one stretch of its positions.
-__global__ void __launch_bounds__(kSelThreads) fa_paged_select_kernel(const EvictArgs e) {
-  __shared__ unsigned keys_lds[kSelHeld];
+// One digit on, given how many of the agreeing keys have the thread's two digits, hi and
+// hi - 1 from the top.  keep: the keys wanted, where this is the first digit.  Returns all that agree.
+__device__ __forceinline__ int descend(Search& s, int n1, int n0, int keep, int wave, int lane, SelShared& sh) {
+  const int hi = kSelBins - 1 - 2 * (int)threadIdx.x;
+  int upto = n0 + n1;  // inclusive, over the wave's lanes
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    const int y = __shfl_up(upto, m);
+    if (lane >= m) upto += y;
+  }
+  const int2 sum = across_waves(__shfl(upto, 63), wave, lane, sh.waves);
+  if (s.shift == 21) s.need = min(keep, sum.y);
+  const int above = sum.x + upto - n0 - n1;
+  if (above < s.need && above + n1 >= s.need) {
+    sh.found[0] = hi;
+    sh.found[1] = above;
+  } else if (above + n1 < s.need && above + n1 + n0 >= s.need) {
+    sh.found[0] = hi - 1;
+    sh.found[1] = above + n1;
+  }
+  __syncthreads();
+  return sum.y;
+}
+// (where there is something to search: some but not all stay)
+__device__ __forceinline__ void take(Search& s, const SelShared& sh) {
+  s.bound |= (unsigned)sh.found[0] << s.shift;
+  s.need -= sh.found[1];
+  s.mask |= (unsigned)(s.width() - 1) << s.shift;
+  s.shift = s.shift > 10 ? s.shift - 11 : s.shift - 10;
+}
+
+// Writes which of a block's positions stay: `before` in front of them do, and so many of
+// equal keys lie there, of which the first `need` stay.  Returns both for what is behind it.
+__device__ __forceinline__ int2 write_kept(const SelRow& row, const SelBlock& x, unsigned bound, int need, int target,
+                                           int above, int same, int wave, int lane, int* waves) {
+  int n = 0;  // of this wave: above the bound, and equal to it in the upper half
+  uint64_t gt[kSelKeys], eq[kSelKeys];
+#pragma unroll
+  for (int u = 0; u < kSelKeys; ++u) {
+    gt[u] = __builtin_amdgcn_ballot_w64(x.k[u] > bound);
+    eq[u] = __builtin_amdgcn_ballot_w64(x.k[u] == bound && x.k[u] != 0);
+    n += __builtin_popcountll(gt[u]) + (__builtin_popcountll(eq[u]) << 16);
+  }
+  const int2 sum = across_waves(n, wave, lane, waves);
+  int a = above + (sum.x & 0xffff), s = same + (sum.x >> 16);
+  const uint64_t lower = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+  for (int u = 0; u < kSelKeys; ++u) {
+    const int ge = a + __builtin_popcountll(gt[u] & lower), se = s + __builtin_popcountll(eq[u] & lower);
+    const bool stays = x.k[u] > bound || (x.k[u] == bound && x.k[u] != 0 && se < need);
+    const int to = ge + min(se, need);
+    if (stays && to < target) {  // (to < target always, unless the weights change meanwhile)
+      row.kept[to] = x.j0 + 64 * u;
+      row.to_w[to] = x.x[u];
+    }
+    a += __builtin_popcountll(gt[u]);
+    s += __builtin_popcountll(eq[u]);
+  }
+  return {above + (sum.y & 0xffff), same + (sum.y >> 16)};
+}
+
+// A workgroup for each (sequence, KV head), where the table has room for one block.  The chain of
+// its steps bounds it (three digits of three barriers): %%%.
+__global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_kernel(const EvictArgs e) {
   __shared__ int bins[kSelBins];
-  __shared__ int scratch[kSelWaves];
-  __shared__ int found[2];
-  const PagedArgs& a = e.p;
+  __shared__ SelShared sh[4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int b = (int)((unsigned)blockIdx.x / (unsigned)a.hkv), h = (int)blockIdx.x - b * a.hkv;
-  const int len = max(0, a.lens[b]);
-  const int keys = min(len, a.max_pages << a.page_shift);
-  const int recent_from = len - min(e.recent, len);
-  const float* const w = e.weights + b * e.wb + h * e.wh;
-  const int32_t* const entries = a.table + b * a.table_stride;
-  const int64_t pair = (int64_t)b * a.hkv + h;
-  int32_t* const kept = e.kept + pair * e.slots;
-  const int room = e.to_pages << a.page_shift;
-  float* const to_w = e.new_weights + pair * room;
-
-  auto make_key = [&](int j) -> unsigned {
-    const int page = entries[j >> a.page_shift];
-    const float x = w[j];
-    if (page < 0 || page >= a.num_pages) return 0;
-    return j >= recent_from ? kRecentKey : order_key(x);
-  };
-  const int part = ((keys + kSelThreads - 1) / kSelThreads) * 64;  // positions of a wave
-  const int j0 = min(keys, wave * part), j1 = min(keys, j0 + part);
-  int held = 0;
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const unsigned k = make_key(j);
-    if (j < kSelHeld) keys_lds[j] = k;
-    held += k != 0;
-  }
-  auto key_at = [&](int j) -> unsigned { return j < kSelHeld ? keys_lds[j] : make_key(j); };
-  const int all = across_waves(wave_sum(held), wave, scratch).all;
-  const int target = min(e.keep, all);
-
-  // The smallest key that stays, and how many of those equal to it do.
-  unsigned bound = 0;  // (all that are held: those above 0)
-  int equal = 0;
-  if (target < all && target > 0) {
-    int need = target;  // of the keys that agree with `bound` above `shift`
-    unsigned mask = 0;
-    for (int shift = 21; shift >= 0; shift = shift > 10 ? shift - 11 : shift - 10) {
-      const int digits = shift == 0 ? 1 << 10 : kSelBins;
-      for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) bins[i] = 0;
-      __syncthreads();
-      for (int j = j0 + lane; j < j1; j += 64) {
-        const unsigned k = key_at(j);
-        if ((k & mask) == bound) atomicAdd(&bins[(k >> shift) & (digits - 1)], 1);
-      }
-      __syncthreads();
-      // Thread t: the two bins t from the top.
-      const int hi = kSelBins - 1 - 2 * (int)threadIdx.x;
-      const int n1 = bins[hi], n0 = bins[hi - 1];
-      int upto = n0 + n1;  // inclusive, over the wave's lanes
+  int2* const own = (int2*)bins + (kSelThreads - 1 - threadIdx.x);
+  *own = {0, 0};
+  const SelRow row(e, (int)blockIdx.x);
+  const SelBlock x(row, 0, INT32_MAX, wave, lane);
+  __syncthreads();
+  Search s = {0, 0, 0, 21};
+  int target = 0;
 #pragma unroll
-      for (int m = 1; m < 64; m *= 2) {
-        const int y = __shfl_up(upto, m);
-        if (lane >= m) upto += y;
-      }
-      const int above = across_waves(__shfl(upto, 63), wave, scratch).before + upto - n0 - n1;
-      if (above < need && above + n1 >= need) {
-        found[0] = hi;
-        found[1] = above;
-      } else if (above + n1 < need && above + n1 + n0 >= need) {
-        found[0] = hi - 1;
-        found[1] = above + n1;
-      }
-      __syncthreads();
-      bound |= (unsigned)found[0] << shift;
-      need -= found[1];
-      mask |= (unsigned)(digits - 1) << shift;
-      __syncthreads();
-      if (shift == 0) break;
-    }
-    equal = need;
+  for (int p = 0; p < 3; ++p) {
+    s.count(x, bins);
+    __syncthreads();
+    const int2 n = *own;  // (digits 2 i and 2 i + 1)
+    *own = {0, 0};
+    const int all = descend(s, n.y, n.x, e.keep, wave, lane, sh[p]);
+    if (p == 0) target = s.need;
+    if (p == 0 && (target == all || target == 0)) break;  // all that are held stay: those above 0
+    take(s, sh[p]);
   }
-
-  // The positions that stay, in order.
-  int above = 0, same = 0;
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const unsigned k = key_at(j);
-    above += k > bound;
-    same += k == bound && k != 0;
-  }
-  const int above_before = across_waves(wave_sum(above), wave, scratch).before;
-  int same_before = across_waves(wave_sum(same), wave, scratch).before;
-  int r = above_before + min(same_before, equal);
   if (target > 0) {
-    for (int j = j0 + lane; j - lane < j1; j += 64) {
-      const unsigned k = j < j1 ? key_at(j) : 0;
-      const bool eq = k == bound && k != 0;
-      const uint64_t eqs = __builtin_amdgcn_ballot_w64(eq);
-      const uint64_t lower = ((uint64_t)1 << lane) - 1;
-      const bool stays = k > bound || (eq && same_before + __builtin_popcountll(eqs & lower) < equal);
-      const uint64_t all_stay = __builtin_amdgcn_ballot_w64(stays);
-      if (stays) {
-        const int to = r + __builtin_popcountll(all_stay & lower);
-        if (to < target) {  // (always, unless the weights change meanwhile)
-          kept[to] = j;
-          to_w[to] = w[j];
-        }
-      }
-      r += __builtin_popcountll(all_stay);
-      same_before += __builtin_popcountll(eqs);
-    }
+    if (s.mask == 0) s.need = 0;
+    write_kept(row, x, s.bound, s.need, target, 0, 0, wave, lane, sh[3].waves);
   }
-  for (int j = target + (int)threadIdx.x; j < room; j += kSelThreads) to_w[j] = 0.0f;
-  if (h == 0 && threadIdx.x == 0) e.new_lens[b] = target;
+  for (int j = target + (int)threadIdx.x; j < row.room; j += kSelThreads) row.to_w[j] = 0.0f;
+  if (row.h == 0 && threadIdx.x == 0) e.new_lens[row.b] = target;
+}
+
+// Longer rows: `chunks` workgroups each, in four launches.  The first three count a digit each over
+// the chunk's keys, into a histogram of its own; each launch adds up those of the ones before it to
+// find their digits, and the last also what of the chunks in front of its own stays.
+template <int PHASE>
+__global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_long_kernel(const EvictArgs e) {
+  __shared__ int bins[kSelBins];
+  __shared__ SelShared sh[3];
+  __shared__ int waves[3][kSelWaves];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int pair = (int)((unsigned)blockIdx.x / (unsigned)e.chunks), chunk = (int)blockIdx.x - pair * e.chunks;
+  const int slot = kSelThreads - 1 - (int)threadIdx.x;
+  int2* const hist = (int2*)e.counts + ((int64_t)pair * 3 * e.chunks) * kSelThreads + slot;
+  const SelRow row(e, pair);
+  Search s = {0, 0, 0, 21};
+  int target = 0, above = 0, same = 0;
+  bool search = true;
+#pragma unroll
+  for (int p = 0; p < PHASE; ++p) {
+    int2 all = {0, 0}, front = {0, 0};
+    for (int c = 0; c < e.chunks; c += 8) {
+      int2 n[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        n[u] = c + u < e.chunks ? hist[((int64_t)p * e.chunks + c + u) * kSelThreads] : int2{0, 0};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        all.x += n[u].x;
+        all.y += n[u].y;
+        front.x += c + u < chunk ? n[u].x : 0;
+        front.y += c + u < chunk ? n[u].y : 0;
+      }
+    }
+    const int total = descend(s, all.y, all.x, e.keep, wave, lane, sh[p]);
+    if (p == 0) {
+      target = s.need;
+      search = target < total && target > 0;
+    }
+    if (!search) {
+      above += front.x + front.y;
+      break;
+    }
+    const int at = sh[p].found[0];
+    above += (2 * slot > at ? front.x : 0) + (2 * slot + 1 > at ? front.y : 0);
+    if (p == 2) same = 2 * slot == at ? front.x : 2 * slot + 1 == at ? front.y : 0;
+    take(s, sh[p]);
+  }
+  const int part = (int)((unsigned)(row.keys + e.chunks * kSelBlock - 1) / (unsigned)(e.chunks * kSelBlock)) * kSelBlock;
+  const int begin = (int)min((int64_t)chunk * part, (int64_t)row.keys), end = min(row.keys, begin + part);
+  if constexpr (PHASE < 3) {
+    if (!search) return;  // (all the workgroups of the row; the histograms are not asked for)
+    int2* const own = (int2*)bins + slot;
+    *own = {0, 0};
+    __syncthreads();
+    for (int j = begin; j < end; j += kSelBlock) s.count(SelBlock(row, j, end, wave, lane), bins);
+    __syncthreads();
+    hist[((int64_t)PHASE * e.chunks + chunk) * kSelThreads] = *own;
+  } else {
+    // What stays in front of the chunk: above the bound, and equal to it.
+    int2 before = {across_waves(wave_sum(above), wave, lane, waves[0]).y,
+                   across_waves(wave_sum(same), wave, lane, waves[1]).y};
+    if (!search) s.need = 0;
+    if (target > 0) {
+      for (int j = begin; j < end; j += kSelBlock) {
+        before = write_kept(row, SelBlock(row, j, end, wave, lane), s.bound, s.need, target, before.x, before.y, wave,
+                            lane, waves[2]);
+        __syncthreads();
+      }
+    }
+    for (int64_t j = target + (int64_t)chunk * kSelThreads + threadIdx.x; j < row.room; j += e.chunks * kSelThreads)
+      row.to_w[j] = 0.0f;
+    if (row.h == 0 && chunk == 0 && threadIdx.x == 0) e.new_lens[row.b] = target;
+  }
 }
 
 // Copies the rows that stay, 16 bytes a lane, kMoveRows rows of K and V at once.
@@ -229,13 +349,37 @@ __global__ void __launch_bounds__(kMoveThreads) fa_paged_move_kernel(const Evict
 
 }  // namespace
 
-int64_t evict_workspace_bytes(const EvictArgs& a) {
-  return ((int64_t)a.p.batch * a.p.hkv * a.slots * (int64_t)sizeof(int32_t) + 15) & ~(int64_t)15;
+// Workgroups of a long row: one for each block of positions, up to 64 (each adds up the histograms of
+// all), and 4096 in all; 0: one workgroup has them in its registers.
+static int evict_chunks(const EvictArgs& e) {
+  const int64_t room = (int64_t)e.p.max_pages << e.p.page_shift, pairs = (int64_t)e.p.batch * e.p.hkv;
+  if (room <= kSelBlock) return 0;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({64, (room + kSelBlock - 1) / kSelBlock, 4096 / pairs}));
+}
+static int64_t kept_bytes(const EvictArgs& e) {
+  return ((int64_t)e.p.batch * e.p.hkv * e.slots * (int64_t)sizeof(int32_t) + 15) & ~(int64_t)15;
 }
 
-int launch_evict(const EvictArgs& e, int head_dim, hipStream_t stream) {
+int64_t evict_workspace_bytes(const EvictArgs& e) {
+  return kept_bytes(e) + (int64_t)e.p.batch * e.p.hkv * 3 * evict_chunks(e) * kSelBins * (int64_t)sizeof(int);
+}
+
+int launch_evict(const EvictArgs& args, int head_dim, void* workspace, hipStream_t stream) {
+  EvictArgs e = args;
+  e.kept = static_cast<int32_t*>(workspace);
+  e.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + kept_bytes(e));
+  e.chunks = evict_chunks(e);
   const int64_t pairs = (int64_t)e.p.batch * e.p.hkv;
-  hipLaunchKernelGGL(fa_paged_select_kernel, dim3((unsigned)pairs), dim3(kSelThreads), 0, stream, e);
+  const dim3 threads(kSelThreads);
+  if (e.chunks == 0) {
+    hipLaunchKernelGGL(fa_paged_select_kernel, dim3((unsigned)pairs), threads, 0, stream, e);
+  } else {
+    const dim3 rows((unsigned)(pairs * e.chunks));
+    hipLaunchKernelGGL(fa_paged_select_long_kernel<0>, rows, threads, 0, stream, e);
+    hipLaunchKernelGGL(fa_paged_select_long_kernel<1>, rows, threads, 0, stream, e);
+    hipLaunchKernelGGL(fa_paged_select_long_kernel<2>, rows, threads, 0, stream, e);
+    hipLaunchKernelGGL(fa_paged_select_long_kernel<3>, rows, threads, 0, stream, e);
+  }
   if (e.slots == 0 || e.p.num_pages == 0) return 0;
   const int bytes = head_dim * (e.p.ks != nullptr ? 1 : 2);
   const int per = kMoveThreads / (bytes / 16) * kMoveRows;

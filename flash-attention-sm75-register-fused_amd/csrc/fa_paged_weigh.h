@@ -3,13 +3,17 @@
 // kv_head * group + r % group) of p_rj = exp(scale q_r k_j - lse_r), where lse_r is the row's
 // log-sum-exp: the probabilities the attention used, computed again from Q and K.
 //
-//   S = Q K^T   rows on the M side of 16x16x32 MFMAs, keys on N: a lane has one key
-//               of a 16-key piece and four rows of each 16, so that a key's sum over
-//               rows is a sum in the lane and, once a tile, over the four lane groups
+//   S = Q K^T   rows on the M side of the MFMAs, keys on N: a lane has one key and
+//               several rows, so that a key's sum over rows is a sum in the lane, and
+//               over the lane groups once, at the end
 //
 // p = 2^(c s - lse log2 e), c = scale log2 e: no maximum is looked for, the lse is one already.
-// Everything from S on is in 32 bits.  Each key has one owner, which adds its rows' terms in
-// their order: the same call gives the same bits.
+// Everything from S on is in 32 bits, and sums go by tiles of 32 rows (one accumulator over 2048
+// rows was off by 1.4e-6 of a weight, by tiles %%%).  Which rows a sum takes, and in which order, follows from
+// the sizes and lengths: the same call gives the same bits.
+//
+// Two kernels: up to 32 rows (one generated token, a few drafted ones) K is the work, which
+// streams through registers; more rows meet a block of keys that stays in registers.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -62,7 +66,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArg
   const int full = a.causal ? uniform(clamp_int(past + 1, 0, sees)) : sees;
   const int t_stop = uniform(clamp_int((sees + kWTile - 1) / kWTile, t_begin, t_end));
   float* const out = w.out + b * w.sb + hkv * w.sh;
-  const float c2 = a.c;
+  const float c2 = a.negate_q ? -a.c : a.c;
 
   // Rows rb R .. + R - 1: their Q, and of each of the lane's four rows of a 16 its lse
   // and the last key it sees.
@@ -82,8 +86,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArg
       for (int kk = 0; kk < KS; ++kk) {
         // (the dimensions of a K row's bytes, see fa_paged_attn.h)
         const int dim = FP8 ? 64 * (kk >> 1) + 16 * g4 + 8 * (kk & 1) : 32 * kk + 8 * g4;
-        const half8 x = *(const half8*)(qp + dim);
-        qf[nt][kk] = ok ? (a.negate_q ? negate16(x) : x) : (half8)(_Float16)0;
+        qf[nt][kk] = ok ? *(const half8*)(qp + dim) : (half8)(_Float16)0;
       }
       const float lse = ok ? weigh_lse2(w.lse[(int64_t)pr.head * a.tokens + pr.token]) : __builtin_inff();
       const int most = !ok ? -1 : a.causal ? min(sees - 1, past + (pr.token - s.t0)) : sees - 1;
@@ -202,7 +205,337 @@ __global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArg
   }
 }
 
+// ---- more than 32 rows ------------------------------------------------------------
+//
+// A unit is 256 keys of one (sequence, KV head), a wave's 64 of them in its registers as the B
+// operand of 32x32x16 MFMAs; the sequence's rows come by, 32 at a time, through LDS (double-buffered,
+// each row's -lse log2 e beside it).  Where units are few, each one's row tiles go to `parts`
+// workgroups in turns (under the causal rule every part then has as many that see the keys), and the last
+// of them to finish adds the parts up in their order.
+constexpr int kWBlock = 256;    // keys of a unit
+constexpr int kWRows = 32;      // rows of a tile
+constexpr int kWTarget = 1024;  // workgroups that units are cut into, where they are fewer
+constexpr int kWMinTiles = 8;   // tiles a part has at least
+
+// The units that hold keys and rows: of every sequence its blocks of keys up to max_len, for
+// each KV head (heads next to each other, so that those of one head meet in one XCD's L2 where
+// the heads divide over the XCDs).  Called by whole waves.
+struct WeighLine {
+  const WeighArgs& w;
+  int lane;
+  PagedSeq own;  // sequence `lane`
+  __device__ __forceinline__ WeighLine(const WeighArgs& args, int ln) : w(args), lane(ln) { own = look(ln); }
+  __device__ __forceinline__ PagedSeq look(int b) const {
+    PagedSeq s = paged_seq(w.p, min(b, w.p.batch - 1), [](const int32_t* p) { return *p; });
+    if (b >= w.p.batch) s.n = s.keys = 0;
+    return s;
+  }
+  __device__ __forceinline__ int blocks(const PagedSeq& s) const {
+    return s.n > 0 ? (int)((unsigned)(min(s.keys, w.max_len) + kWBlock - 1) / kWBlock) : 0;
+  }
+  __device__ __forceinline__ int every() const { return (int)((unsigned)(w.max_len + kWBlock - 1) / kWBlock); }
+  // Units of sequences b0 + lane (empty: of the blocks behind their keys), summed up to the lane.
+  __device__ __forceinline__ int prefix(int b0, bool empty) const {
+    const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
+    const int n = blocks(s);
+    return wave_prefix((b0 + lane < w.p.batch ? empty ? every() - n : n : 0) * w.p.hkv);
+  }
+  // All units, and the most row tiles of a sequence.
+  __device__ __forceinline__ int total(int& tiles) const {
+    int sum = 0;
+    tiles = 0;
+    for (int b0 = 0; b0 < w.p.batch; b0 += 64) {
+      sum += wave_bcast(prefix(b0, false), 63);
+      const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
+      tiles = max(tiles, wave_max((int)((unsigned)(s.n * w.p.group + kWRows - 1) / kWRows)));
+    }
+    return uniform(sum);
+  }
+  // The sequence of unit `at`, which becomes its number in the sequence.
+  __device__ __forceinline__ int find(int& at, bool empty) const {
+    for (int b0 = 0;; b0 += 64) {
+      const int x = prefix(b0, empty);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(x > at);
+      if (past != 0 || b0 + 64 >= w.p.batch) {
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        if (l > 0) at -= wave_bcast(x, l - 1);
+        return uniform(min(b0 + l, w.p.batch - 1));
+      }
+      at -= wave_bcast(x, 63);
+    }
+  }
+};
+
+template <int D, bool BF16, bool FP8>
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const WeighArgs w) {
+  using E = Elem<BF16>;
+  using L = Lds<D>;
+  constexpr int KK = D / 16;               // contraction steps of S
+  constexpr int RL = D / 8;                // threads that bring a row of Q
+  constexpr int QL = kWRows * RL / kThreads;  // loads of a thread
+  constexpr int NS = 2 * KK;               // MFMAs of a tile
+  constexpr int PF = 3;                    // Q operand reads run this many steps ahead
+  __shared__ __attribute__((aligned(16))) _Float16 q_lds[2][kWRows * L::Pitch];
+  __shared__ __attribute__((aligned(16))) float lse_lds[4][kWRows];
+  __shared__ int scratch[kWaves];
+  const PagedArgs& a = w.p;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hi = lane >> 5, l32 = lane & 31;
+  const WeighLine line(w, lane);
+  int most;
+  const int units = line.total(most);
+  // (kWTarget over the units is cut to whole parts: at most kWTarget workgroups where there are several)
+  int parts = 1;
+  if (w.split && units > 0 && units < kWTarget)
+    parts = max(1, min((int)((unsigned)kWTarget / (unsigned)units), (int)((unsigned)most / kWMinTiles)));
+  parts = uniform(parts);
+  const int wg = (int)blockIdx.x;
+  if (wg >= units * parts) {  // blocks behind the keys
+    int at = wg - units * parts;
+    if (w.add || at >= line.every() * a.batch * a.hkv - units) return;
+    const int b = line.find(at, true);
+    const int block = line.blocks(scalar_seq(a, b)) + (int)((unsigned)at / (unsigned)a.hkv), h = at % a.hkv;
+    const int j = block * kWBlock + (int)threadIdx.x;
+    if (j < w.max_len) w.out[b * w.sb + h * w.sh + j] = 0.0f;
+    return;
+  }
+  const int part = (int)((unsigned)wg / (unsigned)units);
+  int at = wg - part * units;
+  at = uniform(at);
+  const int unit = at;
+  const int b = line.find(at, false);
+  const int block = uniform((int)((unsigned)at / (unsigned)a.hkv)), hkv = uniform(at - block * a.hkv);
+  const PagedSeq s = scalar_seq(a, b);
+  const int nrows = s.n * a.group;
+  const int past = s.len - s.n;  // tokens before the new ones
+  const int sees = min(s.keys, w.max_len);
+  const int key0 = block * kWBlock;
+
+  // This lane's two keys.
+  const int key = key0 + 64 * wave + l32;
+  half8 kf[2][KK];
+  bool held[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int j = key + 32 * t;
+    const int page = j < sees ? a.table[b * a.table_stride + (j >> a.page_shift)] : -1;
+    held[t] = page >= 0 && page < a.num_pages;
+    const int64_t off = j & ((1 << a.page_shift) - 1);
+    const uint8_t* const row = a.k + page * a.kp + hkv * a.kh + off * a.kn + 16 * hi;
+    const float ks = FP8 && held[t] ? scale_of(a.ks[page * a.ksp + hkv * a.ksh + off * a.ksn]) : 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (FP8) {  // (16 codes are two steps' dimensions)
+        if (kk & 1) continue;
+        const uint4v c = held[t] ? *(const uint4v*)(row + 16 * kk) : (uint4v)0u;
+        kf[t][kk] = dequantise8<BF16>(c[0], c[1], ks);
+        kf[t][kk + 1] = dequantise8<BF16>(c[2], c[3], ks);
+      } else {
+        kf[t][kk] = held[t] ? *(const half8*)(row + 32 * kk) : (half8)(_Float16)0;
+      }
+    }
+  }
+  // Row r sees key j iff r >= (j - past) group, its token's number not below j - past: from row
+  // `from` on this lane's first key, and 32 tokens later the second.
+  const int first_row = a.causal ? clamp_int(key0 - past, 0, s.n) * a.group : 0;
+  const int64_t from64[2] = {(int64_t)(key - past) * a.group, (int64_t)(key + 32 - past) * a.group};
+  int from[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) from[t] = a.causal ? (int)min(max(from64[t], (int64_t)0), (int64_t)nrows) : 0;
+  // From this row on all of the unit's keys are seen.
+  const int all_from = a.causal ? (int)min((int64_t)max(0, key0 + kWBlock - 1 - past) * a.group, (int64_t)nrows) : 0;
+
+  // Row tiles of this part.
+  const int tiles = (int)((unsigned)(nrows + kWRows - 1) / kWRows);
+  const int tile0 = uniform((int)((unsigned)first_row / kWRows)) + part;
+  const float c2 = a.negate_q ? -a.c : a.c;
+  // Loads of a tile's rows go through windows from its first row's token and the first head of the
+  // group on, with offsets below 2^31 bytes (the launcher sees to it), whose factors have 24 bits.
+  half8 q_next[QL];
+  float lse_next;
+  const int r_own = (int)threadIdx.x / RL;
+  const int q_tok = 2 * (int)a.qt, q_head = 2 * (int)a.qh;  // in bytes
+  const int part_rows = uniform(kWRows * parts);
+  const int tok_step = uniform((int)((unsigned)part_rows / (unsigned)a.group));
+  const int rem_step = part_rows - tok_step * a.group;
+  int ld_row = uniform(tile0 * kWRows);  // of the tile that is loaded next; its token and what is left
+  int ld_tok = uniform((int)((unsigned)ld_row / (unsigned)a.group));
+  int ld_rem = ld_row - ld_tok * a.group;
+  auto load = [&] {
+    const __amdgpu_buffer_rsrc_t rq =
+        make_rsrc(a.q + (int64_t)(s.t0 + ld_tok) * a.qt + (int64_t)hkv * a.group * a.qh, INT32_MAX);
+    const int end = nrows - 1 - ld_row;  // the last row there is, again for those behind it
+    auto place = [&](int r, int& tok, int& head) {
+      const int x = ld_rem + min(r, end);
+      tok = (int)(((float)x + 0.5f) * a.inv_group);
+      head = x - (int)__umul24(tok, a.group);
+    };
+#pragma unroll
+    for (int u = 0; u < QL; ++u) {
+      int tok, head;
+      place(r_own + u * (kThreads / RL), tok, head);
+      const int off = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (int)(threadIdx.x % RL);
+      q_next[u] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rq, off, 0, 0));
+    }
+    if (threadIdx.x < kWRows) {
+      int tok, head;
+      place(threadIdx.x, tok, head);
+      const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
+      lse_next = (int)threadIdx.x <= end ? weigh_lse2(lse[head * a.tokens + tok]) : __builtin_inff();
+    }
+    ld_row += part_rows;
+    ld_tok += tok_step;
+    ld_rem += rem_step;
+    if (ld_rem >= a.group) {
+      ld_rem -= a.group;
+      ++ld_tok;
+    }
+  };
+  auto store = [&](int i) {  // the part's tile number i
+#pragma unroll
+    for (int u = 0; u < QL; ++u) {
+      const int r = (int)threadIdx.x / RL + u * (kThreads / RL), c = threadIdx.x % RL;
+      *(half8*)(q_lds[i & 1] + r * L::Pitch + 8 * (c ^ ((r >> 2) & 3))) = q_next[u];
+    }
+    if (threadIdx.x < kWRows) lse_lds[i & 3][threadIdx.x] = -lse_next;
+  };
+  auto read_q = [&](int i, int kk) -> half8 {
+    const int c = FP8 ? 4 * (kk >> 1) + 2 * hi + (kk & 1) : 2 * kk + hi;
+    return *(const half8*)(q_lds[i & 1] + l32 * L::Pitch + 8 * (c ^ ((l32 >> 2) & 3)));
+  };
+  float sum[2] = {0.0f, 0.0f};
+  float16v st[2][2];
+  const int count = tile0 < tiles ? uniform((int)((unsigned)(tiles - tile0 + parts - 1) / (unsigned)parts)) : 0;
+  // Step i: the probabilities of tile i, whose S is st[U], between the MFMAs of tile i + 1's (behind
+  // the last one: of what is there, for nobody); tile i + 2 goes to LDS in the place of tile i's Q, which
+  // every wave is done with.
+  auto step = [&](int i, auto u_t, auto masked_t) {
+    constexpr int U = decltype(u_t)::value;
+    constexpr bool MASKED = decltype(masked_t)::value;
+    half8 qf[KK];
+    static_for<PF>([&](auto k_c) { qf[decltype(k_c)::value] = read_q(i + 1, decltype(k_c)::value); });
+    float4v nl[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) nl[g] = *(const float4v*)(lse_lds[i & 3] + 8 * g + 4 * hi);
+    const int row0 = (tile0 + i * parts) * kWRows + 4 * hi;
+    const int lim[2] = {from[0] - row0, from[1] - row0};
+    float add[2] = {0.0f, 0.0f};
+    fence_schedule();
+    static_for<NS>([&](auto slot_c) {
+      constexpr int slot = decltype(slot_c)::value;
+      constexpr int kk = slot / 2, v = slot % 2;
+      if constexpr (v == 0 && kk + PF < KK) qf[kk + PF] = read_q(i + 1, kk + PF);
+      if constexpr (slot == NS / 4) {
+        if (i + 2 < count) store(i + 2);
+      }
+      if constexpr (slot == NS / 2) {
+        if (i + 3 < count) load();
+      }
+      st[1 - U][v] = E::mfma(qf[kk], kf[v][kk], kk == 0 ? (float16v)0.0f : st[1 - U][v]);
+      // Rows 8 g + 4 hi + r of the tile in register 4 g + r.
+      static_for<32>([&](auto e_c) {
+        constexpr int e = decltype(e_c)::value;
+        if constexpr (e * NS / 32 == slot) {
+          constexpr int k = e & 1, x = e >> 1;
+          float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[U][k][x], c2, nl[x >> 2][x & 3]));
+          if constexpr (MASKED) y = 8 * (x >> 2) + (x & 3) >= lim[k] ? y : 0.0f;
+          add[k] += y;
+          asm volatile("" : "+v"(add[k]));  // keeps the sum in this slot
+        }
+      });
+      fence_schedule();
+    });
+    sum[0] += add[0];
+    sum[1] += add[1];
+    barrier_after_loads<63>();
+  };
+  if (count > 0) {
+    load();
+    store(0);
+    if (count > 1) {
+      load();
+      store(1);
+    }
+    if (count > 2) load();
+    barrier_after_loads<63>();
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      st[0][v] = (float16v)0.0f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) st[0][v] = E::mfma(read_q(0, kk), kf[v][kk], st[0][v]);
+    }
+    barrier_after_loads<63>();
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    // Tiles before `all_from` hide a key from some row.
+    const int hiding = uniform((int)((unsigned)(max(0, all_from - tile0 * kWRows) + part_rows - 1) / (unsigned)part_rows));
+    for (int i = 0; i < count; i += 2) {
+      if (i < hiding) step(i, I0{}, Flag<true>{});
+      else step(i, I0{}, Flag<false>{});
+      if (i + 1 >= count) break;
+      if (i + 1 < hiding) step(i + 1, I1{}, Flag<true>{});
+      else step(i + 1, I1{}, Flag<false>{});
+    }
+  }
+  // Thread: a key of its wave's 64.
+  sum[0] = halves_sum(sum[0]);
+  sum[1] = halves_sum(sum[1]);
+  const bool mine = hi ? held[1] : held[0];
+  const float x = mine ? (hi ? sum[1] : sum[0]) : 0.0f;
+  const int j = key0 + (int)threadIdx.x;
+  float* const out = w.out + b * w.sb + hkv * w.sh + j;
+  if (parts == 1) {
+    if (j < w.max_len && (mine || !w.add)) *out = w.add ? *out + x : x;
+    return;
+  }
+  // A record for each part, and one of what the first part finds there; coherent over the L2s.
+  const __amdgpu_buffer_rsrc_t rec = make_rsrc(w.partial, 2 * kWTarget * kWBlock * 4);
+  auto at_record = [&](int p) { return ((unit * (parts + 1) + p) * kWBlock + (int)threadIdx.x) * 4; };
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), rec, at_record(part), 0, kPCoherent);
+  if (part == 0 && w.add) {
+    const float before = j < w.max_len ? *out : 0.0f;
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, before), rec, at_record(parts), 0, kPCoherent);
+  }
+  // (see last_to_finish, fa_paged_units.h: whoever sets the last flag sees them all)
+  const __amdgpu_buffer_rsrc_t rf = make_rsrc(w.flags, kWTarget * 8);
+  wait_loads<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, w.mark), rf, (unit * parts + part) * 8, 0, kPCoherent);
+    wait_loads<0>();
+  }
+  __syncthreads();
+  bool set = true;
+  for (int p = threadIdx.x; p < parts; p += kThreads)
+    set = set && __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(rf, (unit * parts + p) * 8, 0,
+                                                                                    kPCoherent)) == w.mark;
+  const bool all = __builtin_amdgcn_ballot_w64(!set) == 0;
+  if (lane == 0) scratch[wave] = all;
+  __syncthreads();
+  if (!(scratch[0] && scratch[1] && scratch[2] && scratch[3])) return;
+  // Two that both get here store the same values.
+  auto get = [&](int p) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rec, at_record(p), 0, kPCoherent));
+  };
+  float y = 0.0f;
+  for (int p = 0; p < parts; p += 8) {
+    float z[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) z[u] = get(min(p + u, parts - 1));
+#pragma unroll
+    for (int u = 0; u < 8; ++u) y += p + u < parts ? z[u] : 0.0f;
+  }
+  if (w.add) y += get(parts);
+  if (j < w.max_len && (mine || !w.add)) *out = y;
+}
+
 }  // namespace
+
+template <int D, bool BF16, bool FP8>
+void launch_weigh_chunk(const WeighArgs& a, int64_t grid, hipStream_t stream) {
+  hipLaunchKernelGGL((fa_paged_weigh_chunk_kernel<D, BF16, FP8>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+}
 
 template <int D, bool BF16, bool FP8>
 void launch_weigh_few(const WeighArgs& a, int rows, int64_t grid, hipStream_t stream) {

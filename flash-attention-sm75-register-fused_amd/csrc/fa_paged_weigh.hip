@@ -7,18 +7,26 @@
 namespace fa {
 
 #define FA_WEIGH_EXTERN(D, BF, F8) \
-  extern template void launch_weigh_few<D, BF, F8>(const WeighArgs&, int, int64_t, hipStream_t);
+  extern template void launch_weigh_few<D, BF, F8>(const WeighArgs&, int, int64_t, hipStream_t); \
+  extern template void launch_weigh_chunk<D, BF, F8>(const WeighArgs&, int64_t, hipStream_t);
 FA_WEIGH_EXTERN(64, false, false) FA_WEIGH_EXTERN(64, true, false)
 FA_WEIGH_EXTERN(64, false, true) FA_WEIGH_EXTERN(64, true, true)
 FA_WEIGH_EXTERN(128, false, false) FA_WEIGH_EXTERN(128, true, false)
 FA_WEIGH_EXTERN(128, false, true) FA_WEIGH_EXTERN(128, true, true)
 #undef FA_WEIGH_EXTERN
 
-WeighPlan plan_weigh(const WeighArgs& a, int head_dim, int64_t max_query_len) {
-  (void)head_dim;
+WeighPlan plan_weigh(const WeighArgs& a, int64_t max_query_len, int64_t workspace_bytes) {
   WeighPlan p{};
-  p.rows = max_query_len * a.p.group <= 16 ? 16 : 32;
   const int64_t pairs = (int64_t)a.p.batch * a.p.hkv;
+  if (max_query_len * a.p.group > 32) {
+    // A workgroup for each block of keys there is room for, and for the parts of those that are cut.
+    constexpr int64_t kBytes = (2 * kWBlock * 4 + 8) * (int64_t)kWTarget;
+    p.split = workspace_bytes >= kBytes;
+    p.workspace_bytes = p.split ? kBytes : 0;
+    p.grid = ((int64_t)a.max_len + kWBlock - 1) / kWBlock * pairs + (p.split ? kWTarget : 0);
+    return p;
+  }
+  p.rows = max_query_len * a.p.group <= 16 ? 16 : 32;
   const int64_t tiles = ((int64_t)a.max_len + kWTile - 1) / kWTile;
   // Tiles of a wave: one where there are few, at most eight.
   const int64_t waves = (int64_t)resident_fused_workgroups() * 8;
@@ -27,21 +35,34 @@ WeighPlan plan_weigh(const WeighArgs& a, int head_dim, int64_t max_query_len) {
   return p;
 }
 
-int launch_weigh(const WeighArgs& args, const WeighPlan& plan, int head_dim, hipStream_t stream) {
+template <int D, bool BF16, bool FP8>
+static void launch_planned(const WeighArgs& a, const WeighPlan& plan, hipStream_t stream) {
+  if (plan.rows == 0) launch_weigh_chunk<D, BF16, FP8>(a, plan.grid, stream);
+  else launch_weigh_few<D, BF16, FP8>(a, plan.rows, plan.grid, stream);
+}
+template <int D>
+static void launch_typed(const WeighArgs& a, const WeighPlan& plan, hipStream_t stream) {
+  if (a.p.ks != nullptr) {
+    if (a.p.bf16) launch_planned<D, true, true>(a, plan, stream);
+    else launch_planned<D, false, true>(a, plan, stream);
+  } else {
+    if (a.p.bf16) launch_planned<D, true, false>(a, plan, stream);
+    else launch_planned<D, false, false>(a, plan, stream);
+  }
+}
+
+int launch_weigh(const WeighArgs& args, const WeighPlan& plan, int head_dim, void* workspace, hipStream_t stream) {
   WeighArgs a = args;
   a.run = plan.run;
+  a.split = plan.split ? 1 : 0;
   a.p.inv_group = 1.0f / (float)a.p.group;
-  const bool fp8 = a.p.ks != nullptr;
-#define FA_WEIGH(D)                                                             \
-  if (fp8) {                                                                    \
-    if (a.p.bf16) launch_weigh_few<D, true, true>(a, plan.rows, plan.grid, stream);   \
-    else launch_weigh_few<D, false, true>(a, plan.rows, plan.grid, stream);     \
-  } else {                                                                      \
-    if (a.p.bf16) launch_weigh_few<D, true, false>(a, plan.rows, plan.grid, stream);  \
-    else launch_weigh_few<D, false, false>(a, plan.rows, plan.grid, stream);    \
+  if (plan.split) {
+    a.partial = static_cast<float*>(workspace);
+    a.flags = reinterpret_cast<uint64_t*>(a.partial + 2 * kWTarget * kWBlock);
+    a.mark = merge_mark(a.flags, kWTarget, stream);
   }
-  if (head_dim == 64) { FA_WEIGH(64) } else { FA_WEIGH(128) }
-#undef FA_WEIGH
+  if (head_dim == 64) launch_typed<64>(a, plan, stream);
+  else launch_typed<128>(a, plan, stream);
   return 0;
 }
 

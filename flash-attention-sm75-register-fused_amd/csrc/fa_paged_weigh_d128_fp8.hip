@@ -4,4 +4,6 @@
 namespace fa {
 template void launch_weigh_few<128, false, true>(const WeighArgs&, int, int64_t, hipStream_t);
 template void launch_weigh_few<128, true, true>(const WeighArgs&, int, int64_t, hipStream_t);
+template void launch_weigh_chunk<128, false, true>(const WeighArgs&, int64_t, hipStream_t);
+template void launch_weigh_chunk<128, true, true>(const WeighArgs&, int64_t, hipStream_t);
 }  // namespace fa

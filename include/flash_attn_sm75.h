@@ -466,22 +466,26 @@ typedef struct fa_paged_weigh_params {
   float* weights;      /* [batch, heads_kv, max_len], strides in elements, positions contiguous */
   int64_t weights_stride_b, weights_stride_h;
   int64_t max_len;     /* positions up to max_len are weighed; batch * heads_kv up to 2^22, times
-                          max_len up to 2^33 */
+                          max_len (in whole 32) up to 2^31 */
   int add;             /* nonzero: add to what is there (positions without a row are left as they
                           are); 0: write (they get 0) */
   int64_t tokens;      /* as in fa_paged_params, as all that follows */
   int64_t heads_q;
-  int64_t q_stride_t, q_stride_h;
+  int64_t q_stride_t, q_stride_h;  /* below 2^23; (heads_q / heads_kv) q_stride_h + 33 q_stride_t below 2^30 */
   const int32_t* cu_seqlens;
   int64_t max_query_len;
   float scale;
   int causal;
   int dtype;
   void* stream;
+  void* workspace;     /* optional, as in fa_paged_params: sums of keys whose rows are split */
+  int64_t workspace_bytes;
 } fa_paged_weigh_params;
 
-/* Asynchronous on p->stream; needs no workspace.  The same call gives the same bits. */
+/* Asynchronous on p->stream; allocates nothing.  The same call, with the same workspace size, gives
+ * the same bits. */
 int fa_sm75_paged_weigh(const fa_paged_weigh_params* p);
+int64_t fa_sm75_paged_weigh_workspace_size(const fa_paged_weigh_params* p);
 
 /* Eviction: of each sequence and KV head, min(keep, rows it holds) rows stay: those of its last
  * `recent` positions, and of the others the ones of the largest weights (of equal ones those at
@@ -499,7 +503,7 @@ typedef struct fa_paged_evict_params {
   int64_t to_pages;         /* to_pages * page_size at least keep, or as many as block_table has
                                room for */
   int64_t to_table_stride;
-  int64_t keep, recent;     /* 0 <= recent <= keep; batch * heads_kv up to 2^20, times keep up to 2^30 */
+  int64_t keep, recent;     /* 0 <= recent <= keep; batch * heads_kv up to 2^20, times keep up to 2^29 */
   int32_t* new_lens;        /* [batch] */
   float* new_weights;       /* contiguous [batch, heads_kv, to_pages * page_size] */
   void* stream;

@@ -492,8 +492,36 @@ def test_evict_heads(device, hkv):
 
 @pytest.mark.parametrize("keep,recent", [(0, 0), (1, 1), (33000, 5), (20000, 1000), (40000, 0)])
 def test_evict_long(device, keep, recent):
-    """More positions than shared memory holds."""
-    evict(Cache([34567, 100], 1, 64, 128, BF16, True), device, keep, recent)
+    """Rows of several workgroups, one of few positions among them."""
+    evict(Cache([34567, 100, 8192, 8193, 0], 1, 64, 128, BF16, True), device, keep, recent)
+
+
+@pytest.mark.parametrize("keep,recent", [(4000, 100), (16000, 0)])
+def test_evict_blocks(device, keep, recent):
+    """Sizes at a block's borders, ties over several of them, pages missing in some."""
+    c = Cache([16384, 16383, 16385, 9000], 2, 64, 256, FP16, False, gone=[(3, 0), (0, 31), (0, 32), (0, 33), (2, 63)])
+    w = torch.randint(0, 6, (4, 2, c.width * 256), generator=torch.Generator().manual_seed(6)).float()
+    evict(c, device, keep, recent, w=w)
+
+
+def test_evict_many_blocks_of_a_workgroup(device):
+    """More rows than workgroups are wanted: each takes several blocks."""
+    batch, room, keep = 2100, 16384 + 256, 5
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn(3 + batch, 2, 256, 64, generator=g).half().to(device)
+    table = torch.zeros(batch, room // 256, dtype=torch.int32, device=device)
+    table[:, 1::2] = 1
+    lens = torch.randint(room - 300, room + 1, (batch,), generator=g).int().to(device)
+    to = torch.arange(3, 3 + batch, dtype=torch.int32, device=device)[:, None]
+    w = torch.rand(batch, 2, room, generator=g).to(device)
+    old = k.clone()
+    got, left = fa.paged_cache_evict(k, k.clone(), table, lens, w, to, keep)
+    assert (got == keep).all()
+    live = torch.where(torch.arange(room, device=device) < lens[:, None, None], w, -1.0)
+    at = live.topk(keep).indices.sort(-1).values
+    assert torch.equal(left[:, :, :keep], w.gather(2, at)) and (left[:, :, keep:] == 0).all()
+    want = old[(at // 256) % 2, torch.arange(2, device=device)[:, None], at % 256]
+    assert torch.equal(k[3:, :, :keep], want)
 
 
 @pytest.mark.parametrize("q8", [False, True])

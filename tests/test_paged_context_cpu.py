@@ -24,7 +24,8 @@ class WeighParams(ctypes.Structure):
     _fields_ = [("cache", ctypes.POINTER(PagedCache)), ("q", PTR), ("lse", PTR), ("weights", PTR),
                 ("weights_stride_b", I64), ("weights_stride_h", I64), ("max_len", I64), ("add", INT),
                 ("tokens", I64), ("heads_q", I64), ("q_stride_t", I64), ("q_stride_h", I64), ("cu_seqlens", PTR),
-                ("max_query_len", I64), ("scale", ctypes.c_float), ("causal", INT), ("dtype", INT), ("stream", PTR)]
+                ("max_query_len", I64), ("scale", ctypes.c_float), ("causal", INT), ("dtype", INT), ("stream", PTR),
+                ("workspace", PTR), ("workspace_bytes", I64)]
 
 
 class EvictParams(ctypes.Structure):
@@ -43,9 +44,9 @@ def lib():
     lib.fa_sm75_paged_prefix_forward.argtypes = [P(PagedParams), P(PagedPrefix)]
     lib.fa_sm75_paged_prefix_workspace_size.argtypes = [P(PagedParams), P(PagedPrefix)]
     lib.fa_sm75_paged_workspace_size.argtypes = [P(PagedParams)]
-    lib.fa_sm75_paged_weigh.argtypes = [P(WeighParams)]
+    lib.fa_sm75_paged_weigh.argtypes = lib.fa_sm75_paged_weigh_workspace_size.argtypes = [P(WeighParams)]
     lib.fa_sm75_paged_evict.argtypes = lib.fa_sm75_paged_evict_workspace_size.argtypes = [P(EvictParams)]
-    for f in ("prefix", "evict"):
+    for f in ("prefix", "weigh", "evict"):
         getattr(lib, f"fa_sm75_paged_{f}_workspace_size").restype = I64
     lib.fa_sm75_paged_workspace_size.restype = I64
     return lib
@@ -146,6 +147,9 @@ def test_prefix_workspace(lib):
     (dict(q=0), 1, b"Q must not be NULL"),
     (dict(q=0x10008), 4, b"Q must be 16-byte aligned"),
     (dict(q_stride_h=12), 4, b"multiples of 8"),
+    (dict(q_stride_h=1 << 23), 5, b"below 2^23"),
+    (dict(q_stride_t=1 << 40), 5, b"below 2^23"),
+    (dict(heads_q=1 << 10, q_stride_h=1 << 21), 5, b"within 2^30"),
     (dict(lse=0), 1, b"lse must not be NULL"),
     (dict(lse=0x1002), 4, b"lse must be 4-byte aligned"),
     (dict(weights=0), 1, b"weights must not be NULL"),
@@ -154,10 +158,16 @@ def test_prefix_workspace(lib):
     (dict(max_len=-1), 1, b"non-negative"),
     (dict(max_len=(1 << 30) + 1), 5, b"max_len exceeds 2^30"),
     (dict(max_query_len=-1), 1, b"non-negative"),
+    (dict(workspace=0x1004, workspace_bytes=64), 4, b"workspace must be 16-byte aligned"),
+    (dict(workspace_bytes=-1), 1, b"non-negative"),
 ])
 def test_weigh_refusals(lib, kw, status, msg):
-    assert lib.fa_sm75_paged_weigh(ctypes.byref(weigh(cache(), **kw))) == status
+    p = weigh(cache(), **kw)
+    assert lib.fa_sm75_paged_weigh(ctypes.byref(p)) == status
     assert msg in lib.fa_sm75_last_error()
+    before = lib.fa_sm75_last_error()
+    assert lib.fa_sm75_paged_weigh_workspace_size(ctypes.byref(p)) == 0
+    assert lib.fa_sm75_last_error() == before
 
 
 def test_weigh_sizes(lib):
@@ -172,6 +182,10 @@ def test_weigh_sizes(lib):
     assert lib.fa_sm75_paged_weigh(ctypes.byref(many)) == 5
     long = weigh(cache(batch=1 << 5), heads_q=0, tokens=1 << 5, max_len=1 << 30)
     assert lib.fa_sm75_paged_weigh(ctypes.byref(long)) == 5
+    size = lambda **kw: lib.fa_sm75_paged_weigh_workspace_size(ctypes.byref(weigh(cache(), **kw)))  # noqa: E731
+    assert size() == 0  # one row block: never cut
+    assert size(cu_seqlens=0x1000, tokens=64) > 0 and size(cu_seqlens=0x1000, tokens=64) % 16 == 0
+    assert size(cu_seqlens=0x1000, tokens=64, max_query_len=16) == 0
     # V may be missing
     assert lib.fa_sm75_paged_weigh(ctypes.byref(weigh(cache(v=0, v_stride_n=3, k_scale=0x1000), max_len=0))) == 0
 
