@@ -69,19 +69,21 @@ struct PagedArgs {
   int pieces;       // most pieces the chunk kernel may cut a unit into, 0: any number
   int stream_v;     // the chunk kernel reads V non-temporally
 
-  // Attention behind shared prefixes, in two launches.  Of the prefixes (stage kPrefix):
-  // `batch` of them, table, lens and max_pages theirs, prefix g's rows those of sequences
-  // groups[g] .. groups[g + 1] - 1 of `seqs`, of all where groups is nullptr; the rows' states
-  // (O unnormalised; max, sum) go to joint_o [tokens, hq, D] and joint_ml [tokens, hq, 2].  Of
-  // the sequences' own keys (stage kOwn): the states of rows whose sequence has one of the
-  // `prefixes` join theirs.
+  // Attention behind shared prefixes, in two launches (their stage a template argument of the
+  // kernels).  Of the prefixes (kPrefix): `batch` of them, table, lens and max_pages theirs,
+  // prefix g's rows those of sequences groups[g] .. groups[g + 1] - 1 of `seqs`, of all where
+  // groups is nullptr; the states of the rows over pieces of their prefix go to records of
+  // joint_o and joint_ml, where which are is in joint_info.  Of the sequences' own keys (kOwn):
+  // rows whose sequence has one of the `prefixes` join those states.
   int stage;
   const int32_t* groups;
   int prefixes, seqs;
   float* joint_o;
   float* joint_ml;
+  int32_t* joint_info;  // of each prefix: first item of its class's, pieces of a unit, first token, tokens
+  int joint_records;
 };
-constexpr int kPrefix = 1, kOwn = 2;  // PagedArgs::stage
+constexpr int kPrefix = 1, kOwn = 2;  // PagedArgs::stage (0: no prefixes)
 
 // Largest key count a block table may cover, and row stride (bytes) of a cache
 // tensor: a window over 64 of its rows stays within 31 bits.
@@ -106,14 +108,17 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
                      int64_t workspace_bytes);
 int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_dim,
                            void* workspace, hipStream_t stream);
-// What joint_o and joint_ml take of a workspace.
-int64_t joint_bytes(const PagedArgs& a, int head_dim);
-// SHARE: instances of the two stages behind shared prefixes.
-template <int D, bool BF16, bool FP8, bool SHARE>
+// The launch over shared prefixes (workspace_bytes: what joint_o, joint_ml and joint_info take).
+PagedPlan plan_prefix(const PagedArgs& a, int head_dim, int64_t max_queries);
+// Sets the joint fields of both stages' arguments, and launches the first.
+int launch_paged_prefix(PagedArgs& prefix, PagedArgs& own, const PagedPlan& plan, int head_dim, void* workspace,
+                        hipStream_t stream);
+// STAGE: 0, or of attention behind shared prefixes kPrefix (chunks only) or kOwn.
+template <int D, bool BF16, bool FP8, int STAGE>
 void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream);
-template <int D, bool BF16, bool FP8, bool SHARE>
+template <int D, bool BF16, bool FP8, int STAGE>
 void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream);
-template <int D, bool BF16, bool SHARE>
+template <int D, bool BF16, int STAGE>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream);
 
 // The weights that attention gave the cached rows: out[b, h, j] (+)= sum over the new tokens
@@ -191,11 +196,11 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 struct PagedSeq {
   int t0, n, len, keys;
 };
-template <bool SHARE = false, class Load>
+template <int STAGE = 0, class Load>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load load) {
   PagedSeq s;
   const int len = load(a.lens + b);  // (all loads together)
-  if (SHARE && a.stage == kPrefix) {  // a prefix: the rows of its sequences
+  if constexpr (STAGE == kPrefix) {  // a prefix: the rows of its sequences
     int b0 = 0, b1 = a.seqs;
     if (a.groups != nullptr) {
       const int g0 = load(a.groups + b), g1 = load(a.groups + b + 1);
@@ -205,7 +210,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load lo
     const int t0 = a.cu != nullptr ? load(a.cu + b0) : b0, t1 = a.cu != nullptr ? load(a.cu + b1) : b1;
     s.t0 = clamp_int(t0, 0, a.tokens);
     s.n = clamp_int(t1, s.t0, a.tokens) - s.t0;
-  } else if (a.cu != nullptr) {
+    s.len = max(0, len);
+    s.keys = min(s.len, a.max_pages << a.page_shift);
+    return s;
+  }
+  if (a.cu != nullptr) {
     const int t0 = load(a.cu + b), t1 = load(a.cu + b + 1);
     s.t0 = clamp_int(t0, 0, a.tokens);
     s.n = clamp_int(t1, s.t0, a.tokens) - s.t0;
@@ -218,9 +227,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load lo
   return s;
 }
 // (b the same in every lane; all of it in scalar registers)
-template <bool SHARE = false>
+template <int STAGE = 0>
 __device__ __forceinline__ PagedSeq scalar_seq(const PagedArgs& a, int b) {
-  const PagedSeq s = paged_seq<SHARE>(a, uniform(b), load_scalar);
+  const PagedSeq s = paged_seq<STAGE>(a, uniform(b), load_scalar);
   return {uniform(s.t0), uniform(s.n), uniform(s.len), uniform(s.keys)};
 }
 

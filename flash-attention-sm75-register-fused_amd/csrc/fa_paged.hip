@@ -10,16 +10,17 @@
 namespace fa {
 
 // The instances of fa_paged_d*.hip.
-#define FA_PAGED_EXTERN_S(D, BF, F8, SH) \
-  extern template void launch_paged_attn<D, BF, F8, SH>(const PagedArgs&, int, int64_t, hipStream_t); \
-  extern template void launch_paged_chunk<D, BF, F8, SH>(const PagedArgs&, int64_t, hipStream_t);
-#define FA_PAGED_EXTERN(D, BF, F8) FA_PAGED_EXTERN_S(D, BF, F8, false) FA_PAGED_EXTERN_S(D, BF, F8, true)
+#define FA_PAGED_EXTERN(D, BF, F8)                                                                   \
+  extern template void launch_paged_attn<D, BF, F8, 0>(const PagedArgs&, int, int64_t, hipStream_t);    \
+  extern template void launch_paged_attn<D, BF, F8, kOwn>(const PagedArgs&, int, int64_t, hipStream_t); \
+  extern template void launch_paged_chunk<D, BF, F8, 0>(const PagedArgs&, int64_t, hipStream_t);        \
+  extern template void launch_paged_chunk<D, BF, F8, kPrefix>(const PagedArgs&, int64_t, hipStream_t);  \
+  extern template void launch_paged_chunk<D, BF, F8, kOwn>(const PagedArgs&, int64_t, hipStream_t);
 FA_PAGED_EXTERN(64, false, false) FA_PAGED_EXTERN(64, true, false)
 FA_PAGED_EXTERN(64, false, true) FA_PAGED_EXTERN(64, true, true)
 FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
 FA_PAGED_EXTERN(128, false, true) FA_PAGED_EXTERN(128, true, true)
 #undef FA_PAGED_EXTERN
-#undef FA_PAGED_EXTERN_S
 
 namespace {
 int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two records and their flags
@@ -33,6 +34,17 @@ constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 1
 static bool fits_line(const PagedArgs& a, int64_t units, int tile, int ahead) {
   const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + tile - 1) / tile;
   return units * (ahead + std::max<int64_t>(1, tiles)) <= INT32_MAX - 64;  // (room to round up)
+}
+
+// V non-temporally, where one block of a sequence reads it and the tables have room for
+// more than stays in the 256 MB cache behind the L2s from one step to the next (us without
+// and with: 16 tokens each of 16 sequences of 4096 to 8192 keys, 32 over 8 heads d128, 400
+// MB 99.9 / 81.2, of 32 in 8 bits 118.7 / 108.8, 10 of 48 of 8192 to 16384 d64, 302 MB 68.2 /
+// 63.8; in the cache: 16 of those 33.0 / 35.4, 16 in 8 bits d128 72.5 / 73.7).
+static bool streams_v(const PagedArgs& a, int head_dim, int64_t max_query_len) {
+  const int64_t room = ((int64_t)a.max_pages << a.page_shift) * a.batch * a.hkv;
+  return max_query_len * a.group <= kChunkRows &&
+         room > kLastCacheBytes / (2 * head_dim * (a.ks != nullptr ? 1 : 2));
 }
 
 // Units of 128 rows, cut into pieces where they may be fewer than the GPU runs at once.
@@ -54,22 +66,11 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t max_query
   // ones d128 60.9 / 59.1, one prompt of 700 tokens 21.8 / 20.3, three of 777 tokens d64 8 bits 50.7 / 47.5)
   const bool few = least * (chunk_pieces(head_dim) - 1) < wgs;
   p.combine = p.split && few;
-  // V non-temporally, where one block of a sequence reads it and the tables have room for
-  // more than stays in the 256 MB cache behind the L2s from one step to the next (us without
-  // and with: 16 tokens each of 16 sequences of 4096 to 8192 keys, 32 over 8 heads d128, 400
-  // MB 99.9 / 81.2, of 32 in 8 bits 118.7 / 108.8, 10 of 48 of 8192 to 16384 d64, 302 MB 68.2 /
-  // 63.8; in the cache: 16 of those 33.0 / 35.4, 16 in 8 bits d128 72.5 / 73.7).
-  const int64_t room = ((int64_t)a.max_pages << a.page_shift) * a.batch * a.hkv;
-  p.stream_v = max_query_len * a.group <= kChunkRows &&
-               room > kLastCacheBytes / (2 * head_dim * (a.ks != nullptr ? 1 : 2));
+  p.stream_v = streams_v(a, head_dim, max_query_len);
   p.pieces = few ? 0 : chunk_pieces(head_dim);
   p.wgs = p.split ? (int)wgs : p.units;
   p.workspace_bytes = p.split ? p.wgs * record + kCombineWord : 0;
   return p;
-}
-
-int64_t joint_bytes(const PagedArgs& a, int head_dim) {
-  return ((int64_t)a.tokens * a.hq * (head_dim + 2) * (int64_t)sizeof(float) + 15) & ~(int64_t)15;
 }
 
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
@@ -87,9 +88,8 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   const int64_t room = (workspace_bytes - kCombineWord) / (partial_bytes(p.rows, head_dim) * p.classes);
   p.wgs = (int)std::min(resident / p.classes, room);
   // Units of a class: blocks of rows, the last of each sequence not full.
-  const bool ones = a.cu == nullptr && a.stage != kPrefix;  // one token in every sequence
   const int64_t blocks =
-      ones ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
+      a.cu == nullptr ? (int64_t)a.batch * ((a.group + p.rows - 1) / p.rows)
                       : (int64_t)a.tokens * a.group / p.rows + std::min(a.batch, a.tokens);
   p.units = (int)(a.hkv / p.classes * blocks);
   // (Of very many units a workgroup each is balanced enough.)
@@ -102,45 +102,63 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   const int64_t pieces = PagedStretch<kPMinTiles>::most_pieces(tiles, p.wgs);
   p.y = (int)std::min<int64_t>(p.rows, max_query_len * a.group);
   // (max_query_len may be wrong: rows are then up to p.rows)
-  p.combine = p.split && !paged_merges_itself((int)pieces, ones ? p.y : p.rows, head_dim);
+  p.combine = p.split && !paged_merges_itself((int)pieces, a.cu == nullptr ? p.y : p.rows, head_dim);
   return p;
 }
 
-template <int D, bool BF16, bool SHARE>
+PagedPlan plan_prefix(const PagedArgs& a, int head_dim, int64_t max_queries) {
+  PagedPlan p{};
+  p.chunk = p.split = true;
+  p.rows = kChunkRows;
+  p.classes = std::gcd(a.hkv, kNumXcds);
+  const int64_t rows = (int64_t)a.tokens * a.group;
+  p.units = (int)(a.hkv / p.classes * ((rows + (p.rows - 1ll) * std::min(a.batch, a.tokens)) / p.rows));
+  p.wgs = std::max(resident_fused_workgroups() / p.classes, p.units);
+  p.stream_v = streams_v(a, head_dim, max_queries);
+  p.workspace_bytes = (int64_t)p.wgs * p.classes * p.rows * (head_dim + 2) * (int64_t)sizeof(float) + 16ll * a.batch;
+  return p;
+}
+
+template <int D, bool BF16, int STAGE>
 void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream) {
   if (rows == kChunkRows) {
-    hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16, SHARE>),
+    hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16, STAGE>),
                        dim3((unsigned)(a.wgs * a.classes), kChunkCombineY), dim3(kThreads), 0, stream, a);
     return;
   }
   const dim3 g((unsigned)(a.units * a.classes), (unsigned)y);
   if (rows == 16)
-    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1, SHARE>), g, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 1, STAGE>), g, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 2, SHARE>), g, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((fa_paged_combine_kernel<D, BF16, 2, STAGE>), g, dim3(kThreads), 0, stream, a);
 }
 
-template <int D, bool BF16, bool FP8, bool SHARE>
+template <int D, bool BF16, bool FP8, int STAGE>
 static void launch_planned(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
-  if (plan.chunk) launch_paged_chunk<D, BF16, FP8, SHARE>(a, grid, stream);
-  else launch_paged_attn<D, BF16, FP8, SHARE>(a, plan.rows, grid, stream);
-  if (plan.combine) launch_paged_combine<D, BF16, SHARE>(a, plan.rows, plan.y, stream);
+  if constexpr (STAGE == kPrefix) {
+    launch_paged_chunk<D, BF16, FP8, STAGE>(a, grid, stream);
+    return;
+  } else if (plan.chunk) {
+    launch_paged_chunk<D, BF16, FP8, STAGE>(a, grid, stream);
+  } else {
+    launch_paged_attn<D, BF16, FP8, STAGE>(a, plan.rows, grid, stream);
+  }
+  if (plan.combine) launch_paged_combine<D, BF16, STAGE>(a, plan.rows, plan.y, stream);
 }
-template <int D, bool SHARE>
+template <int D, int STAGE>
 static void launch_typed(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
   if (a.ks != nullptr) {
-    if (a.bf16) launch_planned<D, true, true, SHARE>(a, plan, stream);
-    else launch_planned<D, false, true, SHARE>(a, plan, stream);
+    if (a.bf16) launch_planned<D, true, true, STAGE>(a, plan, stream);
+    else launch_planned<D, false, true, STAGE>(a, plan, stream);
   } else {
-    if (a.bf16) launch_planned<D, true, false, SHARE>(a, plan, stream);
-    else launch_planned<D, false, false, SHARE>(a, plan, stream);
+    if (a.bf16) launch_planned<D, true, false, STAGE>(a, plan, stream);
+    else launch_planned<D, false, false, STAGE>(a, plan, stream);
   }
 }
 
-int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int head_dim,
-                           void* workspace, hipStream_t stream) {
-  PagedArgs a = args;
+// A plan's fields, and what follows from the sizes.
+static void set_plan(PagedArgs& a, const PagedPlan& plan) {
   a.classes = plan.classes;  // (divides kNumXcds, a power of two)
   a.class_shift = __builtin_ctz(plan.classes);
   a.heads = a.hkv / a.classes;
@@ -152,6 +170,30 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
   a.pieces = plan.pieces;
   a.stream_v = plan.stream_v ? 1 : 0;
   a.split = plan.split ? 1 : 0;
+}
+
+template <int STAGE>
+static void launch_sized(const PagedArgs& a, const PagedPlan& plan, int head_dim, hipStream_t stream) {
+  if (head_dim == 64) launch_typed<64, STAGE>(a, plan, stream);
+  else launch_typed<128, STAGE>(a, plan, stream);
+}
+
+int launch_paged_prefix(PagedArgs& prefix, PagedArgs& own, const PagedPlan& plan, int head_dim, void* workspace,
+                        hipStream_t stream) {
+  set_plan(prefix, plan);
+  const int64_t records = (int64_t)plan.wgs * plan.classes;
+  prefix.joint_records = own.joint_records = (int)records;
+  prefix.joint_info = own.joint_info = static_cast<int32_t*>(workspace);
+  prefix.joint_o = own.joint_o = reinterpret_cast<float*>(prefix.joint_info + 4ll * prefix.batch);
+  prefix.joint_ml = own.joint_ml = prefix.joint_o + records * plan.rows * head_dim;
+  launch_sized<kPrefix>(prefix, plan, head_dim, stream);
+  return 0;
+}
+
+int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int head_dim,
+                           void* workspace, hipStream_t stream) {
+  PagedArgs a = args;
+  set_plan(a, plan);
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
   if (plan.split) {
     a.part_o = static_cast<float*>(workspace);
@@ -159,13 +201,8 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);
     a.mark = merge_mark(a.flags, 2 * grid + 1, stream);
   }
-  if (a.stage != 0) {
-    if (head_dim == 64) launch_typed<64, true>(a, plan, stream);
-    else launch_typed<128, true>(a, plan, stream);
-  } else {
-    if (head_dim == 64) launch_typed<64, false>(a, plan, stream);
-    else launch_typed<128, false>(a, plan, stream);
-  }
+  if (a.stage == kOwn) launch_sized<kOwn>(a, plan, head_dim, stream);
+  else launch_sized<0>(a, plan, head_dim, stream);
   return 0;
 }
 

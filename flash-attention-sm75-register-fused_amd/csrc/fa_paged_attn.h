@@ -85,8 +85,8 @@ __device__ __forceinline__ PagedStretch<kPMinTiles> paged_stretch(const PagedArg
   return s;
 }
 
-// SHARE: either stage of attention behind shared prefixes (PagedArgs::stage).
-template <int D, bool BF16, bool FP8, int NT, bool SHARE>
+// STAGE: 0, or kOwn behind shared prefixes.
+template <int D, bool BF16, bool FP8, int NT, int STAGE>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
   using E = Elem<BF16>;
   constexpr int R = 16 * NT;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
 
-  const PagedLine<R, kPTile, kPAhead, SHARE> line(a, lane, a.split != 0);
+  const PagedLine<R, kPTile, kPAhead> line(a, lane, a.split != 0);
   auto stretch = paged_stretch(a, line);
   if (wg >= stretch.active) return;
   int pos, end;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     // key it sees.
     const int nrows = s.n * a.group;
     const PagedRows row_of(a, s, hkv, rb * R);
-    const PagedJoint joint = joint_of<SHARE>(a, b);
+    const PagedJoint joint = joint_of<STAGE>(a, b, hkv);
     const int past = s.len - s.n;  // tokens before the new ones
     int last[NT];
     half8 qf[NT][KS];
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
 // unit of a class (blockIdx.x) and row (blockIdx.y, and every gridDim.y-th on).
 // The four waves take every fourth piece, D / 4 lanes each piece's row (with
 // several pieces at once where D / 4 < 64 lanes), and meet in LDS.
-template <int D, bool BF16, int NT, bool SHARE>
+template <int D, bool BF16, int NT, int STAGE>
 __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedArgs a) {
   constexpr int R = 16 * NT;
   constexpr int LR = D / 4;               // lanes of a row
@@ -546,13 +546,12 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   if (!combine_asked(a)) return;
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int index = (int)(blockIdx.x >> a.class_shift);  // of the class's units
-  const PagedLine<R, kPTile, kPAhead, SHARE> line(a, threadIdx.x & 63, true);
-  const PagedLine<R, kPTile, kPAhead, SHARE> units(a, threadIdx.x & 63, false);
+  const PagedLine<R, kPTile, kPAhead> line(a, threadIdx.x & 63, true);
+  const PagedLine<R, kPTile, kPAhead> units(a, threadIdx.x & 63, false);
   if (index >= units.total()) return;
   int unit_start;
   const int b = uniform(units.find(index, unit_start));
   const PagedSeq s = line.seq(b);
-  const PagedJoint joint = joint_of<SHARE>(a, b);
   const int unit_len = line.unit_of(s);
   const int unit = index - unit_start;
   const int u0 = line.start_of(b) + unit * unit_len;
@@ -563,6 +562,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   const int hc = unit / blocks;
   const int rb = unit - hc * blocks;
   const int hkv = hc * a.classes + cls;
+  const PagedJoint joint = joint_of<STAGE>(a, b, hkv);
   const int nr = min(R, s.n * a.group - rb * R);
   if (paged_merges_itself(pieces.count, nr, D)) return;
   const int grp = (int)threadIdx.x / LR, ch = (int)threadIdx.x % LR;
@@ -597,13 +597,13 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
 
 }  // namespace
 
-template <int D, bool BF16, bool FP8, bool SHARE>
+template <int D, bool BF16, bool FP8, int STAGE>
 void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream) {
   if (rows == 16)
-    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 1, SHARE>), dim3((unsigned)grid), dim3(kThreads), 0,
+    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 1, STAGE>), dim3((unsigned)grid), dim3(kThreads), 0,
                        stream, a);
   else
-    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 2, SHARE>), dim3((unsigned)grid), dim3(kThreads), 0,
+    hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 2, STAGE>), dim3((unsigned)grid), dim3(kThreads), 0,
                        stream, a);
 }
 

@@ -386,9 +386,7 @@ int64_t fa_sm75_paged_prefix_workspace_size(const fa_paged_params* p, const fa_p
   if (make_forward(p, &a, &empty) != FA_OK || empty || make_prefix(x, a, &prefix, &own) != FA_OK) return 0;
   const int d = (int)p->cache->head_dim;
   const int64_t rest = fa::plan_paged(own, d, longest_query(p), INT64_MAX).workspace_bytes;
-  if (own.stage == 0) return rest;
-  const int64_t first = fa::plan_paged(prefix, d, longest_shared(x, a), INT64_MAX).workspace_bytes;
-  return fa::joint_bytes(a, d) + (first > rest ? first : rest);
+  return own.stage == 0 ? rest : fa::plan_prefix(prefix, d, longest_shared(x, a)).workspace_bytes + rest;
 }
 
 int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix* x) {
@@ -403,16 +401,13 @@ int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix
   char* work = static_cast<char*>(p->workspace);
   int64_t bytes = p->workspace != nullptr ? p->workspace_bytes : 0;
   if (own.stage != 0) {
-    const int64_t joint = fa::joint_bytes(a, d);
-    if (bytes < joint)
+    const fa::PagedPlan plan = fa::plan_prefix(prefix, d, longest_shared(x, a));
+    if (bytes < plan.workspace_bytes)
       return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes at least, got %lld",
-                       (long long)joint, (long long)bytes);
-    prefix.joint_o = own.joint_o = reinterpret_cast<float*>(work);
-    prefix.joint_ml = own.joint_ml = own.joint_o + (int64_t)a.tokens * a.hq * d;
-    work += joint;
-    bytes -= joint;
-    const fa::PagedPlan plan = fa::plan_paged(prefix, d, longest_shared(x, a), bytes);
-    fa::launch_paged_attention(prefix, plan, d, work, stream);
+                       (long long)plan.workspace_bytes, (long long)bytes);
+    fa::launch_paged_prefix(prefix, own, plan, d, work, stream);
+    work += plan.workspace_bytes;
+    bytes -= plan.workspace_bytes;
   }
   const fa::PagedPlan plan = fa::plan_paged(own, d, longest_query(p), bytes);
   fa::launch_paged_attention(own, plan, d, work, stream);

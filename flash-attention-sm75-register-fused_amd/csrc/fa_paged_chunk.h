@@ -46,7 +46,6 @@
 namespace fa {
 namespace {
 
-constexpr int kChunkRows = 128;
 // Tiles a stretch is not cut below (us with 4, 5 and 6: one prompt of 320 tokens d128 17.9 /
 // 14.8 / 14.8, of 384 18.3 / 18.4 / 15.7, of 640 24.9 / 23.0 / 23.0, 64 tokens behind 936
 // 20.4 / 20.5 / 21.0).
@@ -78,24 +77,33 @@ __device__ __forceinline__ void store_pair(_Float16* to, float4v x, float4v y, f
 // O and LSE of a row from its merged state: pairs of groups pair0 .. pair0 + N - 1, 16
 // dimensions each, of which a half-wave holds 4 hi .. + 3 and 8 + 4 hi .. + 3.
 template <int D, bool BF16, int N>
-__device__ __forceinline__ void store_pairs(const PagedArgs& a, const PagedJoint joint, const PagedRow pr, int hi,
+__device__ __forceinline__ void store_pairs(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int hi,
                                             int pair0, float m2, float l, float4v (&x)[N][2]) {
-  if (joint.out) {
-    const int64_t row = joint_row(a, pr);
-    float* const to = a.joint_o + row * D + 16 * pair0 + 4 * hi;
+  if (joint.pieces > 0) {
+    const JointRow j(a, joint, pr);
+    const float* const o = a.joint_o + record_o<D>(j.record, j.row >> 5, 2 * pair0, 32 * hi + (j.row & 31));
+    const float* const ml = a.joint_ml + record_ml(j.record, j.row);
+    auto load_ml = [&](int i) { return *(const v2f*)(ml + record_ml((int64_t)i * joint.step, 0)); };
+    float top = m2;
+    for (int i = 0; i < j.pieces; ++i) top = fmaxf(top, load_ml(i)[0]);
+    const float f = __builtin_amdgcn_exp2f(m2 - over_zero(top));
+    l *= f;
 #pragma unroll
-    for (int q = 0; q < N; ++q)
+    for (int q = 0; q < N; ++q) {
+      x[q][0] *= f;
+      x[q][1] *= f;
+    }
+    m2 = top;
+    for (int i = 0; i < j.pieces; ++i) {
+      const v2f p = load_ml(i);
+      const float w = __builtin_amdgcn_exp2f(p[0] - over_zero(top));
+      l += w * p[1];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) *(float4v*)(to + 16 * q + 8 * e) = x[q][e];
-    if (hi == 0 && pair0 == 0) *(v2f*)(a.joint_ml + 2 * row) = v2f{m2, l};
-    return;
-  }
-  if (joint.in) {
-    const JointState<D> j(a, pr, m2, l);
+      for (int q = 0; q < N; ++q)
 #pragma unroll
-    for (int q = 0; q < N; ++q)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) x[q][e] = j.x(16 * (pair0 + q) + 4 * hi + 8 * e, x[q][e]);
+        for (int e = 0; e < 2; ++e)
+          x[q][e] += w * *(const float4v*)(o + record_o<D>((int64_t)i * joint.step, 0, 2 * q + e, 0));
+    }
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
@@ -113,9 +121,8 @@ constexpr int kChunkMergeBytes = 320 << 10;
 constexpr int chunk_pieces(int d) { return kChunkMergeBytes / (kChunkRows * d * 4); }
 
 // A record of the workspace: a block's partials in the order its waves' registers
-// hold them, so that 64 lanes store and load 1 KB at once (row by row, 16 bytes of
-// 32 rows at once, coherent stores took half of a short launch).  Group 4 mt + g of a wave:
-// dimensions 32 mt + 8 g + 4 (lane / 32) .. + 3 of its row lane % 32.
+// hold them (record_o), so that 64 lanes store and load 1 KB at once (row by row, 16 bytes
+// of 32 rows at once, coherent stores took half of a short launch).
 template <int D>
 struct ChunkRecord {
   static constexpr int Groups = D / 8;
@@ -137,7 +144,7 @@ struct ChunkRecord {
 // l_i, M = max_i m_i.
 template <int D, bool BF16>
 __device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPieces& pieces, int cls,
-                                            const PagedJoint joint, const PagedRows& row_of, int rows, int pair0) {
+                                            const PagedJoint& joint, const PagedRows& row_of, int rows, int pair0) {
   constexpr int PAIRS = 4, AT = 4;  // at once; pieces at once
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -228,9 +235,98 @@ __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const Page
   return s;
 }
 
+// The plan of the launch over shared prefixes.  An item is a piece of a unit (prefix, KV head of
+// the class, block of rows): units of a prefix with T tiles are cut into ceil(T / q) pieces of
+// equal length, q the smallest (found in steps of an eighth) with which the class's workgroups
+// have an item each at most; where the units are more than those, none is cut.  A piece's record is its
+// item's, and the second launch adds the pieces up where it stores a row, so there is no merge (64
+// tokens behind a prefix of 8192, 32 over 8 heads d128: %%%).
+constexpr int kPrefixMinTiles = 4;
+struct PrefixLine {
+  const PagedArgs& a;
+  int lane, q;
+  PagedSeq own;  // prefix `lane`
+  __device__ __forceinline__ PrefixLine(const PagedArgs& args, int ln) : a(args), lane(ln) {
+    own = look(lane);
+    float units = 0.0f, tiles = 0.0f;  // (where cu_prefix falls again and again they may pass 2^31)
+    for (int g0 = 0; g0 < a.batch; g0 += 64) {
+      const PagedSeq s = g0 == 0 ? own : look(g0 + lane);
+      float n = (float)units_of(s), t = n * (float)tiles_of(s);
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        n += __shfl_xor(n, m);
+        t += __shfl_xor(t, m);
+      }
+      units += n;
+      tiles += t;
+    }
+    q = INT32_MAX;
+    if (units >= (float)a.wgs) return;
+    q = max(kPrefixMinTiles, (int)(tiles / (float)a.wgs));
+    while (total() > a.wgs) q += (q + 7) / 8;  // (ends: with the longest prefix's tiles there are `units`)
+    q = uniform(q);
+  }
+  __device__ __forceinline__ PagedSeq look(int g) const {
+    PagedSeq s = paged_seq<kPrefix>(a, min(g, a.batch - 1), [](const int32_t* p) { return *p; });
+    if (g >= a.batch) s.n = 0;
+    return s;
+  }
+  static __device__ __forceinline__ int tiles_of(const PagedSeq& s) {
+    return (int)((unsigned)(s.keys + kBlockN - 1) / kBlockN);
+  }
+  // (none of a prefix without keys: nothing is to be joined)
+  __device__ __forceinline__ int units_of(const PagedSeq& s) const {
+    return s.keys > 0 ? a.heads * paged_blocks<kChunkRows>(a, s) : 0;
+  }
+  __device__ __forceinline__ int pieces_of(const PagedSeq& s) const {
+    const unsigned t = tiles_of(s);
+    return (int)(t / (unsigned)q + (t % (unsigned)q != 0 ? 1 : 0));
+  }
+  __device__ __forceinline__ int prefix(int g0) const {  // items of prefixes g0 .. g0 + lane
+    const PagedSeq s = g0 == 0 ? own : look(g0 + lane);
+    return wave_prefix(units_of(s) * pieces_of(s));
+  }
+  __device__ __forceinline__ int total() const {
+    int sum = 0;
+    for (int g0 = 0; g0 < a.batch; g0 += 64) sum += wave_bcast(prefix(g0), 63);
+    return uniform(sum);
+  }
+  // The prefix of an item (below total), and its first one.
+  __device__ __forceinline__ int find(int item, int& start) const {
+    int before = 0;
+    for (int g0 = 0;; g0 += 64) {
+      const int x = prefix(g0);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + x > item);
+      if (past != 0 || g0 + 64 >= a.batch) {
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        start = uniform(l > 0 ? before + wave_bcast(x, l - 1) : before);
+        return uniform(min(g0 + l, a.batch - 1));
+      }
+      before += wave_bcast(x, 63);
+    }
+  }
+  // What the second launch goes by (PagedArgs::joint_info); one wave of the launch.
+  __device__ __forceinline__ void publish() const {
+    int before = 0;
+    for (int g0 = 0; g0 < a.batch; g0 += 64) {
+      const PagedSeq s = g0 == 0 ? own : look(g0 + lane);
+      const int items = units_of(s) * pieces_of(s);
+      const int x = wave_prefix(items);
+      if (g0 + lane < a.batch) {
+        int32_t* const to = a.joint_info + 4 * (g0 + lane);
+        to[0] = before + x - items;
+        to[1] = items > 0 ? pieces_of(s) : 0;
+        to[2] = s.t0;
+        to[3] = s.n;
+      }
+      before += wave_bcast(x, 63);
+    }
+  }
+};
+
 // STREAM: V's rows are read non-temporally (a sequence's only block is the one that reads them).
-// SHARE: either stage of attention behind shared prefixes (PagedArgs::stage).
-template <int D, bool BF16, bool FP8, bool SPLIT, bool STREAM, bool SHARE>
+// STAGE: 0, or of attention behind shared prefixes kPrefix (SPLIT) or kOwn.
+template <int D, bool BF16, bool FP8, bool SPLIT, bool STREAM, int STAGE>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
   constexpr bool DENSE = D == 64;
   using L = std::conditional_t<DENSE, LdsDense<D>, Lds<D>>;
@@ -257,24 +353,51 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
-  const PagedLine<kChunkRows, kBlockN, kChunkAhead, SHARE> line(a, threadIdx.x & 63, SPLIT);
+  constexpr bool PREFIX = STAGE == kPrefix;
+  const auto line = [&] {
+    if constexpr (PREFIX) return PrefixLine(a, threadIdx.x & 63);
+    else return PagedLine<kChunkRows, kBlockN, kChunkAhead>(a, threadIdx.x & 63, SPLIT);
+  }();
   const auto stretch = [&] {
-    if constexpr (SPLIT) return chunk_stretch<D>(a, line);
+    if constexpr (PREFIX) return 0;
+    else if constexpr (SPLIT) return chunk_stretch<D>(a, line);
     else return PagedStretch<1>(a, line.total());
   }();
-  if (wg >= stretch.active) return;
-  int pos, end;
-  stretch.of(wg, pos, end);
-  if constexpr (!SPLIT) {
-    if (a.causal && stretch.len <= a.resident && pos >= a.resident / 2)
-      pos = stretch.len - 1 + a.resident / 2 - pos;
+  int pos = 0, end = 0;
+  int seq_start, b;
+  if constexpr (PREFIX) {
+    if (blockIdx.x == 0 && wave == 0) line.publish();
+    if (wg >= line.total()) return;
+    b = line.find(wg, seq_start);
+  } else {
+    if (wg >= stretch.active) return;
+    stretch.of(wg, pos, end);
+    if constexpr (!SPLIT) {
+      if (a.causal && stretch.len <= a.resident && pos >= a.resident / 2)
+        pos = stretch.len - 1 + a.resident / 2 - pos;
+    }
+    b = uniform(line.find(pos, seq_start));
   }
-  int seq_start;
-  int b = uniform(line.find(pos, seq_start));
 
   do {
-  const PagedSeq s = line.seq(b);
-  const int blocks = paged_blocks<kChunkRows>(a, s);
+  PagedSeq s;
+  int blocks, first, stop, hc, rb, u0 = 0, u1 = 0;
+  bool whole = false;
+  if constexpr (PREFIX) {
+    s = scalar_seq<kPrefix>(a, b);
+    blocks = paged_blocks<kChunkRows>(a, s);
+    // Pieces next to each other in the order of the items are of units that read the same keys.
+    const int units = line.units_of(s), rel = wg - seq_start;
+    const int tiles = line.tiles_of(s), pieces = line.pieces_of(s);
+    if (units <= 0 || rel < 0 || rel >= units * pieces) return;  // (past 2^31)
+    const int piece = uniform((int)((unsigned)rel / (unsigned)units)), unit = rel - piece * units;
+    first = uniform((int)((uint64_t)(unsigned)tiles * (unsigned)piece / (unsigned)pieces));
+    stop = uniform((int)((uint64_t)(unsigned)tiles * (unsigned)(piece + 1) / (unsigned)pieces));
+    hc = uniform((int)((unsigned)unit / (unsigned)blocks));
+    rb = unit - hc * blocks;
+  } else {
+  s = line.seq(b);
+  blocks = paged_blocks<kChunkRows>(a, s);
   const int unit_len = line.unit_of(s);
   const int len = line.length_of(s);
   if (pos >= seq_start + len || len == 0) {  // on to the next sequence
@@ -283,16 +406,17 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
     continue;
   }
   const int unit = line.unit_at(pos - seq_start, unit_len, blocks);
-  const int u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
-  const int u1 = seq_start + (unit + 1) * unit_len;
-  const int first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
+  u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
+  u1 = seq_start + (unit + 1) * unit_len;
+  first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
   if (SPLIT && u1 <= pos) return;  // (wrapped round)
   pos = SPLIT ? min(u1, end) : u1;
-  const int stop = pos - u0;
+  stop = pos - u0;
   if (SPLIT && stop <= 0) break;
-  const bool whole = !SPLIT || (first == 0 && pos == u1);
-  const int hc = blocks == 1 ? unit : (int)((unsigned)unit / (unsigned)blocks);
-  const int rb = blocks - 1 - (unit - hc * blocks);
+  whole = !SPLIT || (first == 0 && pos == u1);
+  hc = blocks == 1 ? unit : (int)((unsigned)unit / (unsigned)blocks);
+  rb = blocks - 1 - (unit - hc * blocks);
+  }
   const int hkv = hc * a.classes + cls;
 
   // What depends on the lane is derived for each segment from an opaque lane index, so
@@ -759,9 +883,18 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 
   const float l = halves_sum(l_run);
   const float m2 = m_run == -__builtin_inff() ? m_run : m_run * c2;
-  const PagedJoint joint = joint_of<SHARE>(a, b);
+  const PagedJoint joint = joint_of<STAGE>(a, b, hkv);
   if (row < nrows) {
-    if (whole) {
+    if constexpr (PREFIX) {
+      float* const to = a.joint_o + record_o<D>(blockIdx.x, wave, 0, lane);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(float4v*)(to + record_o<D>(0, 0, 4 * mt + g, 0)) =
+              float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
+      if (hi == 0) *(v2f*)(a.joint_ml + record_ml(blockIdx.x, 32 * wave + ql)) = v2f{m2, l};
+    } else if (whole) {
       float4v x[D / 16][2];
 #pragma unroll
       for (int q = 0; q < D / 16; ++q)
@@ -789,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
                                               rec.ml_at(record, wave, ql), 0, kPCoherent);
     }
   }
-  if constexpr (SPLIT) {
+  if constexpr (SPLIT && !PREFIX) {
     if (!whole) {
       const PagedPieces pieces(stretch, a.wgs, u0, u1);
       if (pieces.count > chunk_pieces(D)) {
@@ -801,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
     }
     __syncthreads();  // the next segment's loads go into these tiles
   }
-  } while (SPLIT && pos < end);
+  } while (SPLIT && !PREFIX && pos < end);
 }
 
 // Merges the partials of units whose last workgroup does not.  The kChunkCombineY
@@ -809,14 +942,14 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 // of the unit share its tasks, a pair of groups of one wave's 32 rows each.  Of a task
 // the workgroup's waves take every fourth piece, and meet in LDS.
 constexpr int kChunkCombineY = 2;
-template <int D, bool BF16, bool SHARE>
+template <int D, bool BF16, int STAGE>
 __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
   __shared__ float4v xo[kWaves][2][64];
   __shared__ float xml[kWaves][2][64];
   if (!combine_asked(a)) return;
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
-  const PagedLine<kChunkRows, kBlockN, kChunkAhead, SHARE> line(a, threadIdx.x & 63, true);
+  const PagedLine<kChunkRows, kBlockN, kChunkAhead> line(a, threadIdx.x & 63, true);
   const auto stretch = chunk_stretch<D>(a, line);
   if (wg == 0 || wg >= stretch.active) return;
   int border, end;
@@ -836,7 +969,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int rows = s.n * a.group - rb * kChunkRows;
   const PagedRows row_of(a, s, hc * a.classes + cls, rb * kChunkRows);
-  const PagedJoint joint = joint_of<SHARE>(a, b);
+  const PagedJoint joint = joint_of<STAGE>(a, b, hc * a.classes + cls);
   const ChunkRecord<D> rec(a);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -904,21 +1037,19 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
 
 }  // namespace
 
-// (Behind shared prefixes V is not read non-temporally: a prefix's rows are read by all its blocks.)
-template <int D, bool BF16, bool FP8, bool SHARE>
+template <int D, bool BF16, bool FP8, int STAGE>
 void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream) {
   const dim3 g((unsigned)grid), t(kThreads);
-  if (!a.split) {
-    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false, false, SHARE>), g, t, 0, stream, a);
-    return;
-  }
-  if constexpr (!SHARE) {
-    if (a.stream_v) {
-      hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, true, SHARE>), g, t, 0, stream, a);
+  if constexpr (STAGE != kPrefix) {
+    if (!a.split) {
+      hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, false, false, STAGE>), g, t, 0, stream, a);
       return;
     }
   }
-  hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, false, SHARE>), g, t, 0, stream, a);
+  if (a.stream_v)
+    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, true, STAGE>), g, t, 0, stream, a);
+  else
+    hipLaunchKernelGGL((fa_paged_chunk_kernel<D, BF16, FP8, true, false, STAGE>), g, t, 0, stream, a);
 }
 
 }  // namespace fa

@@ -3,6 +3,6 @@
 #include "fa_paged_chunk.h"
 
 namespace fa {
-template void launch_paged_attn<128, true, true, false>(const PagedArgs&, int, int64_t, hipStream_t);
-template void launch_paged_chunk<128, true, true, false>(const PagedArgs&, int64_t, hipStream_t);
+template void launch_paged_attn<128, true, true, 0>(const PagedArgs&, int, int64_t, hipStream_t);
+template void launch_paged_chunk<128, true, true, 0>(const PagedArgs&, int64_t, hipStream_t);
 }  // namespace fa

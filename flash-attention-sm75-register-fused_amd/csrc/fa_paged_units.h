@@ -52,7 +52,7 @@ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& 
 // again and again, so that sequences share rows, may positions wrap round, and then
 // units are held to those there are, and pieces to the workgroups).  Called by whole
 // waves; the first 64 sequences, one a lane, are looked at once.
-template <int R, int T, int H, bool SHARE = false>
+template <int R, int T, int H>
 struct PagedLine {
   const PagedArgs& a;
   const int lane;
@@ -77,7 +77,7 @@ struct PagedLine {
     first = wave_prefix(length_of(own));
   }
   __device__ __forceinline__ PagedSeq look(int b) const {
-    PagedSeq s = paged_seq<SHARE>(a, min(b, a.batch - 1), [](const int32_t* p) { return *p; });
+    PagedSeq s = paged_seq(a, min(b, a.batch - 1), [](const int32_t* p) { return *p; });
     if (b >= a.batch) s.n = 0;
     return s;
   }
@@ -108,7 +108,7 @@ struct PagedLine {
     return most;
   }
   __device__ __forceinline__ PagedSeq seq(int b) const {
-    if (b >= 64) return scalar_seq<SHARE>(a, b);
+    if (b >= 64) return scalar_seq(a, b);
     return {wave_bcast(own.t0, b), wave_bcast(own.n, b), wave_bcast(own.len, b), wave_bcast(own.keys, b)};
   }
   // The sequence b that holds position pos (0 <= pos < total), and where it starts.
@@ -255,69 +255,6 @@ constexpr int kPCoherent = 16, kPStreamed = 2;
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-// What becomes of a unit's merged states behind shared prefixes: they are kept (of a prefix), or
-// join those of their rows over the prefix (of a sequence that has one).
-struct PagedJoint {
-  bool out, in;
-};
-template <bool SHARE>
-__device__ __forceinline__ PagedJoint joint_of(const PagedArgs& a, int b) {
-  PagedJoint j = {false, false};
-  if constexpr (SHARE) {
-    j.out = a.stage == kPrefix;
-    j.in = !j.out;
-    if (j.in && a.groups != nullptr) {
-      const int first = load_scalar(a.groups), behind = load_scalar(a.groups + a.prefixes);
-      j.in = b >= first && b < behind;
-    }
-  }
-  return j;
-}
-__device__ __forceinline__ int64_t joint_row(const PagedArgs& a, const PagedRow pr) {
-  return (int64_t)pr.token * a.hq + pr.head;
-}
-// A row's own state (m, l, and its x through `x`) joined with the one over its prefix:
-// M = max(m, m'), l = 2^(m - M) l + 2^(m' - M) l', x likewise; all in 32 bits, one rounding
-// to the 16-bit type after both.
-template <int D>
-struct JointState {
-  float f, fp;
-  const float* o;
-  __device__ __forceinline__ JointState(const PagedArgs& a, const PagedRow pr, float& m, float& l) {
-    const int64_t row = joint_row(a, pr);
-    const v2f p = *(const v2f*)(a.joint_ml + 2 * row);
-    o = a.joint_o + row * D;
-    const float top = fmaxf(m, p[0]);
-    f = __builtin_amdgcn_exp2f(m - over_zero(top));
-    fp = __builtin_amdgcn_exp2f(p[0] - over_zero(top));
-    l = f * l + fp * p[1];
-    m = top;
-  }
-  __device__ __forceinline__ float4v x(int dim, float4v own) const { return f * own + fp * *(const float4v*)(o + dim); }
-};
-
-// O and LSE of a row from its merged state, 4 dimensions.
-template <int D, bool BF16>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedJoint joint, const PagedRow pr, int dim,
-                                          float m2, float l, float4v x) {
-  if (joint.out) {
-    const int64_t row = joint_row(a, pr);
-    *(float4v*)(a.joint_o + row * D + dim) = x;
-    if (dim == 0) *(v2f*)(a.joint_ml + 2 * row) = v2f{m2, l};
-    return;
-  }
-  if (joint.in) {
-    const JointState<D> j(a, pr, m2, l);
-    x = j.x(dim, x);
-  }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  half4 y;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = Elem<BF16>::round(x[e] * inv);
-  *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
-  if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
-}
-
 // Folds up to BATCH partials, step apart from i0 among count, into (m, l, x): all their
 // loads are in flight together.  `load` gives a record's (max, sum) and 4 dimensions.
 template <int BATCH, class LoadML, class LoadO>
@@ -350,6 +287,90 @@ __device__ __forceinline__ void fold_partials(int i0, int step, int count, float
     x += w * o[u];
   }
   m = m_new;
+}
+
+// ---- states over shared prefixes ---------------------------------------------------
+
+// Rows of a prefix's unit (fa_paged_chunk.h), and where a record of their states keeps them: in
+// the order its waves' registers hold them.  Group 4 mt + g of a wave: dimensions 32 mt + 8 g +
+// 4 (lane / 32) .. + 3 of its row lane % 32.
+constexpr int kChunkRows = 128;
+template <int D>
+__device__ __forceinline__ int64_t record_o(int64_t record, int wave, int group, int lane) {  // in floats
+  return (((record * 4 + wave) * (D / 8) + group) * 64 + lane) * 4;
+}
+__device__ __forceinline__ int64_t record_ml(int64_t record, int row) { return (record * kChunkRows + row) * 2; }
+
+// The records of one KV head's rows of a sequence over its prefix: `pieces` of them (0: it has
+// none), `step` apart, from rec0 for the prefix's first block of rows.
+struct PagedJoint {
+  int pieces, rec0, step, t0, n, head0;
+};
+template <int STAGE>
+__device__ __forceinline__ PagedJoint joint_of(const PagedArgs& a, int b, int hkv) {
+  PagedJoint j = {0, 0, 0, 0, 0, 0};
+  if constexpr (STAGE == kOwn) {
+    int g = 0;
+    if (a.groups != nullptr) {  // the last that begins at b or before
+      const int lane = threadIdx.x & 63;
+      for (int g0 = 0; g0 <= a.prefixes; g0 += 64) {
+        const bool starts = g0 + lane <= a.prefixes && a.groups[min(g0 + lane, a.prefixes)] <= b;
+        g += __builtin_popcountll(__builtin_amdgcn_ballot_w64(starts));
+      }
+      --g;
+    }
+    if (g >= 0 && g < a.prefixes) {
+      const int32_t* const info = a.joint_info + 4 * g;
+      const int start = load_scalar(info);
+      j.pieces = load_scalar(info + 1);
+      j.t0 = load_scalar(info + 2);
+      j.n = load_scalar(info + 3);
+      const int blocks = (int)((unsigned)(j.n * a.group + kChunkRows - 1) / kChunkRows);
+      j.rec0 = ((start + (hkv >> a.class_shift) * blocks) << a.class_shift) + (hkv & (a.classes - 1));
+      j.step = (a.heads * blocks) << a.class_shift;
+      j.head0 = hkv * a.group;
+    }
+  }
+  return j;
+}
+// A row's own state (m, l, x) joined with those over its prefix's pieces: with M the largest of
+// their maxima l = sum 2^(m_i - M) l_i, x likewise; all in 32 bits, one rounding to the 16-bit type
+// behind it.
+struct JointRow {
+  int pieces;  // 0: none (also of a row that is not the prefix's, where cu_seqlens falls)
+  int row;
+  int64_t record;
+  __device__ __forceinline__ JointRow(const PagedArgs& a, const PagedJoint& j, const PagedRow pr) {
+    pieces = j.pieces;
+    const int i = pr.token - j.t0;
+    const int r = i * a.group + pr.head - j.head0;
+    row = r & (kChunkRows - 1);
+    record = j.rec0 + ((int64_t)(r / kChunkRows) << a.class_shift);
+    if ((unsigned)i >= (unsigned)j.n || record < 0 || record + (int64_t)(pieces - 1) * j.step >= a.joint_records)
+      pieces = 0;
+  }
+};
+
+// O and LSE of a row from its merged state, 4 dimensions.
+template <int D, bool BF16>
+__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int dim,
+                                          float m2, float l, float4v x) {
+  if (joint.pieces > 0) {
+    const JointRow j(a, joint, pr);
+    const float* const o = a.joint_o + record_o<D>(j.record, j.row >> 5, dim >> 3, (dim & 4) * 8 + (j.row & 31));
+    const float* const ml = a.joint_ml + record_ml(j.record, j.row);
+    for (int i = 0; i < j.pieces; i += 8)
+      fold_partials<8>(
+          i, 1, j.pieces, m2, l, x,
+          [&](int i) { return *(const v2f*)(ml + record_ml((int64_t)i * joint.step, 0)); },
+          [&](int i) { return *(const float4v*)(o + record_o<D>((int64_t)i * joint.step, 0, 0, 0)); });
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  half4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = Elem<BF16>::round(x[e] * inv);
+  *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
+  if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
 }
 
 // Waits until at most N of the wave's vector loads and stores are in flight (they

@@ -118,14 +118,15 @@ def test_prefix_too_many_units(lib):
 
 
 def test_prefix_workspace(lib):
-    """The rows' states at least; without them the call is refused, before it asks the device anything."""
+    """The rows' states at least (a record of 128 rows for each of the 512 workgroups that a device runs at
+    once); without them the call is refused, before it asks the device anything."""
     p, x = params(cache()), prefix()
-    states = 2 * 4 * (64 + 2) * 4
+    states = 512 * 128 * (64 + 2) * 4 + 16
     size = lib.fa_sm75_paged_prefix_workspace_size(ctypes.byref(p), ctypes.byref(x))
     assert size >= states and size % 16 == 0
     for kw in (dict(), dict(workspace=0x1000, workspace_bytes=states - 1)):
         assert lib.fa_sm75_paged_prefix_forward(ctypes.byref(params(cache(), **kw)), ctypes.byref(x)) == 1
-        assert b"must hold 2112 bytes at least" in lib.fa_sm75_last_error()
+        assert b"bytes at least, got" in lib.fa_sm75_last_error()
     assert lib.fa_sm75_paged_prefix_forward(ctypes.byref(p), None) == 1
     assert lib.fa_sm75_paged_prefix_forward(None, ctypes.byref(x)) == 1
     none = prefix(count=0, cu_prefix=0x1000)  # no prefix: what the plain call uses
