@@ -27,6 +27,7 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
   return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
 }
 constexpr int64_t kLastCacheBytes = 256 << 20;
+constexpr int kOwnShort = 1536;
 constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 16 bytes
 }  // namespace
 
@@ -94,6 +95,13 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   p.units = (int)(a.hkv / p.classes * blocks);
   // (Of very many units a workgroup each is balanced enough.)
   p.split = p.wgs > 0 && p.units <= 16 * resident / p.classes && fits_line(a, p.units, kPTile, kPAhead);
+  // Behind a shared prefix the own keys are often few: cutting them costs more than it
+  // balances where no sequence has more than a stretch's least, or where units nearly fill the
+  // GPU and are short (us of the launch, cut and not: 64 sequences of 64 to 256 keys, 8 heads d128 17.4 /
+  // 11.0, of 128 to 1024 34.7 / 30.8, 48 of 100 to 1500 8 bits 24.8 / 22.4; of 512 to 4096 95 / 111).
+  const int64_t longest = (int64_t)a.max_pages << a.page_shift;
+  if (a.stage == kOwn && (longest <= kPTile * kPMinTiles || (longest <= kOwnShort && p.units >= p.wgs - p.wgs / 4)))
+    p.split = false;
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) + kCombineWord : 0;

@@ -435,26 +435,65 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
       }
     }
     __syncthreads();
-    // Thread: 4 dimensions of one column, columns in turns.
-    for (int it = tid; it < R * (D / 4); it += kThreads) {
-      const int c = it / (D / 4), ch = it - c * (D / 4), dim = 4 * ch;
-      const int r = rb * R + c;
-      if (r >= nrows) continue;
-      float mw[4], m = -__builtin_inff(), l = 0.0f;
+    // The waves' states of 4 dimensions of a column, merged.
+    auto merged = [&](int c, int ch, float& m2, float& l, float4v& x) {
+      float mw[4], m = -__builtin_inff();
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         mw[w] = ml_lds[w][0][c];
         m = fmaxf(m, mw[w]);
       }
       const float m_use = m == -__builtin_inff() ? 0.0f : m;
-      float4v x = (float4v)0.0f;
+      l = 0.0f;
+      x = (float4v)0.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float f = __builtin_amdgcn_exp2f((mw[w] - m_use) * c2);
         l += f * ml_lds[w][1][c];
         x += f * *o_at(w, c, ch);
       }
-      const float m2 = m == -__builtin_inff() ? m : m * c2;
+      m2 = m == -__builtin_inff() ? m : m * c2;
+    };
+    if constexpr (STAGE == kOwn) {
+      // Few rows leave threads without a column: those take every groups-th piece of the
+      // prefix each (64 tokens of 4 rows behind 32 pieces: %%%).
+      const int items = min(R, nrows - rb * R) * (D / 4);
+      const int groups = min(kThreads / items, joint.pieces);
+      if (whole && groups > 1) {
+        const int grp = tid / items, c = (tid - grp * items) / (D / 4), ch = (tid - grp * items) % (D / 4);
+        float m = -__builtin_inff(), l = 0.0f;
+        float4v x = (float4v)0.0f;
+        if (grp == 0) merged(c, ch, m, l, x);
+        if (grp < groups) fold_joint<D, 16>(a, joint, row_of(c), 4 * ch, grp, groups, m, l, x);
+        __syncthreads();
+        float4v* const xo = (float4v*)v_lds0;
+        float* const xm = (float*)(v_lds0 + 8 * kThreads);  // max, then sum
+        xo[tid] = x;
+        xm[tid] = m;
+        xm[kThreads + tid] = l;
+        __syncthreads();
+        if (tid < items) {
+          for (int g = 1; g < groups; ++g) m = fmaxf(m, xm[g * items + tid]);
+          l = 0.0f;
+          x = (float4v)0.0f;
+          for (int g = 0; g < groups; ++g) {
+            const float w = __builtin_amdgcn_exp2f(xm[g * items + tid] - over_zero(m));
+            l += w * xm[kThreads + g * items + tid];
+            x += w * xo[g * items + tid];
+          }
+          finish_row<BF16>(a, row_of(c), 4 * ch, m, l, x);
+        }
+        __syncthreads();  // the next unit's loads go into these tiles
+        continue;
+      }
+    }
+    // Thread: 4 dimensions of one column, columns in turns.
+    for (int it = tid; it < R * (D / 4); it += kThreads) {
+      const int c = it / (D / 4), ch = it - c * (D / 4), dim = 4 * ch;
+      if (rb * R + c >= nrows) continue;
+      float m2, l;
+      float4v x;
+      merged(c, ch, m2, l, x);
       if (whole) {
         store_row<D, BF16>(a, joint, row_of(c), dim, m2, l, x);
       } else {

@@ -239,8 +239,10 @@ __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const Page
 // the class, block of rows): units of a prefix with T tiles are cut into ceil(T / q) pieces of
 // equal length, q the smallest (found in steps of an eighth) with which the class's workgroups
 // have an item each at most; where the units are more than those, none is cut.  A piece's record is its
-// item's, and the second launch adds the pieces up where it stores a row, so there is no merge (64
-// tokens behind a prefix of 8192, 32 over 8 heads d128: %%%).
+// item's, and the second launch adds the pieces up where it stores a row, so there is no merge.  There
+// each piece costs about as much as half a tile does here, so that pieces of the longest prefix are no
+// shorter than sqrt(T / 2) (us of both launches with 2, 4, 6, 8, 12 tiles: 64 tokens of 32 over 8 heads
+// d128 behind 128 tiles 65.1, 66.7, 62.5, 60.0, 62.1, 4 of 14 over 2 d64 behind 16 tiles 21.6, 20.1, 24.5, 26.0, 26.2).
 constexpr int kPrefixMinTiles = 4;
 struct PrefixLine {
   const PagedArgs& a;
@@ -248,6 +250,7 @@ struct PrefixLine {
   PagedSeq own;  // prefix `lane`
   __device__ __forceinline__ PrefixLine(const PagedArgs& args, int ln) : a(args), lane(ln) {
     own = look(lane);
+    int longest = 0;
     float units = 0.0f, tiles = 0.0f;  // (where cu_prefix falls again and again they may pass 2^31)
     for (int g0 = 0; g0 < a.batch; g0 += 64) {
       const PagedSeq s = g0 == 0 ? own : look(g0 + lane);
@@ -259,10 +262,11 @@ struct PrefixLine {
       }
       units += n;
       tiles += t;
+      longest = max(longest, wave_max(n > 0.0f ? tiles_of(s) : 0));
     }
     q = INT32_MAX;
     if (units >= (float)a.wgs) return;
-    q = max(kPrefixMinTiles, (int)(tiles / (float)a.wgs));
+    q = max(max(kPrefixMinTiles, (int)ceilf(sqrtf(0.5f * (float)longest))), (int)(tiles / (float)a.wgs));
     while (total() > a.wgs) q += (q + 7) / 8;  // (ends: with the longest prefix's tiles there are `units`)
     q = uniform(q);
   }

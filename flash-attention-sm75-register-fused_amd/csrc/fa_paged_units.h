@@ -351,26 +351,36 @@ struct JointRow {
   }
 };
 
-// O and LSE of a row from its merged state, 4 dimensions.
-template <int D, bool BF16>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int dim,
-                                          float m2, float l, float4v x) {
-  if (joint.pieces > 0) {
-    const JointRow j(a, joint, pr);
-    const float* const o = a.joint_o + record_o<D>(j.record, j.row >> 5, dim >> 3, (dim & 4) * 8 + (j.row & 31));
-    const float* const ml = a.joint_ml + record_ml(j.record, j.row);
-    for (int i = 0; i < j.pieces; i += 8)
-      fold_partials<8>(
-          i, 1, j.pieces, m2, l, x,
-          [&](int i) { return *(const v2f*)(ml + record_ml((int64_t)i * joint.step, 0)); },
-          [&](int i) { return *(const float4v*)(o + record_o<D>((int64_t)i * joint.step, 0, 0, 0)); });
-  }
+// Folds pieces first, first + step, .. of a row's states over its prefix into (m, l, x), 4
+// dimensions, BATCH of them asked for at once.
+template <int D, int BATCH>
+__device__ __forceinline__ void fold_joint(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int dim,
+                                           int first, int step, float& m, float& l, float4v& x) {
+  const JointRow j(a, joint, pr);
+  const float* const o = a.joint_o + record_o<D>(j.record, j.row >> 5, dim >> 3, (dim & 4) * 8 + (j.row & 31));
+  const float* const ml = a.joint_ml + record_ml(j.record, j.row);
+  for (int i = first; i < j.pieces; i += BATCH * step)
+    fold_partials<BATCH>(
+        i, step, j.pieces, m, l, x, [&](int i) { return *(const v2f*)(ml + record_ml((int64_t)i * joint.step, 0)); },
+        [&](int i) { return *(const float4v*)(o + record_o<D>((int64_t)i * joint.step, 0, 0, 0)); });
+}
+
+// O and LSE of a row from its state, 4 dimensions.
+template <bool BF16>
+__device__ __forceinline__ void finish_row(const PagedArgs& a, const PagedRow pr, int dim, float m2, float l, float4v x) {
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   half4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = Elem<BF16>::round(x[e] * inv);
   *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
   if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+}
+// The same from that over its own keys, 4 dimensions.
+template <int D, bool BF16>
+__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int dim,
+                                          float m2, float l, float4v x) {
+  if (joint.pieces > 0) fold_joint<D, 8>(a, joint, pr, dim, 0, 1, m2, l, x);
+  finish_row<BF16>(a, pr, dim, m2, l, x);
 }
 
 // Waits until at most N of the wave's vector loads and stores are in flight (they
