@@ -24,7 +24,8 @@
 namespace fa {
 namespace {
 
-constexpr int kWTile = 32;  // keys of a wave's step: two 16-key pieces, each in one page
+constexpr int kWTile = 32;    // keys of a wave's step: two 16-key pieces, each in one page
+constexpr int kWBlock = 256;  // keys of a unit of the kernel for more rows
 
 // A row's log-sum-exp in log2 units.  -inf (a row that saw no key) as +inf: it gives
 // every key 2^-inf = 0.
@@ -32,12 +33,74 @@ __device__ __forceinline__ float weigh_lse2(float lse) {
   return lse == -__builtin_inff() ? __builtin_inff() : lse * 1.4426950408889634f;
 }
 
-// A wave takes `run` tiles of one (sequence, KV head): K goes to registers, the next
-// tile's under the current one's work.  Runs are dealt by their place in the sequence,
-// those of all sequences and heads before the next, so that what lies behind the shorter
-// sequences' ends is dealt last.
+// The steps of STEP keys that hold keys some row sees, up to max_len: of every sequence, those of its
+// KV heads.  And the blocks of 256 positions behind them.  Called by whole waves.
+template <int STEP>
+struct WeighLine {
+  const WeighArgs& w;
+  int lane;
+  PagedSeq own;  // sequence `lane`
+  __device__ __forceinline__ WeighLine(const WeighArgs& args, int ln) : w(args), lane(ln) { own = look(ln); }
+  __device__ __forceinline__ PagedSeq look(int b) const {
+    PagedSeq s = paged_seq(w.p, min(b, w.p.batch - 1), [](const int32_t* p) { return *p; });
+    if (b >= w.p.batch) s.n = 0;
+    return s;
+  }
+  __device__ __forceinline__ int steps(const PagedSeq& s) const {  // for each KV head
+    return s.n > 0 ? (int)((unsigned)(min(s.keys, w.max_len) + STEP - 1) / STEP) : 0;
+  }
+  __device__ __forceinline__ int empty(const PagedSeq& s) const {
+    return (int)((unsigned)(max(0, w.max_len - STEP * steps(s)) + kWBlock - 1) / kWBlock);
+  }
+  // Those of sequences b0 .. b0 + lane.
+  __device__ __forceinline__ int prefix(int b0, bool behind) const {
+    const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
+    return wave_prefix((b0 + lane < w.p.batch ? behind ? empty(s) : steps(s) : 0) * w.p.hkv);
+  }
+  __device__ __forceinline__ int total(bool behind) const {
+    int sum = 0;
+    for (int b0 = 0; b0 < w.p.batch; b0 += 64) sum += wave_bcast(prefix(b0, behind), 63);
+    return uniform(sum);
+  }
+  // The most rows of a sequence, in tiles of R.
+  template <int R>
+  __device__ __forceinline__ int row_tiles() const {
+    int most = 0;
+    for (int b0 = 0; b0 < w.p.batch; b0 += 64) {
+      const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
+      most = max(most, wave_max((int)((unsigned)(s.n * w.p.group + R - 1) / R)));
+    }
+    return most;
+  }
+  // The sequence of number `at` (below the total), which becomes its number in the sequence.
+  __device__ __forceinline__ int find(int& at, bool behind) const {
+    for (int b0 = 0;; b0 += 64) {
+      const int x = prefix(b0, behind);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(x > at);
+      if (past != 0 || b0 + 64 >= w.p.batch) {
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        if (l > 0) at -= wave_bcast(x, l - 1);
+        return uniform(min(b0 + l, w.p.batch - 1));
+      }
+      at -= wave_bcast(x, 63);
+    }
+  }
+  // Zeros into block number `at` of those behind the keys, `threads` threads.
+  __device__ __forceinline__ void clear(int at, int thread, int threads) const {
+    const int b = find(at, true);
+    const int block = (int)((unsigned)at / (unsigned)w.p.hkv), h = at - block * w.p.hkv;
+    const int j0 = STEP * steps(scalar_seq(w.p, b)) + block * kWBlock;
+    float* const out = w.out + b * w.sb + h * w.sh;
+    for (int j = j0 + thread; j < min(j0 + kWBlock, w.max_len); j += threads) out[j] = 0.0f;
+  }
+};
+
+// The tiles of all (sequence, KV head) end to end are a line, of which each of `waves` waves takes an
+// equal stretch, whatever heads and sequences it covers: as many waves as run at once, or one for
+// each tile.  K goes to registers, the next tile's under the current one's work.  (Runs of 8 tiles
+// a wave, as the GPU got round to them, left a last round of half the waves: %%%.)
 template <int D, bool BF16, bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArgs w) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kernel(const WeighArgs w) {
   using E = Elem<BF16>;
   constexpr int R = 16 * NT;
   constexpr int KS = D / 32;             // contraction steps of S
@@ -47,24 +110,34 @@ __global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArg
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l16 = lane & 15;
   const int g4 = lane >> 4;
-  const int pairs = a.batch * a.hkv;
-  const unsigned item = (unsigned)blockIdx.x * kWaves + wave;
-  const int at = uniform((int)(item / (unsigned)pairs));
-  const int bh = uniform((int)(item - (unsigned)at * pairs));
-  const int tiles = (int)((unsigned)(w.max_len + kWTile - 1) / kWTile);
-  const int t_begin = at * w.run;
-  if (t_begin >= tiles) return;
-  const int b = uniform((int)((unsigned)bh / (unsigned)a.hkv));
-  const int hkv = bh - b * a.hkv;
+  const WeighLine<kWTile> line(w, lane);
+  const int total = line.total(false);
+  const int wv = uniform((int)blockIdx.x * kWaves + wave);
+  const int waves = min(w.waves, total);
+  if (wv >= waves) {  // blocks behind the keys
+    if (!w.add && wv - waves < line.total(true)) line.clear(wv - waves, lane, 64);
+    return;
+  }
+  int pos = (int)((int64_t)total * wv / waves);
+  const int end = uniform((int)((int64_t)total * (wv + 1) / waves));
+
+  while (pos < end) {
+  int at = pos;
+  const int b = line.find(at, false);
   const PagedSeq s = scalar_seq(a, b);
-  const int t_end = min(t_begin + w.run, tiles);
+  const int tiles = uniform(line.steps(s));
+  if (tiles == 0) return;  // (the lengths changed meanwhile)
+  const int hkv = uniform((int)((unsigned)at / (unsigned)tiles));
+  const int t_begin = uniform(at - hkv * tiles);
+  const int t_stop = uniform(min(tiles, t_begin + end - pos));
+  pos = uniform(pos + t_stop - t_begin);
+  if (hkv >= a.hkv) return;
 
   // Keys some row sees end at `sees`; those before `full` every row sees.
   const int nrows = s.n * a.group;
   const int past = s.len - s.n;  // tokens before the new ones
   const int sees = s.n > 0 ? uniform(min(s.keys, w.max_len)) : 0;
   const int full = a.causal ? uniform(clamp_int(past + 1, 0, sees)) : sees;
-  const int t_stop = uniform(clamp_int((sees + kWTile - 1) / kWTile, t_begin, t_end));
   float* const out = w.out + b * w.sb + hkv * w.sh;
   const float c2 = a.negate_q ? -a.c : a.c;
 
@@ -200,8 +273,6 @@ __global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArg
     }
     if (t < t_stop) step(t, xa);
   }
-  if (!w.add) {
-    for (int j = t_stop * kWTile + lane; j < min(t_end * kWTile, w.max_len); j += 64) out[j] = 0.0f;
   }
 }
 
@@ -212,59 +283,9 @@ __global__ void __launch_bounds__(kThreads) fa_paged_weigh_kernel(const WeighArg
 // each row's -lse log2 e beside it).  Where units are few, each one's row tiles go to `parts`
 // workgroups in turns (under the causal rule every part then has as many that see the keys), and the last
 // of them to finish adds the parts up in their order.
-constexpr int kWBlock = 256;    // keys of a unit
 constexpr int kWRows = 32;      // rows of a tile
 constexpr int kWTarget = 1024;  // workgroups that units are cut into, where they are fewer
 constexpr int kWMinTiles = 8;   // tiles a part has at least
-
-// The units that hold keys and rows: of every sequence its blocks of keys up to max_len, for
-// each KV head (heads next to each other, so that those of one head meet in one XCD's L2 where
-// the heads divide over the XCDs).  Called by whole waves.
-struct WeighLine {
-  const WeighArgs& w;
-  int lane;
-  PagedSeq own;  // sequence `lane`
-  __device__ __forceinline__ WeighLine(const WeighArgs& args, int ln) : w(args), lane(ln) { own = look(ln); }
-  __device__ __forceinline__ PagedSeq look(int b) const {
-    PagedSeq s = paged_seq(w.p, min(b, w.p.batch - 1), [](const int32_t* p) { return *p; });
-    if (b >= w.p.batch) s.n = s.keys = 0;
-    return s;
-  }
-  __device__ __forceinline__ int blocks(const PagedSeq& s) const {
-    return s.n > 0 ? (int)((unsigned)(min(s.keys, w.max_len) + kWBlock - 1) / kWBlock) : 0;
-  }
-  __device__ __forceinline__ int every() const { return (int)((unsigned)(w.max_len + kWBlock - 1) / kWBlock); }
-  // Units of sequences b0 + lane (empty: of the blocks behind their keys), summed up to the lane.
-  __device__ __forceinline__ int prefix(int b0, bool empty) const {
-    const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
-    const int n = blocks(s);
-    return wave_prefix((b0 + lane < w.p.batch ? empty ? every() - n : n : 0) * w.p.hkv);
-  }
-  // All units, and the most row tiles of a sequence.
-  __device__ __forceinline__ int total(int& tiles) const {
-    int sum = 0;
-    tiles = 0;
-    for (int b0 = 0; b0 < w.p.batch; b0 += 64) {
-      sum += wave_bcast(prefix(b0, false), 63);
-      const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
-      tiles = max(tiles, wave_max((int)((unsigned)(s.n * w.p.group + kWRows - 1) / kWRows)));
-    }
-    return uniform(sum);
-  }
-  // The sequence of unit `at`, which becomes its number in the sequence.
-  __device__ __forceinline__ int find(int& at, bool empty) const {
-    for (int b0 = 0;; b0 += 64) {
-      const int x = prefix(b0, empty);
-      const uint64_t past = __builtin_amdgcn_ballot_w64(x > at);
-      if (past != 0 || b0 + 64 >= w.p.batch) {
-        const int l = past != 0 ? __builtin_ctzll(past) : 63;
-        if (l > 0) at -= wave_bcast(x, l - 1);
-        return uniform(min(b0 + l, w.p.batch - 1));
-      }
-      at -= wave_bcast(x, 63);
-    }
-  }
-};
 
 template <int D, bool BF16, bool FP8>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const WeighArgs w) {
@@ -282,9 +303,9 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int hi = lane >> 5, l32 = lane & 31;
-  const WeighLine line(w, lane);
-  int most;
-  const int units = line.total(most);
+  const WeighLine<kWBlock> line(w, lane);  // (heads next to each other: those of one head meet in one XCD's L2)
+  const int most = line.row_tiles<kWRows>();
+  const int units = line.total(false);
   // (kWTarget over the units is cut to whole parts: at most kWTarget workgroups where there are several)
   int parts = 1;
   if (w.split && units > 0 && units < kWTarget)
@@ -292,12 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   parts = uniform(parts);
   const int wg = (int)blockIdx.x;
   if (wg >= units * parts) {  // blocks behind the keys
-    int at = wg - units * parts;
-    if (w.add || at >= line.every() * a.batch * a.hkv - units) return;
-    const int b = line.find(at, true);
-    const int block = line.blocks(scalar_seq(a, b)) + (int)((unsigned)at / (unsigned)a.hkv), h = at % a.hkv;
-    const int j = block * kWBlock + (int)threadIdx.x;
-    if (j < w.max_len) w.out[b * w.sb + h * w.sh + j] = 0.0f;
+    if (!w.add && wg - units * parts < line.total(true)) line.clear(wg - units * parts, threadIdx.x, kThreads);
     return;
   }
   const int part = (int)((unsigned)wg / (unsigned)units);

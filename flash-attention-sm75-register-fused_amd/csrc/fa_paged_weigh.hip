@@ -27,11 +27,12 @@ WeighPlan plan_weigh(const WeighArgs& a, int64_t max_query_len, int64_t workspac
     return p;
   }
   p.rows = max_query_len * a.p.group <= 16 ? 16 : 32;
-  const int64_t tiles = ((int64_t)a.max_len + kWTile - 1) / kWTile;
-  // Tiles of a wave: one where there are few, at most eight.
-  const int64_t waves = (int64_t)resident_fused_workgroups() * 8;
-  p.run = (int)std::max<int64_t>(1, std::min<int64_t>(8, tiles * pairs / waves));
-  p.grid = ((tiles + p.run - 1) / p.run * pairs + kWaves - 1) / kWaves;
+  // Waves: four a SIMD, of 32 rows three, or one for each tile there is room for; and those that
+  // clear what is behind the keys.
+  const int64_t tiles = ((int64_t)a.max_len + kWTile - 1) / kWTile * pairs;
+  const int64_t blocks = ((int64_t)a.max_len + kWBlock - 1) / kWBlock * pairs;
+  p.waves = (int)std::min<int64_t>(tiles, (int64_t)resident_fused_workgroups() * (p.rows == 16 ? 8 : 6));
+  p.grid = (p.waves + (a.add ? 0 : blocks) + kWaves - 1) / kWaves;
   return p;
 }
 
@@ -53,7 +54,7 @@ static void launch_typed(const WeighArgs& a, const WeighPlan& plan, hipStream_t 
 
 int launch_weigh(const WeighArgs& args, const WeighPlan& plan, int head_dim, void* workspace, hipStream_t stream) {
   WeighArgs a = args;
-  a.run = plan.run;
+  a.waves = plan.waves;
   a.split = plan.split ? 1 : 0;
   a.p.inv_group = 1.0f / (float)a.p.group;
   if (plan.split) {
