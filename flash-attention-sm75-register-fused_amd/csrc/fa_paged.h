@@ -131,7 +131,7 @@ struct WeighArgs {
   int max_len;
   int add;           // to what is there; else positions without a row get 0
   // Plan.
-  int run;           // few rows: 32-key tiles of a wave
+  int waves;         // few rows: most waves that share the tiles
   int split;         // more: units may be cut (with a workspace)
   float* partial;
   uint64_t* flags;
@@ -139,7 +139,7 @@ struct WeighArgs {
 };
 struct WeighPlan {
   int rows;  // rows at once: 16 or 32, 0 for the kernel of more
-  int run;
+  int waves;
   int64_t grid;
   bool split;
   int64_t workspace_bytes;
@@ -164,7 +164,11 @@ struct EvictArgs {
   float* new_weights;       // [batch, hkv, to_pages << page_shift]
   int32_t* kept;            // workspace: [batch, hkv, slots] positions of the rows that stay
   int slots;                // the most rows that can stay: min(keep, room of the table)
-  int* counts;              // workspace: a histogram for each row, digit and chunk
+  // Workspace of long rows: a histogram for each row, digit and chunk, the search behind each
+  // digit, and for each chunk what is above the first two in front of it.
+  int* counts;
+  int* states;
+  int* fronts;
   int chunks;               // workgroups of a row
 };
 int64_t evict_workspace_bytes(const EvictArgs& a);

@@ -15,7 +15,7 @@
 #include <algorithm>
 
 #include "fa_kernel_common.h"
-#include "fa_paged.h"
+#include "fa_paged_units.h"
 
 namespace fa {
 namespace {
@@ -116,23 +116,13 @@ __device__ __forceinline__ int2 across_waves(int x, int wave, int lane, int* wav
   }
   return r;
 }
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m);
-  return x;
-}
 
 // One digit on, given how many of the agreeing keys have the thread's two digits, hi and
 // hi - 1 from the top.  keep: the keys wanted, where this is the first digit.  Returns all that agree.
 __device__ __forceinline__ int descend(Search& s, int n1, int n0, int keep, int wave, int lane, SelShared& sh) {
   const int hi = kSelBins - 1 - 2 * (int)threadIdx.x;
-  int upto = n0 + n1;  // inclusive, over the wave's lanes
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    const int y = __shfl_up(upto, m);
-    if (lane >= m) upto += y;
-  }
-  const int2 sum = across_waves(__shfl(upto, 63), wave, lane, sh.waves);
+  const int upto = wave_prefix(n0 + n1);
+  const int2 sum = across_waves(wave_bcast(upto, 63), wave, lane, sh.waves);
   if (s.shift == 21) s.need = min(keep, sum.y);
   const int above = sum.x + upto - n0 - n1;
   if (above < s.need && above + n1 >= s.need) {
@@ -217,54 +207,75 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_kernel(const E
 }
 
 // Longer rows: `chunks` workgroups each, in four launches.  The first three count a digit each over
-// the chunk's keys, into a histogram of its own; each launch adds up those of the ones before it to
-// find their digits, and the last also what of the chunks in front of its own stays.
+// the chunk's keys, into a histogram of its own; the next launch adds those up to find the digit (and
+// keeps where the search is), and what of the chunks in front of its own stays by it.
+struct SelState {  // a row's search behind a digit
+  unsigned bound;
+  int need, target, search;
+};
 template <int PHASE>
 __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_long_kernel(const EvictArgs e) {
   __shared__ int bins[kSelBins];
-  __shared__ SelShared sh[3];
+  __shared__ SelShared sh;
   __shared__ int waves[3][kSelWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int pair = (int)((unsigned)blockIdx.x / (unsigned)e.chunks), chunk = (int)blockIdx.x - pair * e.chunks;
   const int slot = kSelThreads - 1 - (int)threadIdx.x;
-  int2* const hist = (int2*)e.counts + ((int64_t)pair * 3 * e.chunks) * kSelThreads + slot;
+  SelState* const states = (SelState*)e.states + (int64_t)pair * 3;
+  int* const fronts = e.fronts + (int64_t)pair * 2 * e.chunks;  // above the first two digits
   const SelRow row(e, pair);
+  const int part = (int)((unsigned)(row.keys + e.chunks * kSelBlock - 1) / (unsigned)(e.chunks * kSelBlock)) * kSelBlock;
+  const int begin = (int)min((int64_t)chunk * part, (int64_t)row.keys), end = min(row.keys, begin + part);
   Search s = {0, 0, 0, 21};
   int target = 0, above = 0, same = 0;
   bool search = true;
+  if constexpr (PHASE > 0) {
+    constexpr int p = PHASE - 1;  // the digit that was counted last
+    if constexpr (p > 0) {
+      const SelState before = states[p - 1];
+      s.bound = before.bound;
+      s.need = before.need;
+      s.shift = p == 1 ? 10 : 0;
+      s.mask = p == 1 ? 0xffe00000u : 0xfffffc00u;
+      target = before.target;
+      search = before.search != 0;
+    }
+    if (search) {
+      const int2* const hist = (const int2*)e.counts + ((int64_t)pair * 3 + p) * e.chunks * kSelThreads + slot;
+      int2 all = {0, 0}, front = {0, 0};
+      for (int c = 0; c < e.chunks; c += 8) {
+        int2 n[8];
 #pragma unroll
-  for (int p = 0; p < PHASE; ++p) {
-    int2 all = {0, 0}, front = {0, 0};
-    for (int c = 0; c < e.chunks; c += 8) {
-      int2 n[8];
+        for (int u = 0; u < 8; ++u) n[u] = c + u < e.chunks ? hist[(int64_t)(c + u) * kSelThreads] : int2{0, 0};
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        n[u] = c + u < e.chunks ? hist[((int64_t)p * e.chunks + c + u) * kSelThreads] : int2{0, 0};
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        all.x += n[u].x;
-        all.y += n[u].y;
-        front.x += c + u < chunk ? n[u].x : 0;
-        front.y += c + u < chunk ? n[u].y : 0;
+        for (int u = 0; u < 8; ++u) {
+          all.x += n[u].x;
+          all.y += n[u].y;
+          front.x += c + u < chunk ? n[u].x : 0;
+          front.y += c + u < chunk ? n[u].y : 0;
+        }
       }
+      const int total = descend(s, all.y, all.x, e.keep, wave, lane, sh);
+      if constexpr (p == 0) {
+        target = s.need;
+        search = target < total && target > 0;
+      }
+      const int at = search ? sh.found[0] : -1;
+      above = (2 * slot > at ? front.x : 0) + (2 * slot + 1 > at ? front.y : 0);
+      if constexpr (p == 2) same = 2 * slot == at ? front.x : 2 * slot + 1 == at ? front.y : 0;
+      if (search) take(s, sh);
+      above = across_waves(wave_bcast(wave_prefix(above), 63), wave, lane, waves[0]).y;
+      if constexpr (p < 2) {
+        if (threadIdx.x == 0) {
+          fronts[p * e.chunks + chunk] = above;
+          if (chunk == 0) states[p] = {s.bound, s.need, target, search};
+        }
+      }
+    } else if constexpr (p == 1) {
+      if (threadIdx.x == 0 && chunk == 0) states[1] = states[0];
     }
-    const int total = descend(s, all.y, all.x, e.keep, wave, lane, sh[p]);
-    if (p == 0) {
-      target = s.need;
-      search = target < total && target > 0;
-    }
-    if (!search) {
-      above += front.x + front.y;
-      break;
-    }
-    const int at = sh[p].found[0];
-    above += (2 * slot > at ? front.x : 0) + (2 * slot + 1 > at ? front.y : 0);
-    if (p == 2) same = 2 * slot == at ? front.x : 2 * slot + 1 == at ? front.y : 0;
-    take(s, sh[p]);
   }
-  const int part = (int)((unsigned)(row.keys + e.chunks * kSelBlock - 1) / (unsigned)(e.chunks * kSelBlock)) * kSelBlock;
-  const int begin = (int)min((int64_t)chunk * part, (int64_t)row.keys), end = min(row.keys, begin + part);
   if constexpr (PHASE < 3) {
     if (!search) return;  // (all the workgroups of the row; the histograms are not asked for)
     int2* const own = (int2*)bins + slot;
@@ -272,12 +283,18 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_long_kernel(co
     __syncthreads();
     for (int j = begin; j < end; j += kSelBlock) s.count(SelBlock(row, j, end, wave, lane), bins);
     __syncthreads();
-    hist[((int64_t)PHASE * e.chunks + chunk) * kSelThreads] = *own;
+    ((int2*)e.counts)[(((int64_t)pair * 3 + PHASE) * e.chunks + chunk) * kSelThreads + slot] = *own;
   } else {
-    // What stays in front of the chunk: above the bound, and equal to it.
-    int2 before = {across_waves(wave_sum(above), wave, lane, waves[0]).y,
-                   across_waves(wave_sum(same), wave, lane, waves[1]).y};
-    if (!search) s.need = 0;
+    // What stays in front of the chunk: above the bound, and equal to it.  (Where nothing is searched
+    // for, all that the first digit counted.)
+    int2 before = {fronts[chunk], 0};
+    if (search) {
+      before.x += fronts[e.chunks + chunk] + above;
+      before.y = across_waves(wave_bcast(wave_prefix(same), 63), wave, lane, waves[1]).y;
+    } else {
+      s.bound = 0;
+      s.need = 0;
+    }
     if (target > 0) {
       for (int j = begin; j < end; j += kSelBlock) {
         before = write_kept(row, SelBlock(row, j, end, wave, lane), s.bound, s.need, target, before.x, before.y, wave,
@@ -361,14 +378,19 @@ static int64_t kept_bytes(const EvictArgs& e) {
 }
 
 int64_t evict_workspace_bytes(const EvictArgs& e) {
-  return kept_bytes(e) + (int64_t)e.p.batch * e.p.hkv * 3 * evict_chunks(e) * kSelBins * (int64_t)sizeof(int);
+  const int64_t pairs = (int64_t)e.p.batch * e.p.hkv, chunks = evict_chunks(e);
+  if (chunks == 0) return kept_bytes(e);
+  const int64_t row = 3 * chunks * kSelBins * (int64_t)sizeof(int) + 3 * (int64_t)sizeof(SelState) + 2 * chunks * (int64_t)sizeof(int);
+  return (kept_bytes(e) + pairs * row + 15) & ~(int64_t)15;
 }
 
 int launch_evict(const EvictArgs& args, int head_dim, void* workspace, hipStream_t stream) {
   EvictArgs e = args;
+  e.chunks = evict_chunks(e);
   e.kept = static_cast<int32_t*>(workspace);
   e.counts = reinterpret_cast<int*>(static_cast<char*>(workspace) + kept_bytes(e));
-  e.chunks = evict_chunks(e);
+  e.states = e.counts + (int64_t)e.p.batch * e.p.hkv * 3 * e.chunks * kSelBins;
+  e.fronts = e.states + (int64_t)e.p.batch * e.p.hkv * 3 * (int64_t)(sizeof(SelState) / sizeof(int));
   const int64_t pairs = (int64_t)e.p.batch * e.p.hkv;
   const dim3 threads(kSelThreads);
   if (e.chunks == 0) {
