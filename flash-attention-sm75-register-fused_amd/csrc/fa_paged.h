@@ -15,6 +15,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace fa {
 
 struct PagedArgs {
@@ -68,14 +70,16 @@ struct PagedArgs {
   int resident;     // the chunk kernel's workgroups of a class that run at once
   int pieces;       // most pieces the chunk kernel may cut a unit into, 0: any number
   int stream_v;     // the chunk kernel reads V non-temporally
+};
 
-  // Attention behind shared prefixes, in two launches (their stage a template argument of the
-  // kernels).  Of the prefixes (kPrefix): `batch` of them, table, lens and max_pages theirs,
-  // prefix g's rows those of sequences groups[g] .. groups[g + 1] - 1 of `seqs`, of all where
-  // groups is nullptr; the states of the rows over pieces of their prefix go to records of
-  // joint_o and joint_ml, where which are is in joint_info.  Of the sequences' own keys (kOwn):
-  // rows whose sequence has one of the `prefixes` join those states.
-  int stage;
+// Attention behind shared prefixes, in two launches (their stage a template argument of the
+// kernels).  Of the prefixes (kPrefix): `batch` of them, table, lens and max_pages theirs, prefix g's
+// rows those of sequences groups[g] .. groups[g + 1] - 1 of `seqs`, of all where groups is nullptr;
+// the states of the rows over pieces of their prefix go to records of joint_o and joint_ml, where
+// which are is in joint_info.  Of the sequences' own keys (kOwn): rows whose sequence has one of the
+// `prefixes` join those states.
+constexpr int kPrefix = 1, kOwn = 2;  // (0: no prefixes)
+struct PagedShared : PagedArgs {
   const int32_t* groups;
   int prefixes, seqs;
   float* joint_o;
@@ -83,7 +87,8 @@ struct PagedArgs {
   int32_t* joint_info;  // of each prefix: first item of its class's, pieces of a unit, first token, tokens
   int joint_records;
 };
-constexpr int kPrefix = 1, kOwn = 2;  // PagedArgs::stage (0: no prefixes)
+template <int STAGE>
+using StageArgs = std::conditional_t<STAGE == 0, PagedArgs, PagedShared>;
 
 // Largest key count a block table may cover, and row stride (bytes) of a cache
 // tensor: a window over 64 of its rows stays within 31 bits.
@@ -104,22 +109,25 @@ struct PagedPlan {
   bool stream_v;
   int64_t workspace_bytes;
 };
+// stage: 0 or kOwn.
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
-                     int64_t workspace_bytes);
+                     int64_t workspace_bytes, int stage = 0);
 int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_dim,
                            void* workspace, hipStream_t stream);
+int launch_paged_attention(const PagedShared& own, const PagedPlan& plan, int head_dim,
+                           void* workspace, hipStream_t stream);
 // The launch over shared prefixes (workspace_bytes: what joint_o, joint_ml and joint_info take).
-PagedPlan plan_prefix(const PagedArgs& a, int head_dim, int64_t max_queries);
+PagedPlan plan_prefix(const PagedShared& a, int head_dim, int64_t max_queries);
 // Sets the joint fields of both stages' arguments, and launches the first.
-int launch_paged_prefix(PagedArgs& prefix, PagedArgs& own, const PagedPlan& plan, int head_dim, void* workspace,
+int launch_paged_prefix(PagedShared& prefix, PagedShared& own, const PagedPlan& plan, int head_dim, void* workspace,
                         hipStream_t stream);
 // STAGE: 0, or of attention behind shared prefixes kPrefix (chunks only) or kOwn.
 template <int D, bool BF16, bool FP8, int STAGE>
-void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream);
+void launch_paged_attn(const StageArgs<STAGE>& a, int rows, int64_t grid, hipStream_t stream);
 template <int D, bool BF16, bool FP8, int STAGE>
-void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream);
+void launch_paged_chunk(const StageArgs<STAGE>& a, int64_t grid, hipStream_t stream);
 template <int D, bool BF16, int STAGE>
-void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream);
+void launch_paged_combine(const StageArgs<STAGE>& a, int rows, int y, hipStream_t stream);
 
 // The weights that attention gave the cached rows: out[b, h, j] (+)= sum over the new tokens
 // i of sequence b that see key j, and the query heads of KV head h, of exp(scale q k - lse).
@@ -201,7 +209,7 @@ struct PagedSeq {
   int t0, n, len, keys;
 };
 template <int STAGE = 0, class Load>
-__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load load) {
+__device__ __forceinline__ PagedSeq paged_seq(const StageArgs<STAGE>& a, int b, Load load) {
   PagedSeq s;
   const int len = load(a.lens + b);  // (all loads together)
   if constexpr (STAGE == kPrefix) {  // a prefix: the rows of its sequences
@@ -232,7 +240,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, Load lo
 }
 // (b the same in every lane; all of it in scalar registers)
 template <int STAGE = 0>
-__device__ __forceinline__ PagedSeq scalar_seq(const PagedArgs& a, int b) {
+__device__ __forceinline__ PagedSeq scalar_seq(const StageArgs<STAGE>& a, int b) {
   const PagedSeq s = paged_seq<STAGE>(a, uniform(b), load_scalar);
   return {uniform(s.t0), uniform(s.n), uniform(s.len), uniform(s.keys)};
 }

@@ -10,12 +10,12 @@
 namespace fa {
 
 // The instances of fa_paged_d*.hip.
-#define FA_PAGED_EXTERN(D, BF, F8)                                                                   \
-  extern template void launch_paged_attn<D, BF, F8, 0>(const PagedArgs&, int, int64_t, hipStream_t);    \
-  extern template void launch_paged_attn<D, BF, F8, kOwn>(const PagedArgs&, int, int64_t, hipStream_t); \
-  extern template void launch_paged_chunk<D, BF, F8, 0>(const PagedArgs&, int64_t, hipStream_t);        \
-  extern template void launch_paged_chunk<D, BF, F8, kPrefix>(const PagedArgs&, int64_t, hipStream_t);  \
-  extern template void launch_paged_chunk<D, BF, F8, kOwn>(const PagedArgs&, int64_t, hipStream_t);
+#define FA_PAGED_EXTERN(D, BF, F8)                                                                     \
+  extern template void launch_paged_attn<D, BF, F8, 0>(const PagedArgs&, int, int64_t, hipStream_t);      \
+  extern template void launch_paged_attn<D, BF, F8, kOwn>(const PagedShared&, int, int64_t, hipStream_t); \
+  extern template void launch_paged_chunk<D, BF, F8, 0>(const PagedArgs&, int64_t, hipStream_t);          \
+  extern template void launch_paged_chunk<D, BF, F8, kPrefix>(const PagedShared&, int64_t, hipStream_t);  \
+  extern template void launch_paged_chunk<D, BF, F8, kOwn>(const PagedShared&, int64_t, hipStream_t);
 FA_PAGED_EXTERN(64, false, false) FA_PAGED_EXTERN(64, true, false)
 FA_PAGED_EXTERN(64, false, true) FA_PAGED_EXTERN(64, true, true)
 FA_PAGED_EXTERN(128, false, false) FA_PAGED_EXTERN(128, true, false)
@@ -75,7 +75,7 @@ static PagedPlan plan_chunks(const PagedArgs& a, int head_dim, int64_t max_query
 }
 
 PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
-                     int64_t workspace_bytes) {
+                     int64_t workspace_bytes, int stage) {
   if (max_query_len * a.group > 32) return plan_chunks(a, head_dim, max_query_len, workspace_bytes);
   PagedPlan p{};
   p.rows = max_query_len * a.group <= 16 ? 16 : 32;
@@ -100,7 +100,7 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   // GPU and are short (us of the launch, cut and not: 64 sequences of 64 to 256 keys, 8 heads d128 17.4 /
   // 11.0, of 128 to 1024 34.7 / 30.8, 48 of 100 to 1500 8 bits 24.8 / 22.4; of 512 to 4096 95 / 111).
   const int64_t longest = (int64_t)a.max_pages << a.page_shift;
-  if (a.stage == kOwn && (longest <= kPTile * kPMinTiles || (longest <= kOwnShort && p.units >= p.wgs - p.wgs / 4)))
+  if (stage == kOwn && (longest <= kPTile * kPMinTiles || (longest <= kOwnShort && p.units >= p.wgs - p.wgs / 4)))
     p.split = false;
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
@@ -114,7 +114,7 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   return p;
 }
 
-PagedPlan plan_prefix(const PagedArgs& a, int head_dim, int64_t max_queries) {
+PagedPlan plan_prefix(const PagedShared& a, int head_dim, int64_t max_queries) {
   PagedPlan p{};
   p.chunk = p.split = true;
   p.rows = kChunkRows;
@@ -128,7 +128,7 @@ PagedPlan plan_prefix(const PagedArgs& a, int head_dim, int64_t max_queries) {
 }
 
 template <int D, bool BF16, int STAGE>
-void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t stream) {
+void launch_paged_combine(const StageArgs<STAGE>& a, int rows, int y, hipStream_t stream) {
   if (rows == kChunkRows) {
     hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16, STAGE>),
                        dim3((unsigned)(a.wgs * a.classes), kChunkCombineY), dim3(kThreads), 0, stream, a);
@@ -142,7 +142,7 @@ void launch_paged_combine(const PagedArgs& a, int rows, int y, hipStream_t strea
 }
 
 template <int D, bool BF16, bool FP8, int STAGE>
-static void launch_planned(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
+static void launch_planned(const StageArgs<STAGE>& a, const PagedPlan& plan, hipStream_t stream) {
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
   if constexpr (STAGE == kPrefix) {
     launch_paged_chunk<D, BF16, FP8, STAGE>(a, grid, stream);
@@ -155,7 +155,7 @@ static void launch_planned(const PagedArgs& a, const PagedPlan& plan, hipStream_
   if (plan.combine) launch_paged_combine<D, BF16, STAGE>(a, plan.rows, plan.y, stream);
 }
 template <int D, int STAGE>
-static void launch_typed(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
+static void launch_typed(const StageArgs<STAGE>& a, const PagedPlan& plan, hipStream_t stream) {
   if (a.ks != nullptr) {
     if (a.bf16) launch_planned<D, true, true, STAGE>(a, plan, stream);
     else launch_planned<D, false, true, STAGE>(a, plan, stream);
@@ -181,12 +181,12 @@ static void set_plan(PagedArgs& a, const PagedPlan& plan) {
 }
 
 template <int STAGE>
-static void launch_sized(const PagedArgs& a, const PagedPlan& plan, int head_dim, hipStream_t stream) {
+static void launch_sized(const StageArgs<STAGE>& a, const PagedPlan& plan, int head_dim, hipStream_t stream) {
   if (head_dim == 64) launch_typed<64, STAGE>(a, plan, stream);
   else launch_typed<128, STAGE>(a, plan, stream);
 }
 
-int launch_paged_prefix(PagedArgs& prefix, PagedArgs& own, const PagedPlan& plan, int head_dim, void* workspace,
+int launch_paged_prefix(PagedShared& prefix, PagedShared& own, const PagedPlan& plan, int head_dim, void* workspace,
                         hipStream_t stream) {
   set_plan(prefix, plan);
   const int64_t records = (int64_t)plan.wgs * plan.classes;
@@ -198,9 +198,10 @@ int launch_paged_prefix(PagedArgs& prefix, PagedArgs& own, const PagedPlan& plan
   return 0;
 }
 
-int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int head_dim,
-                           void* workspace, hipStream_t stream) {
-  PagedArgs a = args;
+template <int STAGE>
+static void launch_attention(const StageArgs<STAGE>& args, const PagedPlan& plan, int head_dim, void* workspace,
+                             hipStream_t stream) {
+  StageArgs<STAGE> a = args;
   set_plan(a, plan);
   const int64_t grid = (int64_t)plan.wgs * plan.classes;
   if (plan.split) {
@@ -209,8 +210,17 @@ int launch_paged_attention(const PagedArgs& args, const PagedPlan& plan, int hea
     a.flags = reinterpret_cast<uint64_t*>(a.part_ml + 2 * grid * plan.rows * 2);
     a.mark = merge_mark(a.flags, 2 * grid + 1, stream);
   }
-  if (a.stage == kOwn) launch_sized<kOwn>(a, plan, head_dim, stream);
-  else launch_sized<0>(a, plan, head_dim, stream);
+  launch_sized<STAGE>(a, plan, head_dim, stream);
+}
+
+int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_dim,
+                           void* workspace, hipStream_t stream) {
+  launch_attention<0>(a, plan, head_dim, workspace, stream);
+  return 0;
+}
+int launch_paged_attention(const PagedShared& own, const PagedPlan& plan, int head_dim,
+                           void* workspace, hipStream_t stream) {
+  launch_attention<kOwn>(own, plan, head_dim, workspace, stream);
   return 0;
 }
 

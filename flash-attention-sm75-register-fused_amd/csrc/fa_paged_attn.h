@@ -87,7 +87,7 @@ __device__ __forceinline__ PagedStretch<kPMinTiles> paged_stretch(const PagedArg
 
 // STAGE: 0, or kOwn behind shared prefixes.
 template <int D, bool BF16, bool FP8, int NT, int STAGE>
-__global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageArgs<STAGE> a) {
   using E = Elem<BF16>;
   constexpr int R = 16 * NT;
   constexpr int KS = D / 32;  // contraction steps of S^T
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
     // key it sees.
     const int nrows = s.n * a.group;
     const PagedRows row_of(a, s, hkv, rb * R);
-    const PagedJoint joint = joint_of<STAGE>(a, b, hkv);
+    const auto joint = joint_of(a, b, hkv);
     const int past = s.len - s.n;  // tokens before the new ones
     int last[NT];
     half8 qf[NT][KS];
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const PagedA
 // The four waves take every fourth piece, D / 4 lanes each piece's row (with
 // several pieces at once where D / 4 < 64 lanes), and meet in LDS.
 template <int D, bool BF16, int NT, int STAGE>
-__global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const StageArgs<STAGE> a) {
   constexpr int R = 16 * NT;
   constexpr int LR = D / 4;               // lanes of a row
   constexpr int GROUPS = kThreads / LR;   // pieces at once
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
   const int hc = unit / blocks;
   const int rb = unit - hc * blocks;
   const int hkv = hc * a.classes + cls;
-  const PagedJoint joint = joint_of<STAGE>(a, b, hkv);
+  const auto joint = joint_of(a, b, hkv);
   const int nr = min(R, s.n * a.group - rb * R);
   if (paged_merges_itself(pieces.count, nr, D)) return;
   const int grp = (int)threadIdx.x / LR, ch = (int)threadIdx.x % LR;
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const PagedA
 }  // namespace
 
 template <int D, bool BF16, bool FP8, int STAGE>
-void launch_paged_attn(const PagedArgs& a, int rows, int64_t grid, hipStream_t stream) {
+void launch_paged_attn(const StageArgs<STAGE>& a, int rows, int64_t grid, hipStream_t stream) {
   if (rows == 16)
     hipLaunchKernelGGL((fa_paged_attn_kernel<D, BF16, FP8, 1, STAGE>), dim3((unsigned)grid), dim3(kThreads), 0,
                        stream, a);

@@ -160,7 +160,7 @@ int make_forward(const fa_paged_params* p, fa::PagedArgs* a, bool* empty) {
 }
 
 // Checks the prefixes of a forward call and fills both stages' arguments from its own ones.
-int make_prefix(const fa_paged_prefix* x, const fa::PagedArgs& a, fa::PagedArgs* prefix, fa::PagedArgs* own) {
+int make_prefix(const fa_paged_prefix* x, const fa::PagedArgs& a, fa::PagedShared* prefix, fa::PagedShared* own) {
   if (x == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "prefix must not be NULL");
   if (x->count < 0 || x->max_pages < 0 || x->block_table_stride < 0 || x->max_queries < 0)
     return capi_fail(FA_ERR_INVALID_ARGUMENT, "the prefixes' sizes and strides must be non-negative");
@@ -175,13 +175,11 @@ int make_prefix(const fa_paged_prefix* x, const fa::PagedArgs& a, fa::PagedArgs*
     return capi_fail(FA_ERR_MISALIGNED, "the prefixes' block_table, lens and cu_prefix must be 4-byte aligned");
   if ((int64_t)a.tokens * a.hq + x->count * a.hkv * 32 > (1 << 27))
     return capi_fail(FA_ERR_TOO_LARGE, "tokens * heads_q + 32 * prefixes * heads_kv exceeds 2^27");
-  *own = a;
+  *own = fa::PagedShared{a};
   own->groups = x->cu_prefix;
   own->prefixes = (int)x->count;
   own->seqs = a.batch;
-  own->stage = x->count > 0 ? fa::kOwn : 0;
   *prefix = *own;
-  prefix->stage = fa::kPrefix;
   prefix->batch = (int)x->count;
   prefix->table = x->block_table;
   prefix->lens = x->lens;
@@ -381,36 +379,36 @@ int fa_sm75_paged_forward(const fa_paged_params* p) {
 
 int64_t fa_sm75_paged_prefix_workspace_size(const fa_paged_params* p, const fa_paged_prefix* x) {
   const fa::SavedError keep;  // a size is no error report
-  fa::PagedArgs a, prefix, own;
+  fa::PagedArgs a;
+  fa::PagedShared prefix, own;
   bool empty = true;
   if (make_forward(p, &a, &empty) != FA_OK || empty || make_prefix(x, a, &prefix, &own) != FA_OK) return 0;
+  if (x->count == 0) return fa_sm75_paged_workspace_size(p);
   const int d = (int)p->cache->head_dim;
-  const int64_t rest = fa::plan_paged(own, d, longest_query(p), INT64_MAX).workspace_bytes;
-  return own.stage == 0 ? rest : fa::plan_prefix(prefix, d, longest_shared(x, a)).workspace_bytes + rest;
+  return fa::plan_prefix(prefix, d, longest_shared(x, a)).workspace_bytes +
+         fa::plan_paged(own, d, longest_query(p), INT64_MAX, fa::kOwn).workspace_bytes;
 }
 
 int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix* x) {
   fa::capi_clear_error();
-  fa::PagedArgs a, prefix, own;
+  fa::PagedArgs a;
+  fa::PagedShared prefix, own;
   bool empty = true;
   if (int st = make_forward(p, &a, &empty)) return st;
   if (empty) return FA_OK;
   if (int st = make_prefix(x, a, &prefix, &own)) return st;
+  if (x->count == 0) return fa_sm75_paged_forward(p);
   const int d = (int)p->cache->head_dim;
   const hipStream_t stream = static_cast<hipStream_t>(p->stream);
-  char* work = static_cast<char*>(p->workspace);
-  int64_t bytes = p->workspace != nullptr ? p->workspace_bytes : 0;
-  if (own.stage != 0) {
-    const fa::PagedPlan plan = fa::plan_prefix(prefix, d, longest_shared(x, a));
-    if (bytes < plan.workspace_bytes)
-      return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes at least, got %lld",
-                       (long long)plan.workspace_bytes, (long long)bytes);
-    fa::launch_paged_prefix(prefix, own, plan, d, work, stream);
-    work += plan.workspace_bytes;
-    bytes -= plan.workspace_bytes;
-  }
-  const fa::PagedPlan plan = fa::plan_paged(own, d, longest_query(p), bytes);
-  fa::launch_paged_attention(own, plan, d, work, stream);
+  const int64_t bytes = p->workspace != nullptr ? p->workspace_bytes : 0;
+  const fa::PagedPlan first = fa::plan_prefix(prefix, d, longest_shared(x, a));
+  const int64_t rest = bytes - first.workspace_bytes;
+  if (rest < 0)
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes at least, got %lld",
+                     (long long)first.workspace_bytes, (long long)bytes);
+  fa::launch_paged_prefix(prefix, own, first, d, p->workspace, stream);
+  const fa::PagedPlan plan = fa::plan_paged(own, d, longest_query(p), rest, fa::kOwn);
+  fa::launch_paged_attention(own, plan, d, static_cast<char*>(p->workspace) + first.workspace_bytes, stream);
   return check_launch();
 }
 

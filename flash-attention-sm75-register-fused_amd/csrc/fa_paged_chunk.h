@@ -74,10 +74,21 @@ __device__ __forceinline__ void store_pair(_Float16* to, float4v x, float4v y, f
   *(uint4v*)to = v;
 }
 
-// O and LSE of a row from its merged state: pairs of groups pair0 .. pair0 + N - 1, 16
-// dimensions each, of which a half-wave holds 4 hi .. + 3 and 8 + 4 hi .. + 3.
+// O and LSE of a row from its state: pairs of groups pair0 .. pair0 + N - 1, 16 dimensions
+// each, of which a half-wave holds 4 hi .. + 3 and 8 + 4 hi .. + 3.
 template <int D, bool BF16, int N>
-__device__ __forceinline__ void store_pairs(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int hi,
+__device__ __forceinline__ void store_pairs(const PagedArgs& a, int, const PagedRow pr, int hi, int pair0, float m2,
+                                            float l, float4v (&x)[N][2]) {
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+#pragma unroll
+  for (int q = 0; q < N; ++q) store_pair<BF16>(op + 16 * (pair0 + q) + 8 * hi, x[q][0], x[q][1], inv);
+  if (a.lse != nullptr && hi == 0 && pair0 == 0)
+    a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+}
+// The same of a row that may have a prefix, whose state this is over its own keys.
+template <int D, bool BF16, int N>
+__device__ __forceinline__ void store_pairs(const PagedShared& a, const PagedJoint& joint, const PagedRow pr, int hi,
                                             int pair0, float m2, float l, float4v (&x)[N][2]) {
   if (joint.pieces > 0) {
     const JointRow j(a, joint, pr);
@@ -105,12 +116,7 @@ __device__ __forceinline__ void store_pairs(const PagedArgs& a, const PagedJoint
           x[q][e] += w * *(const float4v*)(o + record_o<D>((int64_t)i * joint.step, 0, 2 * q + e, 0));
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
-#pragma unroll
-  for (int q = 0; q < N; ++q) store_pair<BF16>(op + 16 * (pair0 + q) + 8 * hi, x[q][0], x[q][1], inv);
-  if (a.lse != nullptr && hi == 0 && pair0 == 0)
-    a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+  store_pairs<D, BF16, N>(static_cast<const PagedArgs&>(a), 0, pr, hi, pair0, m2, l, x);
 }
 
 // Whether a unit's last workgroup merges its partials (it reads them at about 50
@@ -142,9 +148,9 @@ struct ChunkRecord {
 // Merges pairs of groups pair0 .. pair0 + 3 of a unit's partials, wave w its rows
 // 32 w .. + 31 (of `rows`), and stores them: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M)
 // l_i, M = max_i m_i.
-template <int D, bool BF16>
-__device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPieces& pieces, int cls,
-                                            const PagedJoint& joint, const PagedRows& row_of, int rows, int pair0) {
+template <int D, bool BF16, class Args, class Joint>
+__device__ __forceinline__ void merge_chunk(const Args& a, const PagedPieces& pieces, int cls, const Joint& joint,
+                                            const PagedRows& row_of, int rows, int pair0) {
   constexpr int PAIRS = 4, AT = 4;  // at once; pieces at once
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -195,7 +201,18 @@ __device__ __forceinline__ void merge_chunk(const PagedArgs& a, const PagedPiece
         for (int e = 0; e < 2; ++e) x[q][e] += w * o[u][q][e];
     }
   }
-  store_pairs<D, BF16, PAIRS>(a, joint, row_of(r), hi, pair0, m, l, x);
+  const PagedRow pr = row_of(r);
+  if constexpr (!std::is_same_v<Args, PagedArgs>) {
+    store_pairs<D, BF16, PAIRS>(a, joint, pr, hi, pair0, m, l, x);
+    return;
+  }
+  // (store_pairs' code for no prefix: called, it left mixed batches 1% slower)
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh;
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q) store_pair<BF16>(op + 16 * (pair0 + q) + 8 * hi, x[q][0], x[q][1], inv);
+  if (a.lse != nullptr && hi == 0 && pair0 == 0)
+    a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m, l);
 }
 
 // A class's stretches.  Where all units are equally long, of units, each into the number q
@@ -245,10 +262,11 @@ __device__ __forceinline__ PagedStretch<kChunkMinTiles> chunk_stretch(const Page
 // d128 behind 128 tiles 65.1, 66.7, 62.5, 60.0, 62.1, 4 of 14 over 2 d64 behind 16 tiles 21.6, 20.1, 24.5, 26.0, 26.2).
 constexpr int kPrefixMinTiles = 4;
 struct PrefixLine {
-  const PagedArgs& a;
+  static constexpr int ahead = 0;
+  const PagedShared& a;
   int lane, q;
   PagedSeq own;  // prefix `lane`
-  __device__ __forceinline__ PrefixLine(const PagedArgs& args, int ln) : a(args), lane(ln) {
+  __device__ __forceinline__ PrefixLine(const PagedShared& args, int ln, bool) : a(args), lane(ln) {
     own = look(lane);
     int longest = 0;
     float units = 0.0f, tiles = 0.0f;  // (where cu_prefix falls again and again they may pass 2^31)
@@ -286,9 +304,21 @@ struct PrefixLine {
     const unsigned t = tiles_of(s);
     return (int)(t / (unsigned)q + (t % (unsigned)q != 0 ? 1 : 0));
   }
-  __device__ __forceinline__ int prefix(int g0) const {  // items of prefixes g0 .. g0 + lane
-    const PagedSeq s = g0 == 0 ? own : look(g0 + lane);
-    return wave_prefix(units_of(s) * pieces_of(s));
+  __device__ __forceinline__ int length_of(const PagedSeq& s) const { return units_of(s) * pieces_of(s); }  // items
+  __device__ __forceinline__ int prefix(int g0) const {  // of prefixes g0 .. g0 + lane
+    return wave_prefix(length_of(g0 == 0 ? own : look(g0 + lane)));
+  }
+  __device__ __forceinline__ PagedSeq seq(int g) const { return scalar_seq<kPrefix>(a, g); }
+  // What item `rel` of a prefix is: pieces next to each other are of units that read the same keys.
+  __device__ __forceinline__ int unit_of(const PagedSeq&) const { return 1; }
+  __device__ __forceinline__ int unit_at(int rel, int, int blocks) const {
+    const unsigned units = (unsigned)(a.heads * blocks);
+    return uniform((int)((unsigned)rel - (unsigned)rel / units * units));
+  }
+  __device__ __forceinline__ void tiles_of_item(const PagedSeq& s, int rel, int& first, int& stop) const {
+    const unsigned tiles = tiles_of(s), pieces = pieces_of(s), piece = (unsigned)rel / (unsigned)units_of(s);
+    first = uniform((int)((uint64_t)tiles * piece / pieces));
+    stop = uniform((int)((uint64_t)tiles * (piece + 1) / pieces));
   }
   __device__ __forceinline__ int total() const {
     int sum = 0;
@@ -314,7 +344,7 @@ struct PrefixLine {
     int before = 0;
     for (int g0 = 0; g0 < a.batch; g0 += 64) {
       const PagedSeq s = g0 == 0 ? own : look(g0 + lane);
-      const int items = units_of(s) * pieces_of(s);
+      const int items = length_of(s);
       const int x = wave_prefix(items);
       if (g0 + lane < a.batch) {
         int32_t* const to = a.joint_info + 4 * (g0 + lane);
@@ -331,7 +361,7 @@ struct PrefixLine {
 // STREAM: V's rows are read non-temporally (a sequence's only block is the one that reads them).
 // STAGE: 0, or of attention behind shared prefixes kPrefix (SPLIT) or kOwn.
 template <int D, bool BF16, bool FP8, bool SPLIT, bool STREAM, int STAGE>
-__global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const StageArgs<STAGE> a) {
   constexpr bool DENSE = D == 64;
   using L = std::conditional_t<DENSE, LdsDense<D>, Lds<D>>;
   using E = Elem<BF16>;
@@ -358,18 +388,16 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
   constexpr bool PREFIX = STAGE == kPrefix;
-  const auto line = [&] {
-    if constexpr (PREFIX) return PrefixLine(a, threadIdx.x & 63);
-    else return PagedLine<kChunkRows, kBlockN, kChunkAhead>(a, threadIdx.x & 63, SPLIT);
-  }();
+  using Line = std::conditional_t<PREFIX, PrefixLine, PagedLine<kChunkRows, kBlockN, kChunkAhead>>;
+  const Line line(a, threadIdx.x & 63, SPLIT);
   const auto stretch = [&] {
     if constexpr (PREFIX) return 0;
     else if constexpr (SPLIT) return chunk_stretch<D>(a, line);
     else return PagedStretch<1>(a, line.total());
   }();
-  int pos = 0, end = 0;
-  int seq_start, b;
+  int pos, end, seq_start, b;
   if constexpr (PREFIX) {
+    pos = end = wg;
     if (blockIdx.x == 0 && wave == 0) line.publish();
     if (wg >= line.total()) return;
     b = line.find(wg, seq_start);
@@ -384,43 +412,29 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
   }
 
   do {
-  PagedSeq s;
-  int blocks, first, stop, hc, rb, u0 = 0, u1 = 0;
-  bool whole = false;
-  if constexpr (PREFIX) {
-    s = scalar_seq<kPrefix>(a, b);
-    blocks = paged_blocks<kChunkRows>(a, s);
-    // Pieces next to each other in the order of the items are of units that read the same keys.
-    const int units = line.units_of(s), rel = wg - seq_start;
-    const int tiles = line.tiles_of(s), pieces = line.pieces_of(s);
-    if (units <= 0 || rel < 0 || rel >= units * pieces) return;  // (past 2^31)
-    const int piece = uniform((int)((unsigned)rel / (unsigned)units)), unit = rel - piece * units;
-    first = uniform((int)((uint64_t)(unsigned)tiles * (unsigned)piece / (unsigned)pieces));
-    stop = uniform((int)((uint64_t)(unsigned)tiles * (unsigned)(piece + 1) / (unsigned)pieces));
-    hc = uniform((int)((unsigned)unit / (unsigned)blocks));
-    rb = unit - hc * blocks;
-  } else {
-  s = line.seq(b);
-  blocks = paged_blocks<kChunkRows>(a, s);
+  const PagedSeq s = line.seq(b);
+  const int blocks = paged_blocks<kChunkRows>(a, s);
   const int unit_len = line.unit_of(s);
   const int len = line.length_of(s);
-  if (pos >= seq_start + len || len == 0) {  // on to the next sequence
+  if (!PREFIX && (pos >= seq_start + len || len == 0)) {  // on to the next sequence
     seq_start += len;
     if (++b >= a.batch) return;
     continue;
   }
+  if (PREFIX && (len <= 0 || wg - seq_start < 0 || wg - seq_start >= len)) return;  // (past 2^31)
   const int unit = line.unit_at(pos - seq_start, unit_len, blocks);
-  u0 = seq_start + unit * unit_len + line.ahead;  // its first tile on the line
-  u1 = seq_start + (unit + 1) * unit_len;
-  first = max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
-  if (SPLIT && u1 <= pos) return;  // (wrapped round)
-  pos = SPLIT ? min(u1, end) : u1;
-  stop = pos - u0;
-  if (SPLIT && stop <= 0) break;
-  whole = !SPLIT || (first == 0 && pos == u1);
-  hc = blocks == 1 ? unit : (int)((unsigned)unit / (unsigned)blocks);
-  rb = blocks - 1 - (unit - hc * blocks);
-  }
+  const int u0 = PREFIX ? 0 : seq_start + unit * unit_len + line.ahead;  // its first tile on the line
+  const int u1 = PREFIX ? 0 : seq_start + (unit + 1) * unit_len;
+  int item_first = 0, item_stop = 0;
+  if constexpr (PREFIX) line.tiles_of_item(s, pos - seq_start, item_first, item_stop);
+  const int first = PREFIX ? item_first : max(0, pos - u0);  // tiles [first, stop) of it are this stretch's
+  if (SPLIT && !PREFIX && u1 <= pos) return;  // (wrapped round)
+  pos = PREFIX ? pos : SPLIT ? min(u1, end) : u1;
+  const int stop = PREFIX ? item_stop : pos - u0;
+  if (SPLIT && !PREFIX && stop <= 0) break;
+  const bool whole = !SPLIT || (first == 0 && pos == u1);
+  const int hc = blocks == 1 ? unit : (int)((unsigned)unit / (unsigned)blocks);
+  const int rb = blocks - 1 - (unit - hc * blocks);
   const int hkv = hc * a.classes + cls;
 
   // What depends on the lane is derived for each segment from an opaque lane index, so
@@ -887,7 +901,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 
   const float l = halves_sum(l_run);
   const float m2 = m_run == -__builtin_inff() ? m_run : m_run * c2;
-  const PagedJoint joint = joint_of<STAGE>(a, b, hkv);
+  const auto joint = [&] {
+    if constexpr (PREFIX) return 0;
+    else return joint_of(a, b, hkv);
+  }();
   if (row < nrows) {
     if constexpr (PREFIX) {
       float* const to = a.joint_o + record_o<D>(blockIdx.x, wave, 0, lane);
@@ -899,15 +916,31 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
               float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
       if (hi == 0) *(v2f*)(a.joint_ml + record_ml(blockIdx.x, 32 * wave + ql)) = v2f{m2, l};
     } else if (whole) {
-      float4v x[D / 16][2];
+      const PagedRow pr = row_of(row - q0);
+      if constexpr (STAGE == kOwn) {
+        float4v x[D / 16][2];
 #pragma unroll
-      for (int q = 0; q < D / 16; ++q)
+        for (int q = 0; q < D / 16; ++q)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int mt = q / 2, g = 2 * (q % 2) + e;
-          x[q][e] = float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
-        }
-      store_pairs<D, BF16, D / 16>(a, joint, row_of(row - q0), hi, 0, m2, l, x);
+          for (int e = 0; e < 2; ++e) {
+            const int mt = q / 2, g = 2 * (q % 2) + e;
+            x[q][e] = float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]};
+          }
+        store_pairs<D, BF16, D / 16>(a, joint, pr, hi, 0, m2, l, x);
+      } else {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        _Float16* const op = a.o + pr.token * a.ot + pr.head * a.oh + 8 * hi;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int g = 0; g < 4; g += 2)
+            store_pair<BF16>(op + 32 * mt + 8 * g,
+                             float4v{oacc[mt][4 * g], oacc[mt][4 * g + 1], oacc[mt][4 * g + 2], oacc[mt][4 * g + 3]},
+                             float4v{oacc[mt][4 * g + 4], oacc[mt][4 * g + 5], oacc[mt][4 * g + 6],
+                                     oacc[mt][4 * g + 7]},
+                             inv);
+        if (a.lse != nullptr && hi == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
+      }
     } else {
       // (see ChunkRecord; coherent over the L2s: the merging workgroup may be on
       // another XCD)
@@ -947,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_chunk_kernel(const Paged
 // the workgroup's waves take every fourth piece, and meet in LDS.
 constexpr int kChunkCombineY = 2;
 template <int D, bool BF16, int STAGE>
-__global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const StageArgs<STAGE> a) {
   __shared__ float4v xo[kWaves][2][64];
   __shared__ float xml[kWaves][2][64];
   if (!combine_asked(a)) return;
@@ -973,7 +1006,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
   const int rb = blocks - 1 - (unit - hc * blocks);
   const int rows = s.n * a.group - rb * kChunkRows;
   const PagedRows row_of(a, s, hc * a.classes + cls, rb * kChunkRows);
-  const PagedJoint joint = joint_of<STAGE>(a, b, hc * a.classes + cls);
+  const auto joint = joint_of(a, b, hc * a.classes + cls);
   const ChunkRecord<D> rec(a);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -1042,7 +1075,7 @@ __global__ void __launch_bounds__(kThreads) fa_paged_chunk_combine_kernel(const 
 }  // namespace
 
 template <int D, bool BF16, bool FP8, int STAGE>
-void launch_paged_chunk(const PagedArgs& a, int64_t grid, hipStream_t stream) {
+void launch_paged_chunk(const StageArgs<STAGE>& a, int64_t grid, hipStream_t stream) {
   const dim3 g((unsigned)grid), t(kThreads);
   if constexpr (STAGE != kPrefix) {
     if (!a.split) {

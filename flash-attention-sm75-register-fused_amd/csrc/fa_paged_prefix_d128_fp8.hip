@@ -3,7 +3,7 @@
 #include "fa_paged_chunk.h"
 
 namespace fa {
-template void launch_paged_attn<128, false, true, kOwn>(const PagedArgs&, int, int64_t, hipStream_t);
-template void launch_paged_chunk<128, false, true, kPrefix>(const PagedArgs&, int64_t, hipStream_t);
-template void launch_paged_chunk<128, false, true, kOwn>(const PagedArgs&, int64_t, hipStream_t);
+template void launch_paged_attn<128, false, true, kOwn>(const PagedShared&, int, int64_t, hipStream_t);
+template void launch_paged_chunk<128, false, true, kPrefix>(const PagedShared&, int64_t, hipStream_t);
+template void launch_paged_chunk<128, false, true, kOwn>(const PagedShared&, int64_t, hipStream_t);
 }  // namespace fa

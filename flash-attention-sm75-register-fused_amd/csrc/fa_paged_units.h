@@ -302,34 +302,32 @@ __device__ __forceinline__ int64_t record_o(int64_t record, int wave, int group,
 __device__ __forceinline__ int64_t record_ml(int64_t record, int row) { return (record * kChunkRows + row) * 2; }
 
 // The records of one KV head's rows of a sequence over its prefix: `pieces` of them (0: it has
-// none), `step` apart, from rec0 for the prefix's first block of rows.
+// none), `step` apart, the first rec0 for the prefix's first block of rows.
 struct PagedJoint {
   int pieces, rec0, step, t0, n, head0;
 };
-template <int STAGE>
-__device__ __forceinline__ PagedJoint joint_of(const PagedArgs& a, int b, int hkv) {
+__device__ __forceinline__ int joint_of(const PagedArgs&, int, int) { return 0; }  // (no prefixes)
+__device__ __forceinline__ PagedJoint joint_of(const PagedShared& a, int b, int hkv) {
   PagedJoint j = {0, 0, 0, 0, 0, 0};
-  if constexpr (STAGE == kOwn) {
-    int g = 0;
-    if (a.groups != nullptr) {  // the last that begins at b or before
-      const int lane = threadIdx.x & 63;
-      for (int g0 = 0; g0 <= a.prefixes; g0 += 64) {
-        const bool starts = g0 + lane <= a.prefixes && a.groups[min(g0 + lane, a.prefixes)] <= b;
-        g += __builtin_popcountll(__builtin_amdgcn_ballot_w64(starts));
-      }
-      --g;
+  int g = 0;
+  if (a.groups != nullptr) {  // the last that begins at b or before
+    const int lane = threadIdx.x & 63;
+    for (int g0 = 0; g0 <= a.prefixes; g0 += 64) {
+      const bool starts = g0 + lane <= a.prefixes && a.groups[min(g0 + lane, a.prefixes)] <= b;
+      g += __builtin_popcountll(__builtin_amdgcn_ballot_w64(starts));
     }
-    if (g >= 0 && g < a.prefixes) {
-      const int32_t* const info = a.joint_info + 4 * g;
-      const int start = load_scalar(info);
-      j.pieces = load_scalar(info + 1);
-      j.t0 = load_scalar(info + 2);
-      j.n = load_scalar(info + 3);
-      const int blocks = (int)((unsigned)(j.n * a.group + kChunkRows - 1) / kChunkRows);
-      j.rec0 = ((start + (hkv >> a.class_shift) * blocks) << a.class_shift) + (hkv & (a.classes - 1));
-      j.step = (a.heads * blocks) << a.class_shift;
-      j.head0 = hkv * a.group;
-    }
+    --g;
+  }
+  if (g >= 0 && g < a.prefixes) {
+    const int32_t* const info = a.joint_info + 4 * g;
+    const int start = load_scalar(info);
+    j.pieces = load_scalar(info + 1);
+    j.t0 = load_scalar(info + 2);
+    j.n = load_scalar(info + 3);
+    const int blocks = (int)((unsigned)(j.n * a.group + kChunkRows - 1) / kChunkRows);
+    j.rec0 = ((start + ((hkv >> a.class_shift) + 1) * blocks - 1) << a.class_shift) + (hkv & (a.classes - 1));
+    j.step = (a.heads * blocks) << a.class_shift;
+    j.head0 = hkv * a.group;
   }
   return j;
 }
@@ -340,12 +338,12 @@ struct JointRow {
   int pieces;  // 0: none (also of a row that is not the prefix's, where cu_seqlens falls)
   int row;
   int64_t record;
-  __device__ __forceinline__ JointRow(const PagedArgs& a, const PagedJoint& j, const PagedRow pr) {
+  __device__ __forceinline__ JointRow(const PagedShared& a, const PagedJoint& j, const PagedRow pr) {
     pieces = j.pieces;
     const int i = pr.token - j.t0;
     const int r = i * a.group + pr.head - j.head0;
     row = r & (kChunkRows - 1);
-    record = j.rec0 + ((int64_t)(r / kChunkRows) << a.class_shift);
+    record = j.rec0 - ((int64_t)(r / kChunkRows) << a.class_shift);  // (blocks go from the last to the first)
     if ((unsigned)i >= (unsigned)j.n || record < 0 || record + (int64_t)(pieces - 1) * j.step >= a.joint_records)
       pieces = 0;
   }
@@ -354,7 +352,7 @@ struct JointRow {
 // Folds pieces first, first + step, .. of a row's states over its prefix into (m, l, x), 4
 // dimensions, BATCH of them asked for at once.
 template <int D, int BATCH>
-__device__ __forceinline__ void fold_joint(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int dim,
+__device__ __forceinline__ void fold_joint(const PagedShared& a, const PagedJoint& joint, const PagedRow pr, int dim,
                                            int first, int step, float& m, float& l, float4v& x) {
   const JointRow j(a, joint, pr);
   const float* const o = a.joint_o + record_o<D>(j.record, j.row >> 5, dim >> 3, (dim & 4) * 8 + (j.row & 31));
@@ -375,9 +373,14 @@ __device__ __forceinline__ void finish_row(const PagedArgs& a, const PagedRow pr
   *(half4*)(a.o + pr.token * a.ot + pr.head * a.oh + dim) = y;
   if (a.lse != nullptr && dim == 0) a.lse[(int64_t)pr.head * a.tokens + pr.token] = natural_lse(m2, l);
 }
-// The same from that over its own keys, 4 dimensions.
+// The same of a row that may have a prefix, whose state this is over its own keys.
 template <int D, bool BF16>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const PagedJoint& joint, const PagedRow pr, int dim,
+__device__ __forceinline__ void store_row(const PagedArgs& a, int, const PagedRow pr, int dim, float m2, float l,
+                                          float4v x) {
+  finish_row<BF16>(a, pr, dim, m2, l, x);
+}
+template <int D, bool BF16>
+__device__ __forceinline__ void store_row(const PagedShared& a, const PagedJoint& joint, const PagedRow pr, int dim,
                                           float m2, float l, float4v x) {
   if (joint.pieces > 0) fold_joint<D, 8>(a, joint, pr, dim, 0, 1, m2, l, x);
   finish_row<BF16>(a, pr, dim, m2, l, x);
