@@ -283,9 +283,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 // each row's -lse log2 e beside it).  Where units are few, each one's row tiles go to `parts`
 // workgroups in turns (under the causal rule every part then has as many that see the keys), and the last
 // of them to finish adds the parts up in their order.
-constexpr int kWRows = 32;      // rows of a tile
+constexpr int kWRows = 64;      // rows of a tile, two of S
 constexpr int kWTarget = 1024;  // workgroups that units are cut into, where they are fewer
-constexpr int kWMinTiles = 8;   // tiles a part has at least
+constexpr int kWMinTiles = 4;   // tiles a part has at least
 
 template <int D, bool BF16, bool FP8>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const WeighArgs w) {
@@ -294,10 +294,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   constexpr int KK = D / 16;               // contraction steps of S
   constexpr int RL = D / 8;                // threads that bring a row of Q
   constexpr int QL = kWRows * RL / kThreads;  // loads of a thread
-  constexpr int NS = 2 * KK;               // MFMAs of a tile
+  constexpr int NS = 2 * KK;               // MFMAs of 32 rows
   constexpr int PF = 3;                    // Q operand reads run this many steps ahead
-  __shared__ __attribute__((aligned(16))) _Float16 q_lds[2][kWRows * L::Pitch];
-  __shared__ __attribute__((aligned(16))) float lse_lds[4][kWRows];
+  __shared__ __attribute__((aligned(16))) _Float16 q_lds[3][kWRows * L::Pitch];
+  __shared__ __attribute__((aligned(16))) float lse_lds[3][kWRows];
   __shared__ int scratch[kWaves];
   const PagedArgs& a = w.p;
   const int lane = threadIdx.x & 63;
@@ -408,53 +408,54 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       ++ld_tok;
     }
   };
-  auto store = [&](int i) {  // the part's tile number i
+  auto store = [&](int buf) {
 #pragma unroll
     for (int u = 0; u < QL; ++u) {
       const int r = (int)threadIdx.x / RL + u * (kThreads / RL), c = threadIdx.x % RL;
-      *(half8*)(q_lds[i & 1] + r * L::Pitch + 8 * (c ^ ((r >> 2) & 3))) = q_next[u];
+      *(half8*)(q_lds[buf] + r * L::Pitch + 8 * (c ^ ((r >> 2) & 3))) = q_next[u];
     }
-    if (threadIdx.x < kWRows) lse_lds[i & 3][threadIdx.x] = -lse_next;
+    if (threadIdx.x < kWRows) lse_lds[buf][threadIdx.x] = -lse_next;
   };
-  auto read_q = [&](int i, int kk) -> half8 {
+  auto read_q = [&](int buf, int half, int kk) -> half8 {
     const int c = FP8 ? 4 * (kk >> 1) + 2 * hi + (kk & 1) : 2 * kk + hi;
-    return *(const half8*)(q_lds[i & 1] + l32 * L::Pitch + 8 * (c ^ ((l32 >> 2) & 3)));
+    return *(const half8*)(q_lds[buf] + (32 * half + l32) * L::Pitch + 8 * (c ^ ((l32 >> 2) & 3)));
   };
   float sum[2] = {0.0f, 0.0f};
   float16v st[2][2];
   const int count = tile0 < tiles ? uniform((int)((unsigned)(tiles - tile0 + parts - 1) / (unsigned)parts)) : 0;
-  // Step i: the probabilities of tile i, whose S is st[U], between the MFMAs of tile i + 1's (behind
-  // the last one: of what is there, for nobody); tile i + 2 goes to LDS in the place of tile i's Q, which
-  // every wave is done with.
-  auto step = [&](int i, auto u_t, auto masked_t) {
-    constexpr int U = decltype(u_t)::value;
+  // Half H of step i: the probabilities of these 32 rows, whose S is st[H], between the MFMAs of the
+  // next 32's (behind the last tile: of what is there, for nobody).  Tiles i and i + 1 are in buffers
+  // `now` and `next`; tile i + 2 goes to `free`, which held tile i - 1, and is loaded a step before.
+  auto half_step = [&](int i, int now, int next, int free, auto half_t, auto masked_t) {
+    constexpr int H = decltype(half_t)::value;
     constexpr bool MASKED = decltype(masked_t)::value;
     half8 qf[KK];
-    static_for<PF>([&](auto k_c) { qf[decltype(k_c)::value] = read_q(i + 1, decltype(k_c)::value); });
+    const int buf = H == 0 ? now : next;
+    static_for<PF>([&](auto k_c) { qf[decltype(k_c)::value] = read_q(buf, 1 - H, decltype(k_c)::value); });
     float4v nl[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) nl[g] = *(const float4v*)(lse_lds[i & 3] + 8 * g + 4 * hi);
-    const int row0 = (tile0 + i * parts) * kWRows + 4 * hi;
+    for (int g = 0; g < 4; ++g) nl[g] = *(const float4v*)(lse_lds[now] + 32 * H + 8 * g + 4 * hi);
+    const int row0 = (tile0 + i * parts) * kWRows + 32 * H + 4 * hi;
     const int lim[2] = {from[0] - row0, from[1] - row0};
     float add[2] = {0.0f, 0.0f};
     fence_schedule();
     static_for<NS>([&](auto slot_c) {
       constexpr int slot = decltype(slot_c)::value;
       constexpr int kk = slot / 2, v = slot % 2;
-      if constexpr (v == 0 && kk + PF < KK) qf[kk + PF] = read_q(i + 1, kk + PF);
-      if constexpr (slot == NS / 4) {
-        if (i + 2 < count) store(i + 2);
+      if constexpr (v == 0 && kk + PF < KK) qf[kk + PF] = read_q(buf, 1 - H, kk + PF);
+      if constexpr (H == 1 && slot == NS / 4) {
+        if (i + 2 < count) store(free);
       }
-      if constexpr (slot == NS / 2) {
+      if constexpr (H == 1 && slot == NS / 2) {
         if (i + 3 < count) load();
       }
-      st[1 - U][v] = E::mfma(qf[kk], kf[v][kk], kk == 0 ? (float16v)0.0f : st[1 - U][v]);
-      // Rows 8 g + 4 hi + r of the tile in register 4 g + r.
+      st[1 - H][v] = E::mfma(qf[kk], kf[v][kk], kk == 0 ? (float16v)0.0f : st[1 - H][v]);
+      // Rows 8 g + 4 hi + r of the 32 in register 4 g + r.
       static_for<32>([&](auto e_c) {
         constexpr int e = decltype(e_c)::value;
         if constexpr (e * NS / 32 == slot) {
           constexpr int k = e & 1, x = e >> 1;
-          float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[U][k][x], c2, nl[x >> 2][x & 3]));
+          float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[H][k][x], c2, nl[x >> 2][x & 3]));
           if constexpr (MASKED) y = 8 * (x >> 2) + (x & 3) >= lim[k] ? y : 0.0f;
           add[k] += y;
           asm volatile("" : "+v"(add[k]));  // keeps the sum in this slot
@@ -464,7 +465,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     });
     sum[0] += add[0];
     sum[1] += add[1];
-    barrier_after_loads<63>();
   };
   if (count > 0) {
     load();
@@ -479,19 +479,26 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     for (int v = 0; v < 2; ++v) {
       st[0][v] = (float16v)0.0f;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) st[0][v] = E::mfma(read_q(0, kk), kf[v][kk], st[0][v]);
+      for (int kk = 0; kk < KK; ++kk) st[0][v] = E::mfma(read_q(0, 0, kk), kf[v][kk], st[0][v]);
     }
-    barrier_after_loads<63>();
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     // Tiles before `all_from` hide a key from some row.
     const int hiding = uniform((int)((unsigned)(max(0, all_from - tile0 * kWRows) + part_rows - 1) / (unsigned)part_rows));
-    for (int i = 0; i < count; i += 2) {
-      if (i < hiding) step(i, I0{}, Flag<true>{});
-      else step(i, I0{}, Flag<false>{});
-      if (i + 1 >= count) break;
-      if (i + 1 < hiding) step(i + 1, I1{}, Flag<true>{});
-      else step(i + 1, I1{}, Flag<false>{});
+    int now = 0, next = 1, free = 2;
+    for (int i = 0; i < count; ++i) {
+      if (i < hiding) {
+        half_step(i, now, next, free, I0{}, Flag<true>{});
+        half_step(i, now, next, free, I1{}, Flag<true>{});
+      } else {
+        half_step(i, now, next, free, I0{}, Flag<false>{});
+        half_step(i, now, next, free, I1{}, Flag<false>{});
+      }
+      barrier_after_loads<63>();
+      const int done = now;
+      now = next;
+      next = free;
+      free = done;
     }
   }
   // Thread: a key of its wave's 64.
