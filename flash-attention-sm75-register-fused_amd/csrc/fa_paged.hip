@@ -121,7 +121,11 @@ PagedPlan plan_prefix(const PagedShared& a, int head_dim, int64_t max_queries) {
   p.classes = std::gcd(a.hkv, kNumXcds);
   const int64_t rows = (int64_t)a.tokens * a.group;
   p.units = (int)(a.hkv / p.classes * ((rows + (p.rows - 1ll) * std::min(a.batch, a.tokens)) / p.rows));
-  p.wgs = std::max(resident_fused_workgroups() / p.classes, p.units);
+  // A workgroup for each unit, or, while they are fewer than run at once, for each piece.
+  const int64_t tiles = (((int64_t)a.max_pages << a.page_shift) + kBlockN - 1) / kBlockN;
+  const int64_t pieces = std::max<int64_t>(1, (tiles + kPrefixMinTiles - 1) / kPrefixMinTiles);
+  const int64_t resident = resident_fused_workgroups() / p.classes;
+  p.wgs = (int)std::max<int64_t>(p.units, std::min<int64_t>(resident, p.units * pieces));
   p.stream_v = streams_v(a, head_dim, max_queries);
   p.workspace_bytes = (int64_t)p.wgs * p.classes * p.rows * (head_dim + 2) * (int64_t)sizeof(float) + 16ll * a.batch;
   return p;

@@ -765,6 +765,185 @@ def test_graph(device, q8, news):
         assert torch.equal(prefix, state["prefix"])
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_graph_large(device, q8):
+    """The same of sizes that are cut: pieces of a prefix, rows of the weights over several workgroups, long
+    rows of the eviction; replays between eager calls of the same sizes."""
+    own = Cache([9000, 700], 2, 64, 64, BF16, q8, news=[600, 300])
+    shared = Cache([3001], 2, 64, 64, BF16, q8, seed=1)
+    args, kw = on(device, own, shared)
+    k, v, ptable, plens, table, lens = args
+    ks = {"k_scale": kw["k_scale"]} if q8 else {}
+    cu = own.cu.to(device)
+    q = torch.randn(900, 8, 64, generator=torch.Generator().manual_seed(5)).bfloat16().to(device)
+    to = torch.full((2, 100), -1, dtype=torch.int32, device=device)  # (rows are dropped: weights and lens count)
+
+    def run():
+        o, lse = fa.flash_attention_paged_prefix(q, *args, cu_seqlens=cu, return_lse=True, **kw)
+        w = fa.paged_attention_weights(q, lse, k, table, lens, cu_seqlens=cu, **ks)
+        return (o, lse, w, *fa.paged_cache_evict(k, v, table, lens, w, to, 6000, 500, **kw))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for i in range(4):
+        lens.copy_(torch.tensor([[9000, 700], [8300, 300], [600, 650], [8999, 301]][i], dtype=torch.int32))
+        plens.fill_([3001, 17, 0, 2900][i])
+        want = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(outs, want):
+            assert torch.equal(x, y)
+        want = run()
+        for x, y in zip(outs, want):
+            assert torch.equal(x, y)
+
+
+def test_calls_at_once(device):
+    """On several streams at once, each with its own cache, sizes that are cut among them."""
+    settings = [Cache([9000 - 700 * i, 300], 2, 64, 64, BF16, i % 2 == 1, seed=i, news=[200 + i, 1]) for i in range(4)]
+    shared = [Cache([2000 + i], 2, 64, 64, BF16, i % 2 == 1, seed=9 + i) for i in range(4)]
+    on_device = [on(device, o, s) for o, s in zip(settings, shared)]
+    qs = [torch.randn(sum(o.news), 4, 64, generator=torch.Generator().manual_seed(i)).bfloat16().to(device)
+          for i, o in enumerate(settings)]
+    cus, to = [o.cu.to(device) for o in settings], torch.full((2, 60), -1, dtype=torch.int32, device=device)
+
+    def run(i):
+        args, kw = on_device[i]
+        ks = {"k_scale": kw["k_scale"]} if kw else {}
+        o, lse = fa.flash_attention_paged_prefix(qs[i], *args, cu_seqlens=cus[i], return_lse=True, **kw)
+        w = fa.paged_attention_weights(qs[i], lse, args[0], *args[4:], cu_seqlens=cus[i], **ks)
+        return (o, lse, w, *fa.paged_cache_evict(*args[:2], *args[4:], w, to, 3700, 100, **kw))
+
+    alone = [run(i) for i in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(4):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(run(i))
+        torch.cuda.synchronize()
+        for x, y in zip(alone, got):
+            assert all(torch.equal(a, b) for a, b in zip(x, y))
+
+
+def test_prefix_groups_that_overlap(device):
+    """cu_prefix that falls again and again makes more units than there are records: what is written is not
+    said, but nothing outside the rows is, and the call ends."""
+    own, shared = Cache([20] * 64, 2, 64, 16, FP16, False), Cache([200], 2, 64, 16, FP16, False, seed=3)
+    k, v, ptable, plens, table, lens = on(device, own, shared)[0]
+    for count in (700, 5000):
+        cu = torch.tensor(([0, 64] * count)[:count + 1], dtype=torch.int32, device=device)
+        room = torch.full((192, 8, 64), 7.0, dtype=FP16, device=device)
+        q = torch.randn(64, 8, 64, dtype=FP16, device=device)
+        fa.flash_attention_paged_prefix(q, k, v, ptable.expand(count, -1).contiguous(), plens.expand(count).contiguous(),
+                                        table, lens, cu_prefix=cu, out=room[64:128])
+        assert (room[:64] == 7).all() and (room[128:] == 7).all()
+
+
+def test_pools_past_32_bits(device):
+    """Pages, codes and scales whose byte offsets pass 2^32."""
+    pages, page, hkv, d = 300000, 64, 4, 64
+    for dtype in (torch.float8_e4m3fn, FP16):
+        q8 = dtype != FP16
+        own, shared = Cache([150, 100], hkv, d, page, FP16, q8, news=[90, 1]), Cache([130], hkv, d, page, FP16, q8, seed=2)
+        k = torch.empty(pages, hkv, page, d, dtype=dtype, device=device)
+        v = torch.empty_like(k)
+        kw = {}
+        if q8:
+            kw = {n: torch.empty(pages, hkv, page, dtype=torch.float8_e8m0fnu, device=device) for n in ("k_scale", "v_scale")}
+        assert k.numel() * k.element_size() > 2 ** 32
+        where = {}
+        for i, c in enumerate((own, shared)):
+            for b in range(len(c.lens)):
+                for j in range(-(-c.lens[b] // page)):
+                    p, to = int(c.table[b, j]), pages - 1 - 1000 * len(where)
+                    where[i, p] = to
+                    k[to], v[to] = c.k[p].to(device), c.v[p].to(device)
+                    if q8:
+                        kw["k_scale"].view(torch.uint8)[to] = c.ks.view(torch.uint8)[p].to(device)
+                        kw["v_scale"].view(torch.uint8)[to] = c.vs.view(torch.uint8)[p].to(device)
+                    c.table[b, j] = to
+            c.pages = pages
+        table, lens, cu = own.table.to(device), own.seq_lens.to(device), own.cu.to(device)
+        q = torch.randn(91, 8, d, generator=torch.Generator().manual_seed(8)).half()
+        o, lse = fa.flash_attention_paged_prefix(q.to(device), k, v, shared.table.to(device), shared.seq_lens.to(device),
+                                                 table, lens, cu_seqlens=cu, return_lse=True, **kw)
+        want, _, tol, _ = ref.attention(con.Joined(own, shared, [0, 0]), q)
+        ref.check(o, want, tol * (1 + 2.0 ** -4), "O")
+        want, tol = con.weights(own, q, lse.cpu())
+        ks = {"k_scale": kw["k_scale"]} if q8 else {}
+        for hint in (1, None):
+            w = fa.paged_attention_weights(q.to(device), lse, k, table, lens, cu_seqlens=cu, max_query_len=hint, **ks)
+            ref.check(w, want, tol, "weights")
+        to = torch.tensor([[pages - 2], [pages - 3]], dtype=torch.int32, device=device)
+        got, left = fa.paged_cache_evict(k, v, table, lens, w, to, 40, 3, **kw)
+        assert got.tolist() == [40, 40]
+        for b in range(2):
+            for h in range(hkv):
+                at = con.stays(w[b, h].tolist(), own.held(b).tolist(), own.lens[b], 40, 3)
+                rows = k[int(to[b, 0]), h, :40].double()
+                if q8:
+                    rows = rows * kw["k_scale"][int(to[b, 0]), h, :40].double()[:, None]
+                assert torch.equal(rows.cpu(), own.rows[b][0][h, at]) and torch.equal(left[b, h, :40], w[b, h, at])
+        del k, v, kw
+        torch.cuda.empty_cache()
+
+
+def test_workspaces_of_the_c_calls(device):
+    """Weights without a workspace (no unit is cut) and prefixes with no more than the states' share of one (own
+    keys are not cut) give the same within the same bounds."""
+    import ctypes
+
+    from capi_types import LIB
+    from test_paged_context_cpu import PagedPrefix, WeighParams
+    from test_paged_cpu import PagedCache, PagedParams
+
+    lib = ctypes.CDLL(LIB)
+    lib.fa_sm75_last_error.restype = ctypes.c_char_p
+    P = ctypes.POINTER
+    lib.fa_sm75_paged_weigh.argtypes = [P(WeighParams)]
+    lib.fa_sm75_paged_prefix_forward.argtypes = [P(PagedParams), P(PagedPrefix)]
+    own, shared = Cache([2500, 33], 2, 64, 64, BF16, False, news=[200, 1]), Cache([700], 2, 64, 64, BF16, False, seed=3)
+    k, v, ptable, plens, table, lens = on(device, own, shared)[0]
+    q, cu = torch.randn(201, 8, 64, generator=torch.Generator().manual_seed(1)).bfloat16(), own.cu.to(device)
+    qd = q.to(device)
+    c = PagedCache(k=k.data_ptr(), v=v.data_ptr(), block_table=table.data_ptr(), seq_lens=lens.data_ptr(), batch=2, heads_kv=2,
+                   head_dim=64, num_pages=k.shape[0], page_size=64, max_pages=table.shape[1], block_table_stride=table.stride(0))
+    for t, x in (("k", k), ("v", v)):
+        for i, n in enumerate("phn"):
+            setattr(c, f"{t}_stride_{n}", x.stride(i))
+    x = PagedPrefix(block_table=ptable.data_ptr(), lens=plens.data_ptr(), count=1, max_pages=ptable.shape[1],
+                    block_table_stride=ptable.shape[1])
+    o, lse = torch.empty_like(qd), torch.empty(8, 201, device=device)
+    work = torch.empty(1 << 26, dtype=torch.uint8, device=device)
+    p = PagedParams(cache=ctypes.pointer(c), q=qd.data_ptr(), o=o.data_ptr(), lse=lse.data_ptr(), tokens=201, heads_q=8,
+                    q_stride_t=512, q_stride_h=64, o_stride_t=512, o_stride_h=64, cu_seqlens=cu.data_ptr(), scale=0.125,
+                    causal=2, dtype=1, stream=torch.cuda.current_stream().cuda_stream, workspace=work.data_ptr())
+    assert lib.fa_sm75_paged_prefix_forward(ctypes.byref(p), ctypes.byref(x)) == 1
+    p.workspace_bytes = int(lib.fa_sm75_last_error().split(b"hold ")[1].split(b" ")[0])  # the least
+    assert p.workspace_bytes < work.numel()
+    work[p.workspace_bytes:] = 77
+    assert lib.fa_sm75_paged_prefix_forward(ctypes.byref(p), ctypes.byref(x)) == 0, lib.fa_sm75_last_error()
+    assert (work[p.workspace_bytes:] == 77).all()
+    want, want_lse, tol, lse_tol = ref.attention(con.Joined(own, shared, [0, 0]), q)
+    ref.check(o, want, tol * (1 + 2.0 ** -4), "O")
+    ref.check(lse, want_lse, lse_tol + 2.0 ** -15, "LSE")
+    weights = torch.empty(2, 2, 2560, device=device)
+    w = WeighParams(cache=ctypes.pointer(c), q=qd.data_ptr(), lse=lse.data_ptr(), weights=weights.data_ptr(),
+                    weights_stride_b=5120, weights_stride_h=2560, max_len=2560, tokens=201, heads_q=8, q_stride_t=512,
+                    q_stride_h=64, cu_seqlens=cu.data_ptr(), scale=0.125, causal=2, dtype=1, stream=p.stream)
+    c.v = 0  # not looked at
+    assert lib.fa_sm75_paged_weigh(ctypes.byref(w)) == 0, lib.fa_sm75_last_error()
+    want, tol = con.weights(own, q, lse.cpu())
+    ref.check(weights, want, tol, "weights")
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_drawn(device, seed):
     """Drawn sizes, tables, hints and types of all three operators."""

@@ -118,10 +118,10 @@ def test_prefix_too_many_units(lib):
 
 
 def test_prefix_workspace(lib):
-    """The rows' states at least (a record of 128 rows for each of the 512 workgroups that a device runs at
-    once); without them the call is refused, before it asks the device anything."""
+    """The rows' states at least (a record of 128 rows for each workgroup: of one block of rows of two heads, and
+    a single tile of keys); without them the call is refused, before it asks the device anything."""
     p, x = params(cache()), prefix()
-    states = 512 * 128 * (64 + 2) * 4 + 16
+    states = 2 * 128 * (64 + 2) * 4 + 16
     size = lib.fa_sm75_paged_prefix_workspace_size(ctypes.byref(p), ctypes.byref(x))
     assert size >= states and size % 16 == 0
     for kw in (dict(), dict(workspace=0x1000, workspace_bytes=states - 1)):
