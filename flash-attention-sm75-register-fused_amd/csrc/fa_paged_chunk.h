@@ -308,7 +308,10 @@ struct PrefixLine {
   __device__ __forceinline__ int prefix(int g0) const {  // of prefixes g0 .. g0 + lane
     return wave_prefix(length_of(g0 == 0 ? own : look(g0 + lane)));
   }
-  __device__ __forceinline__ PagedSeq seq(int g) const { return scalar_seq<kPrefix>(a, g); }
+  __device__ __forceinline__ PagedSeq seq(int g) const {
+    if (g >= 64) return scalar_seq<kPrefix>(a, g);
+    return {wave_bcast(own.t0, g), wave_bcast(own.n, g), wave_bcast(own.len, g), wave_bcast(own.keys, g)};
+  }
   // What item `rel` of a prefix is: pieces next to each other are of units that read the same keys.
   __device__ __forceinline__ int unit_of(const PagedSeq&) const { return 1; }
   __device__ __forceinline__ int unit_at(int rel, int, int blocks) const {
