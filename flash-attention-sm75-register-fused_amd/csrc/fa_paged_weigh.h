@@ -370,7 +370,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   // group on, with offsets below 2^31 bytes (the launcher sees to it), whose factors have 24 bits.
   half8 q_next[QL];
   float lse_next;
-  const int r_own = (int)threadIdx.x / RL;
   const int q_tok = 2 * (int)a.qt, q_head = 2 * (int)a.qh;  // in bytes
   const int part_rows = uniform(kWRows * parts);
   const int tok_step = uniform((int)((unsigned)part_rows / (unsigned)a.group));
@@ -378,27 +377,36 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   int ld_row = uniform(tile0 * kWRows);  // of the tile that is loaded next; its token and what is left
   int ld_tok = uniform((int)((unsigned)ld_row / (unsigned)a.group));
   int ld_rem = ld_row - ld_tok * a.group;
+  // Offsets of the thread's rows: they follow from what is left of the tile's first token, which often is
+  // the same for all tiles, and, of the last tile, from where the rows end (the last row again for those
+  // behind it).
+  int q_off[QL], lse_off = 0, aimed = -1;
   auto load = [&] {
+    const int end = nrows - 1 - ld_row;
+    if (ld_rem != aimed || end < kWRows - 1) {
+      aimed = ld_rem;
+      auto place = [&](int r, int& tok, int& head) {
+        const int x = ld_rem + min(r, end);
+        tok = (int)(((float)x + 0.5f) * a.inv_group);
+        head = x - (int)__umul24(tok, a.group);
+      };
+      int tok, head;
+#pragma unroll
+      for (int u = 0; u < QL; ++u) {
+        place((int)threadIdx.x / RL + u * (kThreads / RL), tok, head);
+        q_off[u] = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (int)(threadIdx.x % RL);
+      }
+      place(threadIdx.x, tok, head);
+      lse_off = head * a.tokens + tok;
+    }
     const __amdgpu_buffer_rsrc_t rq =
         make_rsrc(a.q + (int64_t)(s.t0 + ld_tok) * a.qt + (int64_t)hkv * a.group * a.qh, INT32_MAX);
-    const int end = nrows - 1 - ld_row;  // the last row there is, again for those behind it
-    auto place = [&](int r, int& tok, int& head) {
-      const int x = ld_rem + min(r, end);
-      tok = (int)(((float)x + 0.5f) * a.inv_group);
-      head = x - (int)__umul24(tok, a.group);
-    };
 #pragma unroll
-    for (int u = 0; u < QL; ++u) {
-      int tok, head;
-      place(r_own + u * (kThreads / RL), tok, head);
-      const int off = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (int)(threadIdx.x % RL);
-      q_next[u] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rq, off, 0, 0));
-    }
+    for (int u = 0; u < QL; ++u)
+      q_next[u] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rq, q_off[u], 0, 0));
     if (threadIdx.x < kWRows) {
-      int tok, head;
-      place(threadIdx.x, tok, head);
       const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
-      lse_next = (int)threadIdx.x <= end ? weigh_lse2(lse[head * a.tokens + tok]) : __builtin_inff();
+      lse_next = (int)threadIdx.x <= end ? weigh_lse2(lse[lse_off]) : __builtin_inff();
     }
     ld_row += part_rows;
     ld_tok += tok_step;
@@ -416,9 +424,13 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     }
     if (threadIdx.x < kWRows) lse_lds[buf][threadIdx.x] = -lse_next;
   };
+  // (the swizzle moves the two low bits of a chunk's number: one base for even steps, one for odd)
+  const int swz = (l32 >> 2) & 3;
+  const int q_even = l32 * L::Pitch + 8 * ((FP8 ? 2 * hi : hi) ^ swz);
+  const int q_odd = l32 * L::Pitch + 8 * ((FP8 ? 2 * hi + 1 : 2 + hi) ^ swz);
   auto read_q = [&](int buf, int half, int kk) -> half8 {
-    const int c = FP8 ? 4 * (kk >> 1) + 2 * hi + (kk & 1) : 2 * kk + hi;
-    return *(const half8*)(q_lds[buf] + (32 * half + l32) * L::Pitch + 8 * (c ^ ((l32 >> 2) & 3)));
+    const _Float16* const base = q_lds[0] + buf * (kWRows * L::Pitch) + ((kk & 1) ? q_odd : q_even);
+    return *(const half8*)(base + 32 * half * L::Pitch + 32 * (kk >> 1));
   };
   float sum[2] = {0.0f, 0.0f};
   float16v st[2][2];
