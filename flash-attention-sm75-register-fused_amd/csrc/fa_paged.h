@@ -140,16 +140,15 @@ struct WeighArgs {
   int add;           // to what is there; else positions without a row get 0
   // Plan.
   int waves;         // few rows: most waves that share the tiles
-  int split;         // more: units may be cut (with a workspace)
+  int wgs;           // more: workgroups that units are cut over where they are fewer (0: no workspace)
   float* partial;
   uint64_t* flags;
   uint64_t mark;     // what a written part's flag holds (merge_mark)
 };
 struct WeighPlan {
   int rows;  // rows at once: 16 or 32, 0 for the kernel of more
-  int waves;
+  int waves, wgs;
   int64_t grid;
-  bool split;
   int64_t workspace_bytes;
 };
 WeighPlan plan_weigh(const WeighArgs& a, int64_t max_query_len, int64_t workspace_bytes);

@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
     };
     if constexpr (STAGE == kOwn) {
       // Few rows leave threads without a column: those take every groups-th piece of the
-      // prefix each (64 tokens of 4 rows behind 32 pieces: %%%).
+      // prefix each (64 tokens of 4 rows behind 32 pieces: 36 us of launch for 47 with whole rows).
       const int items = min(R, nrows - rb * R) * (D / 4);
       const int groups = min(kThreads / items, joint.pieces);
       if (whole && groups > 1) {

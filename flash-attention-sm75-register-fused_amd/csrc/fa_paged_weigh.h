@@ -9,7 +9,7 @@
 //
 // p = 2^(c s - lse log2 e), c = scale log2 e: no maximum is looked for, the lse is one already.
 // Everything from S on is in 32 bits, and sums go by tiles of 32 rows (one accumulator over 2048
-// rows was off by 1.4e-6 of a weight, by tiles %%%).  Which rows a sum takes, and in which order, follows from
+// rows was off by 1.4e-6 of a weight, twelve of the sum's own roundings).  Which rows a sum takes, and in which order, follows from
 // the sizes and lengths: the same call gives the same bits.
 //
 // Two kernels: up to 32 rows (one generated token, a few drafted ones) K is the work, which
@@ -19,6 +19,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fa_internal.h"
 #include "fa_paged_units.h"
 
 namespace fa {
@@ -62,16 +63,6 @@ struct WeighLine {
     for (int b0 = 0; b0 < w.p.batch; b0 += 64) sum += wave_bcast(prefix(b0, behind), 63);
     return uniform(sum);
   }
-  // The most rows of a sequence, in tiles of R.
-  template <int R>
-  __device__ __forceinline__ int row_tiles() const {
-    int most = 0;
-    for (int b0 = 0; b0 < w.p.batch; b0 += 64) {
-      const PagedSeq s = b0 == 0 ? own : look(b0 + lane);
-      most = max(most, wave_max((int)((unsigned)(s.n * w.p.group + R - 1) / R)));
-    }
-    return most;
-  }
   // The sequence of number `at` (below the total), which becomes its number in the sequence.
   __device__ __forceinline__ int find(int& at, bool behind) const {
     for (int b0 = 0;; b0 += 64) {
@@ -98,7 +89,11 @@ struct WeighLine {
 // The tiles of all (sequence, KV head) end to end are a line, of which each of `waves` waves takes an
 // equal stretch, whatever heads and sequences it covers: as many waves as run at once, or one for
 // each tile.  K goes to registers, the next tile's under the current one's work.  (Runs of 8 tiles
-// a wave, as the GPU got round to them, left a last round of half the waves: %%%.)
+// a wave, as the GPU got round to them, left a last round of half the waves: 88 us for 80 at 32 sequences
+// of 4096 .. 8192 rows of 128, 8 KV heads, and 40.5 for 36 at 8 bits.)
+//
+// Bound: K comes from HBM once, 403 MB in 80 us (5.0 TB/s, as fast as a copy moves bytes); at 8 bits
+// 211 MB in 36 us (5.8 TB/s).  A token over a few thousand rows is latency, 5 us.
 template <int D, bool BF16, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kernel(const WeighArgs w) {
   using E = Elem<BF16>;
@@ -279,13 +274,43 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 // ---- more than 32 rows ------------------------------------------------------------
 //
 // A unit is 256 keys of one (sequence, KV head), a wave's 64 of them in its registers as the B
-// operand of 32x32x16 MFMAs; the sequence's rows come by, 32 at a time, through LDS (double-buffered,
-// each row's -lse log2 e beside it).  Where units are few, each one's row tiles go to `parts`
-// workgroups in turns (under the causal rule every part then has as many that see the keys), and the last
-// of them to finish adds the parts up in their order.
+// operand of 32x32x16 MFMAs; the sequence's rows that see them come by, 64 at a time, through LDS
+// (three buffers, each row's -lse log2 e beside it), the probabilities of 32 rows between the
+// MFMAs of the next 32.  Where units are many, each is a workgroup's; else their row tiles (under the
+// causal rule a unit of new keys has fewer) are a line, of which each workgroup takes an equal stretch;
+// the workgroups of a unit leave their sums, and the last of them to finish adds those up in their
+// order (each unit's rows dealt to whole parts left a second round and idle CUs: at a prompt of
+// 4096 tokens 116 us for 97, at five of 700 .. 2000 of 14 heads of 64 42 for 35; where the parts came
+// to two whole rounds the line costs 4%, 155 us for 149).
+//
+// Bound: the matrix units and the exponentials take turns on a SIMD.  The last 2048 tokens of 8192,
+// 32 heads of 128 on 8, are 120 GFLOP in 150 us (0.8 PFLOP/s), the matrix units busy 43% of them;
+// without the exponentials 137, without MFMAs 147, without loads 129.
 constexpr int kWRows = 64;      // rows of a tile, two of S
-constexpr int kWTarget = 1024;  // workgroups that units are cut into, where they are fewer
-constexpr int kWMinTiles = 4;   // tiles a part has at least
+constexpr int kWMinTiles = 8;   // tiles a stretch has at least
+
+// How many of a sequence's row tiles see its blocks of keys: `tiles` for those before block k0,
+// where the new tokens begin; block k from there on is hidden from the first 4 group k - c
+// (row r sees key j iff r >= (j - past) group).
+struct WeighTiles {
+  int tiles, k0, group;
+  int64_t c;
+  __device__ __forceinline__ WeighTiles(const PagedArgs& a, const PagedSeq& s) {
+    const int past = s.len - s.n;  // tokens before the new ones
+    group = a.group;
+    tiles = (int)((unsigned)(s.n * a.group + kWRows - 1) / kWRows);
+    k0 = a.causal ? max(0, (int)(((int64_t)past + kWBlock - 1) / kWBlock)) : INT32_MAX;
+    const int64_t rows = (int64_t)past * a.group;
+    c = rows > 0 ? (rows + kWRows - 1) / kWRows : -(-rows / kWRows);
+  }
+  // The first tile that sees block k, and all those of blocks before it (below 2^31 where there
+  // are fewer units than workgroups).
+  __device__ __forceinline__ int first(int k) const { return k < k0 ? 0 : (int)(4ll * group * k - c); }
+  __device__ __forceinline__ int before(int k) const {
+    if (k <= k0) return k * tiles;
+    return (int)((int64_t)k0 * tiles + (k - k0) * (tiles + c) - 2ll * group * ((int64_t)k * (k - 1) - (int64_t)k0 * (k0 - 1)));
+  }
+};
 
 template <int D, bool BF16, bool FP8>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const WeighArgs w) {
@@ -300,31 +325,96 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   __shared__ __attribute__((aligned(16))) float lse_lds[3][kWRows];
   __shared__ int scratch[kWaves];
   const PagedArgs& a = w.p;
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int hi = lane >> 5, l32 = lane & 31;
-  const WeighLine<kWBlock> line(w, lane);  // (heads next to each other: those of one head meet in one XCD's L2)
-  const int most = line.row_tiles<kWRows>();
-  const int units = line.total(false);
-  // (kWTarget over the units is cut to whole parts: at most kWTarget workgroups where there are several)
-  int parts = 1;
-  if (w.split && units > 0 && units < kWTarget)
-    parts = max(1, min((int)((unsigned)kWTarget / (unsigned)units), (int)((unsigned)most / kWMinTiles)));
-  parts = uniform(parts);
   const int wg = (int)blockIdx.x;
-  if (wg >= units * parts) {  // blocks behind the keys
-    if (!w.add && wg - units * parts < line.total(true)) line.clear(wg - units * parts, threadIdx.x, kThreads);
-    return;
+  // The line of row tiles and its workgroups, or one for each unit.  (The sequences are looked at again
+  // for each unit, not kept in registers through its tiles.)
+  auto length_of = [&](const WeighLine<kWBlock>& line, int b0) {  // of sequence b0 + lane
+    const PagedSeq s = b0 == 0 ? line.own : line.look(b0 + line.lane);
+    return s.n > 0 ? WeighTiles(a, s).before(line.steps(s)) * a.hkv : 0;
+  };
+  int total = 0, cuts = 0;
+  {
+    const WeighLine<kWBlock> line(w, threadIdx.x & 63);
+    const int units = line.total(false);
+    if (w.wgs > units) {
+      for (int b0 = 0; b0 < a.batch; b0 += 64) total += wave_bcast(wave_prefix(length_of(line, b0)), 63);
+      total = uniform(total);
+      cuts = uniform(min(w.wgs, (int)((unsigned)total / kWMinTiles)));
+      if (cuts >= kNumXcds) cuts &= -kNumXcds;
+      if (cuts <= units) cuts = 0;
+    }
+    const int active = cuts > 0 ? cuts : units;
+    if (wg >= active) {  // blocks behind the keys
+      if (!w.add && wg - active < line.total(true)) line.clear(wg - active, threadIdx.x, kThreads);
+      return;
+    }
   }
-  const int part = (int)((unsigned)wg / (unsigned)units);
-  int at = wg - part * units;
-  at = uniform(at);
-  const int unit = at;
-  const int b = line.find(at, false);
-  const int block = uniform((int)((unsigned)at / (unsigned)a.hkv)), hkv = uniform(at - block * a.hkv);
+  // Stretch number i is [start(i), start(i + 1)) of the line; an XCD's are next to each other, so that it
+  // reads few heads' rows.
+  auto start = [&](int i) { return (int)((int64_t)total * i / cuts); };
+  auto holder = [&](int pos) { return (int)(((int64_t)(pos + 1) * cuts + total - 1) / total) - 1; };
+  const int place = cuts >= kNumXcds ? (wg & (kNumXcds - 1)) * (cuts / kNumXcds) + wg / kNumXcds : wg;
+  int pos = 0, end = 1;
+  if (cuts > 0) {
+    pos = uniform(start(place));
+    end = uniform(start(place + 1));
+  }
+  while (pos < end) {
+  // The unit, and its tiles [t0, t1) that are this workgroup's, at [u0, u1) of the line.
+  int b, block, hkv, t0 = 0, t1, u0 = 0, u1 = 0;
+  // What depends on the thread is derived for each unit from an opaque index, so that none of it is kept
+  // in registers from one to the next.
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
+  const WeighLine<kWBlock> line(w, lane);
+  if (cuts > 0) {
+    int before = 0;
+    for (int b0 = 0;; b0 += 64) {
+      const int x = wave_prefix(length_of(line, b0));
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + x > pos);
+      if (past != 0 || b0 + 64 >= a.batch) {
+        const int l = past != 0 ? __builtin_ctzll(past) : 63;
+        if (l > 0) before += wave_bcast(x, l - 1);
+        b = uniform(min(b0 + l, a.batch - 1));
+        break;
+      }
+      before += wave_bcast(x, 63);
+    }
+    u0 = before;
+  } else {
+    int at = wg;
+    b = line.find(at, false);
+    block = uniform((int)((unsigned)at / (unsigned)a.hkv));
+    hkv = uniform(at - block * a.hkv);
+  }
   const PagedSeq s = scalar_seq(a, b);
+  const WeighTiles rows(a, s);
+  if (cuts > 0) {
+    const int blocks = line.steps(s), head = rows.before(blocks);
+    if (head <= 0) return;  // (the lengths changed meanwhile)
+    hkv = uniform((int)((unsigned)(pos - u0) / (unsigned)head));
+    const int rel = pos - u0 - hkv * head;
+    int lo = 0, hi_k = blocks;  // before(lo) <= rel < before(hi_k)
+    while (hi_k - lo > 1) {
+      const int mid = (lo + hi_k) / 2;
+      if (rows.before(mid) <= rel) lo = mid;
+      else hi_k = mid;
+    }
+    block = uniform(lo);
+    u0 = uniform(u0 + hkv * head + rows.before(lo));
+    u1 = uniform(u0 + rows.before(lo + 1) - rows.before(lo));
+    t0 = pos - u0;
+    t1 = min(u1, end) - u0;
+    pos = uniform(min(u1, end));
+    if (hkv >= a.hkv || t1 <= t0) return;
+  } else {
+    t1 = rows.tiles - rows.first(block);
+    pos = end;
+  }
   const int nrows = s.n * a.group;
-  const int past = s.len - s.n;  // tokens before the new ones
+  const int past = s.len - s.n;
   const int sees = min(s.keys, w.max_len);
   const int key0 = block * kWBlock;
 
@@ -354,7 +444,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   }
   // Row r sees key j iff r >= (j - past) group, its token's number not below j - past: from row
   // `from` on this lane's first key, and 32 tokens later the second.
-  const int first_row = a.causal ? clamp_int(key0 - past, 0, s.n) * a.group : 0;
   const int64_t from64[2] = {(int64_t)(key - past) * a.group, (int64_t)(key + 32 - past) * a.group};
   int from[2];
 #pragma unroll
@@ -362,18 +451,16 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   // From this row on all of the unit's keys are seen.
   const int all_from = a.causal ? (int)min((int64_t)max(0, key0 + kWBlock - 1 - past) * a.group, (int64_t)nrows) : 0;
 
-  // Row tiles of this part.
-  const int tiles = (int)((unsigned)(nrows + kWRows - 1) / kWRows);
-  const int tile0 = uniform((int)((unsigned)first_row / kWRows)) + part;
+  const int tile0 = uniform(rows.first(block) + t0);
+  const int count = uniform(max(0, t1 - t0));
   const float c2 = a.negate_q ? -a.c : a.c;
   // Loads of a tile's rows go through windows from its first row's token and the first head of the
   // group on, with offsets below 2^31 bytes (the launcher sees to it), whose factors have 24 bits.
   half8 q_next[QL];
   float lse_next;
   const int q_tok = 2 * (int)a.qt, q_head = 2 * (int)a.qh;  // in bytes
-  const int part_rows = uniform(kWRows * parts);
-  const int tok_step = uniform((int)((unsigned)part_rows / (unsigned)a.group));
-  const int rem_step = part_rows - tok_step * a.group;
+  const int tok_step = uniform((int)((unsigned)kWRows / (unsigned)a.group));
+  const int rem_step = kWRows - tok_step * a.group;
   int ld_row = uniform(tile0 * kWRows);  // of the tile that is loaded next; its token and what is left
   int ld_tok = uniform((int)((unsigned)ld_row / (unsigned)a.group));
   int ld_rem = ld_row - ld_tok * a.group;
@@ -393,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       int tok, head;
 #pragma unroll
       for (int u = 0; u < QL; ++u) {
-        place((int)threadIdx.x / RL + u * (kThreads / RL), tok, head);
-        q_off[u] = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (int)(threadIdx.x % RL);
+        place(tid / RL + u * (kThreads / RL), tok, head);
+        q_off[u] = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (int)(tid % RL);
       }
-      place(threadIdx.x, tok, head);
+      place(tid, tok, head);
       lse_off = head * a.tokens + tok;
     }
     const __amdgpu_buffer_rsrc_t rq =
@@ -404,11 +491,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
 #pragma unroll
     for (int u = 0; u < QL; ++u)
       q_next[u] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rq, q_off[u], 0, 0));
-    if (threadIdx.x < kWRows) {
+    if (tid < kWRows) {
       const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
-      lse_next = (int)threadIdx.x <= end ? weigh_lse2(lse[lse_off]) : __builtin_inff();
+      lse_next = tid <= end ? weigh_lse2(lse[lse_off]) : __builtin_inff();
     }
-    ld_row += part_rows;
+    ld_row += kWRows;
     ld_tok += tok_step;
     ld_rem += rem_step;
     if (ld_rem >= a.group) {
@@ -419,10 +506,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   auto store = [&](int buf) {
 #pragma unroll
     for (int u = 0; u < QL; ++u) {
-      const int r = (int)threadIdx.x / RL + u * (kThreads / RL), c = threadIdx.x % RL;
+      const int r = tid / RL + u * (kThreads / RL), c = tid % RL;
       *(half8*)(q_lds[buf] + r * L::Pitch + 8 * (c ^ ((r >> 2) & 3))) = q_next[u];
     }
-    if (threadIdx.x < kWRows) lse_lds[buf][threadIdx.x] = -lse_next;
+    if (tid < kWRows) lse_lds[buf][tid] = -lse_next;
   };
   // (the swizzle moves the two low bits of a chunk's number: one base for even steps, one for odd)
   const int swz = (l32 >> 2) & 3;
@@ -434,7 +521,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   };
   float sum[2] = {0.0f, 0.0f};
   float16v st[2][2];
-  const int count = tile0 < tiles ? uniform((int)((unsigned)(tiles - tile0 + parts - 1) / (unsigned)parts)) : 0;
   // Half H of step i: the probabilities of these 32 rows, whose S is st[H], between the MFMAs of the
   // next 32's (behind the last tile: of what is there, for nobody).  Tiles i and i + 1 are in buffers
   // `now` and `next`; tile i + 2 goes to `free`, which held tile i - 1, and is loaded a step before.
@@ -445,9 +531,9 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     const int buf = H == 0 ? now : next;
     static_for<PF>([&](auto k_c) { qf[decltype(k_c)::value] = read_q(buf, 1 - H, decltype(k_c)::value); });
     float4v nl[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) nl[g] = *(const float4v*)(lse_lds[now] + 32 * H + 8 * g + 4 * hi);
-    const int row0 = (tile0 + i * parts) * kWRows + 32 * H + 4 * hi;
+    auto read_lse = [&](int g) { return *(const float4v*)(lse_lds[now] + 32 * H + 8 * g + 4 * hi); };
+    nl[0] = read_lse(0);
+    const int row0 = (tile0 + i) * kWRows + 32 * H + 4 * hi;
     const int lim[2] = {from[0] - row0, from[1] - row0};
     float add[2] = {0.0f, 0.0f};
     fence_schedule();
@@ -455,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       constexpr int slot = decltype(slot_c)::value;
       constexpr int kk = slot / 2, v = slot % 2;
       if constexpr (v == 0 && kk + PF < KK) qf[kk + PF] = read_q(buf, 1 - H, kk + PF);
+      if constexpr (slot % (NS / 4) == 1 && slot / (NS / 4) < 3) nl[slot / (NS / 4) + 1] = read_lse(slot / (NS / 4) + 1);
       if constexpr (H == 1 && slot == NS / 4) {
         if (i + 2 < count) store(free);
       }
@@ -496,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     // Tiles before `all_from` hide a key from some row.
-    const int hiding = uniform((int)((unsigned)(max(0, all_from - tile0 * kWRows) + part_rows - 1) / (unsigned)part_rows));
+    const int hiding = uniform((int)((unsigned)(max(0, all_from - tile0 * kWRows) + kWRows - 1) / kWRows));
     int now = 0, next = 1, free = 2;
     for (int i = 0; i < count; ++i) {
       if (i < hiding) {
@@ -518,51 +605,60 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   sum[1] = halves_sum(sum[1]);
   const bool mine = hi ? held[1] : held[0];
   const float x = mine ? (hi ? sum[1] : sum[0]) : 0.0f;
-  const int j = key0 + (int)threadIdx.x;
+  const int j = key0 + tid;
   float* const out = w.out + b * w.sb + hkv * w.sh + j;
-  if (parts == 1) {
+  if (cuts == 0 || (t0 == 0 && u0 + t1 == u1)) {
     if (j < w.max_len && (mine || !w.add)) *out = w.add ? *out + x : x;
-    return;
+    barrier_after_loads<63>();  // the next unit's rows go into these buffers
+    continue;
   }
-  // A record for each part, and one of what the first part finds there; coherent over the L2s.
-  const __amdgpu_buffer_rsrc_t rec = make_rsrc(w.partial, 2 * kWTarget * kWBlock * 4);
-  auto at_record = [&](int p) { return ((unit * (parts + 1) + p) * kWBlock + (int)threadIdx.x) * 4; };
-  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), rec, at_record(part), 0, kPCoherent);
-  if (part == 0 && w.add) {
+  // A record for each workgroup's piece of a unit that it begins and of one that it does not, and one of
+  // what the first piece's finds there; coherent over the L2s.
+  const __amdgpu_buffer_rsrc_t rec = make_rsrc(w.partial, 3 * w.wgs * kWBlock * 4);
+  auto at_record = [&](int r) { return (r * kWBlock + tid) * 4; };
+  const int record = 2 * place + (t0 == 0 ? 1 : 0);
+  const int from_place = uniform(holder(u0)), pieces = uniform(holder(u1 - 1)) - from_place + 1;
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), rec, at_record(record), 0, kPCoherent);
+  if (t0 == 0 && w.add) {
     const float before = j < w.max_len ? *out : 0.0f;
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, before), rec, at_record(parts), 0, kPCoherent);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, before), rec, at_record(2 * w.wgs + place), 0,
+                                          kPCoherent);
   }
   // (see last_to_finish, fa_paged_units.h: whoever sets the last flag sees them all)
-  const __amdgpu_buffer_rsrc_t rf = make_rsrc(w.flags, kWTarget * 8);
+  const __amdgpu_buffer_rsrc_t rf = make_rsrc(w.flags, 2 * w.wgs * 8);
+  auto piece = [&](int p) { return 2 * (from_place + p) + (p == 0 ? 1 : 0); };
   wait_loads<0>();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, w.mark), rf, (unit * parts + part) * 8, 0, kPCoherent);
+  if (tid == 0) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, w.mark), rf, record * 8, 0, kPCoherent);
     wait_loads<0>();
   }
   __syncthreads();
   bool set = true;
-  for (int p = threadIdx.x; p < parts; p += kThreads)
-    set = set && __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(rf, (unit * parts + p) * 8, 0,
-                                                                                    kPCoherent)) == w.mark;
+  for (int p = tid; p < pieces; p += kThreads)
+    set = set && __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(rf, piece(p) * 8, 0, kPCoherent)) ==
+                     w.mark;
   const bool all = __builtin_amdgcn_ballot_w64(!set) == 0;
   if (lane == 0) scratch[wave] = all;
   __syncthreads();
-  if (!(scratch[0] && scratch[1] && scratch[2] && scratch[3])) return;
+  const bool last = scratch[0] && scratch[1] && scratch[2] && scratch[3];
+  __syncthreads();
+  if (!last) continue;
   // Two that both get here store the same values.
-  auto get = [&](int p) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rec, at_record(p), 0, kPCoherent));
+  auto get = [&](int r) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rec, at_record(r), 0, kPCoherent));
   };
   float y = 0.0f;
-  for (int p = 0; p < parts; p += 8) {
+  for (int p = 0; p < pieces; p += 8) {
     float z[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) z[u] = get(min(p + u, parts - 1));
+    for (int u = 0; u < 8; ++u) z[u] = get(piece(min(p + u, pieces - 1)));
 #pragma unroll
-    for (int u = 0; u < 8; ++u) y += p + u < parts ? z[u] : 0.0f;
+    for (int u = 0; u < 8; ++u) y += p + u < pieces ? z[u] : 0.0f;
   }
-  if (w.add) y += get(parts);
+  if (w.add) y += get(2 * w.wgs + from_place);
   if (j < w.max_len && (mine || !w.add)) *out = y;
+  }
 }
 
 }  // namespace

@@ -19,11 +19,14 @@ WeighPlan plan_weigh(const WeighArgs& a, int64_t max_query_len, int64_t workspac
   WeighPlan p{};
   const int64_t pairs = (int64_t)a.p.batch * a.p.hkv;
   if (max_query_len * a.p.group > 32) {
-    // A workgroup for each block of keys there is room for, and for the parts of those that are cut.
-    constexpr int64_t kBytes = (2 * kWBlock * 4 + 8) * (int64_t)kWTarget;
-    p.split = workspace_bytes >= kBytes;
-    p.workspace_bytes = p.split ? kBytes : 0;
-    p.grid = ((int64_t)a.max_len + kWBlock - 1) / kWBlock * pairs + (p.split ? kWTarget : 0);
+    // A workgroup for each block of keys there is room for, and as many as run at once for those that
+    // are cut (fewer units than that, whose row tiles' numbers on the line have 31 bits).
+    const int wgs = resident_fused_workgroups();
+    const int64_t bytes = (3ll * kWBlock * 4 + 2 * 8) * wgs;
+    const bool counted = (a.p.tokens * a.p.group / kWRows + 1) * wgs <= INT32_MAX;
+    p.wgs = counted && workspace_bytes >= bytes ? wgs : 0;
+    p.workspace_bytes = p.wgs > 0 ? bytes : 0;
+    p.grid = ((int64_t)a.max_len + kWBlock - 1) / kWBlock * pairs + p.wgs;
     return p;
   }
   p.rows = max_query_len * a.p.group <= 16 ? 16 : 32;
@@ -55,12 +58,12 @@ static void launch_typed(const WeighArgs& a, const WeighPlan& plan, hipStream_t 
 int launch_weigh(const WeighArgs& args, const WeighPlan& plan, int head_dim, void* workspace, hipStream_t stream) {
   WeighArgs a = args;
   a.waves = plan.waves;
-  a.split = plan.split ? 1 : 0;
+  a.wgs = plan.wgs;
   a.p.inv_group = 1.0f / (float)a.p.group;
-  if (plan.split) {
+  if (plan.wgs > 0) {
     a.partial = static_cast<float*>(workspace);
-    a.flags = reinterpret_cast<uint64_t*>(a.partial + 2 * kWTarget * kWBlock);
-    a.mark = merge_mark(a.flags, kWTarget, stream);
+    a.flags = reinterpret_cast<uint64_t*>(a.partial + 3ll * plan.wgs * kWBlock);
+    a.mark = merge_mark(a.flags, 2 * plan.wgs, stream);
   }
   if (head_dim == 64) launch_typed<64>(a, plan, stream);
   else launch_typed<128>(a, plan, stream);
