@@ -132,7 +132,7 @@ void launch_paged_combine(const StageArgs<STAGE>& a, int rows, int y, hipStream_
 // The weights that attention gave the cached rows: out[b, h, j] (+)= sum over the new tokens
 // i of sequence b that see key j, and the query heads of KV head h, of exp(scale q k - lse).
 struct WeighArgs {
-  PagedArgs p;       // q, table, lens, ..; lse_in below in place of lse
+  PagedArgs p;       // q, table, lens, ..; lse below in place of its own
   const float* lse;  // [hq, tokens]
   float* out;        // out[b, h, j] at b * sb + h * sh + j, j < max_len
   int64_t sb, sh;

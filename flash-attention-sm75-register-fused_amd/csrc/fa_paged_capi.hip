@@ -224,7 +224,8 @@ int make_weigh(const fa_paged_weigh_params* p, fa::WeighArgs* w, bool* nothing) 
   bool empty = true;
   if (int st = make_forward(&f, &w->p, &empty)) return st;
   if (!empty && p->lse == nullptr) return capi_fail(FA_ERR_INVALID_ARGUMENT, "lse must not be NULL");
-  // 32 rows of one KV head's queries are read through one window, by products of 24 bits.
+  // 64 rows of one KV head's queries (33 tokens, or of one head 64) are read through one window, by
+  // products of 24 bits.
   constexpr int64_t kStride = 1 << 23;
   if (!empty && (p->q_stride_t >= kStride || p->q_stride_h >= kStride || w->p.group >= kStride ||
                  33 * p->q_stride_t + w->p.group * p->q_stride_h >= 1 << 30))

@@ -342,7 +342,7 @@ struct PrefixLine {
       before += wave_bcast(x, 63);
     }
   }
-  // What the second launch goes by (PagedArgs::joint_info); one wave of the launch.
+  // What the second launch goes by (joint_info); one wave of the launch.
   __device__ __forceinline__ void publish() const {
     int before = 0;
     for (int g0 = 0; g0 < a.batch; g0 += 64) {

@@ -20,11 +20,10 @@ WeighPlan plan_weigh(const WeighArgs& a, int64_t max_query_len, int64_t workspac
   const int64_t pairs = (int64_t)a.p.batch * a.p.hkv;
   if (max_query_len * a.p.group > 32) {
     // A workgroup for each block of keys there is room for, and as many as run at once for those that
-    // are cut (fewer units than that, whose row tiles' numbers on the line have 31 bits).
+    // are cut (fewer units than that, of at most 2^27 rows in all: tiles on the line have 31 bits).
     const int wgs = resident_fused_workgroups();
     const int64_t bytes = (3ll * kWBlock * 4 + 2 * 8) * wgs;
-    const bool counted = (a.p.tokens * a.p.group / kWRows + 1) * wgs <= INT32_MAX;
-    p.wgs = counted && workspace_bytes >= bytes ? wgs : 0;
+    p.wgs = workspace_bytes >= bytes ? wgs : 0;
     p.workspace_bytes = p.wgs > 0 ? bytes : 0;
     p.grid = ((int64_t)a.max_len + kWBlock - 1) / kWBlock * pairs + p.wgs;
     return p;

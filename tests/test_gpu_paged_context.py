@@ -317,6 +317,25 @@ def test_weights_long(device, d, q8):
     weigh(Cache([900], 1, d, 16, FP16, q8, news=[900]), device, 4)
 
 
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 1), (7, 1), (14, 2), (100, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_prompts(device, hq, hkv, causal):
+    """Blocks of new keys, which fewer rows see, next to old ones, dealt in equal stretches."""
+    weigh(Cache([1500], hkv, 64, 16, FP16, False, news=[1500]), device, hq, causal=causal)
+    weigh(Cache([1000, 0, 700, 300], hkv, 128, 16, BF16, True, news=[333, 0, 1000, 7]), device, hq, causal=causal)
+
+
+def test_weights_prompts_of_many_sequences(device):
+    lens = [(37 * i) % 301 for i in range(70)]
+    weigh(Cache(lens, 2, 64, 16, BF16, False, news=[max(0, x - (i % 3) * 50) for i, x in enumerate(lens)]), device, 6)
+
+
+@pytest.mark.parametrize("max_len", [1, 256, 700, 1700])
+def test_weights_prompts_max_len(device, max_len):
+    w = weigh(Cache([1500, 90], 2, 64, 16, FP16, False, news=[1100, 80]), device, 8, max_len=max_len)
+    assert w.shape == (2, 2, max_len)
+
+
 @pytest.mark.parametrize("max_len", [1, 31, 33, 100, 333, 1000])
 def test_weights_max_len(device, max_len):
     """Positions past max_len are not weighed, those past the sequence get 0; rows still see all keys."""
