@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 //
 // A unit is 256 keys of one (sequence, KV head), a wave's 64 of them in its registers as the B
 // operand of 32x32x16 MFMAs; the sequence's rows that see them come by, 64 at a time, through LDS
-// (three buffers, each row's -lse log2 e beside it), the probabilities of 32 rows between the
+// (four buffers, loaded directly two steps ahead, each row's -lse log2 e beside it), the probabilities of 32 rows between the
 // MFMAs of the next 32.  Where units are many, each is a workgroup's; else their row tiles (under the
 // causal rule a unit of new keys has fewer) are a line, of which each workgroup takes an equal stretch;
 // the workgroups of a unit leave their sums, and the last of them to finish adds those up in their
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 // to two whole rounds the line costs 4%, 155 us for 149).
 //
 // Bound: the matrix units and the exponentials take turns on a SIMD.  The last 2048 tokens of 8192,
-// 32 heads of 128 on 8, are 120 GFLOP in 150 us (0.8 PFLOP/s), the matrix units busy 43% of them;
-// without the exponentials 137, without MFMAs 147, without loads 129.
+// 32 heads of 128 on 8, are 120 GFLOP in 142 us (0.85 PFLOP/s); rows loaded through registers, one
+// step ahead, 154.
 constexpr int kWRows = 64;      // rows of a tile, two of S
 constexpr int kWMinTiles = 8;   // tiles a stretch has at least
 
@@ -312,17 +312,27 @@ struct WeighTiles {
   }
 };
 
+template <int D>
+__device__ __forceinline__ int weigh_swizzle(int r) {
+  if constexpr (D == 64) return dense_swizzle(r);
+  return r & 15;
+}
+
 template <int D, bool BF16, bool FP8>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const WeighArgs w) {
   using E = Elem<BF16>;
-  using L = Lds<D>;
   constexpr int KK = D / 16;               // contraction steps of S
-  constexpr int RL = D / 8;                // threads that bring a row of Q
-  constexpr int QL = kWRows * RL / kThreads;  // loads of a thread
+  constexpr int QL = kWRows * D * 2 / 1024 / kWaves;  // 1 KB loads of a wave's 16 rows
   constexpr int NS = 2 * KK;               // MFMAs of 32 rows
   constexpr int PF = 3;                    // Q operand reads run this many steps ahead
-  __shared__ __attribute__((aligned(16))) _Float16 q_lds[3][kWRows * L::Pitch];
-  __shared__ __attribute__((aligned(16))) float lse_lds[3][kWRows];
+  // Tile t's rows are in buffer t % 4.  (Distinct objects, so that the compiler sees that loads in
+  // flight into one do not touch those being read.)  Chunk c of 8 dimensions of row r is at
+  // c ^ weigh_swizzle(r): 16 rows' chunks of one number are in 16 different places of the banks.
+  __shared__ __attribute__((aligned(1024))) _Float16 q_lds0[kWRows * D];
+  __shared__ __attribute__((aligned(1024))) _Float16 q_lds1[kWRows * D];
+  __shared__ __attribute__((aligned(1024))) _Float16 q_lds2[kWRows * D];
+  __shared__ __attribute__((aligned(1024))) _Float16 q_lds3[kWRows * D];
+  __shared__ __attribute__((aligned(16))) float lse_lds[4][kWRows];
   __shared__ int scratch[kWaves];
   const PagedArgs& a = w.p;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -456,7 +466,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   const float c2 = a.negate_q ? -a.c : a.c;
   // Loads of a tile's rows go through windows from its first row's token and the first head of the
   // group on, with offsets below 2^31 bytes (the launcher sees to it), whose factors have 24 bits.
-  half8 q_next[QL];
   float lse_next;
   const int q_tok = 2 * (int)a.qt, q_head = 2 * (int)a.qh;  // in bytes
   const int tok_step = uniform((int)((unsigned)kWRows / (unsigned)a.group));
@@ -464,11 +473,15 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   int ld_row = uniform(tile0 * kWRows);  // of the tile that is loaded next; its token and what is left
   int ld_tok = uniform((int)((unsigned)ld_row / (unsigned)a.group));
   int ld_rem = ld_row - ld_tok * a.group;
-  // Offsets of the thread's rows: they follow from what is left of the tile's first token, which often is
+  // Offsets of the lane's rows: they follow from what is left of the tile's first token, which often is
   // the same for all tiles, and, of the last tile, from where the rows end (the last row again for those
   // behind it).
   int q_off[QL], lse_off = 0, aimed = -1;
-  auto load = [&] {
+  auto q_buf = [&](auto t_c) -> _Float16* {
+    constexpr int B = decltype(t_c)::value % 4;
+    return B == 0 ? q_lds0 : B == 1 ? q_lds1 : B == 2 ? q_lds2 : q_lds3;
+  };
+  auto load = [&](auto t_c) {  // (t_c: the tile's number, modulo 4)
     const int end = nrows - 1 - ld_row;
     if (ld_rem != aimed || end < kWRows - 1) {
       aimed = ld_rem;
@@ -480,20 +493,23 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       int tok, head;
 #pragma unroll
       for (int u = 0; u < QL; ++u) {
-        place(tid / RL + u * (kThreads / RL), tok, head);
-        q_off[u] = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (int)(tid % RL);
+        const int at = 1024 * u + 16 * lane, r = 16 * wave + at / (2 * D);
+        place(r, tok, head);
+        q_off[u] = __umul24(tok, q_tok) + __umul24(head, q_head) + 16 * (((at >> 4) & (D / 8 - 1)) ^ weigh_swizzle<D>(r));
       }
-      place(tid, tok, head);
+      place(lane, tok, head);
       lse_off = head * a.tokens + tok;
     }
+    const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
+    lse_next = lane <= end ? lse[lse_off] : -__builtin_inff();
+    fence_schedule();  // (the LSE is waited for first)
     const __amdgpu_buffer_rsrc_t rq =
         make_rsrc(a.q + (int64_t)(s.t0 + ld_tok) * a.qt + (int64_t)hkv * a.group * a.qh, INT32_MAX);
 #pragma unroll
-    for (int u = 0; u < QL; ++u)
-      q_next[u] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rq, q_off[u], 0, 0));
-    if (tid < kWRows) {
-      const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
-      lse_next = tid <= end ? weigh_lse2(lse[lse_off]) : __builtin_inff();
+    for (int u = 0; u < QL; ++u) {
+      int off = (QL * wave + u) * 512;
+      asm volatile("" : "+s"(off));  // recomputed at each load, not kept in a register
+      direct_load16(rq, (lds_void*)(q_buf(t_c) + off), q_off[u]);
     }
     ld_row += kWRows;
     ld_tok += tok_step;
@@ -503,35 +519,30 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       ++ld_tok;
     }
   };
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int u = 0; u < QL; ++u) {
-      const int r = tid / RL + u * (kThreads / RL), c = tid % RL;
-      *(half8*)(q_lds[buf] + r * L::Pitch + 8 * (c ^ ((r >> 2) & 3))) = q_next[u];
-    }
-    if (tid < kWRows) lse_lds[buf][tid] = -lse_next;
+  auto store_lse = [&](int buf) {
+    if (tid < kWRows) lse_lds[buf][tid] = -weigh_lse2(lse_next);
   };
-  // (the swizzle moves the two low bits of a chunk's number: one base for even steps, one for odd)
-  const int swz = (l32 >> 2) & 3;
-  const int q_even = l32 * L::Pitch + 8 * ((FP8 ? 2 * hi : hi) ^ swz);
-  const int q_odd = l32 * L::Pitch + 8 * ((FP8 ? 2 * hi + 1 : 2 + hi) ^ swz);
-  auto read_q = [&](int buf, int half, int kk) -> half8 {
-    const _Float16* const base = q_lds[0] + buf * (kWRows * L::Pitch) + ((kk & 1) ? q_odd : q_even);
-    return *(const half8*)(base + 32 * half * L::Pitch + 32 * (kk >> 1));
+  int q_base[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)
+    q_base[kk] = l32 * D + 8 * ((FP8 ? 4 * (kk >> 1) + 2 * hi + (kk & 1) : 2 * kk + hi) ^ weigh_swizzle<D>(l32));
+  auto read_q = [&](const _Float16* buf, int half, int kk) -> half8 {
+    return *(const half8*)(buf + q_base[kk] + 32 * half * D);
   };
   float sum[2] = {0.0f, 0.0f};
   float16v st[2][2];
-  // Half H of step i: the probabilities of these 32 rows, whose S is st[H], between the MFMAs of the
-  // next 32's (behind the last tile: of what is there, for nobody).  Tiles i and i + 1 are in buffers
-  // `now` and `next`; tile i + 2 goes to `free`, which held tile i - 1, and is loaded a step before.
-  auto half_step = [&](int i, int now, int next, int free, auto half_t, auto masked_t) {
+  // Half H of step i (I: modulo 4): the probabilities of these 32 rows, whose S is st[H], between the
+  // MFMAs of the next 32's (behind the last tile: of what is there, for nobody).  Tile i + 3 is loaded
+  // to where tile i - 1 was, straight to LDS.
+  auto half_step = [&](int i, auto i_t, auto half_t, auto masked_t) {
+    constexpr int I = decltype(i_t)::value;
     constexpr int H = decltype(half_t)::value;
     constexpr bool MASKED = decltype(masked_t)::value;
     half8 qf[KK];
-    const int buf = H == 0 ? now : next;
+    const _Float16* const buf = q_buf(std::integral_constant<int, I + H>{});
     static_for<PF>([&](auto k_c) { qf[decltype(k_c)::value] = read_q(buf, 1 - H, decltype(k_c)::value); });
     float4v nl[4];
-    auto read_lse = [&](int g) { return *(const float4v*)(lse_lds[now] + 32 * H + 8 * g + 4 * hi); };
+    auto read_lse = [&](int g) { return *(const float4v*)(lse_lds[I] + 32 * H + 8 * g + 4 * hi); };
     nl[0] = read_lse(0);
     const int row0 = (tile0 + i) * kWRows + 32 * H + 4 * hi;
     const int lim[2] = {from[0] - row0, from[1] - row0};
@@ -542,11 +553,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       constexpr int kk = slot / 2, v = slot % 2;
       if constexpr (v == 0 && kk + PF < KK) qf[kk + PF] = read_q(buf, 1 - H, kk + PF);
       if constexpr (slot % (NS / 4) == 1 && slot / (NS / 4) < 3) nl[slot / (NS / 4) + 1] = read_lse(slot / (NS / 4) + 1);
-      if constexpr (H == 1 && slot == NS / 4) {
-        if (i + 2 < count) store(free);
+      if constexpr (H == 0 && slot == NS / 4) {
+        if (i + 2 < count) store_lse((I + 2) % 4);
       }
-      if constexpr (H == 1 && slot == NS / 2) {
-        if (i + 3 < count) load();
+      if constexpr (H == 0 && slot == NS / 2) {
+        if (i + 3 < count) load(std::integral_constant<int, I + 3>{});
       }
       st[1 - H][v] = E::mfma(qf[kk], kf[v][kk], kk == 0 ? (float16v)0.0f : st[1 - H][v]);
       // Rows 8 g + 4 hi + r of the 32 in register 4 g + r.
@@ -566,38 +577,47 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     sum[1] += add[1];
   };
   if (count > 0) {
-    load();
-    store(0);
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+    load(I0{});
+    store_lse(0);
     if (count > 1) {
-      load();
-      store(1);
+      load(I1{});
+      store_lse(1);
     }
-    if (count > 2) load();
-    barrier_after_loads<63>();
+    if (count > 2) load(I2{});
+    barrier_after_loads<0>();
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
       st[0][v] = (float16v)0.0f;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) st[0][v] = E::mfma(read_q(0, 0, kk), kf[v][kk], st[0][v]);
+      for (int kk = 0; kk < KK; ++kk) st[0][v] = E::mfma(read_q(q_lds0, 0, kk), kf[v][kk], st[0][v]);
     }
-    using I0 = std::integral_constant<int, 0>;
-    using I1 = std::integral_constant<int, 1>;
     // Tiles before `all_from` hide a key from some row.
     const int hiding = uniform((int)((unsigned)(max(0, all_from - tile0 * kWRows) + kWRows - 1) / kWRows));
-    int now = 0, next = 1, free = 2;
-    for (int i = 0; i < count; ++i) {
+    auto step = [&](int i, auto i_t) {
       if (i < hiding) {
-        half_step(i, now, next, free, I0{}, Flag<true>{});
-        half_step(i, now, next, free, I1{}, Flag<true>{});
+        half_step(i, i_t, I0{}, Flag<true>{});
+        half_step(i, i_t, I1{}, Flag<true>{});
       } else {
-        half_step(i, now, next, free, I0{}, Flag<false>{});
-        half_step(i, now, next, free, I1{}, Flag<false>{});
+        half_step(i, i_t, I0{}, Flag<false>{});
+        half_step(i, i_t, I1{}, Flag<false>{});
       }
-      barrier_after_loads<63>();
-      const int done = now;
-      now = next;
-      next = free;
-      free = done;
+      // Tile i + 2 has landed, tile i + 3 need not have.
+      if (i + 3 < count) barrier_after_loads<QL>();
+      else barrier_after_loads<0>();
+    };
+    for (int i = 0;; i += 4) {
+      step(i, I0{});
+      if (i + 1 >= count) break;
+      step(i + 1, I1{});
+      if (i + 2 >= count) break;
+      step(i + 2, I2{});
+      if (i + 3 >= count) break;
+      step(i + 3, I3{});
+      if (i + 4 >= count) break;
     }
   }
   // Thread: a key of its wave's 64.
