@@ -275,17 +275,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 //
 // A unit is 256 keys of one (sequence, KV head), a wave's 64 of them in its registers as the B
 // operand of 32x32x16 MFMAs; the sequence's rows that see them come by, 64 at a time, through LDS
-// (four buffers, loaded directly two steps ahead, each row's -lse log2 e beside it), the probabilities of 32 rows between the
-// MFMAs of the next 32.  Where units are many, each is a workgroup's; else their row tiles (under the
-// causal rule a unit of new keys has fewer) are a line, of which each workgroup takes an equal stretch;
-// the workgroups of a unit leave their sums, and the last of them to finish adds those up in their
-// order (each unit's rows dealt to whole parts left a second round and idle CUs: at a prompt of
-// 4096 tokens 116 us for 97, at five of 700 .. 2000 of 14 heads of 64 42 for 35; where the parts came
-// to two whole rounds the line costs 4%, 155 us for 149).
+// (four buffers, loaded directly, two steps ahead; each row's -lse log2 e beside them), the
+// probabilities of 32 rows between the MFMAs of the next 32.  Where units are many, each is a
+// workgroup's; else their row tiles (under the causal rule a unit of new keys has fewer) are a line, of
+// which each workgroup takes an equal stretch; the workgroups of a unit leave their sums, and the last
+// of them to finish adds those up in their order (each unit's rows dealt to whole parts left a second
+// round and idle CUs: at a prompt of 4096 tokens 116 us for 97, at five of 700 .. 2000 of 14 heads of
+// 64 42 for 35; where the parts came to two whole rounds the line costs 4%).
 //
-// Bound: the matrix units and the exponentials take turns on a SIMD.  The last 2048 tokens of 8192,
-// 32 heads of 128 on 8, are 120 GFLOP in 142 us (0.85 PFLOP/s); rows loaded through registers, one
-// step ahead, 154.
+// Bound: the matrix units, the exponentials and the sums share a SIMD's two waves.  The last 2048
+// tokens of 8192, 32 heads of 128 on 8, are 120 GFLOP in 142 us (0.85 PFLOP/s), the matrix units 44%
+// busy; rows loaded through registers, one step ahead, 154.
 constexpr int kWRows = 64;      // rows of a tile, two of S
 constexpr int kWMinTiles = 8;   // tiles a stretch has at least
 
