@@ -78,10 +78,16 @@ struct PagedArgs {
 // the states of the rows over pieces of their prefix go to records of joint_o and joint_ml, where
 // which are is in joint_info.  Of the sequences' own keys (kOwn): rows whose sequence has one of the
 // `prefixes` join those states.
-constexpr int kPrefix = 1, kOwn = 2;  // (0: no prefixes)
+// Or in one (kBoth), where few bytes are read again and again: a sequence's tiles are those of its
+// prefix, the last one not full, and then its own.
+constexpr int kPrefix = 1, kOwn = 2, kBoth = 3;  // (0: no prefixes)
 struct PagedShared : PagedArgs {
   const int32_t* groups;
   int prefixes, seqs;
+  const int32_t* pre_table;  // the prefixes' table and lens
+  const int32_t* pre_lens;
+  int64_t pre_stride;
+  int pre_pages;
   float* joint_o;
   float* joint_ml;
   int32_t* joint_info;  // of each prefix: first item of its class's, pieces of a unit, first token, tokens
@@ -116,12 +122,16 @@ int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_d
                            void* workspace, hipStream_t stream);
 int launch_paged_attention(const PagedShared& own, const PagedPlan& plan, int head_dim,
                            void* workspace, hipStream_t stream);
+// Whether prefixes and own keys are one launch, and its plan and launch.
+bool joins_prefixes(const PagedShared& own, int head_dim, int64_t max_query_len);
+PagedPlan plan_joined(const PagedShared& own, int head_dim, int64_t max_query_len, int64_t workspace_bytes);
+int launch_paged_joined(const PagedShared& own, const PagedPlan& plan, int head_dim, void* workspace, hipStream_t stream);
 // The launch over shared prefixes (workspace_bytes: what joint_o, joint_ml and joint_info take).
 PagedPlan plan_prefix(const PagedShared& a, int head_dim, int64_t max_queries);
 // Sets the joint fields of both stages' arguments, and launches the first.
 int launch_paged_prefix(PagedShared& prefix, PagedShared& own, const PagedPlan& plan, int head_dim, void* workspace,
                         hipStream_t stream);
-// STAGE: 0, or of attention behind shared prefixes kPrefix (chunks only) or kOwn.
+// STAGE: 0, or of attention behind shared prefixes kPrefix (chunks only), kOwn or kBoth (no chunks).
 template <int D, bool BF16, bool FP8, int STAGE>
 void launch_paged_attn(const StageArgs<STAGE>& a, int rows, int64_t grid, hipStream_t stream);
 template <int D, bool BF16, bool FP8, int STAGE>

@@ -13,6 +13,7 @@ namespace fa {
 #define FA_PAGED_EXTERN(D, BF, F8)                                                                     \
   extern template void launch_paged_attn<D, BF, F8, 0>(const PagedArgs&, int, int64_t, hipStream_t);      \
   extern template void launch_paged_attn<D, BF, F8, kOwn>(const PagedShared&, int, int64_t, hipStream_t); \
+  extern template void launch_paged_attn<D, BF, F8, kBoth>(const PagedShared&, int, int64_t, hipStream_t); \
   extern template void launch_paged_chunk<D, BF, F8, 0>(const PagedArgs&, int64_t, hipStream_t);          \
   extern template void launch_paged_chunk<D, BF, F8, kPrefix>(const PagedShared&, int64_t, hipStream_t);  \
   extern template void launch_paged_chunk<D, BF, F8, kOwn>(const PagedShared&, int64_t, hipStream_t);
@@ -28,6 +29,7 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
 }
 constexpr int64_t kLastCacheBytes = 256 << 20;
 constexpr int kOwnShort = 1536;
+constexpr int64_t kJoinBytes = 128 << 20;
 constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 16 bytes
 }  // namespace
 
@@ -114,6 +116,24 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   return p;
 }
 
+// Up to 32 rows of a KV head, where every sequence reads its prefix anew: mostly from the caches, at 12
+// TB/s, which up to the bytes that the tables have room for costs less than a launch over the prefixes, their
+// records and what joins them (us in two launches and in one: 4 tokens of 14 over 2 heads d64 behind 1000,
+// 2 MB in all, 16.7 / 13.2; of 32 over 8 d128 behind 1000, 2 of them 8 MB 22.4 / 11.9, 8 31 MB 26.7 /
+// 15.5, 32 125 MB 32.4 / 25.1, 64 250 MB 29.3 / 37.9; 8 behind 8000 250 MB 32.5 / 32.7, 8 bits 125 MB
+// 35.7 / 27.3; 64 of 2 heads d64 behind 4000, 125 MB, 20.2 / 22.3).
+bool joins_prefixes(const PagedShared& own, int head_dim, int64_t max_query_len) {
+  const int64_t room = ((int64_t)own.pre_pages << own.page_shift) * own.hkv * own.batch;
+  return max_query_len * own.group <= 32 && own.batch <= 64 && own.prefixes <= 63 &&
+         room * 2 * head_dim * (own.ks != nullptr ? 1 : 2) <= kJoinBytes;
+}
+
+PagedPlan plan_joined(const PagedShared& own, int head_dim, int64_t max_query_len, int64_t workspace_bytes) {
+  PagedArgs a = own;  // as wide as both tables (and a tile that the prefix's last leaves open)
+  a.max_pages += own.pre_pages + (kPTile >> std::min(a.page_shift, 5));
+  return plan_paged(a, head_dim, max_query_len, workspace_bytes);
+}
+
 PagedPlan plan_prefix(const PagedShared& a, int head_dim, int64_t max_queries) {
   PagedPlan p{};
   p.chunk = p.split = true;
@@ -133,7 +153,7 @@ PagedPlan plan_prefix(const PagedShared& a, int head_dim, int64_t max_queries) {
 
 template <int D, bool BF16, int STAGE>
 void launch_paged_combine(const StageArgs<STAGE>& a, int rows, int y, hipStream_t stream) {
-  if (rows == kChunkRows) {
+  if (STAGE != kBoth && rows == kChunkRows) {
     hipLaunchKernelGGL((fa_paged_chunk_combine_kernel<D, BF16, STAGE>),
                        dim3((unsigned)(a.wgs * a.classes), kChunkCombineY), dim3(kThreads), 0, stream, a);
     return;
@@ -151,6 +171,8 @@ static void launch_planned(const StageArgs<STAGE>& a, const PagedPlan& plan, hip
   if constexpr (STAGE == kPrefix) {
     launch_paged_chunk<D, BF16, FP8, STAGE>(a, grid, stream);
     return;
+  } else if constexpr (STAGE == kBoth) {
+    launch_paged_attn<D, BF16, FP8, STAGE>(a, plan.rows, grid, stream);
   } else if (plan.chunk) {
     launch_paged_chunk<D, BF16, FP8, STAGE>(a, grid, stream);
   } else {
@@ -225,6 +247,11 @@ int launch_paged_attention(const PagedArgs& a, const PagedPlan& plan, int head_d
 int launch_paged_attention(const PagedShared& own, const PagedPlan& plan, int head_dim,
                            void* workspace, hipStream_t stream) {
   launch_attention<kOwn>(own, plan, head_dim, workspace, stream);
+  return 0;
+}
+int launch_paged_joined(const PagedShared& own, const PagedPlan& plan, int head_dim, void* workspace,
+                        hipStream_t stream) {
+  launch_attention<kBoth>(own, plan, head_dim, workspace, stream);
   return 0;
 }
 

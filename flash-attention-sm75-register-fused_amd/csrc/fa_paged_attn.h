@@ -38,6 +38,8 @@
 // heads d128, 807 MB: 130 us, 6.2 TB/s; 8 bits, 406 MB: 73 us, 5.6 TB/s; 4 tokens over 131072
 // keys 8 bits: 52 us with its merge kernel, 5.2 TB/s), else the chain of one workgroup (its
 // plan, two tiles a wave, two merges: one token of 4097 keys, 2 KV heads d64, 8.7 us).
+// Behind shared prefixes that each sequence reads for itself (kBoth): 4 tokens of 14 over 2 heads d64 behind
+// 1000 keys 13 us, the chain again.
 // 8-bit tiles cost conversions and LDS stores, whose instructions are not what bounds them:
 // laid out without the stores' bank conflicts, or with deeper loads, they took as long.
 #pragma once
@@ -85,7 +87,7 @@ __device__ __forceinline__ PagedStretch<kPMinTiles> paged_stretch(const PagedArg
   return s;
 }
 
-// STAGE: 0, or kOwn behind shared prefixes.
+// STAGE: 0, or behind shared prefixes kOwn or kBoth.
 template <int D, bool BF16, bool FP8, int NT, int STAGE>
 __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageArgs<STAGE> a) {
   using E = Elem<BF16>;
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int wg = (int)(blockIdx.x >> a.class_shift);
 
-  const PagedLine<R, kPTile, kPAhead> line(a, lane, a.split != 0);
+  const PagedLine<R, kPTile, kPAhead, STAGE == kBoth ? kBoth : 0> line(a, lane, a.split != 0);
   auto stretch = paged_stretch(a, line);
   if (wg >= stretch.active) return;
   int pos, end;
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
   const int r0 = 4 * g4 + (l16 >> 2);
 
   while (pos < end) {
-    const PagedSeq s = line.seq(b);
+    PagedSeq s = line.seq(b);
     const int blocks = paged_blocks<R>(a, s);
     const int unit_len = line.unit_of(s);
     const int len = line.length_of(s);
@@ -167,12 +169,17 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
     const bool whole = first == 0 && pos == u1;
     const int t_begin = first;
     const int t_end = a.split ? stop : (s.keys + kPTile - 1) / kPTile;
+    const PagedPre pre = line.pre_of(b);
+    s.keys -= kPTile * pre.tiles;  // its own
 
     // Columns of this lane, one for each nt: whether they hold a row, and the last
     // key it sees.
     const int nrows = s.n * a.group;
     const PagedRows row_of(a, s, hkv, rb * R);
-    const auto joint = joint_of(a, b, hkv);
+    const auto joint = [&] {
+      if constexpr (STAGE == kBoth) return 0;
+      else return joint_of(a, b, hkv);
+    }();
     const int past = s.len - s.n;  // tokens before the new ones
     int last[NT];
     half8 qf[NT][KS];
@@ -209,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
     const int tok_last = uniform(row_of(min(nrows - rb * R, R) - 1).token) - s.t0;
     const int sees = a.causal ? uniform(clamp_int(past + tok_last + 1, 0, s.keys)) : s.keys;
     const int full = a.causal ? uniform(clamp_int(past + tok_first + 1, 0, s.keys)) : s.keys;
-    const int t_stop = min(t_end, (sees + kPTile - 1) / kPTile);
+    const int t_stop = min(t_end, pre.tiles + (sees + kPTile - 1) / kPTile);
 
     float4v o[NT][MT];
     float m_run[NT], l_run[NT], thr[NT], mc[NT];
@@ -234,18 +241,30 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
     const uint8_t* const vh = a.v + hkv * a.vh;
     // Table entries of a tile's pieces (of the last page, past the table).
     auto look_up = [&](int t, int (&e)[2]) {
+      if constexpr (STAGE == kBoth) {  // (there is a tile to load: one of the tables has pages)
+        const bool shared = t < pre.tiles || a.max_pages == 0;
+        const int32_t* const of = shared ? a.pre_table + pre.group * a.pre_stride : entries;
+        const int t0 = shared ? 0 : pre.tiles, pages = shared ? a.pre_pages : a.max_pages;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          e[p] = load_scalar(of + min(((t - t0) * kPTile + 16 * p) >> a.page_shift, pages - 1));
+        return;
+      }
 #pragma unroll
       for (int p = 0; p < 2; ++p)
         e[p] = load_scalar(entries + min((t * kPTile + 16 * p) >> a.page_shift, a.max_pages - 1));
     };
+    // Tile t's first key, of the prefix's or the own ones, and where those end.
+    auto key_of = [&](int t) { return STAGE == kBoth && t >= pre.tiles ? (t - pre.tiles) * kPTile : t * kPTile; };
+    auto is_shared = [&](int t) { return STAGE == kBoth && t < pre.tiles; };
     // Issues a tile's loads.  A piece in no page or past the keys reads through an
     // empty window: zeros, and no traffic.
     auto load = [&](int t, const int (&e)[2], Tile& x, _Float16* vt) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int key = t * kPTile + 16 * p;
+        const int key = key_of(t) + 16 * p;
         const bool paged = e[p] >= 0 && e[p] < a.num_pages;
-        x.rows[p] = uniform(paged && t < t_stop ? clamp_int(sees - key, 0, 16) : 0);
+        x.rows[p] = uniform(paged && t < t_stop ? clamp_int((is_shared(t) ? pre.keys : sees) - key, 0, 16) : 0);
         const int64_t page = paged ? e[p] : 0;
         const int off = key & ((1 << a.page_shift) - 1);
         const __amdgpu_buffer_rsrc_t rk = make_rsrc(kh + page * a.kp + off * a.kn, x.rows[p] * (int)a.kn);
@@ -281,14 +300,16 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_attn_kernel(const StageA
     // Scores to probabilities of one tile, then P V.
     auto compute = [&](int t, const int (&rows)[2], float4v (&st)[2][NT], const _Float16* vt, auto wait) {
       // Lane group g4 holds keys 16 p + 4 g4 + i of column l16.
-      if ((t + 1) * kPTile > full || rows[0] == 0 || rows[1] == 0) {
+      const bool shared = is_shared(t);
+      const int key0 = key_of(t);
+      if (key0 + kPTile > (shared ? pre.keys : full) || rows[0] == 0 || rows[1] == 0) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (t * kPTile + 16 * p + 4 * g4 + i > last[nt] || rows[p] == 0)
+              if (key0 + 16 * p + 4 * g4 + i > (shared ? pre.keys - 1 : last[nt]) || rows[p] == 0)
                 st[p][nt][i] = -__builtin_inff();
       }
       half8 pf[NT];
@@ -585,8 +606,9 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const StageA
   if (!combine_asked(a)) return;
   const int cls = (int)blockIdx.x & (a.classes - 1);
   const int index = (int)(blockIdx.x >> a.class_shift);  // of the class's units
-  const PagedLine<R, kPTile, kPAhead> line(a, threadIdx.x & 63, true);
-  const PagedLine<R, kPTile, kPAhead> units(a, threadIdx.x & 63, false);
+  using Line = PagedLine<R, kPTile, kPAhead, STAGE == kBoth ? kBoth : 0>;
+  const Line line(a, threadIdx.x & 63, true);
+  const Line units(a, threadIdx.x & 63, false);
   if (index >= units.total()) return;
   int unit_start;
   const int b = uniform(units.find(index, unit_start));
@@ -601,7 +623,10 @@ __global__ void __launch_bounds__(kThreads) fa_paged_combine_kernel(const StageA
   const int hc = unit / blocks;
   const int rb = unit - hc * blocks;
   const int hkv = hc * a.classes + cls;
-  const auto joint = joint_of(a, b, hkv);
+  const auto joint = [&] {
+    if constexpr (STAGE == kBoth) return 0;
+    else return joint_of(a, b, hkv);
+  }();
   const int nr = min(R, s.n * a.group - rb * R);
   if (paged_merges_itself(pieces.count, nr, D)) return;
   const int grp = (int)threadIdx.x / LR, ch = (int)threadIdx.x % LR;

@@ -179,6 +179,10 @@ int make_prefix(const fa_paged_prefix* x, const fa::PagedArgs& a, fa::PagedShare
   own->groups = x->cu_prefix;
   own->prefixes = (int)x->count;
   own->seqs = a.batch;
+  own->pre_table = x->block_table;
+  own->pre_lens = x->lens;
+  own->pre_stride = x->block_table_stride;
+  own->pre_pages = (int)x->max_pages;
   *prefix = *own;
   prefix->batch = (int)x->count;
   prefix->table = x->block_table;
@@ -386,6 +390,8 @@ int64_t fa_sm75_paged_prefix_workspace_size(const fa_paged_params* p, const fa_p
   if (make_forward(p, &a, &empty) != FA_OK || empty || make_prefix(x, a, &prefix, &own) != FA_OK) return 0;
   if (x->count == 0) return fa_sm75_paged_workspace_size(p);
   const int d = (int)p->cache->head_dim;
+  if (fa::joins_prefixes(own, d, longest_query(p)))
+    return fa::plan_joined(own, d, longest_query(p), INT64_MAX).workspace_bytes;
   return fa::plan_prefix(prefix, d, longest_shared(x, a)).workspace_bytes +
          fa::plan_paged(own, d, longest_query(p), INT64_MAX, fa::kOwn).workspace_bytes;
 }
@@ -402,6 +408,10 @@ int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix
   const int d = (int)p->cache->head_dim;
   const hipStream_t stream = static_cast<hipStream_t>(p->stream);
   const int64_t bytes = p->workspace != nullptr ? p->workspace_bytes : 0;
+  if (fa::joins_prefixes(own, d, longest_query(p))) {
+    fa::launch_paged_joined(own, fa::plan_joined(own, d, longest_query(p), bytes), d, p->workspace, stream);
+    return check_launch();
+  }
   const fa::PagedPlan first = fa::plan_prefix(prefix, d, longest_shared(x, a));
   const int64_t rest = bytes - first.workspace_bytes;
   if (rest < 0)

@@ -4,6 +4,7 @@
 
 namespace fa {
 template void launch_paged_attn<128, false, true, kOwn>(const PagedShared&, int, int64_t, hipStream_t);
+template void launch_paged_attn<128, false, true, kBoth>(const PagedShared&, int, int64_t, hipStream_t);
 template void launch_paged_chunk<128, false, true, kPrefix>(const PagedShared&, int64_t, hipStream_t);
 template void launch_paged_chunk<128, false, true, kOwn>(const PagedShared&, int64_t, hipStream_t);
 }  // namespace fa

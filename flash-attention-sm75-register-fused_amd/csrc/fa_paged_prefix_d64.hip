@@ -4,6 +4,7 @@
 
 namespace fa {
 template void launch_paged_attn<64, false, false, kOwn>(const PagedShared&, int, int64_t, hipStream_t);
+template void launch_paged_attn<64, false, false, kBoth>(const PagedShared&, int, int64_t, hipStream_t);
 template void launch_paged_chunk<64, false, false, kPrefix>(const PagedShared&, int64_t, hipStream_t);
 template void launch_paged_chunk<64, false, false, kOwn>(const PagedShared&, int64_t, hipStream_t);
 }  // namespace fa

@@ -42,6 +42,11 @@ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& 
   return (int)((unsigned)(s.n * a.group + R - 1) / R);  // (below 2^28)
 }
 
+// A sequence's prefix: which, its keys and their tiles (0: none).
+struct PagedPre {
+  int group, keys, tiles;
+};
+
 // The line of a class of KV heads (every classes-th head): the units of its
 // sequences (blocks of R rows, for each head) end to end, each as long as its sequence
 // has tiles of T keys (one at least, so that the rows of a sequence without keys are
@@ -52,19 +57,25 @@ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& 
 // again and again, so that sequences share rows, may positions wrap round, and then
 // units are held to those there are, and pieces to the workgroups).  Called by whole
 // waves; the first 64 sequences, one a lane, are looked at once.
-template <int R, int T, int H>
+template <int R, int T, int H, int STAGE = 0>
 struct PagedLine {
-  const PagedArgs& a;
+  const std::conditional_t<STAGE == kBoth, PagedShared, PagedArgs>& a;
   const int lane;
   const bool by_tiles;
   int ahead;     // H or 0: a unit's first `ahead` are no tiles
   int same;      // every unit's length, 0 where they differ or are not looked at
-  PagedSeq own;  // sequence `lane`
+  PagedSeq own;  // sequence `lane` (kBoth: its keys behind its prefix's tiles)
   int first;     // prefix(0)
+  PagedPre pre;  // kBoth: the sequence's prefix
 
-  __device__ __forceinline__ PagedLine(const PagedArgs& args, int ln, bool tiles)
+  __device__ __forceinline__ PagedLine(const std::conditional_t<STAGE == kBoth, PagedShared, PagedArgs>& args, int ln,
+                                       bool tiles)
       : a(args), lane(ln), by_tiles(tiles) {
     own = look(lane);
+    if constexpr (STAGE == kBoth) {
+      pre = shared();
+      own.keys += T * pre.tiles;
+    }
     ahead = 0;
     same = 0;
     if (tiles) {
@@ -80,6 +91,26 @@ struct PagedLine {
     PagedSeq s = paged_seq(a, min(b, a.batch - 1), [](const int32_t* p) { return *p; });
     if (b >= a.batch) s.n = 0;
     return s;
+  }
+  // (kBoth: at most 64 sequences and 63 prefixes)
+  __device__ __forceinline__ PagedPre shared() const {
+    PagedPre p = {0, 0, 0};
+    if (a.groups != nullptr) {  // the last that begins at the sequence or before
+      const int begin = a.groups[min(lane, a.prefixes)];
+      for (int i = 0; i <= a.prefixes; ++i) p.group += wave_bcast(begin, i) <= lane ? 1 : 0;
+      --p.group;
+    }
+    const bool has = lane < a.batch && p.group >= 0 && p.group < a.prefixes;
+    if (!has) p.group = 0;
+    const int len = a.pre_lens[p.group];
+    p.keys = has ? clamp_int(len, 0, a.pre_pages << a.page_shift) : 0;
+    p.tiles = (int)((unsigned)(p.keys + T - 1) / T);
+    return p;
+  }
+  // Sequence b's prefix.
+  __device__ __forceinline__ PagedPre pre_of(int b) const {
+    if constexpr (STAGE != kBoth) return {0, 0, 0};
+    return {wave_bcast(pre.group, b), wave_bcast(pre.keys, b), wave_bcast(pre.tiles, b)};
   }
   static __device__ __forceinline__ int tiles_of(const PagedSeq& s) { return (int)((unsigned)(s.keys + T - 1) / T); }
   // A unit's length on the line.

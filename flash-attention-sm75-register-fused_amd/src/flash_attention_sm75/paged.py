@@ -151,7 +151,8 @@ def flash_attention_paged_prefix(Q, k_cache, v_cache, prefix_table, prefix_lens,
                                  max_prefix_queries=None, causal="bottom_right", scale=None, k_scale=None,
                                  v_scale=None, return_lse=False, out=None):
     """Attention of new tokens whose sequences share prefixes (an instruction, a document): a
-    prefix's rows are read once for all of its sequences.
+    prefix's rows are read once for all of its sequences (or, where few rows and short tables make
+    that faster, by each in one launch).
 
     What :func:`flash_attention_paged` gives where each sequence's table lists its prefix's pages
     first, with these differences: block_table and seq_lens are of a sequence's own tokens

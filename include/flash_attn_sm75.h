@@ -448,8 +448,9 @@ typedef struct fa_paged_prefix {
                                  as max_query_len */
 } fa_paged_prefix;
 
-/* As fa_sm75_paged_forward (p->lse: over the prefix and the own keys), but for the workspace, which
- * is needed: 32-bit states of the rows over their prefixes.  Of fa_sm75_paged_prefix_workspace_size()
+/* As fa_sm75_paged_forward (p->lse: over the prefix and the own keys), but for the workspace: 32-bit
+ * states of the rows over their prefixes, which are needed, except where rows and the prefixes' tables are
+ * small enough for a sequence to read its prefix itself.  Of fa_sm75_paged_prefix_workspace_size()
  * bytes the share of the own keys may be missing (the error of a smaller one says the least). */
 int fa_sm75_paged_prefix_forward(const fa_paged_params* p, const fa_paged_prefix* prefix);
 int64_t fa_sm75_paged_prefix_workspace_size(const fa_paged_params* p, const fa_paged_prefix* prefix);

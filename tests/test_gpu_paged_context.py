@@ -47,13 +47,20 @@ def attend(own, shared, cu_prefix, device, hq, seed=1, causal=True, scale=None, 
     args, scales = on(device, own, shared, strided)
     ones = all(n == 1 for n in own.news)
     cu_prefix = None if cu_prefix is None else torch.tensor(cu_prefix, dtype=torch.int32, device=device)
-    for own_hint, shared_hint in hints or ([(None, None), (None, 1)] if ones else [(1, 1), (1, 10 ** 6), (10 ** 6, 1), (None, None)]):
+    # A table with room for more than 128 MB of prefix rows (one read for each sequence) makes two launches of few rows.
+    pools, table, rest = args[:2], args[2], args[3:]
+    room = (128 << 20) // (len(own.lens) * own.hkv * 2 * own.d * (1 if own.q8 else 2)) + own.page
+    wide = torch.nn.functional.pad(table, (0, max(0, room // own.page + 1 - table.shape[1])), value=-1)
+    calls = [(a, b, t) for a, b in hints or ([(None, None), (None, 1)] if ones else
+                                             [(1, 1), (1, 10 ** 6), (10 ** 6, 1), (None, None)])
+             for t in (table, wide)]
+    for own_hint, shared_hint, table in calls:
         o, lse = fa.flash_attention_paged_prefix(
-            q.to(device), *args, cu_seqlens=None if ones else own.cu.to(device), cu_prefix=cu_prefix,
+            q.to(device), *pools, table, *rest, cu_seqlens=None if ones else own.cu.to(device), cu_prefix=cu_prefix,
             max_query_len=own_hint, max_prefix_queries=shared_hint, causal="bottom_right" if causal else False,
             scale=scale, return_lse=True, **scales, **kw)
-        ref.check(o, want, tol, f"O (hints {own_hint}, {shared_hint})")
-        ref.check(lse, want_lse, lse_tol, f"LSE (hints {own_hint}, {shared_hint})")
+        ref.check(o, want, tol, f"O (hints {own_hint}, {shared_hint}, table {tuple(table.shape)})")
+        ref.check(lse, want_lse, lse_tol, f"LSE (hints {own_hint}, {shared_hint}, table {tuple(table.shape)})")
     return o, lse
 
 
@@ -119,6 +126,33 @@ def test_prefix_of_some(device):
     attend(own, shared, [1, 3, 3, 4], device, 4)
     attend(own, shared, [5, 5, 5, 5], device, 4)
     attend(own, shared, [0, 0, 0, 0], device, 4)
+
+
+@pytest.mark.parametrize("sequences,prefixes", [(64, 63), (64, 64), (65, 63)])
+def test_prefix_most_in_one_launch(device, sequences, prefixes):
+    """Up to 64 sequences and 63 prefixes a few rows' prefixes and own keys are one launch."""
+    own = Cache([(5 * i) % 40 for i in range(sequences)], 1, 64, 16, BF16, False, news=[1] * sequences)
+    shared = Cache([(7 * i) % 71 for i in range(prefixes)], 1, 64, 16, BF16, False, seed=3)
+    attend(own, shared, [min(i + 1, sequences - 1) for i in range(prefixes)] + [sequences - 1], device, 4)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_prefix_tables_without_columns(device, q8):
+    """No page of a sequence's own, or none of a prefix's."""
+    q = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(1)).half()
+    for lens, plens in (([0, 0, 0], [77, 0]), ([40, 0, 33], [0, 0]), ([0, 0, 0], [0, 0])):
+        own, shared = Cache(lens, 2, 64, 16, FP16, q8, news=[1, 1, 1]), Cache(plens, 2, 64, 16, FP16, q8, seed=3)
+        want, want_lse, tol, lse_tol = ref.attention(con.Joined(own, shared, [0, 0, 1]), q, True, None)
+        (k, v, ptable, pl, table, sl), scales = on(device, own, shared)
+        if not any(lens):
+            table = table[:, :0]
+        if not any(plens):
+            ptable = ptable[:, :0]
+        cu = torch.tensor([0, 2, 3], dtype=torch.int32, device=device)
+        o, lse = fa.flash_attention_paged_prefix(q.to(device), k, v, ptable, pl, table, sl, cu_prefix=cu,
+                                                 return_lse=True, **scales)
+        ref.check(o, want, tol * (1 + 2.0 ** -4), "O")
+        ref.check(lse, want_lse, lse_tol + 2.0 ** -15, "LSE")
 
 
 def test_prefix_more_new_tokens_than_keys(device):
@@ -953,6 +987,14 @@ def test_workspaces_of_the_c_calls(device):
     want, want_lse, tol, lse_tol = ref.attention(con.Joined(own, shared, [0, 0]), q)
     ref.check(o, want, tol * (1 + 2.0 ** -4), "O")
     ref.check(lse, want_lse, lse_tol + 2.0 ** -15, "LSE")
+    # Few rows and short tables: one launch, which needs none.
+    p.cu_seqlens, p.tokens, p.workspace, p.workspace_bytes = 0, 2, 0, 0
+    assert lib.fa_sm75_paged_prefix_forward(ctypes.byref(p), ctypes.byref(x)) == 0, lib.fa_sm75_last_error()
+    ones = Cache([2500, 33], 2, 64, 64, BF16, False, news=[1, 1])
+    want, want_lse2, tol, lse_tol = ref.attention(con.Joined(ones, shared, [0, 0]), q[:2])
+    ref.check(o[:2], want, tol * (1 + 2.0 ** -4), "O of single tokens")
+    ref.check(lse.flatten()[:16].view(8, 2), want_lse2, lse_tol + 2.0 ** -15, "LSE of single tokens")
+    lse.copy_(want_lse.float())
     weights = torch.empty(2, 2, 2560, device=device)
     w = WeighParams(cache=ctypes.pointer(c), q=qd.data_ptr(), lse=lse.data_ptr(), weights=weights.data_ptr(),
                     weights_stride_b=5120, weights_stride_h=2560, max_len=2560, tokens=201, heads_q=8, q_stride_t=512,

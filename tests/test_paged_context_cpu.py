@@ -118,9 +118,10 @@ def test_prefix_too_many_units(lib):
 
 
 def test_prefix_workspace(lib):
-    """The rows' states at least (a record of 128 rows for each workgroup: of one block of rows of two heads, and
-    a single tile of keys); without them the call is refused, before it asks the device anything."""
-    p, x = params(cache()), prefix()
+    """The rows' states at least (a record of 128 rows for each workgroup: of one block of rows of two heads), where
+    the prefixes' tables have more room than each sequence would read for itself; without them the call is refused,
+    before it asks the device anything."""
+    p, x = params(cache()), prefix(max_pages=1 << 20, block_table_stride=1 << 20)
     states = 2 * 128 * (64 + 2) * 4 + 16
     size = lib.fa_sm75_paged_prefix_workspace_size(ctypes.byref(p), ctypes.byref(x))
     assert size >= states and size % 16 == 0
