@@ -56,26 +56,27 @@ struct SelRow {
   }
 };
 
-// kSelBlock positions of a row, a wave's kSelKeys * 64 next to each other, in registers.  (Loads do
-// not wait for the sequence's length: the weights have the table's room.)
-constexpr int kSelKeys = 8;
+// KEYS * kSelThreads positions of a row, a wave's KEYS * 64 next to each other, in registers.  (Loads
+// do not wait for the sequence's length: the weights have the table's room.)
+constexpr int kSelKeys = 8;  // the most
 constexpr int kSelBlock = kSelKeys * kSelThreads;
+template <int KEYS>
 struct SelBlock {
-  unsigned k[kSelKeys];
-  float x[kSelKeys];
+  unsigned k[KEYS];
+  float x[KEYS];
   int j0;  // this lane's first; 64 apart
   __device__ __forceinline__ SelBlock(const SelRow& row, int base, int end, int wave, int lane) {
-    j0 = base + wave * (64 * kSelKeys) + lane;
-    int page[kSelKeys];
+    j0 = base + wave * (64 * KEYS) + lane;
+    int page[KEYS];
 #pragma unroll
-    for (int u = 0; u < kSelKeys; ++u) {
+    for (int u = 0; u < KEYS; ++u) {
       const int j = j0 + 64 * u;
       const bool there = j < row.from_room;
       x[u] = there ? row.w[j] : 0.0f;
       page[u] = there ? row.entries[j >> row.e.p.page_shift] : -1;
     }
 #pragma unroll
-    for (int u = 0; u < kSelKeys; ++u) {
+    for (int u = 0; u < KEYS; ++u) {
       const int j = j0 + 64 * u;
       const bool held = j < min(end, row.keys) && page[u] >= 0 && page[u] < row.e.p.num_pages;
       k[u] = !held ? 0 : j >= row.recent_from ? kRecentKey : order_key(x[u]);
@@ -90,9 +91,10 @@ struct Search {
   int need, shift;  // shift: 21, 10, 0
   __device__ __forceinline__ int width() const { return shift == 0 ? 1 << 10 : kSelBins; }
   __device__ __forceinline__ int digit(unsigned k) const { return (k >> shift) & (width() - 1); }
-  __device__ __forceinline__ void count(const SelBlock& x, int* bins) const {
+  template <int KEYS>
+  __device__ __forceinline__ void count(const SelBlock<KEYS>& x, int* bins) const {
 #pragma unroll
-    for (int u = 0; u < kSelKeys; ++u)
+    for (int u = 0; u < KEYS; ++u)
       if (x.k[u] != 0 && (x.k[u] & mask) == bound) atomicAdd(&bins[digit(x.k[u])], 1);
   }
 };
@@ -145,12 +147,13 @@ __device__ __forceinline__ void take(Search& s, const SelShared& sh) {
 
 // Writes which of a block's positions stay: `before` in front of them do, and so many of
 // equal keys lie there, of which the first `need` stay.  Returns both for what is behind it.
-__device__ __forceinline__ int2 write_kept(const SelRow& row, const SelBlock& x, unsigned bound, int need, int target,
+template <int KEYS>
+__device__ __forceinline__ int2 write_kept(const SelRow& row, const SelBlock<KEYS>& x, unsigned bound, int need, int target,
                                            int above, int same, int wave, int lane, int* waves) {
   int n = 0;  // of this wave: above the bound, and equal to it in the upper half
-  uint64_t gt[kSelKeys], eq[kSelKeys];
+  uint64_t gt[KEYS], eq[KEYS];
 #pragma unroll
-  for (int u = 0; u < kSelKeys; ++u) {
+  for (int u = 0; u < KEYS; ++u) {
     gt[u] = __builtin_amdgcn_ballot_w64(x.k[u] > bound);
     eq[u] = __builtin_amdgcn_ballot_w64(x.k[u] == bound && x.k[u] != 0);
     n += __builtin_popcountll(gt[u]) + (__builtin_popcountll(eq[u]) << 16);
@@ -159,7 +162,7 @@ __device__ __forceinline__ int2 write_kept(const SelRow& row, const SelBlock& x,
   int a = above + (sum.x & 0xffff), s = same + (sum.x >> 16);
   const uint64_t lower = ((uint64_t)1 << lane) - 1;
 #pragma unroll
-  for (int u = 0; u < kSelKeys; ++u) {
+  for (int u = 0; u < KEYS; ++u) {
     const int ge = a + __builtin_popcountll(gt[u] & lower), se = s + __builtin_popcountll(eq[u] & lower);
     const bool stays = x.k[u] > bound || (x.k[u] == bound && x.k[u] != 0 && se < need);
     const int to = ge + min(se, need);
@@ -175,7 +178,9 @@ __device__ __forceinline__ int2 write_kept(const SelRow& row, const SelBlock& x,
 
 // A workgroup for each (sequence, KV head), where the table has room for one block.  The chain of
 // its steps bounds it (three digits of three barriers): 8.5 us for two rows of 1025 positions, 12.5 for
-// 256 of 4096 .. 8192 (8 MB of weights).
+// 256 of 4096 .. 8192 (8 MB of weights).  With as few keys a thread as the table has room for: of 2 and 8
+// 10.9 and 13.2 us for 8 rows of 1000 positions with the copy, 31.5 and 36.2 for 512.
+template <int KEYS>
 __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_kernel(const EvictArgs e) {
   __shared__ int bins[kSelBins];
   __shared__ SelShared sh[4];
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_kernel(const E
   int2* const own = (int2*)bins + (kSelThreads - 1 - threadIdx.x);
   *own = {0, 0};
   const SelRow row(e, (int)blockIdx.x);
-  const SelBlock x(row, 0, INT32_MAX, wave, lane);
+  const SelBlock<KEYS> x(row, 0, INT32_MAX, wave, lane);
   __syncthreads();
   Search s = {0, 0, 0, 21};
   int target = 0;
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_long_kernel(co
   Search s = {0, 0, 0, 21};
   int target = 0, above = 0, same = 0;
   bool search = true;
-  const SelBlock first(row, begin, end, wave, lane);  // (loads under the search)
+  const SelBlock<kSelKeys> first(row, begin, end, wave, lane);  // (loads under the search)
   if constexpr (PHASE > 0) {
     constexpr int p = PHASE - 1;  // the digit that was counted last
     if constexpr (p > 0) {
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_long_kernel(co
     *own = {0, 0};
     __syncthreads();
     if (begin < end) s.count(first, bins);
-    for (int j = begin + kSelBlock; j < end; j += kSelBlock) s.count(SelBlock(row, j, end, wave, lane), bins);
+    for (int j = begin + kSelBlock; j < end; j += kSelBlock) s.count(SelBlock<kSelKeys>(row, j, end, wave, lane), bins);
     __syncthreads();
     ((int2*)e.counts)[(((int64_t)pair * 3 + PHASE) * e.chunks + chunk) * kSelThreads + slot] = *own;
   } else {
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_long_kernel(co
         __syncthreads();
       }
       for (int j = begin + kSelBlock; j < end; j += kSelBlock) {
-        before = write_kept(row, SelBlock(row, j, end, wave, lane), s.bound, s.need, target, before.x, before.y, wave,
+        before = write_kept(row, SelBlock<kSelKeys>(row, j, end, wave, lane), s.bound, s.need, target, before.x, before.y, wave,
                             lane, waves[2]);
         __syncthreads();
       }
@@ -404,7 +409,11 @@ int launch_evict(const EvictArgs& args, int head_dim, void* workspace, hipStream
   const int64_t pairs = (int64_t)e.p.batch * e.p.hkv;
   const dim3 threads(kSelThreads);
   if (e.chunks == 0) {
-    hipLaunchKernelGGL(fa_paged_select_kernel, dim3((unsigned)pairs), threads, 0, stream, e);
+    const int64_t room = (int64_t)e.p.max_pages << e.p.page_shift;
+    const dim3 rows((unsigned)pairs);
+    if (room <= 2 * kSelThreads) hipLaunchKernelGGL(fa_paged_select_kernel<2>, rows, threads, 0, stream, e);
+    else if (room <= 4 * kSelThreads) hipLaunchKernelGGL(fa_paged_select_kernel<4>, rows, threads, 0, stream, e);
+    else hipLaunchKernelGGL(fa_paged_select_kernel<kSelKeys>, rows, threads, 0, stream, e);
   } else {
     const dim3 rows((unsigned)(pairs * e.chunks));
     hipLaunchKernelGGL(fa_paged_select_long_kernel<0>, rows, threads, 0, stream, e);
