@@ -382,11 +382,14 @@ __global__ void __launch_bounds__(kMoveThreads) fa_paged_move_kernel(const Evict
 }  // namespace
 
 // Workgroups of a long row: one for each block of positions, up to 64 (each adds up the histograms of
-// all), and 4096 in all; 0: one workgroup has them in its registers.
+// all), and 256 in all; 0: one workgroup has them in its registers.  (us with 256, 512 and 4096 in all, 1024
+// rows kept: 64 rows of 60000 51.5 / 59 / 59, 128 of 60000 83 / 83 / 105, of 130000 125 / 117 / 173, 256 of
+// 20000 93 / 104 / 104, 512 of 30000 204 / 204 / 238.  Blocks of 2, 4 and 16 keys a thread in place of 8: 8
+// rows of 131072 93, 58 and 71 for 56.)
 static int evict_chunks(const EvictArgs& e) {
   const int64_t room = (int64_t)e.p.max_pages << e.p.page_shift, pairs = (int64_t)e.p.batch * e.p.hkv;
   if (room <= kSelBlock) return 0;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({64, (room + kSelBlock - 1) / kSelBlock, 4096 / pairs}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({64, (room + kSelBlock - 1) / kSelBlock, 256 / pairs}));
 }
 static int64_t kept_bytes(const EvictArgs& e) {
   return ((int64_t)e.p.batch * e.p.hkv * e.slots * (int64_t)sizeof(int32_t) + 15) & ~(int64_t)15;
