@@ -17,6 +17,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "fa_internal.h"
@@ -28,11 +29,7 @@ namespace {
 constexpr int kWTile = 32;    // keys of a wave's step: two 16-key pieces, each in one page
 constexpr int kWBlock = 256;  // keys of a unit of the kernel for more rows
 
-// A row's log-sum-exp in log2 units.  -inf (a row that saw no key) as +inf: it gives
-// every key 2^-inf = 0.
-__device__ __forceinline__ float weigh_lse2(float lse) {
-  return lse == -__builtin_inff() ? __builtin_inff() : lse * 1.4426950408889634f;
-}
+constexpr float kWLog2e = 1.4426950408889634f;
 
 // The steps of STEP keys that hold keys some row sees, up to max_len: of every sequence, those of its
 // KV heads.  And the blocks of 256 positions behind them.  Called by whole waves.
@@ -128,11 +125,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
   pos = uniform(pos + t_stop - t_begin);
   if (hkv >= a.hkv) return;
 
-  // Keys some row sees end at `sees`; those before `full` every row sees.
+  // Keys some row sees end at `sees`.
   const int nrows = s.n * a.group;
   const int past = s.len - s.n;  // tokens before the new ones
   const int sees = s.n > 0 ? uniform(min(s.keys, w.max_len)) : 0;
-  const int full = a.causal ? uniform(clamp_int(past + 1, 0, sees)) : sees;
   float* const out = w.out + b * w.sb + hkv * w.sh;
   const float c2 = a.negate_q ? -a.c : a.c;
 
@@ -156,11 +152,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
         const int dim = FP8 ? 64 * (kk >> 1) + 16 * g4 + 8 * (kk & 1) : 32 * kk + 8 * g4;
         qf[nt][kk] = ok ? *(const half8*)(qp + dim) : (half8)(_Float16)0;
       }
-      const float lse = ok ? weigh_lse2(w.lse[(int64_t)pr.head * a.tokens + pr.token]) : __builtin_inff();
-      const int most = !ok ? -1 : a.causal ? min(sees - 1, past + (pr.token - s.t0)) : sees - 1;
+      // Rows of LSE -inf and places without a row see no key: their products with one that is not finite may be
+      // NaN.
+      const float lse = ok ? w.lse[(int64_t)pr.head * a.tokens + pr.token] : -__builtin_inff();
+      const int most = lse == -__builtin_inff() ? -1 : a.causal ? min(sees - 1, past + (pr.token - s.t0)) : sees - 1;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        lse2[nt][i] = __shfl(lse, 4 * g4 + i);
+        lse2[nt][i] = __shfl(lse * kWLog2e, 4 * g4 + i);
         last[nt][i] = __shfl(most, 4 * g4 + i);
       }
     }
@@ -219,7 +217,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const int key = t * kWTile + 16 * p + l16;
-        const bool masked = (t + 1) * kWTile > full || x.rows[p] < 16;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float4v st = (float4v)0.0f;
@@ -227,9 +224,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
           for (int kk = 0; kk < KS; ++kk) st = E::mfma16(qf[nt][kk], kf[p][kk], st);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], c2, -lse2[nt][i]));
-            if (masked) y = key <= last[nt][i] ? y : 0.0f;
-            acc[p] += y;
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], c2, -lse2[nt][i]));
+            acc[p] += key <= last[nt][i] ? y : 0.0f;
           }
         }
       }
@@ -467,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   // Loads of a tile's rows go through windows from its first row's token and the first head of the
   // group on, with offsets below 2^31 bytes (the launcher sees to it), whose factors have 24 bits.
   float lse_next;
+  bool lse_copy;
   const int q_tok = 2 * (int)a.qt, q_head = 2 * (int)a.qh;  // in bytes
   const int tok_step = uniform((int)((unsigned)kWRows / (unsigned)a.group));
   const int rem_step = kWRows - tok_step * a.group;
@@ -501,7 +498,8 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       lse_off = head * a.tokens + tok;
     }
     const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
-    lse_next = lane <= end ? lse[lse_off] : -__builtin_inff();
+    lse_next = lse[lse_off];
+    lse_copy = lane > end;
     fence_schedule();  // (the LSE is waited for first)
     const __amdgpu_buffer_rsrc_t rq =
         make_rsrc(a.q + (int64_t)(s.t0 + ld_tok) * a.qt + (int64_t)hkv * a.group * a.qh, INT32_MAX);
@@ -519,8 +517,16 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       ++ld_tok;
     }
   };
+  // Of rows of LSE -inf, which are left out, +inf; bit `buf` of `out_tiles` says that its tile has one (every
+  // wave has all the tile's LSE).  Their products with a key that is not finite may be NaN.  Copies of the last row
+  // behind it get a finite least, with which a score that the row itself makes 0, infinite or NaN stays so.
+  int out_tiles = 0;
   auto store_lse = [&](int buf) {
-    if (tid < kWRows) lse_lds[buf][tid] = -weigh_lse2(lse_next);
+    const bool out = lse_next == -__builtin_inff();
+    const float nl = -lse_next * kWLog2e;
+    if (tid < kWRows)
+      lse_lds[buf][tid] = out ? __builtin_inff() : lse_copy ? -FLT_MAX : nl == __builtin_inff() ? FLT_MAX : nl;
+    out_tiles = uniform((out_tiles & ~(1 << buf)) | (__builtin_amdgcn_ballot_w64(out) != 0 ? 1 << buf : 0));
   };
   int q_base[KK];
 #pragma unroll
@@ -531,13 +537,15 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   };
   float sum[2] = {0.0f, 0.0f};
   float16v st[2][2];
+  // MASK: 1 where keys may be hidden from rows, 2 where rows may be left out as well (a variant of its own: the select
+  // in 1 too cost all steps 4 to 10%).
   // Half H of step i (I: modulo 4): the probabilities of these 32 rows, whose S is st[H], between the
   // MFMAs of the next 32's (behind the last tile: of what is there, for nobody).  Tile i + 3 is loaded
   // to where tile i - 1 was, straight to LDS.
-  auto half_step = [&](int i, auto i_t, auto half_t, auto masked_t) {
+  auto half_step = [&](int i, auto i_t, auto half_t, auto mask_t) {
     constexpr int I = decltype(i_t)::value;
     constexpr int H = decltype(half_t)::value;
-    constexpr bool MASKED = decltype(masked_t)::value;
+    constexpr int MASK = decltype(mask_t)::value;
     half8 qf[KK];
     const _Float16* const buf = q_buf(std::integral_constant<int, I + H>{});
     static_for<PF>([&](auto k_c) { qf[decltype(k_c)::value] = read_q(buf, 1 - H, decltype(k_c)::value); });
@@ -566,7 +574,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
         if constexpr (e * NS / 32 == slot) {
           constexpr int k = e & 1, x = e >> 1;
           float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[H][k][x], c2, nl[x >> 2][x & 3]));
-          if constexpr (MASKED) y = 8 * (x >> 2) + (x & 3) >= lim[k] ? y : 0.0f;
+          if constexpr (MASK != 0) y = 8 * (x >> 2) + (x & 3) >= lim[k] ? y : 0.0f;
+          if constexpr (MASK == 2) {
+            asm volatile("" : "+v"(y));
+            y = nl[x >> 2][x & 3] != __builtin_inff() ? y : 0.0f;
+          }
           add[k] += y;
           asm volatile("" : "+v"(add[k]));  // keeps the sum in this slot
         }
@@ -598,12 +610,15 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     // Tiles before `all_from` hide a key from some row.
     const int hiding = uniform((int)((unsigned)(max(0, all_from - tile0 * kWRows) + kWRows - 1) / kWRows));
     auto step = [&](int i, auto i_t) {
-      if (i < hiding) {
-        half_step(i, i_t, I0{}, Flag<true>{});
-        half_step(i, i_t, I1{}, Flag<true>{});
+      if (out_tiles >> decltype(i_t)::value & 1) {
+        half_step(i, i_t, I0{}, std::integral_constant<int, 2>{});
+        half_step(i, i_t, I1{}, std::integral_constant<int, 2>{});
+      } else if (i < hiding) {
+        half_step(i, i_t, I0{}, std::integral_constant<int, 1>{});
+        half_step(i, i_t, I1{}, std::integral_constant<int, 1>{});
       } else {
-        half_step(i, i_t, I0{}, Flag<false>{});
-        half_step(i, i_t, I1{}, Flag<false>{});
+        half_step(i, i_t, I0{}, std::integral_constant<int, 0>{});
+        half_step(i, i_t, I1{}, std::integral_constant<int, 0>{});
       }
       // Tile i + 2 has landed, tile i + 3 need not have.
       if (i + 3 < count) barrier_after_loads<QL>();

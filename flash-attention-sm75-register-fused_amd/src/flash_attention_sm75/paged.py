@@ -192,7 +192,7 @@ def paged_attention_weights(Q, LSE, k_cache, block_table, seq_lens, cu_seqlens=N
     Args:
         Q, k_cache, block_table, seq_lens, cu_seqlens, max_query_len, causal, scale, k_scale: the
             attention call's.
-        LSE: the log-sum-exp it returned, [H_q, tokens] float32; a row of -inf adds nothing.
+        LSE: the log-sum-exp it returned, [H_q, tokens] float32; a row of -inf adds nothing, whatever its query.
         max_len: positions to weigh (default: all that block_table has room for).
         add_to: [B, H_kv, max_len] float32, positions contiguous: the weights are added to
             those of the positions that hold a row, the others are left as they are.  Its rows
@@ -206,7 +206,7 @@ def paged_attention_weights(Q, LSE, k_cache, block_table, seq_lens, cu_seqlens=N
     The rows of a shared prefix get theirs from a call over its table (prefix_table, prefix_lens, and for
     cu_seqlens the bounds of its sequences' tokens) with causal=False and the LSE of
     :func:`flash_attention_paged_prefix`.  A key that is not finite gives its own weight only;
-    a query or LSE that is NaN gives every row it sees NaN.
+    a query that is NaN (of a row whose LSE is not -inf) or an LSE that is gives every row it sees NaN.
     """
     if torch.is_grad_enabled() and (Q.requires_grad or LSE.requires_grad or k_cache.requires_grad
                                     or (add_to is not None and add_to.requires_grad)):

@@ -435,6 +435,56 @@ def test_weights_nonfinite(device, news):
         assert w[1, 0, :90].isnan().all() and (w[1, 0, 90:] == 0).all() and int(w[0].isnan().sum()) == 1
 
 
+@pytest.mark.parametrize("news", [[1, 1], [5, 3], [40, 3], [130, 90]])
+@pytest.mark.parametrize("at", [0, 3, 60, 255, 395, 399])
+@pytest.mark.parametrize("scale", [None, -0.3])
+def test_weights_infinite_key(device, news, at, scale):
+    """A key that all rows score -inf has weight 0, wherever it stands and whatever the number of rows."""
+    c = Cache([400, 90], 1, 64, 16, BF16, False, news=news)
+    q = torch.rand(sum(news), 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16() + 0.125
+    c.k[int(c.table[0, at // 16]), 0, at % 16, 7] = -math.inf if scale is None else math.inf
+    c.rows[0][0][0, at, 7] = -math.inf if scale is None else math.inf
+    lse = lse_of(c, q, device, scale=scale)
+    assert lse.isfinite().all()  # attention gives the key no weight
+    want, tol = con.weights(c, q, lse.cpu(), scale=scale)
+    assert want[0, 0, at] == 0 and not want.isnan().any()
+    (args, _) = c.args(device)
+    for hint in (1, 10 ** 6):
+        w = fa.paged_attention_weights(q.to(device), lse, args[0], *args[2:], cu_seqlens=c.cu.to(device), scale=scale,
+                                       max_query_len=hint)
+        ref.check(w, want, tol, f"weights (hint {hint})")
+        assert w[0, 0, at] == 0
+
+
+@pytest.mark.parametrize("news", [[1, 1], [5, 3], [40, 3], [130, 90]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_rows_left_out(device, news, causal):
+    """A row of LSE -inf adds nothing, whatever its query and the keys hold: the last row, the first, all of a sequence's.
+    One of LSE +inf gives finite scores 0."""
+    c = Cache([400, 90], 1, 64, 16, BF16, False, news=news)
+    q = torch.randn(sum(news), 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16()
+    lse = lse_of(c, q, device, causal)
+    out = [(0, 0), (3, news[0] - 1)] + [(h, t) for h in range(4) for t in range(news[0], sum(news))]
+    for h, t in out:
+        lse[h, t] = -math.inf
+        q[t, h, 5] = math.nan
+    lse[1, 0] = math.inf
+    # What only rows that are left out see: the last sequence's keys.
+    for j, x in ((2, math.inf), (33, math.nan), (70, -math.inf)):
+        c.k[int(c.table[1, j // 16]), 0, j % 16, 7] = x
+    rows = q.clone()
+    for h, t in out:
+        rows[t, h] = 0
+    want, tol = con.weights(c, rows, lse.cpu(), causal)
+    assert (want[1] == 0).all() and want.isfinite().all()
+    (args, _) = c.args(device)
+    for hint in (1, 10 ** 6):
+        w = fa.paged_attention_weights(q.to(device), lse, args[0], *args[2:], cu_seqlens=c.cu.to(device), max_query_len=hint,
+                                       causal="bottom_right" if causal else False)
+        ref.check(w, want, tol, f"weights (hint {hint})")
+        assert (w[1] == 0).all()
+
+
 def test_weights_indexes_are_held_to_their_ranges(device):
     c = Cache([50, 30], 2, 64, 16, FP16, False, news=[3, 1])
     (args, _), q = c.args(device), torch.randn(4, 4, 64).half().to(device)
