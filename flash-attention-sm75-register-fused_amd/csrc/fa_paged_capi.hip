@@ -14,6 +14,12 @@ using fa::capi_fail;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// Whether two ranges of bytes share none.
+bool apart(const void* x, int64_t nx, const void* y, int64_t ny) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+  return nx == 0 || ny == 0 || a + nx <= b || b + ny <= a;
+}
+
 int check_launch() {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return capi_fail(FA_ERR_HIP, "HIP launch failed: %s", hipGetErrorString(e));
@@ -461,6 +467,14 @@ int fa_sm75_paged_evict(const fa_paged_evict_params* p) {
     return capi_fail(FA_ERR_INVALID_ARGUMENT, "the workspace must hold %lld bytes, got %lld", (long long)need,
                      (long long)(p->workspace != nullptr ? p->workspace_bytes : 0));
   if (!aligned(p->workspace, 16)) return capi_fail(FA_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  // (a row's workgroups read a length and weights while others write what stays)
+  const fa::PagedArgs& a = e.p;
+  const int64_t pairs = (int64_t)a.batch * a.hkv, room = (int64_t)a.max_pages << a.page_shift;
+  const int64_t span = room > 0 ? (a.batch - 1) * e.wb + (a.hkv - 1) * e.wh + room : 0;
+  if (!apart(e.new_lens, 4ll * a.batch, a.lens, 4ll * a.batch))
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "new_lens must not share seq_lens' memory");
+  if (!apart(e.new_weights, 4 * pairs * (p->to_pages << a.page_shift), e.weights, 4 * span))
+    return capi_fail(FA_ERR_INVALID_ARGUMENT, "new_weights must not share the weights' memory");
   fa::launch_evict(e, (int)p->cache->head_dim, p->workspace, static_cast<hipStream_t>(p->stream));
   return check_launch();
 }

@@ -505,8 +505,8 @@ typedef struct fa_paged_evict_params {
                                room for */
   int64_t to_table_stride;
   int64_t keep, recent;     /* 0 <= recent <= keep; batch * heads_kv up to 2^20, times keep up to 2^29 */
-  int32_t* new_lens;        /* [batch] */
-  float* new_weights;       /* contiguous [batch, heads_kv, to_pages * page_size] */
+  int32_t* new_lens;        /* [batch], none of seq_lens' memory */
+  float* new_weights;       /* contiguous [batch, heads_kv, to_pages * page_size], none of the weights' memory */
   void* stream;
   void* workspace;          /* 16-byte aligned, fa_sm75_paged_evict_workspace_size() bytes; calls that
                                share one race */

@@ -219,6 +219,20 @@ def test_evict_refusals(lib, kw, status, msg):
     assert msg in lib.fa_sm75_last_error()
 
 
+def test_evict_in_place_is_refused(lib):
+    """Lengths and weights are read while others are written: neither may be the same memory, in part or whole."""
+    far = dict(new_lens=0x40000, weights=0x50000, new_weights=0x60000)
+    for kw, msg in ((dict(far, new_lens=0x1000), b"new_lens must not share"),
+                    (dict(far, new_lens=0x1004), b"new_lens must not share"),
+                    (dict(far, new_weights=0x50000), b"new_weights must not share"),
+                    (dict(far, new_weights=0x50000 + 4 * 255), b"new_weights must not share"),
+                    (dict(far, new_weights=0x50000 - 4 * (2 * 2 * 32 - 1)), b"new_weights must not share")):
+        p = evict(cache(), **kw)
+        assert p.cache.contents.seq_lens == 0x1000 and p.weights_stride_b == 128
+        assert lib.fa_sm75_paged_evict(ctypes.byref(p)) == 1
+        assert msg in lib.fa_sm75_last_error()
+
+
 def test_evict_sizes(lib):
     assert lib.fa_sm75_paged_evict(None) == 1
     assert lib.fa_sm75_paged_evict(ctypes.byref(evict(cache(heads_kv=0)))) == 1
