@@ -28,7 +28,7 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
   return 2 * (rows * (head_dim + 2ll) * (int64_t)sizeof(float) + (int64_t)sizeof(uint64_t));
 }
 constexpr int64_t kLastCacheBytes = 256 << 20;
-constexpr int kOwnShort = 1536;
+constexpr int kOwnShort = 640, kOwnShare = 1024;
 constexpr int64_t kJoinBytes = 128 << 20;
 constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 16 bytes
 }  // namespace
@@ -97,13 +97,31 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   p.units = (int)(a.hkv / p.classes * blocks);
   // (Of very many units a workgroup each is balanced enough.)
   p.split = p.wgs > 0 && p.units <= 16 * resident / p.classes && fits_line(a, p.units, kPTile, kPAhead);
-  // Behind a shared prefix the own keys are often few: cutting them costs more than it
-  // balances where no sequence has more than a stretch's least, or where units nearly fill the
-  // GPU and are short (us of the launch, cut and not: 64 sequences of 64 to 256 keys, 8 heads d128 17.4 /
-  // 11.0, of 128 to 1024 34.7 / 30.8, 48 of 100 to 1500 8 bits 24.8 / 22.4; of 512 to 4096 95 / 111).
-  const int64_t longest = (int64_t)a.max_pages << a.page_shift;
-  if (stage == kOwn && (longest <= kPTile * kPMinTiles || (longest <= kOwnShort && p.units >= p.wgs - p.wgs / 4)))
-    p.split = false;
+  // Behind a shared prefix the own keys are often few, and cutting them (a plan by tiles, records, a merge: about 8
+  // us) costs more than it balances: up to 640 keys whatever the units, and more keys the more of the GPU the
+  // units fill, twice as many more where a row is half as wide.  us of both launches, units whole and cut, of
+  // sequences of a tenth to all of the keys (and of as many each), caches cold:
+  //   32 over 8 heads d128, 16 bits   512 keys     1024        1536        2048         border
+  //     2 sequences                   22.9 / 24.0  27.8 / 22.0 32.8 / 22.5 37.5 / 22.8   672
+  //     (each as long)                23.0 / 22.6  27.9 / 22.6 32.9 / 22.9
+  //     16                            23.4 / 28.2  28.7 / 31.2 35.5 / 33.1 41.6 / 36.2   896
+  //     (each as long)                23.8 / 25.0  31.6 / 32.4 38.1 / 37.2 44.7 / 42.3
+  //     32                            25.6 / 31.5  34.0 / 37.3 40.6 / 42.8 48.5 / 48.1  1152
+  //     64                            35.7 / 44.6  50.6 / 53.5 63.8 / 66.1 79.7 / 75.9  1664
+  //     96                            47.8 / 49.0  67.3 / 65.8 88.8 / 83.4              1664
+  //   8 bits
+  //     16                            25.6 / 30.2  30.7 / 32.1 35.6 / 37.0 40.8 / 34.7  1152
+  //     48                            31.3 / 37.1  37.7 / 40.2 44.2 / 47.6 48.5 / 54.0  2176 (4096: 74.6 / 69.0)
+  //     64                            31.6 / 41.6  39.7 / 48.4 47.6 / 55.4 55.9 / 60.2  2688 (4096: 82.9 / 79.5)
+  //   14 over 2 heads d64, 16 bits
+  //     4                             17.4 / 26.1  19.8 / 23.9 22.6 / 24.3 25.0 / 22.6   672
+  //     (each as long)                17.8 / 19.2  20.4 / 19.3 22.9 / 19.1 25.4 / 19.4
+  //     128                           20.1 / 30.1  23.3 / 31.7 27.3 / 34.5 31.7 / 36.6  1664 (4096: 45.3 / 47.1)
+  if (stage == kOwn && p.split) {
+    const int64_t longest = (int64_t)a.max_pages << a.page_shift;
+    const int share = head_dim == 128 && a.ks == nullptr ? kOwnShare : 2 * kOwnShare;
+    if (longest <= kOwnShort + (int64_t)share * std::min(p.units, p.wgs) / p.wgs) p.split = false;
+  }
   if (!p.split) p.wgs = p.units;
   p.workspace_bytes =
       p.split ? (int64_t)p.wgs * p.classes * partial_bytes(p.rows, head_dim) + kCombineWord : 0;

@@ -139,6 +139,42 @@ def test_prefix_workspace(lib):
         assert lib.fa_sm75_paged_prefix_workspace_size(ctypes.byref(p), ctypes.byref(x)) == 0
 
 
+def prefix_call(hq, hkv, d, q8, b, keys, prefix_keys, prefixes=1, page=16):
+    """One token of each of b sequences with room for `keys` own ones behind prefixes with room for prefix_keys."""
+    c = cache(batch=b, heads_kv=hkv, head_dim=d, page_size=page, max_pages=-(-keys // page), k_stride_n=d, v_stride_n=d,
+              block_table_stride=-(-keys // page), **(dict(k_scale=0x1000, v_scale=0x1000) if q8 else {}))
+    p = params(c, heads_q=hq, tokens=b)
+    x = prefix(count=prefixes, max_pages=-(-prefix_keys // page), cu_prefix=0x1000)
+    return p, x
+
+
+def cut_bytes(rows, d):
+    """A plan's records where 512 workgroups run at once."""
+    return 512 * 2 * (rows * (d + 2) * 4 + 8) + 16
+
+
+# Sequences, keys and whether units are left whole: sizes of which both were measured, those apart by 3% or less left out.
+OWN_KEYS = [
+    (32, 8, 128, False, [(1, 512, True), (2, 1024, False), (8, 512, True), (16, 768, True), (32, 1024, True), (48, 1024, True),
+                         (64, 1536, True), (48, 2048, False), (64, 2048, False), (96, 2048, False), (128, 4096, False)]),
+    (32, 8, 128, True, [(4, 1536, False), (16, 1024, True), (47, 1504, True), (48, 1504, True), (49, 1504, True),
+                        (48, 2048, True), (64, 2048, True), (32, 2048, False), (48, 4096, False), (64, 4096, False)]),
+    (14, 2, 64, False, [(4, 512, True), (4, 2048, False), (96, 768, True), (128, 1536, True), (256, 1536, True), (256, 2048, True),
+                        (64, 4096, False), (256, 4096, False)]),
+]
+
+
+@pytest.mark.parametrize("hq,hkv,d,q8,sizes", OWN_KEYS)
+def test_prefix_own_keys_cut_or_whole(lib, hq, hkv, d, q8, sizes):
+    """Behind a prefix, units of the own keys are cut where that was measured to be faster, and no workspace is asked
+    for where they are not: the border rises with the share of the GPU that the units fill."""
+    for b, keys, whole in sizes:
+        p, x = prefix_call(hq, hkv, d, q8, b, keys, 1 << 20)
+        size = lib.fa_sm75_paged_prefix_workspace_size(ctypes.byref(p), ctypes.byref(x))
+        states = (size - cut_bytes(16, d) * (not whole) - 16) / (128 * (d + 2) * 4)
+        assert states == 512 * max(1, -(-b * (hq // hkv) // 128) * hkv // 512), (b, keys, whole)
+
+
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(tokens=-1), 1, b"tokens must be non-negative"),
     (dict(tokens=1), 1, b"a token for each of the 2 sequences"),
