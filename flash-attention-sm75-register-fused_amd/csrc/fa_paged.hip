@@ -29,7 +29,7 @@ int64_t partial_bytes(int rows, int head_dim) {  // of one workgroup: two record
 }
 constexpr int64_t kLastCacheBytes = 256 << 20;
 constexpr int kOwnShort = 640, kOwnShare = 1024;
-constexpr int64_t kJoinBytes = 128 << 20;
+constexpr int64_t kJoinBytes = 128 << 20, kJoinAgain = 96 << 20;
 constexpr int64_t kCombineWord = 16;  // behind them, to keep workspaces whole 16 bytes
 }  // namespace
 
@@ -134,16 +134,22 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
   return p;
 }
 
-// Up to 32 rows of a KV head, where every sequence reads its prefix anew: mostly from the caches, at 12
-// TB/s, which up to the bytes that the tables have room for costs less than a launch over the prefixes, their
-// records and what joins them (us in two launches and in one: 4 tokens of 14 over 2 heads d64 behind 1000,
-// 2 MB in all, 16.7 / 13.2; of 32 over 8 d128 behind 1000, 2 of them 8 MB 22.4 / 11.9, 8 31 MB 26.7 /
-// 15.5, 32 125 MB 32.4 / 25.1, 64 250 MB 29.3 / 37.9; 8 behind 8000 250 MB 32.5 / 32.7, 8 bits 125 MB
-// 35.7 / 27.3; 64 of 2 heads d64 behind 4000, 125 MB, 20.2 / 22.3).
+// Up to 32 rows of a KV head, where every sequence reads its prefix itself: what is read again comes mostly from the
+// caches, at 12 TB/s, which while the tables have room for no more than 128 MB so read, 96 MB of it again, costs
+// less than a launch over the prefixes, their records and what joins them; up to 128 MB again where a second launch would cut
+// its own keys, whose plan and merge one launch has anyway.  One launch's time over that of two, caches cold, at
+// 1634 sizes (2 to 64 sequences of 100 to 1800 own keys, 1 or 4 prefixes of 128 to 16000, nine layouts; least, median, most):
+//   MB read again           up to 16     16 .. 48     48 .. 80     80 .. 100    100 .. 130   130 .. 200
+//     own keys whole        .49 .81 1.30 .57 .87 1.14 .64 .95 1.20 .81 .96 1.19 .80 1.03 1.32 .88 1.15 1.41
+//     cut                   .38 .57 .84  .57 .67 .83  .60 .75 .88  .68 .82 .99  .70 .87 .93   .89 1.02 1.09
+// (The rule's choice is 0.8% slower than the better of the two on average; most, 26.7 us for 34.7, with 8 tokens each of 24 sequences of
+// 200 keys behind 4 prefixes of 128.)
 bool joins_prefixes(const PagedShared& own, int head_dim, int64_t max_query_len) {
-  const int64_t room = ((int64_t)own.pre_pages << own.page_shift) * own.hkv * own.batch;
-  return max_query_len * own.group <= 32 && own.batch <= 64 && own.prefixes <= 63 &&
-         room * 2 * head_dim * (own.ks != nullptr ? 1 : 2) <= kJoinBytes;
+  if (max_query_len * own.group > 32 || own.batch > 64 || own.prefixes > 63) return false;
+  const int64_t bytes = ((int64_t)own.pre_pages << own.page_shift) * own.hkv * 2 * head_dim * (own.ks != nullptr ? 1 : 2);
+  return bytes * own.batch <= kJoinBytes &&
+         (bytes * (own.batch - own.prefixes) <= kJoinAgain ||
+          plan_paged(own, head_dim, max_query_len, INT64_MAX, kOwn).split);
 }
 
 PagedPlan plan_joined(const PagedShared& own, int head_dim, int64_t max_query_len, int64_t workspace_bytes) {

@@ -175,6 +175,27 @@ def test_prefix_own_keys_cut_or_whole(lib, hq, hkv, d, q8, sizes):
         assert states == 512 * max(1, -(-b * (hq // hkv) // 128) * hkv // 512), (b, keys, whole)
 
 
+# Sequences, own keys, prefixes, their keys, and whether one launch has both; measured as OWN_KEYS.
+JOINED = [
+    (32, 8, 128, False, [(2, 300, 1, 16000, True), (4, 300, 1, 8000, True), (16, 300, 1, 1000, True), (16, 300, 1, 2000, False),
+                         (16, 1344, 1, 2000, True), (32, 300, 1, 1000, False), (32, 1344, 1, 1000, True), (8, 300, 1, 8000, False),
+                         (64, 300, 4, 1000, False)]),
+    (32, 8, 128, True, [(16, 300, 1, 2000, True), (32, 300, 1, 2000, False), (48, 1344, 1, 600, True)]),
+    (14, 2, 64, False, [(4, 60, 1, 1000, True), (64, 60, 1, 4000, False), (64, 1344, 1, 4000, True), (64, 300, 4, 1000, True)]),
+    (8, 8, 64, False, [(64, 300, 1, 1000, False), (32, 300, 1, 2000, False), (16, 1344, 1, 4000, True), (4, 300, 4, 8000, True)]),
+]
+
+
+@pytest.mark.parametrize("hq,hkv,d,q8,sizes", JOINED)
+def test_prefix_one_launch_or_two(lib, hq, hkv, d, q8, sizes):
+    """One launch has prefixes and own keys where that was measured to be faster."""
+    for b, keys, count, prefix_keys, one in sizes:
+        p, x = prefix_call(hq, hkv, d, q8, b, keys, prefix_keys, count, page=64 if keys % 64 == 0 else 16)
+        size = lib.fa_sm75_paged_prefix_workspace_size(ctypes.byref(p), ctypes.byref(x))
+        cut = cut_bytes(16, d)
+        assert size == cut if one else size not in (0, cut), (b, keys, count, prefix_keys)
+
+
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(tokens=-1), 1, b"tokens must be non-negative"),
     (dict(tokens=1), 1, b"a token for each of the 2 sequences"),
