@@ -212,7 +212,45 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_kernel(const E
   if (row.h == 0 && threadIdx.x == 0) e.new_lens[row.b] = target;
 }
 
-// Longer rows: `chunks` workgroups each, in four launches.  The first three count a digit each over
+// Longer rows where they are many: the same, a block of positions after the other, for each digit anew.
+// (Through the kernels below with one chunk a row they were four launches with a histogram of each digit in memory, 24 KB
+// a row: with the copy 93.0 us for 78.9 at 256 rows of 20000 positions, 203 for 183 at 512 of 30000.)
+__global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_blocks_kernel(const EvictArgs e) {
+  __shared__ int bins[kSelBins];
+  __shared__ SelShared sh[4];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  int2* const own = (int2*)bins + (kSelThreads - 1 - threadIdx.x);
+  *own = {0, 0};
+  const SelRow row(e, (int)blockIdx.x);
+  const int keys = row.keys;
+  __syncthreads();
+  Search s = {0, 0, 0, 21};
+  int target = 0;
+  for (int p = 0; p < 3; ++p) {
+    for (int j = 0; j < keys; j += kSelBlock) s.count(SelBlock<kSelKeys>(row, j, keys, wave, lane), bins);
+    __syncthreads();
+    const int2 n = *own;
+    *own = {0, 0};
+    const int all = descend(s, n.y, n.x, e.keep, wave, lane, sh[p]);
+    if (p == 0) target = s.need;
+    if (p == 0 && (target == all || target == 0)) break;
+    take(s, sh[p]);
+  }
+  if (target > 0) {
+    if (s.mask == 0) s.need = 0;
+    int2 before = {0, 0};
+    for (int j = 0; j < keys; j += kSelBlock) {
+      before = write_kept(row, SelBlock<kSelKeys>(row, j, keys, wave, lane), s.bound, s.need, target, before.x, before.y, wave,
+                          lane, sh[3].waves);
+      __syncthreads();
+    }
+  }
+  for (int j = target + (int)threadIdx.x; j < row.room; j += kSelThreads) row.to_w[j] = 0.0f;
+  if (row.h == 0 && threadIdx.x == 0) e.new_lens[row.b] = target;
+}
+
+// Longer rows, few: `chunks` workgroups each, in four launches.  The first three count a digit each over
 // the chunk's keys, into a histogram of its own; the next launch adds those up to find the digit (and
 // keeps where the search is), and what of the chunks in front of its own stays by it.  The launches'
 // own chains bound them: 5, 8, 8 and 12 us at eight rows of 131072 positions (4 MB of weights, read four
@@ -382,9 +420,9 @@ __global__ void __launch_bounds__(kMoveThreads) fa_paged_move_kernel(const Evict
 }  // namespace
 
 // Workgroups of a long row: one for each block of positions, up to 64 (each adds up the histograms of
-// all), and 256 in all; 0: one workgroup has them in its registers.  (us with 256, 512 and 4096 in all, 1024
+// all), and 256 in all; 1: one takes block after block; 0: one has them in its registers.  (us with 256, 512 and 4096 in all, 1024
 // rows kept: 64 rows of 60000 51.5 / 59 / 59, 128 of 60000 83 / 83 / 105, of 130000 125 / 117 / 173, 256 of
-// 20000 93 / 104 / 104, 512 of 30000 204 / 204 / 238.  Blocks of 2, 4 and 16 keys a thread in place of 8: 8
+// 20000 79 / 104 / 104, 512 of 30000 183 / 204 / 238.  Blocks of 2, 4 and 16 keys a thread in place of 8: 8
 // rows of 131072 93, 58 and 71 for 56.)
 static int evict_chunks(const EvictArgs& e) {
   const int64_t room = (int64_t)e.p.max_pages << e.p.page_shift, pairs = (int64_t)e.p.batch * e.p.hkv;
@@ -397,7 +435,7 @@ static int64_t kept_bytes(const EvictArgs& e) {
 
 int64_t evict_workspace_bytes(const EvictArgs& e) {
   const int64_t pairs = (int64_t)e.p.batch * e.p.hkv, chunks = evict_chunks(e);
-  if (chunks == 0) return kept_bytes(e);
+  if (chunks <= 1) return kept_bytes(e);
   const int64_t row = 3 * chunks * kSelBins * (int64_t)sizeof(int) + 3 * (int64_t)sizeof(SelState) + 2 * chunks * (int64_t)sizeof(int);
   return (kept_bytes(e) + pairs * row + 15) & ~(int64_t)15;
 }
@@ -417,6 +455,8 @@ int launch_evict(const EvictArgs& args, int head_dim, void* workspace, hipStream
     if (room <= 2 * kSelThreads) hipLaunchKernelGGL(fa_paged_select_kernel<2>, rows, threads, 0, stream, e);
     else if (room <= 4 * kSelThreads) hipLaunchKernelGGL(fa_paged_select_kernel<4>, rows, threads, 0, stream, e);
     else hipLaunchKernelGGL(fa_paged_select_kernel<kSelKeys>, rows, threads, 0, stream, e);
+  } else if (e.chunks == 1) {
+    hipLaunchKernelGGL(fa_paged_select_blocks_kernel, dim3((unsigned)pairs), threads, 0, stream, e);
   } else {
     const dim3 rows((unsigned)(pairs * e.chunks));
     hipLaunchKernelGGL(fa_paged_select_long_kernel<0>, rows, threads, 0, stream, e);

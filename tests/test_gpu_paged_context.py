@@ -627,6 +627,18 @@ def test_evict_many_blocks_of_a_workgroup(device):
     assert torch.equal(k[3:, :, :keep], want)
 
 
+@pytest.mark.parametrize("keep,recent", [(0, 0), (1, 1), (700, 33), (9000, 0), (17000, 0)])
+def test_evict_many_long_rows(device, keep, recent):
+    """Rows of several blocks, of each a workgroup: lengths at a block's borders and none, ties, pages missing."""
+    lens = [17000, 8191, 8192, 8193, 0, 1, 16384, 16385, 9999] + [(61 * i) % 400 for i in range(57)]
+    c = Cache(lens, 2, 64, 256, BF16, False, gone=[(0, 0), (0, 32), (3, 32), (6, 5)])
+    g = torch.Generator().manual_seed(6)
+    w = torch.rand(66, 2, c.width * 256, generator=g)
+    w[:9] = torch.randint(0, 6, w[:9].shape, generator=g).float()
+    w[7, 1, ::3] = math.nan
+    evict(c, device, keep, recent, w=w)
+
+
 @pytest.mark.parametrize("q8", [False, True])
 def test_evict_missing_pages(device, q8):
     """Positions without a page hold no row: what stays closes up; to_table may lack pages too."""

@@ -290,6 +290,13 @@ def test_evict_in_place_is_refused(lib):
         assert msg in lib.fa_sm75_last_error()
 
 
+def test_evict_workspace_of_many_long_rows(lib):
+    """The positions of those that stay, and nothing for each digit of each row."""
+    size = lambda c, **kw: lib.fa_sm75_paged_evict_workspace_size(ctypes.byref(evict(c, **kw)))  # noqa: E731
+    assert size(cache(batch=65, max_pages=1024), weights_len=1 << 14) == 65 * 2 * 20 * 4
+    assert size(cache(batch=1 << 18, max_pages=1 << 16), weights_len=1 << 20) == (1 << 18) * 2 * 20 * 4
+
+
 def test_evict_sizes(lib):
     assert lib.fa_sm75_paged_evict(None) == 1
     assert lib.fa_sm75_paged_evict(ctypes.byref(evict(cache(heads_kv=0)))) == 1
