@@ -229,6 +229,36 @@ def test_prefix_nonfinite(device):
         ref.check(o[2, h], want[2, h], tol[2, h] * (1 + 2.0 ** -4), "O")
 
 
+@pytest.mark.parametrize("news", [[1, 1, 1], [5, 3, 8], [70, 5, 33]])
+@pytest.mark.parametrize("which", ["prefix", "own", "all of a prefix"])
+def test_prefix_infinite_keys(device, news, which):
+    """Keys that all rows score -inf have no part in O and LSE, alone in a tile or a whole prefix of them."""
+    lens = [max(n, x) for n, x in zip(news, [20, 90, 40])]
+    own, shared = Cache(lens, 1, 64, 16, BF16, False, news=news), Cache([64, 70], 1, 64, 16, BF16, False, seed=3)
+    at = {"prefix": [(shared, 0, 3), (shared, 0, 33), (shared, 1, 69)], "own": [(own, 0, 2), (own, 1, 40)],
+          "all of a prefix": [(shared, 1, j) for j in range(70)]}[which]
+    q = torch.rand(sum(news), 4, 64, generator=torch.Generator().manual_seed(1)).bfloat16() + 0.125
+    joined = con.Joined(own, shared, [0, 1, None])  # of it those keys are left out
+    left = [joined.held(b) for b in range(3)]
+    for c, b, j in at:
+        c.k[int(c.table[b, j // 16]), 0, j % 16, 7] = -math.inf
+        c.rows[b][0][0, j, 7] = -math.inf
+        left[b][j + (len(left[b]) - own.lens[b] if c is own else 0)] = False
+    joined.held = lambda b: left[b]
+    want, want_lse, tol, lse_tol = ref.attention(joined, q)
+    tol, lse_tol = tol * (1 + 2.0 ** -4), lse_tol + 2.0 ** -15  # (as in attend)
+    args, _ = on(device, own, shared)
+    pools, table, rest = args[:2], args[2], args[3:]
+    wide = torch.nn.functional.pad(table, (0, (160 << 20) // (3 * 256 * 16)), value=-1)
+    for t in (table, wide):
+        for hint in (1, 10 ** 6):
+            o, lse = fa.flash_attention_paged_prefix(
+                q.to(device), *pools, t, *rest, cu_seqlens=own.cu.to(device), max_query_len=hint, return_lse=True,
+                cu_prefix=torch.tensor([0, 1, 2], dtype=torch.int32, device=device))
+            ref.check(o, want, tol, f"O (hint {hint})")
+            ref.check(lse, want_lse, lse_tol, f"LSE (hint {hint})")
+
+
 def test_prefix_indexes_are_held_to_their_ranges(device):
     """cu_prefix and cu_seqlens that fall or pass their ends: nothing outside the rows is written."""
     own, shared = Cache([50, 30], 2, 64, 16, FP16, False, news=[3, 1]), Cache([50, 20], 2, 64, 16, FP16, False, seed=3)
