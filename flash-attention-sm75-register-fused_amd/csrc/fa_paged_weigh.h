@@ -463,7 +463,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   // Loads of a tile's rows go through windows from its first row's token and the first head of the
   // group on, with offsets below 2^31 bytes (the launcher sees to it), whose factors have 24 bits.
   float lse_next;
-  bool lse_copy;
   const int q_tok = 2 * (int)a.qt, q_head = 2 * (int)a.qh;  // in bytes
   const int tok_step = uniform((int)((unsigned)kWRows / (unsigned)a.group));
   const int rem_step = kWRows - tok_step * a.group;
@@ -499,7 +498,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     }
     const float* const lse = w.lse + (int64_t)hkv * a.group * a.tokens + s.t0 + ld_tok;
     lse_next = lse[lse_off];
-    lse_copy = lane > end;
     fence_schedule();  // (the LSE is waited for first)
     const __amdgpu_buffer_rsrc_t rq =
         make_rsrc(a.q + (int64_t)(s.t0 + ld_tok) * a.qt + (int64_t)hkv * a.group * a.qh, INT32_MAX);
@@ -521,11 +519,11 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   // wave has all the tile's LSE).  Their products with a key that is not finite may be NaN.  Copies of the last row
   // behind it get a finite least, with which a score that the row itself makes 0, infinite or NaN stays so.
   int out_tiles = 0;
-  auto store_lse = [&](int buf) {
+  auto store_lse = [&](int buf, int tile) {
     const bool out = lse_next == -__builtin_inff();
     const float nl = -lse_next * kWLog2e;
     if (tid < kWRows)
-      lse_lds[buf][tid] = out ? __builtin_inff() : lse_copy ? -FLT_MAX : nl == __builtin_inff() ? FLT_MAX : nl;
+      lse_lds[buf][tid] = out ? __builtin_inff() : tid > nrows - 1 - (tile0 + tile) * kWRows ? -FLT_MAX : nl == __builtin_inff() ? FLT_MAX : nl;
     out_tiles = uniform((out_tiles & ~(1 << buf)) | (__builtin_amdgcn_ballot_w64(out) != 0 ? 1 << buf : 0));
   };
   int q_base[KK];
@@ -537,11 +535,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   };
   float sum[2] = {0.0f, 0.0f};
   float16v st[2][2];
-  // MASK: 1 where keys may be hidden from rows, 2 where rows may be left out as well (a variant of its own: the select
-  // in 1 too cost all steps 4 to 10%).
   // Half H of step i (I: modulo 4): the probabilities of these 32 rows, whose S is st[H], between the
   // MFMAs of the next 32's (behind the last tile: of what is there, for nobody).  Tile i + 3 is loaded
-  // to where tile i - 1 was, straight to LDS.
+  // to where tile i - 1 was, straight to LDS.  MASK: 1 where keys may be hidden from rows, 2 where rows may be
+  // left out as well (a variant of its own: that select in 1 too cost all steps 4 to 10%).
   auto half_step = [&](int i, auto i_t, auto half_t, auto mask_t) {
     constexpr int I = decltype(i_t)::value;
     constexpr int H = decltype(half_t)::value;
@@ -562,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
       if constexpr (v == 0 && kk + PF < KK) qf[kk + PF] = read_q(buf, 1 - H, kk + PF);
       if constexpr (slot % (NS / 4) == 1 && slot / (NS / 4) < 3) nl[slot / (NS / 4) + 1] = read_lse(slot / (NS / 4) + 1);
       if constexpr (H == 0 && slot == NS / 4) {
-        if (i + 2 < count) store_lse((I + 2) % 4);
+        if (i + 2 < count) store_lse((I + 2) % 4, i + 2);
       }
       if constexpr (H == 0 && slot == NS / 2) {
         if (i + 3 < count) load(std::integral_constant<int, I + 3>{});
@@ -594,10 +591,10 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
     load(I0{});
-    store_lse(0);
+    store_lse(0, 0);
     if (count > 1) {
       load(I1{});
-      store_lse(1);
+      store_lse(1, 1);
     }
     if (count > 2) load(I2{});
     barrier_after_loads<0>();
