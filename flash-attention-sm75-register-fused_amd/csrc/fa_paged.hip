@@ -142,8 +142,8 @@ PagedPlan plan_paged(const PagedArgs& a, int head_dim, int64_t max_query_len,
 //   MB read again           up to 16     16 .. 48     48 .. 80     80 .. 100    100 .. 130   130 .. 200
 //     own keys whole        .49 .81 1.30 .57 .87 1.14 .64 .95 1.20 .81 .96 1.19 .80 1.03 1.32 .88 1.15 1.41
 //     cut                   .38 .57 .84  .57 .67 .83  .60 .75 .88  .68 .82 .99  .70 .87 .93   .89 1.02 1.09
-// (The rule's choice is 0.8% slower than the better of the two on average; most, 26.7 us for 34.7, with 8 tokens each of 24 sequences of
-// 200 keys behind 4 prefixes of 128.)
+// (The rule's choice is 0.8% slower than the better of the two on average; at the most 34.7 us where two launches take 26.7, with 8
+// tokens each of 24 sequences of 100 to 300 keys behind 4 prefixes of 128.)
 bool joins_prefixes(const PagedShared& own, int head_dim, int64_t max_query_len) {
   if (max_query_len * own.group > 32 || own.batch > 64 || own.prefixes > 63) return false;
   const int64_t bytes = ((int64_t)own.pre_pages << own.page_shift) * own.hkv * 2 * head_dim * (own.ks != nullptr ? 1 : 2);

@@ -177,7 +177,7 @@ __device__ __forceinline__ int2 write_kept(const SelRow& row, const SelBlock<KEY
 }
 
 // A workgroup for each (sequence, KV head), where the table has room for one block.  The chain of
-// its steps bounds it (three digits of three barriers): 8.5 us for two rows of 1025 positions, 12.5 for
+// its steps bounds it (three digits of three barriers): 5.5 us for two rows of 1025 positions, 12.6 for
 // 256 of 4096 .. 8192 (8 MB of weights).  With as few keys a thread as the table has room for: of 2 and 8
 // 10.9 and 13.2 us for 8 rows of 1000 positions with the copy, 31.5 and 36.2 for 512.
 template <int KEYS>
@@ -253,8 +253,9 @@ __global__ void __launch_bounds__(kSelThreads, 8) fa_paged_select_blocks_kernel(
 // Longer rows, few: `chunks` workgroups each, in four launches.  The first three count a digit each over
 // the chunk's keys, into a histogram of its own; the next launch adds those up to find the digit (and
 // keeps where the search is), and what of the chunks in front of its own stays by it.  The launches'
-// own chains bound them: 5, 8, 8 and 12 us at eight rows of 131072 positions (4 MB of weights, read four
-// times).  The chunk's first keys are loaded under the search for the digit: 55.6 us with the move for 57.0.
+// own chains bound them: 5, 8, 8 and 11 us at eight rows of 131072 positions (4 MB of weights, read four
+// times), with the move 56 where the caches have them and 66 cold.  The chunk's first keys are loaded under the
+// search for the digit (without, 57.0 for 55.6).
 struct SelState {  // a row's search behind a digit
   unsigned bound;
   int need, target, search;

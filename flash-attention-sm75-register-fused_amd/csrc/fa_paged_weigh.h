@@ -87,10 +87,11 @@ struct WeighLine {
 // equal stretch, whatever heads and sequences it covers: as many waves as run at once, or one for
 // each tile.  K goes to registers, the next tile's under the current one's work.  (Runs of 8 tiles
 // a wave, as the GPU got round to them, left a last round of half the waves: 88 us for 80 at 32 sequences
-// of 4096 .. 8192 rows of 128, 8 KV heads, and 40.5 for 36 at 8 bits.)
+// of 4096 .. 8192 rows of 128, 8 KV heads.)
 //
-// Bound: K comes from HBM once, 403 MB in 80 us (5.0 TB/s, as fast as a copy moves bytes); at 8 bits
-// 211 MB in 36 us (5.8 TB/s).  A token over a few thousand rows is latency, 5 us.
+// Bound: K comes from HBM once, 403 MB in 79 us (5.1 TB/s, as fast as a copy moves bytes); at 8 bits
+// 211 MB in 46 us with cold caches (4.5 TB/s), 36 where the 256 MB cache has part of it.  A token over a
+// few thousand rows is latency, 5 us.
 template <int D, bool BF16, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kernel(const WeighArgs w) {
   using E = Elem<BF16>;
@@ -280,8 +281,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) fa_paged_weigh_kern
 // 64 42 for 35; where the parts came to two whole rounds the line costs 4%).
 //
 // Bound: the matrix units, the exponentials and the sums share a SIMD's two waves.  The last 2048
-// tokens of 8192, 32 heads of 128 on 8, are 120 GFLOP in 142 us (0.85 PFLOP/s), the matrix units 44%
-// busy; rows loaded through registers, one step ahead, 154.
+// tokens of 8192, 32 heads of 128 on 8, are 120 GFLOP in 142 us (0.85 PFLOP/s), the matrix units 42%
+// busy, 8-bit keys 136; rows loaded through registers, one step ahead, 154.
 constexpr int kWRows = 64;      // rows of a tile, two of S
 constexpr int kWMinTiles = 8;   // tiles a stretch has at least
 
@@ -522,8 +523,9 @@ __global__ void __launch_bounds__(kThreads, 2) fa_paged_weigh_chunk_kernel(const
   auto store_lse = [&](int buf, int tile) {
     const bool out = lse_next == -__builtin_inff();
     const float nl = -lse_next * kWLog2e;
+    const bool copy = tid > nrows - 1 - (tile0 + tile) * kWRows;
     if (tid < kWRows)
-      lse_lds[buf][tid] = out ? __builtin_inff() : tid > nrows - 1 - (tile0 + tile) * kWRows ? -FLT_MAX : nl == __builtin_inff() ? FLT_MAX : nl;
+      lse_lds[buf][tid] = out ? __builtin_inff() : copy ? -FLT_MAX : nl == __builtin_inff() ? FLT_MAX : nl;
     out_tiles = uniform((out_tiles & ~(1 << buf)) | (__builtin_amdgcn_ballot_w64(out) != 0 ? 1 << buf : 0));
   };
   int q_base[KK];

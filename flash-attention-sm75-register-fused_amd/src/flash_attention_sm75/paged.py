@@ -162,8 +162,8 @@ def flash_attention_paged_prefix(Q, k_cache, v_cache, prefix_table, prefix_lens,
         prefix_table: [G, max_prefix_pages] int32, the pages of each prefix, as block_table.
         prefix_lens: [G] int32, tokens of each prefix.
         cu_prefix: [G + 1] int32, rising: sequences cu_prefix[g] .. cu_prefix[g + 1] - 1 have
-            prefix g, those before cu_prefix[0] and from cu_prefix[G] on none.  None: there is
-            one prefix, and every sequence has it.
+            prefix g, those before cu_prefix[0] and from cu_prefix[G] on none.  (Where it falls, which
+            prefix a sequence gets is not said.)  None: there is one prefix, and every sequence has it.
         max_prefix_queries: the most new tokens behind one prefix, if the caller knows: a hint
             as max_query_len.
         causal: by which a new token sees its sequence's own keys; it sees all of its prefix.

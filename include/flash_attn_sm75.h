@@ -431,12 +431,14 @@ int fa_sm75_paged_forward(const fa_paged_params* p);
  * depend on the sizes and the current device only, not on what the tables hold. */
 int64_t fa_sm75_paged_workspace_size(const fa_paged_params* p);
 
-/* Attention of sequences that share a prefix, whose rows are read once for all of them.
+/* Attention of sequences that share a prefix, whose rows are read once for all of them (or, of few rows
+ * and short tables, by each in one launch).
  * Sequences cu_prefix[g] .. cu_prefix[g + 1] - 1 of the call's batch have prefix g: their new
  * tokens see all of its keys, whatever p->causal is, and their own (the cache's block_table
  * and seq_lens, which do not count the prefix) by p->causal; sequences before cu_prefix[0] and
- * from cu_prefix[count] on have none.  The pages are the cache's.  cu_prefix is held to
- * [0, batch] and to rising. */
+ * from cu_prefix[count] on have none.  The pages are the cache's.  cu_prefix has to rise: where it
+ * falls, which prefix a sequence gets, or none, is not said and depends on the tables' sizes; nothing outside the
+ * arrays is read or written then either. */
 typedef struct fa_paged_prefix {
   const int32_t* block_table; /* [count, max_pages], rows block_table_stride apart, as the cache's */
   const int32_t* lens;        /* [count]: tokens of each prefix */
